@@ -287,6 +287,81 @@ int q3c_transformer(q3c_ctx* ctx, const float* x_dev, int32_t batch, int32_t fra
  * so that half the bytes cross PCIe.  Asynchronous on the stream; wav and pcm are device pointers. */
 int q3c_wav_to_pcm16(const float* wav_dev, int64_t samples, int16_t* pcm_dev, void* hip_stream);
 
+/* -- paged key/value cache of an autoregressive transformer ---------------------------------------------------------------
+ * The reference's codes come from an autoregressive model (Qwen3TTSModel.generate_*, reference server.py:245-251, models.py:86-101)
+ * whose attention it leaves to a library chosen by name (models.py:22).  These operators are what such a model needs of a cache
+ * on this GPU: grouped heads, per-head norms and rotation on the way in, a sliding window with first tokens that stay visible,
+ * 4-bit storage, and pages that requests share (one cached voice prompt, many requests).  They take no context, do not allocate,
+ * do not synchronise and read nothing on the host, so every one of them can be captured into a HIP graph.
+ *
+ * A q3c_kv describes device memory that the CALLER owns:
+ *   k, v     [layers][pages][kv_heads][page_size][head_dim], 16-byte aligned.  F32 / BF16; INT4: [..][head_dim / 2] bytes, byte
+ *            m * (head_dim / 32) + g of a row (m < 16) packing dimensions 32 g + m (low half) and 32 g + 16 + m, a value n = -7 .. 7
+ *            held as n + 8; and
+ *   k_scale, v_scale (INT4 only): bf16 steps [layers][pages][kv_heads][page_size][head_dim / 32]; a value is n * step
+ *   table    [rows][pages_per_row] int32: the pages of each row's tokens in order, -1 = none
+ *   lens     [rows] int32: tokens of each row;   refs [pages] int32: table entries that name a page (0 = free)
+ *   status   one int32: bits of q3c_kv_status that calls found on the device (sticky; the caller clears it)
+ * page_size: a power of two, 8 .. 256.  head_dim: a multiple of 16, at most 256 (INT4: 64, 128 or 256).  F32 caches take and give
+ * f32 activations, BF16 and INT4 caches bf16.
+ *
+ * A call names its requests by `rows` [sequences] (table rows, distinct) and their new tokens by `offsets` [sequences + 1]: request
+ * i's are tokens offsets[i] .. offsets[i + 1] - 1 of the call's `tokens`; NULL: one each (tokens == sequences).  The last new token of
+ * a request stands at position lens[row] - 1: q3c_kv_reserve first makes room (lens grows), then every layer appends and attends.
+ * Tokens from offsets[sequences] on are neither read nor written.  What a list, an offset or a table entry says is checked on the
+ * device: a token whose row is bad or named before in the call, or that has no page, is not stored (its query is zeros if its row or
+ * position is bad), keys without a page are seen by nobody, and the bit in `status` says so. */
+typedef enum q3c_kv_dtype { Q3C_KV_F32 = 0, Q3C_KV_BF16 = 1, Q3C_KV_INT4 = 2 } q3c_kv_dtype;
+typedef enum q3c_kv_status {
+    Q3C_KV_BAD_ROW = 1,      /* a row id outside the table, named twice, or offsets that do not fit the row's length */
+    Q3C_KV_NO_PAGE = 2,      /* no free page was left, or a token was appended that has no page */
+    Q3C_KV_BAD_PAGE = 4,     /* a page id outside the pool, a count below zero, or a copy pair that was refused */
+    Q3C_KV_FULL_ROW = 8      /* a row's length passed page_size * pages_per_row */
+} q3c_kv_status;
+typedef struct q3c_kv {
+    int32_t struct_size;     /* sizeof(q3c_kv) */
+    int32_t dtype;           /* q3c_kv_dtype */
+    int32_t layers, pages, kv_heads, page_size, head_dim, rows, pages_per_row;
+    void *k, *v, *k_scale, *v_scale;
+    int32_t *table, *lens, *refs, *status;
+} q3c_kv;
+/* Make room for the new tokens: lens[row] grows by each request's count, pages are taken lowest free first, in the order of the call. */
+int q3c_kv_reserve(const q3c_kv* kv, const int32_t* rows, const int32_t* offsets, int32_t sequences, int32_t tokens, void* hip_stream);
+/* Per head of q and k: y = x * rsqrt(mean(x^2) + eps) * weight (NULL weight: no norm), then the first rot_dim dimensions turned by
+ * the token's position: (a, b) = (y[i], y[i + rot_dim / 2]) -> (a cos - b sin, b cos + a sin), tables [positions][rot_dim / 2] fp32 with
+ * positions >= page_size * pages_per_row (rot_dim 0: no rotation; rot_dim a multiple of 8, INT4: 0 or head_dim).  fp32 throughout, rounded once.  k and
+ * v go to the pages (INT4: groups of 32 dimensions, step = bf16(max |x| / 7), n = rint(x / step); a group with an infinity or a NaN
+ * reads back as NaN), q to q_out [tokens][q_heads][head_dim].  q, k, v: [token][head][dim], strides in elements (multiples of 4), dim contiguous. */
+int q3c_kv_append(const q3c_kv* kv, int32_t layer, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                  int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride, int32_t q_heads,
+                  const int32_t* rows, const int32_t* offsets, int32_t sequences, int32_t tokens, const float* q_weight, const float* k_weight,
+                  const float* cos_table, const float* sin_table, int64_t positions, int32_t rot_dim, float eps, void* q_out, void* hip_stream);
+/* What append stored for the same tokens, in one piece: k_out, v_out [tokens][kv_heads][head_dim] in out_precision (q3c_precision);
+ * zeros where there is no page. */
+int q3c_kv_gather(const q3c_kv* kv, int32_t layer, const int32_t* rows, const int32_t* offsets, int32_t sequences, int32_t tokens, void* k_out,
+                  void* v_out, int32_t out_precision, void* hip_stream);
+/* out[t][h] = sum_j softmax_j(scale * q[t][h] . k_j) v_j over the keys j that token t at position p sees: j <= p, and with window > 0
+ * also j > p - window or j < sinks.  Head h reads kv head h / (q_heads / kv_heads).  A token that sees nothing gives zeros.  A
+ * key or value that a token does not see never reaches its output, whatever it holds.  max_len: no row's length is above it (0:
+ * not known); it only steers how the work is split.  Workspace: q3c_kv_attend_workspace_bytes of the same arguments, 16-byte aligned. */
+int q3c_kv_attend_workspace_bytes(const q3c_kv* kv, int32_t q_heads, int32_t sequences, int32_t tokens, int32_t window, int32_t sinks,
+                                  int32_t max_len, size_t* bytes);
+int q3c_kv_attend(const q3c_kv* kv, int32_t layer, const void* q, int64_t q_token_stride, int64_t q_head_stride, int32_t q_heads,
+                  const int32_t* rows, const int32_t* offsets, int32_t sequences, int32_t tokens, int32_t window, int32_t sinks, float scale,
+                  int32_t max_len, void* out, void* workspace, size_t workspace_bytes, void* hip_stream);
+/* Pages.  fork: each child row (empty, named once, no parent of the call) becomes its parent: full pages are shared, a partly
+ * filled last one is copied to a free page (every layer).  release: the rows' pages go back, their lengths become 0.  trim: pages that no
+ * later query of a sliding window sees go back (all their tokens >= sinks and at least `window` before the row's end).  copy: page
+ * dst[i] = page src[i] in every layer; of pairs with one destination the last counts, a pair whose source is another's destination
+ * is refused.  compact: the live pages move to the front of the pool (live pages behind the first *live_dev ones, ascending, to the
+ * free ones before, ascending); table and counts follow, *live_dev = their number.  Workspaces in device memory, 4-byte aligned:
+ * fork 12 * count bytes, copy 4 * count, compact 8 * pages + 16. */
+int q3c_kv_fork(const q3c_kv* kv, const int32_t* parents, const int32_t* children, int32_t count, void* workspace, size_t workspace_bytes, void* hip_stream);
+int q3c_kv_release(const q3c_kv* kv, const int32_t* rows, int32_t count, void* hip_stream);
+int q3c_kv_trim(const q3c_kv* kv, const int32_t* rows, int32_t count, int32_t window, int32_t sinks, void* hip_stream);
+int q3c_kv_copy_pages(const q3c_kv* kv, const int32_t* src, const int32_t* dst, int32_t count, void* workspace, size_t workspace_bytes, void* hip_stream);
+int q3c_kv_compact(const q3c_kv* kv, int32_t* live_dev, void* workspace, size_t workspace_bytes, void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

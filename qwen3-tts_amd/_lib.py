@@ -24,7 +24,9 @@ EXPORTS = ["q3c_create", "q3c_destroy", "q3c_last_error", "q3c_version", "q3c_lo
            "q3c_profile_read", "q3c_stream_pool_create", "q3c_stream_pool_destroy", "q3c_stream_state_bytes",
            "q3c_stream_reset", "q3c_stream_workspace_bytes", "q3c_stream_push", "q3c_stream_push_graph", "q3c_residual_unit", "q3c_convnext_block",
            "q3c_transformer", "q3c_wav_to_pcm16", "q3c_encoder_configure", "q3c_encode_frames", "q3c_encode_workspace_bytes", "q3c_encode",
-           "q3c_debug_set_tuning", "q3c_debug_set_timeline", "q3c_debug_set_operator_context"]
+           "q3c_debug_set_tuning", "q3c_debug_set_timeline", "q3c_debug_set_operator_context",
+           "q3c_kv_reserve", "q3c_kv_append", "q3c_kv_gather", "q3c_kv_attend_workspace_bytes", "q3c_kv_attend", "q3c_kv_fork",
+           "q3c_kv_release", "q3c_kv_trim", "q3c_kv_copy_pages", "q3c_kv_compact"]
 
 
 class Q3cProfileEntry(C.Structure):
@@ -60,6 +62,14 @@ class Q3cEncoderConfig(C.Structure):
         ("downsample_stride", C.c_int32), ("max_positions", C.c_int32),
         ("norm_eps", C.c_float),
     ]
+
+
+class Q3cKv(C.Structure):
+    _fields_ = [("struct_size", C.c_int32), ("dtype", C.c_int32),
+                ("layers", C.c_int32), ("pages", C.c_int32), ("kv_heads", C.c_int32), ("page_size", C.c_int32), ("head_dim", C.c_int32),
+                ("rows", C.c_int32), ("pages_per_row", C.c_int32),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("table", C.c_void_p), ("lens", C.c_void_p), ("refs", C.c_void_p), ("status", C.c_void_p)]
 
 
 def make_encoder_config(ecfg, max_positions: int) -> Q3cEncoderConfig:
@@ -141,6 +151,17 @@ def load() -> C.CDLL:
     lib.q3c_encode_frames.argtypes = [vp, C.c_int64, i64p]
     lib.q3c_encode_workspace_bytes.argtypes = [vp, i32, i32, C.POINTER(C.c_size_t)]
     lib.q3c_encode.argtypes = [vp, vp, i32, i32, vp, vp, vp, C.c_size_t, vp]
+    kv, i64, f32, sz = C.POINTER(Q3cKv), C.c_int64, C.c_float, C.c_size_t
+    lib.q3c_kv_reserve.argtypes = [kv, vp, vp, i32, i32, vp]
+    lib.q3c_kv_append.argtypes = [kv, i32, vp, i64, i64, vp, i64, i64, vp, i64, i64, i32, vp, vp, i32, i32, vp, vp, vp, vp, i64, i32, f32, vp, vp]
+    lib.q3c_kv_gather.argtypes = [kv, i32, vp, vp, i32, i32, vp, vp, i32, vp]
+    lib.q3c_kv_attend_workspace_bytes.argtypes = [kv, i32, i32, i32, i32, i32, i32, C.POINTER(sz)]
+    lib.q3c_kv_attend.argtypes = [kv, i32, vp, i64, i64, i32, vp, vp, i32, i32, i32, i32, f32, i32, vp, vp, sz, vp]
+    lib.q3c_kv_fork.argtypes = [kv, vp, vp, i32, vp, sz, vp]
+    lib.q3c_kv_release.argtypes = [kv, vp, i32, vp]
+    lib.q3c_kv_trim.argtypes = [kv, vp, i32, i32, i32, vp]
+    lib.q3c_kv_copy_pages.argtypes = [kv, vp, vp, i32, vp, sz, vp]
+    lib.q3c_kv_compact.argtypes = [kv, vp, vp, sz, vp]
     for name in EXPORTS:
         fn = getattr(lib, name)
         if name not in ("q3c_destroy", "q3c_last_error", "q3c_version", "q3c_stream_pool_destroy"):

@@ -12,7 +12,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libq3c.so")
 SOURCES = ["convgemm.hip", "convgemm_f32_f32.hip", "convgemm_bf16_bf16.hip", "convgemm_f32_bf16.hip", "convgemm_bf16_f32.hip",
-           "kernels.hip", "decoder.cpp"]
+           "kernels.hip", "kvcache.hip", "kvattend.hip", "decoder.cpp", "kvcache.cpp"]
 # no -ffast-math: the RVQ dequantiser and the fp32 parity path rely on IEEE adds / divides
 # packed fp32 arithmetic (v_pk_add / mul / fma_f32) is kept out of the generated code: some of its forms have given wrong results
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-x", "hip", "-Wall", "-Wno-unused-function",
@@ -32,7 +32,7 @@ def build(force: bool = False, verbose: bool = True) -> str:
     objdir = os.path.join(HERE, "build")
     os.makedirs(objdir, exist_ok=True)
     headers = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "convgemm_impl.h"), os.path.join(CSRC, "encoder_impl.h"),
-               os.path.join(HERE, "..", "include", "q3c.h"), os.path.abspath(__file__)]
+               os.path.join(CSRC, "kv.h"), os.path.join(HERE, "..", "include", "q3c.h"), os.path.abspath(__file__)]
     jobs = []
     for src in SOURCES:
         s = os.path.join(CSRC, src)

@@ -1,0 +1,553 @@
+// Attention over the paged key/value cache (include/q3c.h, q3c_kv_attend): causal by position, optional sliding window with first
+// tokens that stay visible, grouped heads, f32 / bf16 / 4-bit pages, any number of new tokens per request.
+#include "kv.h"
+
+namespace {
+
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+// What one tile of 16 query columns works on.  The new tokens of a request and the heads that share a kv head make its columns: column
+// c is token c / group, head c % group of the kv head, so one new token of a grouped model fills part of one tile and a prompt many.
+// Tiles of all requests are numbered through: request b's start at offsets[b] * group / 16 + b, which leaves room for its
+// rounded-up last one, so the grid needs only the totals that the host knows.
+struct Tile {
+    int seq, row, tok0, ncols, col0;    // request, table row (-1: bad), its first token, columns in all, first column of the tile
+    int first_pos;                      // position of its first new token
+    int pmin, pmax;                     // positions that exist among the tile's columns (pmax < pmin: none)
+    bool on;
+};
+__device__ __forceinline__ Tile kv_tile(const KvAttendArgs& a, int x, int cols, int lane) {
+    Tile t;
+    const int S = a.b.sequences, G = a.group;
+    int n = 1;
+    t.on = false;
+    if (a.b.offsets) {
+        int b = 0;
+        for (int i = 0; i < S; i += 64) {
+            const int j = min(i + lane, S - 1) + 1;
+            const int o = min(max(a.b.offsets[j], 0), a.b.tokens);
+            b += __popcll(__ballot(i + lane < S && (int)((long long)o * G / cols) + j <= x));
+        }
+        if (b >= S) return t;
+        t.tok0 = min(max(a.b.offsets[b], 0), a.b.tokens);
+        n = min(max(a.b.offsets[b + 1], 0), a.b.tokens) - t.tok0;
+        t.seq = b;
+        t.col0 = (x - ((int)((long long)t.tok0 * G / cols) + b)) * cols;
+    } else {
+        const int per = (G + cols - 1) / cols;
+        t.seq = t.tok0 = x / per;
+        if (t.seq >= S) return t;
+        t.col0 = (x - t.seq * per) * cols;
+    }
+    if (n < 1 || t.col0 < 0 || t.col0 >= (long long)n * G) return t;
+    t.ncols = n * G;
+    t.on = true;
+    const int row = a.b.rows[t.seq];
+    t.row = row >= 0 && row < a.c.rows ? row : -1;
+    t.pmin = 0;
+    t.pmax = -1;
+    if (t.row < 0) return t;
+    t.first_pos = a.c.lens[row] - n;
+    const int i0 = t.col0 / G, i1 = min(t.col0 + cols, t.ncols) - 1;
+    t.pmin = max(t.first_pos + i0, 0);
+    t.pmax = min(t.first_pos + i1 / G, (a.c.width << a.c.ps_shift) - 1);
+    return t;
+}
+// The keys a tile can see, in aligned chunks of TB tokens: the first `sinks` tokens' chunks, then from the window's start to the end.
+struct Span {
+    int sink_chunks, first, total;
+    __device__ __forceinline__ int chunk(int i) const { return i < sink_chunks ? i : first + i - sink_chunks; }
+};
+__device__ __forceinline__ Span kv_span(const KvAttendArgs& a, const Tile& t, int tb) {
+    Span s;
+    s.sink_chunks = s.first = s.total = 0;
+    if (t.pmax < t.pmin) return s;
+    int lo = 0;
+    if (a.window > 0) {
+        s.sink_chunks = (min(a.sinks, t.pmax + 1) + tb - 1) / tb;
+        lo = max(0, t.pmin - a.window + 1);
+    }
+    s.first = max(lo / tb, s.sink_chunks);
+    s.total = s.sink_chunks + max(0, t.pmax / tb - s.first + 1);
+    return s;
+}
+
+__device__ __forceinline__ unsigned perm(unsigned hi, unsigned lo, unsigned sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
+__device__ __forceinline__ f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ unsigned pack2(float a, float b) {
+    const bf16 x = (bf16)a, y = (bf16)b;
+    return (unsigned)__builtin_bit_cast(unsigned short, x) | (unsigned)__builtin_bit_cast(unsigned short, y) << 16;
+}
+__device__ __forceinline__ float lo_f(unsigned x) { return __uint_as_float(x << 16); }
+__device__ __forceinline__ float hi_f(unsigned x) { return __uint_as_float(x & 0xffff0000u); }
+
+// ---- the cache types: how a wave holds one chunk of keys and values, and multiplies with it --------------------------------------------
+// Scores are computed transposed, S^T = K Q^T with 16 keys x 16 columns per tile: lane (c, g) = (lane & 15, lane >> 4) reads key
+// row c as the A operand, and gets in return the scores of column c with keys 4 g .. 4 g + 3.  Those are, register for register, the
+// B operand of O^T = V^T P^T when the contraction takes the keys in that order, so probabilities never leave the lane; and because
+// the order of the output rows is free too, lane (m, g) loads for the A operand the DV = DP / 16 consecutive dimensions m DV .. of its
+// keys - whole rows, straight from memory - and transposes that small block in registers (one v_perm per two values).  Nothing
+// passes through LDS.  A chunk is two tiles (32 keys) for bf16 and 4 bits, one (16 keys) for f32.
+template <typename T, int DP> struct Chunk;
+
+template <int DP> struct Chunk<bf16, DP> {
+    static constexpr int TILES = 2, NS = DP / 32, DV = DP / 16, VW = DV / 2;
+    typedef bf16 act;
+    struct Q { u32x4 f[NS]; };
+    u32x4 k[2][NS];
+    unsigned v[8][VW];
+    static __device__ __forceinline__ void load_q(Q& q, const bf16* p, int D, int g, bool on) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            u32x2 x = {0, 0}, y = x;
+            if (on && 32 * s + 8 * g < D) { x = *(const u32x2*)(p + 32 * s + 8 * g); y = *(const u32x2*)(p + 32 * s + 8 * g + 4); }
+            q.f[s] = u32x4{x[0], x[1], y[0], y[1]};
+        }
+    }
+    // row: element offset of this lane's key in its page tensor; dimensions past the head's size read its first ones (their q is 0)
+    __device__ __forceinline__ void load_k(int u, const void* base, long long row, int D, int g, const KvView&, long long) {
+        const bf16* p = (const bf16*)base + row * D;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) { const int d = 32 * s + 8 * g; k[u][s] = *(const u32x4*)(p + (d < D ? d : 0)); }
+    }
+    __device__ __forceinline__ void load_v(int u, const void* base, long long row, int D, int m, const KvView&) {
+        const bf16* p = (const bf16*)base + row * D + (m * DV < D ? m * DV : 0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            if constexpr (VW == 2) { const u32x2 x = *(const u32x2*)(p + r * D); v[4 * u + r][0] = x[0]; v[4 * u + r][1] = x[1]; }
+            else
+#pragma unroll
+                for (int w = 0; w < VW; w += 4) {
+                    const u32x4 x = *(const u32x4*)(p + r * D + 2 * w);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[4 * u + r][w + e] = x[e];
+                }
+        }
+    }
+    __device__ __forceinline__ void drop_v(int j) {
+#pragma unroll
+        for (int w = 0; w < VW; ++w) v[j][w] = 0;
+    }
+    __device__ __forceinline__ f32x4 scores(int u, const Q& q) const {
+        f32x4 s = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < NS; ++i) s = mfma_bf16(k[u][i], q.f[i], s);
+        return s;
+    }
+    __device__ __forceinline__ void weigh(const float* p, f32x4* o) const {
+        u32x4 b;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[j] = pack2(p[2 * j], p[2 * j + 1]);
+#pragma unroll
+        for (int i = 0; i < DV; ++i) {
+            u32x4 x;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = perm(v[2 * j + 1][i / 2], v[2 * j][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+            o[i] = mfma_bf16(x, b, o[i]);
+        }
+    }
+    static __device__ __forceinline__ int dim(int i, int m) { return m * DV + i; }      // of row m of output tile i
+};
+
+template <int DP> struct Chunk<float, DP> {
+    static constexpr int TILES = 1, NS = DP / 16, DV = DP / 16;
+    typedef float act;
+    struct Q { f32x4 f[NS]; };
+    f32x4 k[1][NS];
+    f32x4 v[4][DV / 4];
+    static __device__ __forceinline__ void load_q(Q& q, const float* p, int D, int g, bool on) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            q.f[s] = f32x4{0, 0, 0, 0};
+            if (on && 16 * s < D) q.f[s] = *(const f32x4*)(p + 16 * s + 4 * g);
+        }
+    }
+    __device__ __forceinline__ void load_k(int, const void* base, long long row, int D, int g, const KvView&, long long) {
+        const float* p = (const float*)base + row * D + 4 * g;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) k[0][s] = *(const f32x4*)(p + (16 * s < D ? 16 * s : 0));
+    }
+    __device__ __forceinline__ void load_v(int, const void* base, long long row, int D, int m, const KvView&) {
+        const float* p = (const float*)base + row * D + (m * DV < D ? m * DV : 0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int w = 0; w < DV / 4; ++w) v[r][w] = *(const f32x4*)(p + r * D + 4 * w);
+    }
+    __device__ __forceinline__ void drop_v(int j) {
+#pragma unroll
+        for (int w = 0; w < DV / 4; ++w) v[j][w] = f32x4{0, 0, 0, 0};
+    }
+    __device__ __forceinline__ f32x4 scores(int, const Q& q) const {
+        f32x4 s = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[0][i][e], q.f[i][e], s, 0, 0, 0);
+        return s;
+    }
+    __device__ __forceinline__ void weigh(const float* p, f32x4* o) const {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int i = 0; i < DV; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][i >> 2][i & 3], p[r], o[i], 0, 0, 0);
+    }
+    static __device__ __forceinline__ int dim(int i, int m) { return m * DV + i; }
+};
+
+// 4 bits: a half byte n + 8 under the exponent of 128 IS the bf16 number 128 + (n + 8) (7 fraction bits), one and-or per two values.
+// Keys: the accumulator starts at -136 sum(q) of the group, so a group's product comes out as sum(q n) and is scaled by the key's step.
+// Values: the step goes into the probability, p step in bf16, and a second product with the constant -136 takes the offset out
+// again, chunk by chunk, from the same rounded numbers (one offset for a whole row would cancel against 136 times its sum).
+struct Int4 {};
+template <int D> struct Chunk<Int4, D> {
+    static constexpr int TILES = 2, S = D / 32, DV = D / 16;        // S groups; a lane's keys: 4 S bytes, its values: S bytes a key
+    typedef bf16 act;
+    struct Q { u32x4 f[S]; float bias[S]; };
+    unsigned k[2][S], v[8][(S + 3) / 4], ks[2][2 * S], vs[2][2 * S];
+    static __device__ __forceinline__ void load_q(Q& q, const bf16* p, int, int g, bool on) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            u32x2 x = {0, 0}, y = x;
+            if (on) { x = *(const u32x2*)(p + 32 * s + 4 * g); y = *(const u32x2*)(p + 32 * s + 16 + 4 * g); }
+            q.f[s] = u32x4{x[0], x[1], y[0], y[1]};
+            float t = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t += lo_f(q.f[s][e]) + hi_f(q.f[s][e]);
+            t += __shfl_xor(t, 16);
+            t += __shfl_xor(t, 32);
+            q.bias[s] = -136.f * t;
+        }
+    }
+    template <int N> static __device__ __forceinline__ void load_dw(unsigned* d, const void* p) {
+        if constexpr (N == 1) d[0] = *(const unsigned*)p;
+        else if constexpr (N == 2) { const u32x2 x = *(const u32x2*)p; d[0] = x[0]; d[1] = x[1]; }
+        else
+#pragma unroll
+            for (int w = 0; w < N; w += 4) {
+                const u32x4 x = *(const u32x4*)((const char*)p + 4 * w);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) d[w + e] = x[e];
+            }
+    }
+    __device__ __forceinline__ void load_k(int u, const void* base, long long row, int, int g, const KvView& c, long long row4) {
+        load_dw<S>(k[u], (const char*)base + row * (D / 2) + g * 4 * S);
+        load_dw<2 * S>(ks[u], c.ks + row4 * S);
+    }
+    __device__ __forceinline__ void load_v(int u, const void* base, long long row, int, int m, const KvView& c) {
+        const char* p = (const char*)base + row * (D / 2) + m * S;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            if constexpr (S == 2) v[4 * u + r][0] = *(const unsigned short*)(p + r * (D / 2));
+            else load_dw<S / 4>(v[4 * u + r], p + r * (D / 2));
+        }
+        load_dw<2 * S>(vs[u], c.vs + row * S);
+    }
+    __device__ __forceinline__ void drop_v(int j) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) {                               // the step of key j (a NaN there must not meet its probability 0)
+            unsigned& w = vs[j >> 2][((j & 3) * S + s) >> 1];
+            w &= ((j & 3) * S + s) & 1 ? 0x0000ffffu : 0xffff0000u;
+        }
+    }
+    static __device__ __forceinline__ float step(const unsigned* d, int i) { return i & 1 ? hi_f(d[i >> 1]) : lo_f(d[i >> 1]); }
+    __device__ __forceinline__ f32x4 scores(int u, const Q& q) const {
+        f32x4 t = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            u32x4 x;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {                           // bytes s of the lane's m = 4 g + 2 e and + 1
+                unsigned z;
+                if constexpr (S == 2) z = perm(0, k[u][e], 0x0c000c00u | (unsigned)(s + 2) << 16 | (unsigned)s);
+                else z = perm(k[u][(2 * e + 1) * (S / 4) + s / 4], k[u][2 * e * (S / 4) + s / 4], 0x0c000c00u | (unsigned)(s % 4 + 4) << 16 | (unsigned)(s % 4));
+                x[e] = (z & 0x000f000fu) | 0x43004300u;
+                x[e + 2] = ((z >> 4) & 0x000f000fu) | 0x43004300u;
+            }
+            const f32x4 d = mfma_bf16(x, q.f[s], f32x4{q.bias[s], q.bias[s], q.bias[s], q.bias[s]});
+#pragma unroll
+            for (int r = 0; r < 4; ++r) t[r] = fmaf(step(ks[u], r * S + s), d[r], t[r]);
+        }
+        return t;
+    }
+    __device__ __forceinline__ void weigh(const float* p, f32x4* o) const {
+        const u32x4 off = {0xc308c308u, 0xc308c308u, 0xc308c308u, 0xc308c308u};       // -136
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            u32x4 b, lo, hi;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int u = j >> 1, r = 2 * (j & 1);
+                b[j] = pack2(p[2 * j] * step(vs[u], r * S + s), p[2 * j + 1] * step(vs[u], (r + 1) * S + s));
+                const unsigned z = perm(v[2 * j + 1][s / 4], v[2 * j][s / 4], 0x0c000c00u | (unsigned)(s % 4 + 4) << 16 | (unsigned)(s % 4));
+                lo[j] = (z & 0x000f000fu) | 0x43004300u;
+                hi[j] = ((z >> 4) & 0x000f000fu) | 0x43004300u;
+            }
+            o[2 * s] = mfma_bf16(lo, b, mfma_bf16(off, b, o[2 * s]));
+            o[2 * s + 1] = mfma_bf16(hi, b, mfma_bf16(off, b, o[2 * s + 1]));
+        }
+    }
+    static __device__ __forceinline__ int dim(int i, int m) { return 16 * i + m; }
+};
+
+// One workgroup = one tile of columns, one kv head, one of `splits` equal shares of the chunks the tile sees; its four waves take the
+// share's chunks in turn, each with a running maximum and sum of its own, and are joined through LDS at the end.  With splits > 1 the
+// unnormalised sums go to the workspace and kv_join_kernel joins them.  Bound by memory for single tokens: the next chunk's keys are
+// requested before this one's softmax, its values before this one's scores.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) kv_attend_kernel(const KvAttendArgs a) {
+    typedef Chunk<T, DP> C;
+    typedef typename C::act A;
+    constexpr int TB = 16 * C::TILES, NT = DP / 16, LD = DP + 4;
+    __shared__ __attribute__((aligned(16))) float so[4][16][LD];
+    __shared__ float sm[4][16], sl[4][16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int cq = lane & 15, g = lane >> 4;
+    const Tile t = kv_tile(a, blockIdx.x, 16, lane);
+    if (!t.on) return;
+    const int hk = blockIdx.y, G = a.group, D = a.c.dim, sh = a.c.ps_shift;
+    const int col = t.col0 + cq, qtok = col / G;
+    const bool col_on = col < t.ncols;
+    int mypos = col_on && t.row >= 0 ? t.first_pos + qtok : -1;
+    if (mypos > t.pmax) mypos = -1;
+    typename C::Q q;
+    C::load_q(q, (const A*)a.q.p + (long long)(t.tok0 + qtok) * a.q.ts + (long long)(hk * G + col - qtok * G) * a.q.hs, D, g, mypos >= 0);
+
+    const Span span = kv_span(a, t, TB);
+    const int per = (span.total + a.splits - 1) / a.splits;
+    const int c_end = min(span.total, (int)(blockIdx.z + 1) * per), c_begin = (int)blockIdx.z * per + wave;
+    const int* table = a.c.table + (long long)max(t.row, 0) * a.c.width;
+    const long long page_rows = (long long)a.c.heads << sh;                    // rows of one page, all heads
+    const long long head0 = ((long long)a.layer * a.c.pages * a.c.heads + hk) << sh;
+    const int in_page = (1 << sh) - 1, last_entry = a.c.width - 1;
+    const int W = a.window > 0 ? a.window : 0x7fffffff, sinks = a.window > 0 ? a.sinks : 0;
+
+    const float cs = a.scale_log2e;
+    int only = t.pmin - 1;                     // pmin - 1: all columns at once; else the one position whose columns are wanted (below)
+    for (;;) {
+        const bool all = only < t.pmin;
+        const int vlo = (all ? t.pmin : only) - W, vhi = all ? t.pmax : only;       // a value row counts if vlo < its position <= vhi
+        f32x4 o[NT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) o[i] = f32x4{0, 0, 0, 0};
+        float m = -INFINITY, l = 0.f;
+        int ek[C::TILES], ev[C::TILES];
+        C ch;
+        auto entries = [&](int tb) {
+#pragma unroll
+            for (int u = 0; u < C::TILES; ++u) {
+                ek[u] = table[min((tb + 16 * u + cq) >> sh, last_entry)];
+                ev[u] = table[min((tb + 16 * u + 4 * g) >> sh, last_entry)];
+            }
+        };
+        auto row_of = [&](int e, int tok) { return head0 + (long long)((unsigned)e < (unsigned)a.c.pages ? e : 0) * page_rows + (tok & in_page); };
+        auto keys = [&](int tb) {
+#pragma unroll
+            for (int u = 0; u < C::TILES; ++u)
+                ch.load_k(u, a.c.k, row_of(ek[u], tb + 16 * u + cq), D, g, a.c, row_of(ev[u], tb + 16 * u + 4 * g));
+        };
+        int c = c_begin, tb = 0;
+        if (c < c_end) {
+            tb = span.chunk(c) * TB;
+            entries(tb);
+            keys(tb);
+        }
+        while (c < c_end) {
+            bool pages_ok = true;
+            int ok[C::TILES];
+#pragma unroll
+            for (int u = 0; u < C::TILES; ++u) {
+                ch.load_v(u, a.c.v, row_of(ev[u], tb + 16 * u + 4 * g), D, cq, a.c);
+                ok[u] = (unsigned)ev[u] < (unsigned)a.c.pages;
+                pages_ok = pages_ok && ok[u];
+            }
+            const int now = tb;
+            c += 4;
+            if (c < c_end) {
+                tb = span.chunk(c) * TB;
+                entries(tb);
+            }
+            float x[4 * C::TILES];
+#pragma unroll
+            for (int u = 0; u < C::TILES; ++u) {
+                const f32x4 s = ch.scores(u, q);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[4 * u + r] = s[r];
+            }
+            if (c < c_end) keys(tb);
+            const bool whole = now + TB - 1 <= t.pmin && (now > t.pmax - W || now + TB - 1 < sinks) && __all(pages_ok);
+            if (!whole) {
+#pragma unroll
+                for (int j = 0; j < 4 * C::TILES; ++j) {
+                    const int tok = now + 16 * (j >> 2) + 4 * g + (j & 3);
+                    const bool sees = ok[j >> 2] && tok <= mypos && (tok > mypos - W || tok < sinks);
+                    x[j] = sees ? x[j] : -INFINITY;
+                    if (!(ok[j >> 2] && tok <= vhi && (tok > vlo || tok < sinks))) ch.drop_v(j);
+                }
+            }
+            float top = x[0];
+#pragma unroll
+            for (int j = 1; j < 4 * C::TILES; ++j) top = fmaxf(top, x[j]);
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float mn = fmaxf(m, top * cs), mu = mn == -INFINITY ? 0.f : mn;
+            if (__any(mn > m)) {
+                const float f = __builtin_amdgcn_exp2f(m - mu);
+                l *= f;
+#pragma unroll
+                for (int i = 0; i < NT; ++i) o[i] *= f;
+            }
+            m = mn;
+#pragma unroll
+            for (int j = 0; j < 4 * C::TILES; ++j) {
+                x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], cs, -mu));
+                l += x[j];
+            }
+            ch.weigh(x, o);
+        }
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        if (all || mypos == only) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) so[wave][cq][C::dim(i, 4 * g + r)] = o[i][r];
+            if (g == 0) { sm[wave][cq] = mypos < 0 ? -INFINITY : m; sl[wave][cq] = mypos < 0 ? 0.f : l; }
+        }
+        // A matrix product spreads an infinite or NaN value row to columns that do not see it (0 times it is NaN).  So when a result is
+        // not finite and the tile's columns differ in what they see, each position is computed again with the rows it does not see
+        // taken out, and only its own columns kept.  Finite data never comes here.
+        if (all) {
+            float bad = 0.f;
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) bad += o[i][r] * 0.f;
+            if (t.pmax <= t.pmin || !__any(mypos >= 0 && bad != 0.f)) break;
+        }
+        if (++only > t.pmax) break;
+    }
+    __syncthreads();
+    // join the four waves; thread (c, j) takes DP / 16 dimensions of column c
+    const int c = tid >> 4, d0 = (tid & 15) * (DP / 16);
+    if (t.col0 + c >= t.ncols || d0 >= D) return;
+    float mx = -INFINITY, l = 0.f, f[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mx = fmaxf(mx, sm[w][c]);
+    const float mu = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        f[w] = __builtin_amdgcn_exp2f(sm[w][c] - mu);
+        l = fmaf(sl[w][c], f[w], l);
+    }
+    f32x4 r[DP / 64];
+#pragma unroll
+    for (int i = 0; i < DP / 64; ++i) {
+        r[i] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) r[i] += *(const f32x4*)&so[w][c][d0 + 4 * i] * f[w];
+    }
+    if (a.splits > 1) {
+        float* ws = a.ws + (((long long)blockIdx.x * gridDim.y + hk) * a.splits + blockIdx.z) * (16 * (DP + 2)) + c * (DP + 2);
+#pragma unroll
+        for (int i = 0; i < DP / 64; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) ws[2 + d0 + 4 * i + e] = r[i][e];
+        if (d0 == 0) { ws[0] = mx; ws[1] = l; }
+        return;
+    }
+    const int tk = (t.col0 + c) / G, h = hk * G + t.col0 + c - tk * G;
+    const bool none = l == 0.f;
+    const float inv = 1.0f / l;
+    A* out = (A*)a.out + ((long long)(t.tok0 + tk) * a.q_heads + h) * D + d0;
+#pragma unroll
+    for (int i = 0; i < DP / 64; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[4 * i + e] = (A)(none ? 0.f : r[i][e] * inv);
+}
+
+// out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the shares of one tile and head
+template <typename A, int DP>
+__global__ void __launch_bounds__(256) kv_join_kernel(const KvAttendArgs a) {
+    const int tid = threadIdx.x;
+    const Tile t = kv_tile(a, blockIdx.x, 16, tid & 63);
+    if (!t.on) return;
+    const int hk = blockIdx.y, G = a.group, D = a.c.dim, c = tid >> 4, d0 = (tid & 15) * (DP / 16);
+    if (t.col0 + c >= t.ncols || d0 >= D) return;
+    const float* ws = a.ws + ((long long)blockIdx.x * gridDim.y + hk) * a.splits * (16 * (DP + 2)) + c * (DP + 2);
+    float mx = -INFINITY, l = 0.f;
+    for (int s = 0; s < a.splits; ++s) mx = fmaxf(mx, ws[(long long)s * (16 * (DP + 2))]);
+    const float mu = mx == -INFINITY ? 0.f : mx;
+    float r[DP / 16];
+#pragma unroll
+    for (int e = 0; e < DP / 16; ++e) r[e] = 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+        const float* w = ws + (long long)s * (16 * (DP + 2));
+        const float ls = w[1], f = __builtin_amdgcn_exp2f(w[0] - mu);
+        if (ls == 0.f) continue;
+        l = fmaf(ls, f, l);
+#pragma unroll
+        for (int e = 0; e < DP / 16; ++e) r[e] = fmaf(w[2 + d0 + e], f, r[e]);
+    }
+    const int tk = (t.col0 + c) / G, h = hk * G + t.col0 + c - tk * G;
+    const bool none = l == 0.f;
+    const float inv = 1.0f / l;
+    A* out = (A*)a.out + ((long long)(t.tok0 + tk) * a.q_heads + h) * D + d0;
+#pragma unroll
+    for (int e = 0; e < DP / 16; ++e) out[e] = (A)(none ? 0.f : r[e] * inv);
+}
+
+int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+long long tiles_of(int tokens, int sequences, int group, bool ragged) {
+    return ragged ? (long long)tokens * group / 16 + sequences : (long long)sequences * ((group + 15) / 16);
+}
+
+}  // namespace
+
+// How many shares a tile's keys are cut into: as many workgroups as keep 256 compute units busy, each with at least 8 chunks' work
+// (two rounds of its four waves).
+int q3_kv_attend_splits(const KvView& c, int tokens, int sequences, int q_heads, int window, int sinks, int max_len) {
+    const int group = q_heads / c.heads, tb = c.dtype == Q3C_KV_F32 ? 16 : 32;
+    long long len = (long long)c.width << c.ps_shift;
+    if (max_len > 0 && max_len < len) len = max_len;
+    if (window > 0 && (long long)window + sinks + tb < len) len = (long long)window + sinks + tb;
+    const long long chunks = len / tb + 1, base = (tokens == sequences ? (long long)sequences * ((group + 15) / 16) : (long long)tokens * group / 16 + 1) * c.heads;
+    long long n = (1024 + base - 1) / (base ? base : 1);
+    if (n > (chunks + 7) / 8) n = (chunks + 7) / 8;
+    return (int)(n < 1 ? 1 : n > 128 ? 128 : n);
+}
+size_t q3_kv_attend_ws(const KvView& c, int tokens, int sequences, int q_heads, int splits) {
+    if (splits < 2) return 0;
+    const int group = q_heads / c.heads;
+    const long long tiles = tiles_of(tokens, sequences, group, true);
+    const long long flat = tiles_of(tokens, sequences, group, false);
+    return (size_t)((tiles > flat ? tiles : flat) * c.heads * splits) * (16 * (padded_dim(c.dim) + 2)) * sizeof(float);
+}
+
+hipError_t q3_launch_kv_attend(const KvAttendArgs& a, hipStream_t s) {
+    const unsigned tiles = (unsigned)tiles_of(a.b.tokens, a.b.sequences, a.group, a.b.offsets != nullptr);
+    if (!tiles || !a.b.tokens) return hipSuccess;
+    const dim3 grid(tiles, a.c.heads, a.splits), join(tiles, a.c.heads);
+    const int dp = padded_dim(a.c.dim);
+#define Q3_ATTEND(T, A, DP)                                                        \
+    do {                                                                           \
+        kv_attend_kernel<T, DP><<<grid, 256, 0, s>>>(a);                           \
+        if (a.splits > 1) kv_join_kernel<A, DP><<<join, 256, 0, s>>>(a);           \
+    } while (0)
+#define Q3_ATTEND_DIM(T, A)                        \
+    do {                                           \
+        if (dp == 64) Q3_ATTEND(T, A, 64);         \
+        else if (dp == 128) Q3_ATTEND(T, A, 128);  \
+        else Q3_ATTEND(T, A, 256);                 \
+    } while (0)
+    if (a.c.dtype == Q3C_KV_F32) Q3_ATTEND_DIM(float, float);
+    else if (a.c.dtype == Q3C_KV_BF16) Q3_ATTEND_DIM(bf16, bf16);
+    else Q3_ATTEND_DIM(Int4, bf16);
+#undef Q3_ATTEND_DIM
+#undef Q3_ATTEND
+    return hipGetLastError();
+}

@@ -107,3 +107,51 @@ def snake_beta(x: torch.Tensor, alpha: torch.Tensor, beta: torch.Tensor, eps: fl
 @snake_beta.register_fake
 def _(x, alpha, beta, eps):
     return torch.empty_like(x, dtype=torch.float32)
+
+
+# ---- paged key/value cache (kvcache.PagedKV, registered under a handle like a decoder) ---------------------------------------------
+#     h = torch_ops.register_kv(kv)
+#     q = torch.ops.q3tts.kv_append(q, k, v, rows, None, wq, wk, cos, sin, 1e-6, h, layer)      # writes the cache behind the handle
+#     o = torch.ops.q3tts.kv_attend(q, rows, None, 4096, 4, h, layer)
+_caches: Dict[int, object] = {}
+
+
+def register_kv(cache) -> int:
+    h = _next[0]
+    _next[0] += 1
+    _caches[h] = cache
+    return h
+
+
+def unregister_kv(handle: int) -> None:
+    _caches.pop(handle, None)
+
+
+def _kv(handle: int):
+    try:
+        return _caches[handle]
+    except KeyError:
+        raise KeyError(f"no cache registered under handle {handle}") from None
+
+
+@torch.library.custom_op("q3tts::kv_append", mutates_args=(), device_types="cuda")
+def kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rows: torch.Tensor, offsets: Optional[torch.Tensor],
+              q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
+              eps: float, handle: int, layer: int) -> torch.Tensor:
+    return _kv(handle).append(layer, q, k, v, rows, offsets, q_weight=q_weight, k_weight=k_weight,
+                              rope=None if cos is None else (cos, sin), eps=eps)
+
+
+@kv_append.register_fake
+def _(q, k, v, rows, offsets, q_weight, k_weight, cos, sin, eps, handle, layer):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("q3tts::kv_attend", mutates_args=(), device_types="cuda")
+def kv_attend(q: torch.Tensor, rows: torch.Tensor, offsets: Optional[torch.Tensor], window: int, sinks: int, handle: int, layer: int) -> torch.Tensor:
+    return _kv(handle).attend(layer, q, rows, offsets, window=window, sinks=sinks)
+
+
+@kv_attend.register_fake
+def _(q, rows, offsets, window, sinks, handle, layer):
+    return q.new_empty(q.shape)

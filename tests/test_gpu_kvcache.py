@@ -1,0 +1,649 @@
+"""The paged key/value cache (kvcache.PagedKV) on the GPU against plain 64-bit restatements of each operator (kv_reference.py).
+
+Tolerances count roundings, u = eps / 2 of a type (bf16 2^-8, fp32 2^-24):
+  append  the head norm's sum (14 additions deep), mean, root, quotient, weight and the rotation's three operations are under 32
+          fp32 roundings of numbers no larger than |a| + |b| of the rotated pair; storing rounds once more.
+  attend  bf16: one rounding of the output, one of each probability (averaged by the weights they are: u times the weighted mean of
+          |v|); 4 bits: the probability times its step is what is rounded.  fp32: a score is off by at most (D + 4) u sum |q k| scale, and a
+          relative error of e^score follows; sums of N terms add N u.  4 bits also subtracts 136 times a sum: 144 u per value."""
+import math
+
+import pytest
+import torch
+
+from kv_reference import Pages, attention, norm_rotate
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+ACT = {"f32": torch.float32, "bf16": torch.bfloat16, "int4": torch.bfloat16}
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _randn(g, *shape, dtype=torch.float32):
+    return torch.randn(shape, generator=g, device=DEV).to(dtype)
+
+
+def _cache(dtype, G, D, ps, lens, rows=None, spare=3, layers=1, seed=0, width=None):
+    """A cache whose rows hold `lens` tokens on shuffled pages, every place filled with NaN."""
+    from qwen3_tts_amd.kvcache import PagedKV
+    n = [-(-x // ps) for x in lens]
+    width = max(n) + 2 if width is None else width
+    kv = PagedKV(layers, G, D, sum(n) + spare, ps, rows or len(lens), width, dtype, DEV)
+    order = torch.randperm(kv.pages, generator=torch.Generator().manual_seed(seed)).tolist()
+    for r, c in enumerate(n):
+        ids = [order.pop() for _ in range(c)]
+        kv.table[r, :c] = torch.tensor(ids, dtype=torch.int32)
+        kv.refs[torch.tensor(ids, dtype=torch.long, device=DEV)] += 1
+        kv.lens[r] = lens[r]
+    if dtype == "int4":
+        for t in (kv.k, kv.v):
+            t.fill_(0x11)
+        for t in (kv.k_scale, kv.v_scale):
+            t.fill_(float("nan"))
+    else:
+        for t in (kv.k, kv.v):
+            t.fill_(float("nan"))
+    return kv
+
+
+def _fill(kv, layer, lens, g, spread=1.0):
+    """Random K and V for all tokens of all rows, through append without norm and rotation.  -> per row (k, v) float64, as stored"""
+    off = torch.tensor([0] + lens, dtype=torch.int32).cumsum(0).to(torch.int32).to(DEV)
+    T = sum(lens)
+    k, v = (_randn(g, T, kv.kv_heads, kv.head_dim).mul_(spread).to(kv.activations) for _ in range(2))
+    rows = torch.arange(len(lens), dtype=torch.int32, device=DEV)
+    kv.append(layer, k, k, v, rows, off)
+    kk, vv = kv.gather(layer, rows, off, tokens=T, dtype="f32")
+    if kv.dtype != "int4":
+        assert torch.equal(kk, k.float()) and torch.equal(vv, v.float())
+    return list(zip(kk.double().split(lens), vv.double().split(lens)))
+
+
+def _offsets(counts):
+    return torch.tensor([0] + list(counts), dtype=torch.int32).cumsum(0).to(torch.int32).to(DEV)
+
+
+def _check_attend(got, want, mag, dot, kv, N, scale, q=None):
+    u = U[got.dtype]
+    score = (kv.head_dim + 4) * 2.0 ** -24 * dot * scale
+    if kv.dtype == "int4":                          # 136 sum q of each group is taken out again, in fp32
+        top = float(kv.k_scale.float().nan_to_num(0.0).max())
+        score += 8 * 144 * 2.0 ** -24 * float(q.abs().sum(-1).max()) * top * scale
+    rel = 2 * score + 2.0 ** -20 + N * 2.0 ** -24
+    if got.dtype == torch.float32:
+        bound = rel * mag + u * want.abs()
+    else:
+        bound = u * mag * 1.01 + rel * mag + u * want.abs() * 1.01
+    if kv.dtype == "int4":
+        bound = bound + 144 * 16 * 2.0 ** -24 * float(kv.v_scale.float().nan_to_num(0.0).max())
+    off = (got.double() - want).abs()
+    assert bool((off <= bound + 1e-30).all()), f"max excess {float((off - bound).max()):.3e}, max error {float(off.max()):.3e}"
+
+
+# ---- append ----------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,D,rot,G,H,ps,norm", [
+    ("bf16", 128, 128, 8, 16, 32, True), ("bf16", 128, 64, 2, 14, 8, True), ("bf16", 64, 64, 16, 16, 16, False),
+    ("bf16", 16, 16, 1, 3, 256, True), ("bf16", 80, 40, 3, 3, 16, True), ("bf16", 256, 0, 1, 8, 64, True), ("bf16", 112, 8, 5, 10, 32, False),
+    ("f32", 64, 64, 16, 16, 16, True), ("f32", 128, 128, 2, 6, 128, True), ("f32", 80, 80, 3, 12, 8, False), ("f32", 256, 256, 1, 1, 16, True),
+])
+@pytest.mark.parametrize("counts", [None, [5, 0, 1, 70]])
+def test_append_norms_rotates_and_stores(dtype, D, rot, G, H, ps, norm, counts):
+    from qwen3_tts_amd.kvcache import rope_tables
+    g = _gen(D + H)
+    new = [1] * 4 if counts is None else counts
+    lens = [n + p for n, p in zip(new, (0, 9, 300, 31))]
+    kv = _cache(dtype, G, D, ps, lens, rows=6, layers=2)
+    before_k, before_v = kv.k.clone(), kv.v.clone()
+    T, extra = sum(new), 3                                        # three tokens behind the last request
+    if counts is None:
+        extra = 0
+    qkv = _randn(g, T + extra, (H + 2 * G) * D).mul_(4).to(kv.activations)
+    q, k, v = (x.view(T + extra, -1, D) for x in qkv.split([H * D, G * D, G * D], 1))
+    wq, wk = ((torch.rand(D, generator=g, device=DEV) + 0.5) for _ in range(2)) if norm else (None, None)
+    cos, sin = rope_tables(kv.max_tokens, rot, device=DEV) if rot else (None, None)
+    rows = torch.tensor([0, 1, 2, 3], dtype=torch.int32, device=DEV)
+    off = None if counts is None else _offsets(new)
+    out = torch.full((T + extra, H, D), 7.0, dtype=kv.activations, device=DEV)
+    got = kv.append(1, q, k, v, rows, off, q_weight=wq, k_weight=wk, rope=None if not rot else (cos, sin), eps=1e-6, out=out)
+    assert got is out and bool((out[T:] == 7.0).all())
+    kv.check()
+    pos = torch.cat([torch.arange(L - n, L) for L, n in zip(lens, new)]).to(DEV)
+    u = U[kv.activations]
+    at = [(r, int(p)) for r, (L, n) in enumerate(zip(lens, new)) for p in range(L - n, L)]
+    pages = torch.tensor([int(kv.table[r, p // ps]) for r, p in at], device=DEV, dtype=torch.long)
+    slots = torch.tensor([p % ps for _, p in at], device=DEV, dtype=torch.long)
+    for what, x, w, stored in (("q", q, wq, out[:T]), ("k", k, wk, kv.k[1, pages, :, slots])):
+        want = norm_rotate(x[:T], w, cos, sin, pos, 1e-6)
+        plain = norm_rotate(x[:T], w, None, None, pos, 1e-6).abs()
+        pair = plain.clone()
+        if rot:
+            h = rot // 2
+            pair[..., :h] = pair[..., h:rot] = plain[..., :h] + plain[..., h:rot]
+        bound = (u * want.abs() if dtype == "bf16" else 0) + 32 * 2.0 ** -24 * pair + 1e-37
+        off_by = (stored.double() - want).abs()
+        assert bool((off_by <= bound * 1.01).all()), f"{what}: {float((off_by - bound).max())}"
+    assert torch.equal(kv.v[1, pages, :, slots], v[:T])
+    back_k, back_v = kv.gather(1, rows, off, tokens=T)
+    assert torch.equal(back_k, kv.k[1, pages, :, slots]) and torch.equal(back_v, v[:T])
+    for new_t, old_t in ((kv.k, before_k), (kv.v, before_v)):     # and nothing else was touched
+        rest = new_t.clone()
+        rest[1, pages, :, slots] = old_t[1, pages, :, slots]
+        bits = torch.int16 if dtype == "bf16" else torch.int32
+        assert torch.equal(rest.view(bits), old_t.view(bits))
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("rot", [True, False])
+def test_append_int4_holds_each_group_to_half_a_step(D, rot):
+    from qwen3_tts_amd.kvcache import rope_tables
+    g = _gen(D)
+    new, lens, G, H, ps = [3, 1, 40], [3, 77, 40], 3, 6, 16
+    kv = _cache("int4", G, D, ps, lens)
+    T = sum(new)
+    q, k, v = (_randn(g, T, n, D).mul_(3).to(torch.bfloat16) for n in (H, G, G))
+    k[2] = 0.0                                                    # a row of zeros
+    v[1, 0, :32] = 0.0
+    v[0, 1, 5] = float("inf")
+    v[0, 2, 40] = float("nan")
+    wq, wk = ((torch.rand(D, generator=g, device=DEV) + 0.5) for _ in range(2))
+    rope = rope_tables(kv.max_tokens, D, device=DEV) if rot else None
+    rows = torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV)
+    out = kv.append(0, q, k, v, rows, _offsets(new), q_weight=wq, k_weight=wk, rope=rope)
+    kv.check()
+    pos = torch.cat([torch.arange(L - n, L) for L, n in zip(lens, new)]).to(DEV)
+    cos, sin = rope or (None, None)
+    wq64 = norm_rotate(q, wq, cos, sin, pos, 1e-6)
+    assert bool(((out.double() - wq64).abs() <= 2.0 ** -8 * wq64.abs() + 64 * 2.0 ** -24 * wq64.abs().amax(-1, keepdim=True)).all())
+    got_k, got_v = kv.gather(0, rows, _offsets(new), tokens=T, dtype="f32")
+    for got, want in ((got_k, norm_rotate(k, wk, cos, sin, pos, 1e-6)), (got_v, v.double())):
+        w, x = want.view(T, G, D // 32, 32), got.double().view(T, G, D // 32, 32)
+        top = w.abs().amax(-1, keepdim=True)
+        good = torch.isfinite(w).all(-1, keepdim=True).expand_as(w)
+        # step = top / 7 rounded to bf16 (1 + 2^-8), a value to half a step, and top itself is at most 7.5 steps: clamping costs nothing more
+        bound = top / 7 * (1 + 2.0 ** -8) / 2 * (1 + 2.0 ** -10) + 64 * 2.0 ** -24 * top
+        assert bool(((x - w).abs() <= bound)[good].all())
+        assert bool((x[good] == 0)[(top.expand_as(w) == 0)[good]].all())
+        assert bool(torch.isnan(x[~good]).all())                  # a group with an infinity or a NaN reads back as NaN
+    assert torch.isfinite(got_v).sum() == T * G * D - 64
+
+
+def test_append_and_attend_read_any_strides():
+    g = _gen(3)
+    lens = [40, 7]
+    kv = _cache("bf16", 2, 64, 16, lens)
+    store = _fill(kv, 0, lens, g)
+    rows = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    base = _randn(g, 2, 4, 64, dtype=torch.bfloat16)
+    want = kv.attend(0, base, rows)
+    heads_first = base.transpose(0, 1).contiguous().transpose(0, 1)         # [token][head] over a [head][token] tensor
+    wide = torch.zeros(2, 4, 80, dtype=torch.bfloat16, device=DEV)
+    wide[..., 4:68] = base
+    odd = torch.zeros(2 * 4 * 64 + 1, dtype=torch.bfloat16, device=DEV)[1:].view(2, 4, 64)     # not aligned to four values
+    odd.copy_(base)
+    spaced = torch.zeros(2, 4, 64, 2, dtype=torch.bfloat16, device=DEV)[..., 0]                  # dim not contiguous
+    spaced.copy_(base)
+    for x in (heads_first, wide[..., 4:68], odd, spaced, base[:1].expand(2, 4, 64)):
+        ref = want if x.stride(0) else kv.attend(0, base[:1].repeat(2, 1, 1), rows)
+        assert torch.equal(kv.attend(0, x, rows), ref)
+    kn = _randn(g, 2, 2, 64, dtype=torch.bfloat16)
+    ref_q = kv.append(0, base, kn, kn, rows)
+    ref = kv.gather(0, rows)
+    for x in (heads_first, wide[..., 4:68], odd, spaced):
+        kv.k.zero_()
+        assert torch.equal(kv.append(0, x, kn.transpose(0, 1).contiguous().transpose(0, 1), kn, rows), ref_q)
+        assert all(torch.equal(a, b) for a, b in zip(kv.gather(0, rows), ref))
+    assert store
+
+
+# ---- attend ----------------------------------------------------------------------------------------------------------------------
+SHAPES = [("bf16", 128, 2, 2, 32), ("bf16", 64, 1, 1, 8), ("bf16", 128, 1, 7, 16), ("bf16", 256, 2, 4, 64), ("bf16", 80, 3, 1, 16), ("bf16", 16, 1, 20, 128),
+          ("f32", 64, 2, 1, 16), ("f32", 128, 1, 4, 8), ("f32", 256, 1, 2, 256), ("f32", 48, 2, 3, 32),
+          ("int4", 64, 2, 2, 8), ("int4", 128, 2, 4, 32), ("int4", 256, 1, 1, 16)]
+
+
+@pytest.mark.parametrize("dtype,D,G,group,ps", SHAPES)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (40, 0), (33, 5), (64, 100)])
+def test_attend_prompts_and_pieces(dtype, D, G, group, ps, window, sinks):
+    """Whole prompts (new == length), a piece behind a past, one token, none at all, and a row of nothing."""
+    g = _gen(D + group + window)
+    lens, new = [67, 130, 1, 55, 0, 18], [67, 19, 1, 0, 0, 17]
+    kv = _cache(dtype, G, D, ps, lens)
+    store = _fill(kv, 0, lens, g)
+    T = sum(new)
+    q = _randn(g, T + 2, G * group, D).mul_(2).to(kv.activations)
+    out = torch.full_like(q, 5.0)
+    rows = torch.arange(6, dtype=torch.int32, device=DEV)
+    kv.attend(0, q, rows, _offsets(new), window=window, sinks=sinks, out=out)
+    kv.check()
+    assert bool((out[T:] == 5.0).all())
+    scale, at = D ** -0.5, 0
+    for r, (L, n) in enumerate(zip(lens, new)):
+        want, mag, dot = attention(q[at:at + n], *store[r], list(range(L - n, L)), window, sinks, scale) if n else (None, None, 0)
+        if n:
+            _check_attend(out[at:at + n], want, mag, dot, kv, L, scale, q[at:at + n].double())
+        at += n
+
+
+@pytest.mark.parametrize("dtype,D,G,group,ps", SHAPES)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (200, 3)])
+def test_attend_single_tokens(dtype, D, G, group, ps, window, sinks):
+    """One new token per row, from the first token on; long rows are split over workgroups."""
+    g = _gen(D * 3 + group + window)
+    lens = [1, 2, 15, 16, 17, 31, 33, 64, 250, 1030]
+    kv = _cache(dtype, G, D, ps, lens)
+    store = _fill(kv, 0, lens, g, 1.5)
+    q = _randn(g, len(lens), G * group, D).mul_(2).to(kv.activations)
+    rows = torch.tensor([9, 0, 1, 2, 3, 4, 5, 6, 7, 8], dtype=torch.int32, device=DEV)
+    scale = 0.7 * D ** -0.5
+    for max_len in (0, 1030):
+        out = kv.attend(0, q, rows, window=window, sinks=sinks, scale=scale, max_len=max_len)
+        for i, r in enumerate(rows.tolist()):
+            want, mag, dot = attention(q[i:i + 1], *store[r], [lens[r] - 1], window, sinks, scale)
+            _check_attend(out[i:i + 1], want, mag, dot, kv, lens[r], scale, q[i:i + 1].double())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32", "int4"])
+def test_attend_long_prompt_agrees_with_its_tokens_one_by_one(dtype):
+    """A prompt of many tiles, ragged against the tile and page sizes, and each of its tokens asked for alone."""
+    g = _gen(17)
+    G, group, D, ps, lens, new = 2, 3, 128, 32, [701, 333], [523, 333]
+    kv = _cache(dtype, G, D, ps, lens)
+    _fill(kv, 0, lens, g)
+    q = _randn(g, sum(new), G * group, D).mul_(2).to(kv.activations)
+    rows = torch.arange(2, dtype=torch.int32, device=DEV)
+    for window, sinks in ((0, 0), (150, 4)):
+        out = kv.attend(0, q, rows, _offsets(new), window=window, sinks=sinks)
+        for r, i in ((0, 0), (0, 31), (0, 522), (1, 0), (1, 200), (1, 332)):
+            kv.lens[r] = lens[r] - new[r] + i + 1
+            t = (0 if r == 0 else new[0]) + i
+            alone = kv.attend(0, q[t:t + 1], rows[r:r + 1], window=window, sinks=sinks)
+            kv.lens[r] = lens[r]
+            u = U[kv.activations]
+            tol = 4 * u * (6.0 if dtype != "f32" else 64.0)       # both are within the bounds above; |v| <= 6 here
+            assert float((alone.float() - out[t:t + 1].float()).abs().max()) <= tol
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32", "int4"])
+def test_attend_leaves_out_what_is_not_seen(dtype):
+    """Infinities and NaN in keys and values: a token's output depends on the rows it sees alone (others of its tile may see them)."""
+    g = _gen(5)
+    G, group, D, ps, lens = 1, 2, 64, 8, [60, 45]
+    kv = _cache(dtype, G, D, ps, lens)
+    store = _fill(kv, 0, lens, g)
+    q = _randn(g, sum(lens), G * group, D).to(kv.activations)
+    rows = torch.arange(2, dtype=torch.int32, device=DEV)
+    clean = kv.attend(0, q, rows, _offsets(lens), window=20, sinks=2)
+
+    def poison(row, pos, which, value):
+        page, slot = int(kv.table[row, pos // ps]), pos % ps
+        if dtype == "int4":
+            getattr(kv, which + "_scale")[0, page, 0, slot, 0] = value
+        else:
+            getattr(kv, which)[0, page, 0, slot, 3] = value
+    poison(0, 25, "v", float("inf"))
+    poison(0, 40, "v", float("nan"))
+    poison(1, 30, "k", float("nan"))
+    got = kv.attend(0, q, rows, _offsets(lens), window=20, sinks=2)
+    for row, start, bad in ((0, 0, set(range(25, 60))), (1, 60, set(range(30, 45)))):
+        for p in range(lens[row]):
+            sees = p in bad and any(b <= p < b + 20 for b in ((25, 40) if row == 0 else (30,)))
+            if sees:
+                assert not bool(torch.isfinite(got[start + p]).all()), (row, p)
+            else:
+                assert torch.equal(got[start + p], clean[start + p]), (row, p)
+    assert store
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "int4"])
+def test_attend_missing_pages_and_bad_rows(dtype):
+    g = _gen(6)
+    G, group, D, ps, lens = 2, 2, 64, 16, [100, 50, 20]
+    kv = _cache(dtype, G, D, ps, lens, rows=3)
+    store = _fill(kv, 0, lens, g)
+    kv.table[0, 2] = -1                                            # positions 32 .. 47
+    kv.table[0, 4] = kv.pages + 7                                  # 64 .. 79: outside the pool
+    kv.table[1, :] = -1
+    q = _randn(g, 5, G * group, D).mul_(2).to(kv.activations)
+    out = kv.attend(0, q, torch.tensor([0, 1, 2, -1, 3], dtype=torch.int32, device=DEV))
+    there = torch.ones(100, dtype=torch.bool, device=DEV)
+    there[32:48] = there[64:80] = False
+    scale = D ** -0.5
+    want, mag, dot = attention(q[:1], *store[0], [99], 0, 0, scale, there)
+    _check_attend(out[:1], want, mag, dot, kv, 100, scale, q[:1].double())
+    want, mag, dot = attention(q[2:3], *store[2], [19], 0, 0, scale)
+    _check_attend(out[2:3], want, mag, dot, kv, 20, scale, q[2:3].double())
+    assert bool((out[[1, 3, 4]] == 0).all())
+    # more new tokens than the row holds: those before its beginning see nothing
+    kv.lens[2] = 3
+    out = kv.attend(0, q, torch.tensor([2], dtype=torch.int32, device=DEV), _offsets([5]))
+    assert bool((out[:2] == 0).all())
+    want, mag, dot = attention(q[2:], store[2][0][:3], store[2][1][:3], [0, 1, 2], 0, 0, scale)
+    _check_attend(out[2:], want, mag, dot, kv, 3, scale, q[2:].double())
+
+
+def test_append_bad_rows_and_missing_pages_are_flagged_not_written():
+    from qwen3_tts_amd import _lib
+    g = _gen(8)
+    kv = _cache("bf16", 1, 64, 8, [5, 9])
+    before = kv.k.clone()
+    q, k = _randn(g, 4, 2, 64, dtype=torch.bfloat16), _randn(g, 4, 1, 64, dtype=torch.bfloat16)
+    kv.table[1, 1] = -1
+    out = kv.append(0, q, k, k, torch.tensor([-1, 1, 7, 0], dtype=torch.int32, device=DEV))
+    assert bool((out[[0, 2]] == 0).all()) and torch.equal(out[[1, 3]], q[[1, 3]])
+    with pytest.raises(_lib.Q3cError, match="row id.*no free page"):
+        kv.check()
+    kv.check()                                                     # cleared
+    page, slot = int(kv.table[0, 0]), 4
+    assert torch.equal(kv.k[0, page, :, slot], k[3])
+    kv.k[0, page, :, slot] = before[0, page, :, slot]
+    assert torch.equal(kv.k.view(torch.int16), before.view(torch.int16))
+    kv.append(0, q[:2], k[:2], k[:2], torch.tensor([0, 0], dtype=torch.int32, device=DEV))       # a row named twice: the first counts
+    assert torch.equal(kv.k[0, page, :, slot], k[0])
+    with pytest.raises(_lib.Q3cError, match="row id"):
+        kv.check()
+    kv.append(0, q, k, k, torch.tensor([0], dtype=torch.int32, device=DEV), _offsets([4]))       # fits
+    kv.lens[0] = 2
+    out = kv.append(0, q, k, k, torch.tensor([0], dtype=torch.int32, device=DEV), _offsets([4])) # two tokens before the row's beginning
+    assert bool((out[:2] == 0).all()) and torch.equal(out[2:], q[2:])
+    with pytest.raises(_lib.Q3cError, match="row id"):
+        kv.check()
+
+
+def test_places_past_two_to_the_31():
+    """Element offsets beyond 32 bits: the last page of the last layer of a pool of 2.2e9 values."""
+    from qwen3_tts_amd.kvcache import PagedKV
+    g = _gen(9)
+    G, D, ps, P = 8, 128, 128, 8400
+    kv = PagedKV(2, G, D, P, ps, rows=3, pages_per_row=4, dtype="bf16", device=DEV)
+    assert kv.k.numel() > 2 ** 31
+    kv.table[0, :2] = torch.tensor([P - 1, P - 2], dtype=torch.int32)
+    kv.refs[-2:] = 1
+    kv.lens[0] = 200
+    k, v, q = (_randn(g, 200, n, D, dtype=torch.bfloat16) for n in (G, G, 16))
+    rows = torch.zeros(1, dtype=torch.int32, device=DEV)
+    kv.append(1, q, k, v, rows, _offsets([200]))
+    assert torch.equal(kv.k[1, P - 1].transpose(0, 1), k[:128]) and torch.equal(kv.v[1, P - 2].transpose(0, 1)[:72], v[128:])
+    out = kv.attend(1, q[-1:].contiguous(), rows)
+    want, mag, dot = attention(q[-1:], k, v, [199], 0, 0, D ** -0.5)
+    _check_attend(out, want, mag, dot, kv, 200, D ** -0.5)
+    kv.fork([0], [1])
+    kv.copy_pages([P - 1], [P - 3])
+    kv.check()
+    assert kv.table[1, :3].tolist() == [P - 1, 0, -1] and kv.refs[P - 1] == 2
+    assert torch.equal(kv.k[:, 0], kv.k[:, P - 2]) and torch.equal(kv.v[:, P - 3], kv.v[:, P - 1])
+    assert int(kv.compact()) == 3
+    kv.check()
+    assert kv.table[:2, :2].tolist() == [[2, 1], [2, 0]]
+    assert torch.equal(kv.attend(1, q[-1:].contiguous(), rows), out)
+
+
+# ---- pages -----------------------------------------------------------------------------------------------------------------------
+def _same(kv, ref):
+    assert kv.table.tolist() == ref.table and kv.lens.tolist() == ref.lens and kv.refs.tolist() == ref.refs
+    assert int(kv.status) == ref.status
+
+
+@pytest.mark.parametrize("dtype,pages,rows,width,seed", [("bf16", 40, 7, 9, 0), ("int4", 23, 5, 6, 1), ("f32", 20000, 40, 30, 2), ("bf16", 9, 3, 4, 3)])
+def test_page_operations_follow_the_rules(dtype, pages, rows, width, seed):
+    """A random life of a pool, checked after every operation against lists; pools that run out and rows that fill up among it."""
+    import random
+
+    from qwen3_tts_amd.kvcache import PagedKV
+    rng, ps = random.Random(seed), 8
+    kv = PagedKV(2, 1, 64 if dtype == "int4" else 16, pages, ps, rows, width, dtype, DEV)
+    tensors = [t for t in (kv.k, kv.v, kv.k_scale, kv.v_scale) if t is not None]
+    g = _gen(seed)
+    for t in tensors:
+        t.copy_(torch.randint(0, 200, t.shape, generator=g, device=DEV).to(t.dtype))
+    ref = Pages(pages, ps, rows, width)
+    dev = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    for step in range(60):
+        want = [t.clone() for t in tensors]
+        op = rng.choice(["reserve", "reserve", "tokens", "fork", "release", "trim", "copy", "compact"])
+        some = [rng.randrange(rows) for _ in range(rng.randint(1, rows))]
+        if op == "reserve":
+            if step % 7 == 0:
+                some += [-1, rows]
+            counts = [rng.choice([0, 1, 7, 8, 30]) for _ in some]
+            kv.reserve(dev(some), _offsets(counts), tokens=sum(counts))
+            ref.reserve(some, counts)
+        elif op == "tokens":
+            some = sorted(set(some))
+            kv.reserve(some)
+            ref.reserve(some, [1] * len(some))
+        elif op == "fork":
+            up = [rng.randrange(-1, rows) for _ in some]
+            kv.fork(dev(up), dev(some))
+            for s, d in ref.fork(up, some):
+                for t in want:
+                    t[:, d] = t[:, s].clone()
+        elif op == "release":
+            kv.release(dev(some))
+            ref.release(some)
+        elif op == "trim":
+            w, s = rng.randint(1, 40), rng.choice([0, 3, 8, 9])
+            kv.trim(dev(some), w, s)
+            ref.trim(some, w, s)
+        elif op == "copy":
+            n = rng.randint(0, 6)
+            src, dst = [rng.randrange(-1, pages) for _ in range(n)], [rng.randrange(pages + 1) for _ in range(n)]
+            kv.copy_pages(dev(src), dev(dst))
+            old = [t.clone() for t in want]
+            for s, d in ref.copy(src, dst):
+                for t, o in zip(want, old):
+                    t[:, d] = o[:, s]
+        else:
+            live = kv.compact()
+            old = [t.clone() for t in want]
+            pairs, n = ref.compact()
+            assert int(live) == n
+            for s, d in pairs:
+                for t, o in zip(want, old):
+                    t[:, d] = o[:, s]
+        _same(kv, ref)
+        assert all(torch.equal(a, b) for a, b in zip(tensors, want)), op
+        if ref.status:
+            with pytest.raises(Exception):
+                kv.check()
+            ref.status = 0
+
+
+def test_reserve_and_fork_of_more_rows_than_a_workgroup():
+    from qwen3_tts_amd.kvcache import PagedKV
+    rows, ps = 2300, 8
+    kv = PagedKV(1, 1, 16, 9000, ps, 2 * rows, 3, "bf16", DEV)
+    ref = Pages(9000, ps, 2 * rows, 3)
+    order = torch.randperm(rows, generator=torch.Generator().manual_seed(1)).tolist()
+    counts = [(7 * i) % 19 for i in range(rows)]
+    kv.reserve(torch.tensor(order, dtype=torch.int32, device=DEV), _offsets(counts), tokens=sum(counts))
+    ref.reserve(order, counts)
+    _same(kv, ref)
+    up, ch = list(range(rows)), list(range(rows, 2 * rows))
+    kv.fork(up, ch)
+    ref.fork(up, ch)
+    _same(kv, ref)
+    twice = order + order[:5]
+    kv.reserve(torch.tensor(twice, dtype=torch.int32, device=DEV))
+    ref.reserve(twice, [1] * len(twice))
+    _same(kv, ref)
+
+
+def test_empty_calls_do_nothing():
+    g = _gen(1)
+    kv = _cache("bf16", 1, 64, 16, [20])
+    none = torch.empty(0, dtype=torch.int32, device=DEV)
+    q = _randn(g, 0, 2, 64, dtype=torch.bfloat16)
+    kv.reserve(none)
+    kv.release(none)
+    kv.trim(none, 5)
+    kv.fork(none, none)
+    kv.copy_pages(none, none)
+    assert kv.append(0, q, q[:, :1], q[:, :1], none).shape == (0, 2, 64) and kv.attend(0, q, none).shape == (0, 2, 64)
+    assert kv.gather(0, none)[0].shape == (0, 1, 64)
+    one = torch.zeros(1, dtype=torch.int32, device=DEV)
+    assert kv.attend(0, q, one, _offsets([0])).shape == (0, 2, 64)
+    kv.check()
+    assert kv.lens.tolist() == [20]
+
+
+# ---- together --------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["bf16", "f32", "int4"])
+def test_a_generation_with_forks_trims_and_a_compaction(dtype):
+    """Two layers, a prompt, three requests forked from it, steps of one token under a window with sinks, pages given back and the pool
+    compacted on the way: every output against 64-bit attention over all keys the row ever had."""
+    from qwen3_tts_amd.kvcache import PagedKV, rope_tables
+    g = _gen(21)
+    G, H, D, ps, window, sinks = 2, 4, 64, 8, 24, 4
+    kv = PagedKV(2, G, D, 40, ps, rows=5, pages_per_row=12, dtype=dtype, device=DEV)
+    rope = rope_tables(kv.max_tokens, D, device=DEV)
+    wq, wk = ((torch.rand(D, generator=g, device=DEV) + 0.5) for _ in range(2))
+    history = {}                                                    # (layer, row) -> [k, v] as stored
+
+    def tokens(rows, counts):
+        off, T = (None, len(rows)) if counts is None else (_offsets(counts), sum(counts))
+        counts = counts or [1] * len(rows)
+        ids = torch.tensor(rows, dtype=torch.int32, device=DEV)
+        kv.reserve(ids, off, tokens=T)
+        for layer in range(2):
+            qkv = _randn(g, T, (H + 2 * G) * D).mul_(2).to(kv.activations)
+            q, k, v = (x.view(T, -1, D) for x in qkv.split([H * D, G * D, G * D], 1))
+            q = kv.append(layer, q, k, v, ids, off, q_weight=wq, k_weight=wk, rope=rope)
+            out = kv.attend(layer, q, ids, off, window=window, sinks=sinks)
+            kk, vv = kv.gather(layer, ids, off, tokens=T, dtype="f32")
+            at = 0
+            for r, n in zip(rows, counts):
+                h = history.setdefault((layer, r), [torch.empty(0, G, D, device=DEV, dtype=torch.float64)] * 2)
+                h[0], h[1] = torch.cat([h[0], kk[at:at + n].double()]), torch.cat([h[1], vv[at:at + n].double()])
+                L = h[0].shape[0]
+                want, mag, dot = attention(q[at:at + n], h[0], h[1], list(range(L - n, L)), window, sinks, D ** -0.5)
+                _check_attend(out[at:at + n], want, mag, dot, kv, L, D ** -0.5, q[at:at + n].double())
+                at += n
+
+    tokens([0, 4], [21, 6])
+    kv.fork([0, 0, 0], [1, 2, 3])
+    for layer in range(2):
+        for r in (1, 2, 3):
+            history[layer, r] = list(history[layer, 0])
+    for step in range(40):
+        tokens([3, 0, 1, 2] if step < 20 else [3, 1], None if step % 5 else [2] * (4 if step < 20 else 2))
+        kv.trim([0, 1, 2, 3], window, sinks)
+        if step == 19:
+            kv.release([0, 2])
+            kv.compact()
+    kv.check()
+    kv.release([1, 3, 4])
+    assert kv.free_pages() == kv.pages and int(kv.lens.sum()) == 0 and bool((kv.table == -1).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "int4"])
+def test_captured_steps_replay_beside_each_other(dtype):
+    """A step (reserve, append, attend, trim) captured once and replayed token by token, beside a second graph of another cache on
+    another stream and eager work between: every replay equals the same step run eagerly."""
+    from qwen3_tts_amd.kvcache import PagedKV, rope_tables
+    G, H, D, ps = 2, 4, 128, 8
+    sides = []
+    for seed in (1, 2):
+        g = _gen(seed)
+        pair = [PagedKV(1, G, D, 200, ps, rows=3, pages_per_row=60, dtype=dtype, device=DEV) for _ in range(2)]
+        rope = rope_tables(pair[0].max_tokens, D, device=DEV)
+        rows = torch.tensor([2, 0, 1], dtype=torch.int32, device=DEV)
+        qkv = [torch.empty(3, n, D, dtype=torch.bfloat16, device=DEV) for n in (H, G, G)]
+        for kv in pair:
+            kv.reserve(rows, _offsets([100, 201, 5]), tokens=306)
+            gg = _gen(seed + 10)
+            x = [_randn(gg, 306, n, D, dtype=torch.bfloat16) for n in (H, G, G)]
+            kv.append(0, *x, rows, _offsets([100, 201, 5]), rope=rope)
+
+        def step(kv, qkv=qkv, rows=rows, rope=rope):
+            kv.reserve(rows)
+            out = kv.attend(0, kv.append(0, *qkv, rows, rope=rope), rows, window=64, sinks=3)
+            kv.trim(rows, 64, 3)
+            return out
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        for t in qkv:
+            t.copy_(_randn(g, *t.shape))
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            out = step(pair[0])
+        sides.append((pair, qkv, step, graph, out, stream, g))
+    torch.cuda.synchronize()
+    for i in range(6):
+        for pair, qkv, step, graph, out, stream, g in sides:
+            for t in qkv:
+                t.copy_(_randn(g, *t.shape))
+        torch.cuda.synchronize()
+        for pair, qkv, step, graph, out, stream, g in sides:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for pair, qkv, step, graph, out, stream, g in sides:
+            assert torch.equal(out, step(pair[1])), i
+            assert torch.equal(pair[0].table, pair[1].table) and torch.equal(pair[0].lens, pair[1].lens)
+            for kv in pair:
+                kv.check()
+
+
+def test_another_stream_and_the_torch_ops():
+    from qwen3_tts_amd import torch_ops
+    g = _gen(4)
+    kv = _cache("bf16", 2, 64, 16, [33, 90])
+    _fill(kv, 0, [33, 90], g)
+    rows = torch.tensor([1, 0], dtype=torch.int32, device=DEV)
+    q = _randn(g, 2, 4, 64, dtype=torch.bfloat16)
+    want = kv.attend(0, q, rows, window=50, sinks=1)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        got = kv.attend(0, q, rows, window=50, sinks=1)
+    s.synchronize()
+    assert torch.equal(got, want)
+    h = torch_ops.register_kv(kv)
+    assert torch.equal(torch.ops.q3tts.kv_attend(q, rows, None, 50, 1, h, 0), want)
+    k = _randn(g, 2, 2, 64, dtype=torch.bfloat16)
+    w = torch.rand(64, generator=g, device=DEV)
+    a = torch.ops.q3tts.kv_append(q, k, k, rows, None, w, w, None, None, 1e-6, h, 0)
+    assert torch.equal(a, kv.append(0, q, k, k, rows, q_weight=w, k_weight=w))
+    torch_ops.unregister_kv(h)
+    with pytest.raises(KeyError):
+        torch.ops.q3tts.kv_attend(q, rows, None, 50, 1, h, 0)
+
+
+def test_refusals_with_tensors_on_the_gpu():
+    kv = _cache("bf16", 2, 64, 16, [33, 90])
+    rows = torch.tensor([1, 0], dtype=torch.int32, device=DEV)
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device=DEV)
+    k = q[:, :2]
+    cos = torch.zeros(kv.max_tokens, 32, device=DEV)
+    for bad in (dict(q=q.float()), dict(q=q[..., :32]), dict(k=q), dict(rows=rows.long()), dict(rows=rows.cpu()), dict(rows=rows[:1]),
+                dict(q=q[:1]), dict(q_weight=torch.ones(64, dtype=torch.bfloat16, device=DEV)), dict(q_weight=torch.ones(32, device=DEV)),
+                dict(rope=(cos[:-1], cos[:-1])), dict(rope=(cos, cos[:, :16])), dict(rope=(cos[:, :3].contiguous(),) * 2), dict(out=q.float()),
+                dict(offsets=torch.tensor([0, 2], dtype=torch.int32, device=DEV)), dict(rows=[0, 0]), dict(q=q.cpu())):
+        a = dict(q=q, k=k, v=k, rows=rows, offsets=None, q_weight=None, k_weight=None, rope=None, out=None)
+        a.update(bad)
+        with pytest.raises(ValueError):
+            kv.append(0, a["q"], a["k"], a["v"], a["rows"], a["offsets"], q_weight=a["q_weight"], k_weight=a["k_weight"], rope=a["rope"], out=a["out"])
+    for kw in (dict(window=-1), dict(sinks=-1), dict(scale=0.0), dict(scale=float("inf")), dict(scale=float("nan")), dict(max_len=-2)):
+        with pytest.raises(ValueError):
+            kv.attend(0, q, rows, **kw)
+    with pytest.raises(ValueError):
+        kv.attend(0, q[:, :3], rows)                                # three heads on two kv heads
+    for layer in (-1, 1):
+        with pytest.raises(IndexError):
+            kv.attend(layer, q, rows)
+    for ids in ([2], [-1]):
+        with pytest.raises(IndexError):
+            kv.release(ids)
+    with pytest.raises(ValueError):
+        kv.trim(rows, 0)
+    with pytest.raises(ValueError):
+        kv.fork([0], [1, 0])
+    with pytest.raises(ValueError):
+        kv.gather(0, rows, _offsets([1, 1]))                        # how many tokens is not said
+    kv.check()
+    assert math.isnan(float(kv.k.float().sum()))                    # and nothing was written

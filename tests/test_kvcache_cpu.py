@@ -1,0 +1,134 @@
+"""What the paged key/value cache refuses on the host, without a GPU: sizes and layouts through the class, pointers, sizes and
+workspaces through the C entry points (each refusal comes before any launch), and the fixed points of the plain restatement."""
+import ctypes as C
+
+import pytest
+import torch
+
+import qwen3_tts_amd  # noqa: F401
+from kv_reference import Pages, attention, norm_rotate
+from qwen3_tts_amd import _lib
+from qwen3_tts_amd.kvcache import PagedKV, rope_tables
+
+OK, INVALID, WORKSPACE, UNSUPPORTED = 0, -1, -4, -7
+PTR = 1 << 20                     # an aligned address that no refused call touches
+
+
+def _tensors(L=1, P=4, G=2, ps=16, D=64, dtype=torch.bfloat16, rows=3, width=2):
+    i = dict(dtype=torch.int32)
+    k = torch.zeros(L, P, G, ps, D, dtype=dtype)
+    return dict(k=k, v=k.clone(), table=torch.zeros(rows, width, **i), lens=torch.zeros(rows, **i), refs=torch.zeros(P, **i))
+
+
+@pytest.mark.parametrize("change", [
+    dict(ps=12), dict(ps=4), dict(ps=512), dict(D=24), dict(D=272), dict(dtype=torch.float16), dict(dtype=torch.uint8), dict(P=0), dict(rows=0)])
+def test_layouts_that_are_refused(change):
+    with pytest.raises(ValueError):
+        PagedKV.from_tensors(**_tensors(**change))
+
+
+def test_tensors_that_are_refused():
+    good = _tensors()
+    for name, t in (("v", good["v"][..., :32]), ("v", good["v"].float()), ("table", good["table"].long()), ("table", good["table"][0]),
+                    ("lens", good["lens"][:2]), ("refs", torch.zeros(5, dtype=torch.int32)), ("status", torch.zeros(2, dtype=torch.int32)),
+                    ("k_scale", torch.zeros(1)), ("k", torch.zeros(1, 4, 16, 2, 64, dtype=torch.bfloat16).transpose(2, 3)),
+                    ("k", good["k"][0])):
+        with pytest.raises(ValueError):
+            PagedKV.from_tensors(**{**good, name: t})
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        PagedKV.from_tensors(**good)
+    for kw in (dict(dtype="fp16"), dict(layers=0), dict(pages_per_row=0), dict(dtype="int4", head_dim=80)):
+        with pytest.raises(ValueError):
+            PagedKV(**{**dict(layers=1, kv_heads=1, head_dim=64, pages=2, device="cpu"), **kw})
+
+
+def _kv(**change):
+    c = _lib.Q3cKv()
+    c.struct_size = C.sizeof(_lib.Q3cKv)
+    c.dtype, c.layers, c.pages, c.kv_heads, c.page_size, c.head_dim, c.rows, c.pages_per_row = 1, 2, 8, 2, 16, 64, 4, 3
+    for n in ("k", "v", "table", "lens", "refs", "status"):
+        setattr(c, n, PTR)
+    for n, v in change.items():
+        setattr(c, n, v)
+    return C.byref(c)
+
+
+def test_c_entry_points_refuse_bad_descriptions():
+    lib = _lib.load()
+    for change, rc in ((dict(struct_size=8), INVALID), (dict(dtype=3), INVALID), (dict(dtype=-1), INVALID), (dict(layers=0), INVALID), (dict(pages=0), INVALID),
+                       (dict(rows=0), INVALID), (dict(pages_per_row=0), INVALID), (dict(k=None), INVALID), (dict(k=PTR + 8), INVALID), (dict(status=None), INVALID),
+                       (dict(page_size=24), UNSUPPORTED), (dict(page_size=512), UNSUPPORTED), (dict(page_size=4), UNSUPPORTED), (dict(head_dim=72), UNSUPPORTED),
+                       (dict(head_dim=512), UNSUPPORTED), (dict(dtype=2), INVALID), (dict(dtype=2, head_dim=80, k_scale=PTR, v_scale=PTR), UNSUPPORTED),
+                       (dict(pages_per_row=1 << 27), UNSUPPORTED), (dict(kv_heads=1 << 17), UNSUPPORTED)):
+        kv = _kv(**change)
+        n = C.c_size_t()
+        assert lib.q3c_kv_reserve(kv, PTR, None, 1, 1, None) == rc, change
+        assert lib.q3c_kv_append(kv, 0, PTR, 64, 64, PTR, 64, 64, PTR, 64, 64, 2, PTR, None, 1, 1, None, None, None, None, 0, 0, 1e-6, PTR, None) == rc, change
+        assert lib.q3c_kv_gather(kv, 0, PTR, None, 1, 1, PTR, PTR, 1, None) == rc, change
+        assert lib.q3c_kv_attend_workspace_bytes(kv, 1 << 17 if "kv_heads" in change else 2, 1, 1, 0, 0, 0, C.byref(n)) == rc, change
+        assert lib.q3c_kv_attend(kv, 0, PTR, 64, 64, 2, PTR, None, 1, 1, 0, 0, 1.0, 0, PTR, PTR, 1 << 30, None) == rc, change
+        assert lib.q3c_kv_fork(kv, PTR, PTR, 1, PTR, 12, None) == rc, change
+        assert lib.q3c_kv_release(kv, PTR, 1, None) == rc and lib.q3c_kv_trim(kv, PTR, 1, 4, 0, None) == rc, change
+        assert lib.q3c_kv_copy_pages(kv, PTR, PTR, 1, PTR, 4, None) == rc and lib.q3c_kv_compact(kv, PTR, PTR, 1 << 20, None) == rc, change
+    assert lib.q3c_kv_reserve(None, PTR, None, 1, 1, None) == INVALID
+
+
+def test_c_entry_points_refuse_bad_calls():
+    lib, kv = _lib.load(), _kv()
+
+    def append(layer=0, q=PTR, q_ts=256, q_hs=64, k_hs=64, heads=2, rows=PTR, offsets=None, seqs=1, tokens=1, w=None, cos=None, positions=0, rot=0, out=PTR, kv=kv):
+        return lib.q3c_kv_append(kv, layer, q, q_ts, q_hs, PTR, 128, k_hs, PTR, 128, 64, heads, rows, offsets, seqs, tokens, w, None, cos, cos, positions, rot, 1e-6, out, None)
+    for kw, rc in ((dict(layer=2), INVALID), (dict(layer=-1), INVALID), (dict(q=None), INVALID), (dict(q=PTR + 2), INVALID), (dict(q_ts=66), INVALID), (dict(k_hs=-64), INVALID),
+                   (dict(heads=0), INVALID), (dict(rows=None), INVALID), (dict(seqs=2), INVALID), (dict(seqs=0, offsets=PTR), INVALID), (dict(tokens=-1), INVALID),
+                   (dict(w=PTR + 4), INVALID), (dict(rot=64), INVALID), (dict(rot=64, cos=PTR, positions=47), INVALID), (dict(rot=12, cos=PTR, positions=48), UNSUPPORTED),
+                   (dict(rot=72, cos=PTR, positions=48), UNSUPPORTED), (dict(out=None), INVALID), (dict(out=PTR + 4), INVALID),
+                   (dict(rot=32, cos=PTR, positions=48, kv=_kv(dtype=2, k_scale=PTR, v_scale=PTR)), UNSUPPORTED), (dict(seqs=1 << 25, tokens=1 << 25), UNSUPPORTED)):
+        assert append(**kw) == rc, kw
+
+    def attend(layer=0, q=PTR, heads=4, rows=PTR, offsets=None, seqs=1, tokens=1, window=0, sinks=0, scale=1.0, max_len=0, out=PTR, ws=PTR, size=1 << 30):
+        return lib.q3c_kv_attend(kv, layer, q, 256, 64, heads, rows, offsets, seqs, tokens, window, sinks, scale, max_len, out, ws, size, None)
+    for kw, rc in ((dict(layer=2), INVALID), (dict(q=None), INVALID), (dict(heads=3), INVALID), (dict(heads=0), INVALID), (dict(window=-1), INVALID), (dict(sinks=-1), INVALID),
+                   (dict(scale=0.0), INVALID), (dict(scale=float("nan")), INVALID), (dict(scale=float("inf")), INVALID), (dict(max_len=-1), INVALID), (dict(out=None), INVALID),
+                   (dict(tokens=3), INVALID), (dict(rows=None), INVALID)):
+        assert attend(**kw) == rc, kw
+    long = _kv(pages_per_row=4096)
+    n = C.c_size_t()
+    assert lib.q3c_kv_attend_workspace_bytes(long, 4, 1, 1, 0, 0, 0, C.byref(n)) == OK and n.value > 0
+    assert lib.q3c_kv_attend(long, 0, PTR, 256, 64, 4, PTR, None, 1, 1, 0, 0, 1.0, 0, PTR, PTR, n.value - 1, None) == WORKSPACE
+    assert lib.q3c_kv_attend(long, 0, PTR, 256, 64, 4, PTR, None, 1, 1, 0, 0, 1.0, 0, PTR, None, n.value, None) == INVALID
+    assert lib.q3c_kv_attend_workspace_bytes(long, 4, 1, 1, 0, 0, 0, None) == INVALID
+    assert lib.q3c_kv_fork(kv, PTR, PTR, 2, PTR, 23, None) == WORKSPACE and lib.q3c_kv_fork(kv, None, PTR, 2, PTR, 24, None) == INVALID
+    assert lib.q3c_kv_fork(_kv(layers=1 << 16, page_size=256), PTR, PTR, 1 << 20, PTR, 1 << 40, None) == UNSUPPORTED
+    assert lib.q3c_kv_copy_pages(kv, PTR, PTR, 2, PTR, 7, None) == WORKSPACE and lib.q3c_kv_copy_pages(kv, PTR, PTR, -1, PTR, 7, None) == INVALID
+    assert lib.q3c_kv_compact(kv, PTR, PTR, 79, None) == WORKSPACE and lib.q3c_kv_compact(kv, None, PTR, 80, None) == INVALID
+    assert lib.q3c_kv_trim(kv, PTR, 1, 0, 0, None) == INVALID and lib.q3c_kv_trim(kv, PTR, 1, 1, -1, None) == INVALID
+    assert lib.q3c_kv_release(kv, None, 1, None) == INVALID and lib.q3c_kv_release(kv, PTR, -1, None) == INVALID
+    assert lib.q3c_kv_gather(kv, 0, PTR, None, 1, 1, PTR, PTR, 2, None) == INVALID and lib.q3c_kv_gather(kv, 0, PTR, None, 1, 1, None, PTR, 1, None) == INVALID
+
+
+def test_rope_tables_of_far_positions():
+    cos, sin = rope_tables(200001, 8, theta=1e6, device="cpu")
+    import math
+    for p in (0, 1, 199999, 200000):
+        for i in range(4):
+            a = p * 1e6 ** (-i / 4)
+            assert abs(float(cos[p, i]) - math.cos(a)) < 1e-7 and abs(float(sin[p, i]) - math.sin(a)) < 1e-7
+
+
+def test_the_plain_restatement_itself():
+    """Fixed points that need no second implementation: uniform weights, a window of one token, rotation keeps lengths."""
+    g = torch.Generator().manual_seed(0)
+    v = torch.randn(6, 1, 4, generator=g, dtype=torch.float64)
+    out, _, _ = attention(torch.zeros(1, 2, 4), torch.randn(6, 1, 4, generator=g), v, [5], 3, 1, 1.0)
+    assert torch.allclose(out[0, 0], v[[0, 3, 4, 5], 0].mean(0)) and torch.equal(out[0, 0], out[0, 1])
+    out, _, _ = attention(torch.randn(6, 1, 4, generator=g), v, v, list(range(6)), 1, 0, 1.0)
+    assert torch.allclose(out[:, 0], v[:, 0])
+    x = torch.randn(5, 2, 16, generator=g)
+    cos, sin = rope_tables(9, 16, device="cpu")
+    y = norm_rotate(x, None, cos, sin, torch.arange(5) + 2, 0.0)
+    assert torch.allclose(y.norm(dim=-1), x.double().norm(dim=-1), rtol=1e-6) and not torch.allclose(y, x.double())
+    p = Pages(6, 8, 3, 4)
+    p.reserve([0], [20])
+    assert p.fork([0], [1]) == [(2, 3)] and p.refs == [2, 2, 1, 1, 0, 0]
+    p.release([0])
+    assert p.refs == [1, 1, 0, 1, 0, 0] and p.compact() == ([(3, 2)], 3) and p.table[1] == [0, 1, 2, -1]
