@@ -79,8 +79,9 @@ __device__ __forceinline__ f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 __device__ __forceinline__ unsigned pack2(float a, float b) {
-    const bf16 x = (bf16)a, y = (bf16)b;
-    return (unsigned)__builtin_bit_cast(unsigned short, x) | (unsigned)__builtin_bit_cast(unsigned short, y) << 16;
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{a, b}), bf16x2));
 }
 __device__ __forceinline__ float lo_f(unsigned x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float hi_f(unsigned x) { return __uint_as_float(x & 0xffff0000u); }
@@ -501,9 +502,287 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const KvAttendArgs a) {
     for (int e = 0; e < DP / 16; ++e) out[e] = (A)(none ? 0.f : r[e] * inv);
 }
 
+// ---- prompts -----------------------------------------------------------------------------------------------------------------------------
+// Many columns per request (prompts, long pieces; bf16 and 4 bits): bound by the matrix cores and the LDS that feeds them.  One
+// workgroup = 128 columns of one request and kv head, 32 per wave; keys and values go through LDS in tiles of KT, two buffers
+// deep: while a tile is multiplied the next one's rows are on their way to registers, and one barrier per tile hands them over.
+// A wave computes S^T = K Q^T on 32 x 32 x 16 products, so that a lane holds scores of one column and its probabilities are, register
+// for register, the B operand of O^T = V^T P^T; V^T comes from the row-major image by transposed LDS reads.  The probabilities' maximum
+// is allowed to lag: the sums are rescaled only when a column's maximum has grown by more than 2^8 (fp32 sums and bf16 probabilities have
+// the range), which a causal row does a few times in all.
+// Workgroups of one (request, kv head) sit eight apart in launch order, heads fastest: on the eight XCDs, whose workgroups are dealt
+// round robin, a head's keys stay in one L2.  Long columns start first.
+// 4 bits: values n * step are rounded to bf16 on their way into LDS (operands of the matrix cores), four bytes of the row = one 16-byte
+// chunk; the order of dimensions in a row is then the packed one, which Q's load and the output's store follow.
+template <typename T, int DP> struct Row;                       // chunk ch of a row: 8 values as 16 bytes
+template <int DP> struct Row<bf16, DP> {
+    static constexpr int WORDS = 4;
+    struct Raw { u32x4 x; };
+    static __device__ __forceinline__ void load(Raw& r, const void* base, const bf16*, long long row, int D, int ch) {
+        r.x = *(const u32x4*)((const bf16*)base + row * D + 8 * ch);
+    }
+    static __device__ __forceinline__ void zero(Raw& r) { r.x = u32x4{0, 0, 0, 0}; }
+    static __device__ __forceinline__ u32x4 value(const Raw& r) { return r.x; }
+    static __device__ __forceinline__ int dim(int d) { return d; }      // of place d of a row
+};
+template <int D> struct Row<Int4, D> {
+    static constexpr int S = D / 32;
+    struct Raw { unsigned x; u32x2 st; };
+    static __device__ __forceinline__ void load(Raw& r, const void* base, const bf16* steps, long long row, int, int ch) {
+        r.x = *(const unsigned*)((const char*)base + row * (D / 2) + 4 * ch);
+        if constexpr (S == 2) { r.st[0] = *(const unsigned*)(steps + row * S); r.st[1] = r.st[0]; }
+        else r.st = *(const u32x2*)(steps + row * S + (S == 8 ? 4 * (ch & 1) : 0));
+    }
+    static __device__ __forceinline__ void zero(Raw& r) { r.x = 0x88888888u; r.st = u32x2{0, 0}; }
+    static __device__ __forceinline__ u32x4 value(const Raw& r) {
+        u32x4 v;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const float st = b & 1 ? hi_f(r.st[b >> 1]) : lo_f(r.st[b >> 1]);
+            v[b] = pack2((float)((int)(r.x >> (8 * b) & 15u) - 8) * st, (float)((int)(r.x >> (8 * b + 4) & 15u) - 8) * st);
+        }
+        return v;
+    }
+    static __device__ __forceinline__ int dim(int d) {
+        const int byte = d >> 1;
+        return 32 * (byte % S) + 16 * (d & 1) + byte / S;
+    }
+};
+
+template <int DP> __device__ __forceinline__ int lds_k(int row, int ch) { return 2 * DP * row + 16 * (ch ^ (DP == 64 ? (row >> 1) & 7 : row & 15)); }
+template <int DP> __device__ __forceinline__ int lds_v(int row, int ch) { return 2 * DP * row + 16 * (ch ^ (DP == 64 ? (row >> 1 & 1) << 2 : (row & 3) << 2)); }
+
+template <int N> struct Const { static constexpr int value = N; };
+
+template <typename T, int DP, int KT>
+__global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const KvAttendArgs a, int tiles) {
+    typedef Row<T, DP> R;
+    constexpr int RB = 2 * DP, NCH = DP / 8, KS = DP / 16, ND = DP / 32, NT = KT / 32, RP = 256 / NCH, NR = KT / RP;
+    __shared__ __attribute__((aligned(16))) unsigned char sk[2][KT * RB], sv[2][KT * RB];
+    __shared__ int sok[2][KT];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int hk = blockIdx.x % a.c.heads, G = a.group, D = a.c.dim, sh = a.c.ps_shift;
+    const Tile t = kv_tile(a, tiles - 1 - (int)(blockIdx.x / a.c.heads), 128, lane);
+    if (!t.on) return;
+    const int r = lane & 31, hh = lane >> 5;
+    const int col = t.col0 + 32 * wave + r, qtok = col / G;
+    int mypos = col < t.ncols && t.row >= 0 ? t.first_pos + qtok : -1;
+    if (mypos > t.pmax) mypos = -1;
+    const int c0 = t.col0 + 32 * wave, c1 = min(c0 + 32, t.ncols) - 1;              // the wave's columns and the positions they span
+    const int wmin = max(t.first_pos + c0 / G, 0), wmax = c1 < c0 || t.row < 0 ? -1 : min(t.first_pos + c1 / G, t.pmax);
+    bf16x8 qf[KS];
+    {
+        const bf16* q = (const bf16*)a.q.p + (long long)(t.tok0 + qtok) * a.q.ts + (long long)(hk * G + col - qtok * G) * a.q.hs;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) qf[s][e] = (bf16)0.f;
+            const int d = 16 * s + 8 * hh;
+            if (mypos >= 0 && d < D) {
+                if constexpr (__is_same(T, Int4)) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) qf[s][e] = q[R::dim(d + e)];
+                } else {
+                    const bf16x4 x = *(const bf16x4*)(q + d), y = *(const bf16x4*)(q + d + 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { qf[s][e] = x[e]; qf[s][4 + e] = y[e]; }
+                }
+            }
+        }
+    }
+    const Span span = kv_span(a, t, KT);
+    const int* table = a.c.table + (long long)max(t.row, 0) * a.c.width;
+    const long long page_rows = (long long)a.c.heads << sh, head0 = ((long long)a.layer * a.c.pages * a.c.heads + hk) << sh;
+    const int in_page = (1 << sh) - 1, last_entry = a.c.width - 1;
+    const int W = a.window > 0 ? a.window : 0x7fffffff, sinks = a.window > 0 ? a.sinks : 0;
+    const int ch = tid & (NCH - 1), row0 = tid / NCH;                                // this thread stages chunk ch of rows row0 + i RP
+    const float cs = a.scale_log2e;
+    // LDS places of this lane's operands; tiles, halves and buffers are constants added to them
+    int ak[KS], av[ND];
+    {
+        const int q4 = (lane >> 2) & 3, p4 = lane & 3, c16 = (lane >> 4) & 1;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) ak[k] = lds_k<DP>(r, 2 * k + hh);
+#pragma unroll
+        for (int n = 0; n < ND; ++n) av[n] = lds_v<DP>(4 * hh + q4, 4 * n + 2 * c16 + (p4 >> 1)) + 8 * (p4 & 1);
+    }
+
+    int only = t.pmin - 1;                     // as in kv_attend_kernel: a second look, position by position, where a result is not finite
+    for (;;) {
+        const bool all = only < t.pmin;
+        const int vlo = (all ? t.pmin : only) - W, vhi = all ? t.pmax : only;
+        int e[NR];
+        typename R::Raw kr[NR], vr[NR];
+        auto entries = [&](int c) {
+#pragma unroll
+            for (int i = 0; i < NR; ++i) e[i] = table[min((span.chunk(c) * KT + row0 + i * RP) >> sh, last_entry)];
+        };
+        unsigned there;
+        auto fetch = [&](int c) {
+            there = 0;
+#pragma unroll
+            for (int i = 0; i < NR; ++i) {
+                const int tok = span.chunk(c) * KT + row0 + i * RP;
+                const bool page = (unsigned)e[i] < (unsigned)a.c.pages;
+                there |= (unsigned)page << i;
+                const bool ok = page && tok <= vhi && (tok > vlo || tok < sinks) && 8 * ch < D;
+                R::zero(kr[i]);
+                R::zero(vr[i]);
+                if (ok) {
+                    const long long at = head0 + (long long)e[i] * page_rows + (tok & in_page);
+                    R::load(kr[i], a.c.k, a.c.ks, at, D, ch);
+                    R::load(vr[i], a.c.v, a.c.vs, at, D, ch);
+                }
+            }
+        };
+        auto stage = [&](int buf) {
+#pragma unroll
+            for (int i = 0; i < NR; ++i) {
+                const int row = row0 + i * RP;
+                *(u32x4*)(sk[buf] + lds_k<DP>(row, ch)) = R::value(kr[i]);
+                *(u32x4*)(sv[buf] + lds_v<DP>(row, ch)) = R::value(vr[i]);
+                if (ch == 0) sok[buf][row] = there >> i & 1;
+            }
+        };
+        f32x16 o[ND];
+#pragma unroll
+        for (int n = 0; n < ND; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
+        float m = -INFINITY, l = 0.f;
+        if (span.total > 0) {
+            entries(0);
+            fetch(0);
+            if (span.total > 1) entries(1);
+            stage(0);
+        }
+        __syncthreads();
+        auto tile = [&](int c, auto which) {
+            constexpr int buf = decltype(which)::value;
+            const int kb = span.chunk(c) * KT;
+            const bool more = c + 1 < span.total;
+            if (more) {
+                fetch(c + 1);
+                if (c + 2 < span.total) entries(c + 2);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (kb <= wmax && (kb + KT - 1 > wmin - W || kb < sinks)) {
+                const unsigned long long okm = __ballot(sok[buf][lane & (KT - 1)]);
+                f32x16 s[NT];
+#pragma unroll
+                for (int u = 0; u < NT; ++u) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
+#pragma unroll
+                    for (int k = 0; k < KS; ++k)
+                        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(sk[buf] + 32 * u * RB + ak[k]), qf[k], s[u], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                const bool whole = kb + KT - 1 <= wmin && (kb > wmax - W || kb + KT - 1 < sinks) && okm == ~0ull;
+                if (!whole) {                  // key 32 u + 8 (i >> 2) + 4 hh + (i & 3), counted from kb + 32 u + 4 hh
+#pragma unroll
+                    for (int u = 0; u < NT; ++u) {
+                        const int from = kb + 32 * u + 4 * hh, hi = mypos - from, lo = mypos - W - from, sink = sinks - from;
+                        const unsigned pages = (unsigned)(okm >> (32 * u + 4 * hh));
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int key = 8 * (i >> 2) + (i & 3);
+                            s[u][i] = (pages & 1u << key) && key <= hi && (key > lo || key < sink) ? s[u][i] : -INFINITY;
+                        }
+                    }
+                }
+                float top = s[0][0];
+#pragma unroll
+                for (int u = 0; u < NT; ++u)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
+                top = fmaxf(top, __shfl_xor(top, 32)) * cs;
+                if (__any(top > m + 8.0f || (m == -INFINITY && top > m))) {
+                    const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+                    l *= f;
+#pragma unroll
+                    for (int n = 0; n < ND; ++n)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[n][i] *= f;
+                    m = mn;
+                }
+                const float mu = m == -INFINITY ? 0.f : m;
+                u32x4 p[NT][2];
+#pragma unroll
+                for (int u = 0; u < NT; ++u)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        const float x = __builtin_amdgcn_exp2f(fmaf(s[u][i], cs, -mu)), y = __builtin_amdgcn_exp2f(fmaf(s[u][i + 1], cs, -mu));
+                        l += x + y;
+                        p[u][i >> 3][(i & 7) >> 1] = pack2(x, y);
+                    }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < NT; ++u)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                        for (int n = 0; n < ND; ++n) {
+                            bf16x8 x;
+#pragma unroll
+                            for (int jj = 0; jj < 2; ++jj) {
+                                const unsigned char* ad = sv[buf] + (32 * u + 16 * h + 8 * jj) * RB + av[n];
+                                const bf16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)ad);
+#pragma unroll
+                                for (int w = 0; w < 4; ++w) x[4 * jj + w] = v[w];
+                            }
+                            o[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, __builtin_bit_cast(bf16x8, p[u][h]), o[n], 0, 0, 0);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+            }
+            if (more) stage(buf ^ 1);
+            __syncthreads();
+        };
+        for (int c = 0; c < span.total; c += 2) {
+            tile(c, Const<0>());
+            if (c + 1 < span.total) tile(c + 1, Const<1>());
+        }
+        l += __shfl_xor(l, 32);
+        if (col < t.ncols && (all || mypos == only)) {
+            const float inv = 1.0f / l;
+            const bool none = mypos < 0 || l == 0.f;
+            bf16* out = (bf16*)a.out + ((long long)(t.tok0 + qtok) * a.q_heads + hk * G + col - qtok * G) * D;
+#pragma unroll
+            for (int n = 0; n < ND; ++n)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int d = 32 * n + 8 * g + 4 * hh;
+                    bf16x4 x;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) x[w] = (bf16)(none ? 0.f : o[n][4 * g + w] * inv);
+                    if constexpr (__is_same(T, Int4)) {
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) out[R::dim(d + w)] = x[w];
+                    } else if (d < D) {
+                        *(bf16x4*)(out + d) = x;
+                    }
+                }
+        }
+        if (all) {
+            float bad = 0.f;
+#pragma unroll
+            for (int n = 0; n < ND; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) bad += o[n][i] * 0.f;
+            if (!__syncthreads_or(t.pmax > t.pmin && mypos >= 0 && bad != 0.f)) return;
+        }
+        if (++only > t.pmax) return;
+    }
+}
+
 int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
-long long tiles_of(int tokens, int sequences, int group, bool ragged) {
-    return ragged ? (long long)tokens * group / 16 + sequences : (long long)sequences * ((group + 15) / 16);
+long long tiles_of(int tokens, int sequences, int group, bool ragged, int cols = 16) {
+    return ragged ? (long long)tokens * group / cols + sequences : (long long)sequences * ((group + cols - 1) / cols);
+}
+// Which kernel: 16-column tiles re-read a request's keys for every tile, 128-column ones feed them to four waves through LDS
+bool prompts(const KvView& c, int tokens, int sequences, int q_heads, bool ragged) {
+    return c.dtype != Q3C_KV_F32 && ragged && (long long)tokens * (q_heads / c.heads) >= 64ll * sequences;
 }
 
 }  // namespace
@@ -533,6 +812,20 @@ hipError_t q3_launch_kv_attend(const KvAttendArgs& a, hipStream_t s) {
     if (!tiles || !a.b.tokens) return hipSuccess;
     const dim3 grid(tiles, a.c.heads, a.splits), join(tiles, a.c.heads);
     const int dp = padded_dim(a.c.dim);
+    if (prompts(a.c, a.b.tokens, a.b.sequences, a.q_heads, a.b.offsets != nullptr)) {
+        const int n = (int)tiles_of(a.b.tokens, a.b.sequences, a.group, true, 128);
+        const unsigned blocks = (unsigned)n * a.c.heads;
+        if (a.c.dtype == Q3C_KV_BF16) {
+            if (dp == 64) kv_prompt_kernel<bf16, 64, 64><<<blocks, 256, 0, s>>>(a, n);
+            else if (dp == 128) kv_prompt_kernel<bf16, 128, 64><<<blocks, 256, 0, s>>>(a, n);
+            else kv_prompt_kernel<bf16, 256, 32><<<blocks, 256, 0, s>>>(a, n);
+        } else {
+            if (dp == 64) kv_prompt_kernel<Int4, 64, 64><<<blocks, 256, 0, s>>>(a, n);
+            else if (dp == 128) kv_prompt_kernel<Int4, 128, 64><<<blocks, 256, 0, s>>>(a, n);
+            else kv_prompt_kernel<Int4, 256, 32><<<blocks, 256, 0, s>>>(a, n);
+        }
+        return hipGetLastError();
+    }
 #define Q3_ATTEND(T, A, DP)                                                        \
     do {                                                                           \
         kv_attend_kernel<T, DP><<<grid, 256, 0, s>>>(a);                           \

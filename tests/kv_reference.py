@@ -17,11 +17,13 @@ def norm_rotate(x, weight, cos, sin, pos, eps):
 
 def attention(q, k, v, pos, window, sinks, scale, there=None):
     """q [n, H, D] at positions pos [n], keys k, v [L, G, D] at positions 0 .. L - 1 (`there` [L]: which exist) -> (out [n, H, D], the
-    mean of |v| under the same weights, the largest sum over d of |q_d k_d| of a visible pair): float64.  Only what a query sees enters."""
+    mean of |v| under the same weights, the largest sum over d of |q_d k_d| of a visible pair): float64.  Only what a query sees enters.
+    The middle one carries, as .rounded_keys, how far out moves (first order) when each product q_d k_d is off by a share of itself: the
+    weighted mean of |v - out| sum |q_d k_d| scale, per unit of that share."""
     n, H, D = q.shape
     L, G, _ = k.shape
     out = torch.zeros((n, H, D), dtype=torch.float64, device=q.device)
-    mag, dot = torch.zeros_like(out), 0.0
+    mag, moved, dot = torch.zeros_like(out), torch.zeros_like(out), 0.0
     at = torch.arange(L, device=q.device)
     for i in range(n):
         see = at <= pos[i]
@@ -40,7 +42,10 @@ def attention(q, k, v, pos, window, sinks, scale, there=None):
             w = torch.softmax(x, 0)
             out[i, h] = w @ vv[:, g]
             mag[i, h] = w @ vv[:, g].abs()
-            dot = max(dot, float(prod.abs().sum(-1).max()))
+            dots = prod.abs().sum(-1)
+            moved[i, h] = (w * dots * scale) @ (vv[:, g] - out[i, h]).abs()
+            dot = max(dot, float(dots.max()))
+    mag.rounded_keys = moved
     return out, mag, dot
 
 

@@ -67,7 +67,10 @@ def _offsets(counts):
     return torch.tensor([0] + list(counts), dtype=torch.int32).cumsum(0).to(torch.int32).to(DEV)
 
 
-def _check_attend(got, want, mag, dot, kv, N, scale, q=None):
+def _check_attend(got, want, mag, dot, kv, N, scale, q=None, prompt=False):
+    """`prompt`: many tokens of a request at once, whose 4-bit keys and values n * step the kernel rounds to bf16 as operands: a product q_d k_d is
+    off by u of itself, which moves the output by u mag.rounded_keys (1.05: the second order, e^x - 1 - x for x <= 0.1), and the mean of the values
+    by u of the mean of |v|."""
     u = U[got.dtype]
     score = (kv.head_dim + 4) * 2.0 ** -24 * dot * scale
     if kv.dtype == "int4":                          # 136 sum q of each group is taken out again, in fp32
@@ -78,6 +81,8 @@ def _check_attend(got, want, mag, dot, kv, N, scale, q=None):
         bound = rel * mag + u * want.abs()
     else:
         bound = u * mag * 1.01 + rel * mag + u * want.abs() * 1.01
+    if kv.dtype == "int4" and prompt:
+        bound = bound + u * 1.05 * mag.rounded_keys + u * 1.05 * mag
     if kv.dtype == "int4":
         bound = bound + 144 * 16 * 2.0 ** -24 * float(kv.v_scale.float().nan_to_num(0.0).max())
     off = (got.double() - want).abs()
@@ -224,7 +229,7 @@ def test_attend_prompts_and_pieces(dtype, D, G, group, ps, window, sinks):
     for r, (L, n) in enumerate(zip(lens, new)):
         want, mag, dot = attention(q[at:at + n], *store[r], list(range(L - n, L)), window, sinks, scale) if n else (None, None, 0)
         if n:
-            _check_attend(out[at:at + n], want, mag, dot, kv, L, scale, q[at:at + n].double())
+            _check_attend(out[at:at + n], want, mag, dot, kv, L, scale, q[at:at + n].double(), prompt=True)
         at += n
 
 
@@ -520,7 +525,7 @@ def test_a_generation_with_forks_trims_and_a_compaction(dtype):
                 h[0], h[1] = torch.cat([h[0], kk[at:at + n].double()]), torch.cat([h[1], vv[at:at + n].double()])
                 L = h[0].shape[0]
                 want, mag, dot = attention(q[at:at + n], h[0], h[1], list(range(L - n, L)), window, sinks, D ** -0.5)
-                _check_attend(out[at:at + n], want, mag, dot, kv, L, D ** -0.5, q[at:at + n].double())
+                _check_attend(out[at:at + n], want, mag, dot, kv, L, D ** -0.5, q[at:at + n].double(), prompt=counts[0] > 1)
                 at += n
 
     tokens([0, 4], [21, 6])
@@ -647,3 +652,26 @@ def test_refusals_with_tensors_on_the_gpu():
         kv.gather(0, rows, _offsets([1, 1]))                        # how many tokens is not said
     kv.check()
     assert math.isnan(float(kv.k.float().sum()))                    # and nothing was written
+
+
+@pytest.mark.parametrize("dtype,D,G,group,ps", SHAPES)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (72, 0), (90, 10)])
+def test_attend_prompts_of_many_tiles(dtype, D, G, group, ps, window, sinks):
+    """Prompts long enough for the kernel that shares key tiles between waves: ragged ends, a past, a row of one token, an empty one."""
+    g = _gen(D * 5 + group + window)
+    lens, new = [300, 211, 1, 0], [300, 150, 1, 0]
+    kv = _cache(dtype, G, D, ps, lens)
+    store = _fill(kv, 0, lens, g)
+    T = sum(new)
+    q = _randn(g, T + 1, G * group, D).mul_(2).to(kv.activations)
+    out = torch.full_like(q, 5.0)
+    rows = torch.arange(4, dtype=torch.int32, device=DEV)
+    kv.attend(0, q, rows, _offsets(new), window=window, sinks=sinks, out=out)
+    kv.check()
+    assert bool((out[T:] == 5.0).all())
+    scale = D ** -0.5
+    for r, start, some in ((0, 0, [0, 1, 31, 32, 63, 64, 127, 128, 200, 299]), (1, 300, [0, 5, 63, 100, 149]), (2, 450, [0])):
+        i = torch.tensor(some, device=DEV)
+        pos = [lens[r] - new[r] + p for p in some]
+        want, mag, dot = attention(q[start + i], *store[r], pos, window, sinks, scale)
+        _check_attend(out[start + i], want, mag, dot, kv, lens[r], scale, q[start + i].double(), prompt=True)
