@@ -518,8 +518,10 @@ template <typename T, int DP> struct Row;                       // chunk ch of a
 template <int DP> struct Row<bf16, DP> {
     static constexpr int WORDS = 4;
     struct Raw { u32x4 x; };
-    static __device__ __forceinline__ void load(Raw& r, const void* base, const bf16*, long long row, int D, int ch) {
-        r.x = *(const u32x4*)((const bf16*)base + row * D + 8 * ch);
+    static __device__ __forceinline__ const char* base(const void* p, long long row, int D) { return (const char*)p + row * D * 2; }
+    static __device__ __forceinline__ const bf16* steps(const bf16* p, long long) { return p; }
+    static __device__ __forceinline__ void load(Raw& r, const char* base, const bf16*, int row, int D, int ch) {
+        r.x = *(const u32x4*)(base + (unsigned)(row * D * 2 + 16 * ch));
     }
     static __device__ __forceinline__ void zero(Raw& r) { r.x = u32x4{0, 0, 0, 0}; }
     static __device__ __forceinline__ u32x4 value(const Raw& r) { return r.x; }
@@ -528,8 +530,10 @@ template <int DP> struct Row<bf16, DP> {
 template <int D> struct Row<Int4, D> {
     static constexpr int S = D / 32;
     struct Raw { unsigned x; u32x2 st; };
-    static __device__ __forceinline__ void load(Raw& r, const void* base, const bf16* steps, long long row, int, int ch) {
-        r.x = *(const unsigned*)((const char*)base + row * (D / 2) + 4 * ch);
+    static __device__ __forceinline__ const char* base(const void* p, long long row, int) { return (const char*)p + row * (D / 2); }
+    static __device__ __forceinline__ const bf16* steps(const bf16* p, long long row) { return p + row * S; }
+    static __device__ __forceinline__ void load(Raw& r, const char* base, const bf16* steps, int row, int, int ch) {
+        r.x = *(const unsigned*)(base + (unsigned)(row * (D / 2) + 4 * ch));
         if constexpr (S == 2) { r.st[0] = *(const unsigned*)(steps + row * S); r.st[1] = r.st[0]; }
         else r.st = *(const u32x2*)(steps + row * S + (S == 8 ? 4 * (ch & 1) : 0));
     }
@@ -552,14 +556,37 @@ template <int D> struct Row<Int4, D> {
 template <int DP> __device__ __forceinline__ int lds_k(int row, int ch) { return 2 * DP * row + 16 * (ch ^ (DP == 64 ? (row >> 1) & 7 : row & 15)); }
 template <int DP> __device__ __forceinline__ int lds_v(int row, int ch) { return 2 * DP * row + 16 * (ch ^ (DP == 64 ? (row >> 1 & 1) << 2 : (row & 3) << 2)); }
 
+__device__ __forceinline__ float max_halves(float x) {           // over lanes l and l ^ 32
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 template <int N> struct Const { static constexpr int value = N; };
+
+typedef __attribute__((address_space(3))) void lds_void;
+__device__ const u32x4 kv_zeros = {0, 0, 0, 0};                 // what a row that nobody sees is read from
+
+// 16 bytes per lane from memory to LDS at `lds` (uniform) + 16 lane, outside the compiler's count of loads: `landed` waits for them.
+// (M0 belongs to no value of the compiler's; its own uses write it right before.)
+__device__ __forceinline__ void to_lds(const char* base, unsigned off, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory");
+}
+__device__ __forceinline__ void to_lds(const void* p, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(p), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory");
+}
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void meet() {                        // a barrier that leaves loads in flight
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ unsigned lds_of(const void* p) { return (unsigned)(unsigned long long)(lds_void*)p; }
 
 template <typename T, int DP, int KT>
 __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const KvAttendArgs a, int tiles) {
     typedef Row<T, DP> R;
-    constexpr int RB = 2 * DP, NCH = DP / 8, KS = DP / 16, ND = DP / 32, NT = KT / 32, RP = 256 / NCH, NR = KT / RP;
+    constexpr bool DMA = !__is_same(T, Int4);
+    constexpr int RB = 2 * DP, NCH = DP / 8, KS = DP / 16, ND = DP / 32, NT = KT / 32, RP = 256 / NCH, NR = KT / RP, RW = RP / 4;
     __shared__ __attribute__((aligned(16))) unsigned char sk[2][KT * RB], sv[2][KT * RB];
-    __shared__ int sok[2][KT];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hk = blockIdx.x % a.c.heads, G = a.group, D = a.c.dim, sh = a.c.ps_shift;
     const Tile t = kv_tile(a, tiles - 1 - (int)(blockIdx.x / a.c.heads), 128, lane);
@@ -579,7 +606,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
             for (int e = 0; e < 8; ++e) qf[s][e] = (bf16)0.f;
             const int d = 16 * s + 8 * hh;
             if (mypos >= 0 && d < D) {
-                if constexpr (__is_same(T, Int4)) {
+                if constexpr (!DMA) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) qf[s][e] = q[R::dim(d + e)];
                 } else {
@@ -595,7 +622,8 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
     const long long page_rows = (long long)a.c.heads << sh, head0 = ((long long)a.layer * a.c.pages * a.c.heads + hk) << sh;
     const int in_page = (1 << sh) - 1, last_entry = a.c.width - 1;
     const int W = a.window > 0 ? a.window : 0x7fffffff, sinks = a.window > 0 ? a.sinks : 0;
-    const int ch = tid & (NCH - 1), row0 = tid / NCH;                                // this thread stages chunk ch of rows row0 + i RP
+    // This thread stages 16-byte slot `slot` of rows row0 + i RP; the rows of a wave and i are RW consecutive ones, which lie in one page.
+    const int slot = tid & (NCH - 1), row0 = tid / NCH, sub = lane / NCH;
     const float cs = a.scale_log2e;
     // LDS places of this lane's operands; tiles, halves and buffers are constants added to them
     int ak[KS], av[ND];
@@ -611,133 +639,154 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
     for (;;) {
         const bool all = only < t.pmin;
         const int vlo = (all ? t.pmin : only) - W, vhi = all ? t.pmax : only;
-        int e[NR];
-        typename R::Raw kr[NR], vr[NR];
-        auto entries = [&](int c) {
-#pragma unroll
-            for (int i = 0; i < NR; ++i) e[i] = table[min((span.chunk(c) * KT + row0 + i * RP) >> sh, last_entry)];
-        };
-        unsigned there;
-        auto fetch = [&](int c) {
-            there = 0;
+        typename R::Raw kr[DMA ? 1 : NR], vr[DMA ? 1 : NR];
+        // the page of each of a tile's keys, one per lane
+        auto entries = [&](int c) { return table[min((span.chunk(c) * KT + (lane & (KT - 1))) >> sh, last_entry)]; };
+        // Rows of one tensor of tile c on their way, to LDS (bf16) or to registers (4 bits: `stage` puts them there).  A row that no column sees is
+        // read as zeros: its probabilities are 0, but 0 times an old NaN would still be NaN.
+        auto fetch = [&](int c, int e, const void* tensor, const bf16* steps, unsigned char* lds, bool keys, typename R::Raw* raw) {
+            const int kb = span.chunk(c) * KT;
+            const bool inner = all && kb + KT - 1 <= vhi && (kb > vlo || kb + KT - 1 < sinks);
 #pragma unroll
             for (int i = 0; i < NR; ++i) {
-                const int tok = span.chunk(c) * KT + row0 + i * RP;
-                const bool page = (unsigned)e[i] < (unsigned)a.c.pages;
-                there |= (unsigned)page << i;
-                const bool ok = page && tok <= vhi && (tok > vlo || tok < sinks) && 8 * ch < D;
-                R::zero(kr[i]);
-                R::zero(vr[i]);
-                if (ok) {
-                    const long long at = head0 + (long long)e[i] * page_rows + (tok & in_page);
-                    R::load(kr[i], a.c.k, a.c.ks, at, D, ch);
-                    R::load(vr[i], a.c.v, a.c.vs, at, D, ch);
+                const int first = i * RP + wave * RW, tok = kb + first, mine = tok + sub;
+                if constexpr (DMA) {
+                    const int page = __builtin_amdgcn_readlane(e, first);
+                    const bool there = (unsigned)page < (unsigned)a.c.pages;
+                    const int place = (keys ? lds_k<DP>(row0 + i * RP, slot) : lds_v<DP>(row0 + i * RP, slot)) - RB * (row0 + i * RP);     // the chunk whose place this slot is
+                    const unsigned off = (unsigned)(sub * D * 2 + (place < 2 * D ? place : 0));
+                    const char* base = (const char*)tensor + (head0 + (long long)page * page_rows + (tok & in_page)) * D * 2;
+                    const unsigned to = lds_of(lds) + first * RB;
+                    if (there && inner) to_lds(base, off, to);
+                    else to_lds(there && mine <= vhi && (mine > vlo || mine < sinks) ? (const void*)(base + off) : (const void*)&kv_zeros, to);
+                } else {
+                    const int page = __shfl(e, row0 + i * RP);
+                    R::zero(raw[i]);
+                    if ((unsigned)page < (unsigned)a.c.pages && mine <= vhi && (mine > vlo || mine < sinks)) {
+                        const long long at = head0 + (long long)page * page_rows + ((kb + row0 + i * RP) & in_page);
+                        R::load(raw[i], R::base(tensor, at, D), R::steps(steps, at), 0, D, slot);
+                    }
                 }
             }
         };
-        auto stage = [&](int buf) {
+        auto stage = [&](unsigned char* lds, bool keys, const typename R::Raw* raw) {
+            if constexpr (!DMA) {
 #pragma unroll
-            for (int i = 0; i < NR; ++i) {
-                const int row = row0 + i * RP;
-                *(u32x4*)(sk[buf] + lds_k<DP>(row, ch)) = R::value(kr[i]);
-                *(u32x4*)(sv[buf] + lds_v<DP>(row, ch)) = R::value(vr[i]);
-                if (ch == 0) sok[buf][row] = there >> i & 1;
+                for (int i = 0; i < NR; ++i) {
+                    const int row = row0 + i * RP;
+                    *(u32x4*)(lds + (keys ? lds_k<DP>(row, slot) : lds_v<DP>(row, slot))) = R::value(raw[i]);
+                }
             }
         };
-        f32x16 o[ND];
+        auto exists = [&](int e) { return (unsigned long long)__ballot((unsigned)e < (unsigned)a.c.pages); };
+        f32x16 s[2][NT], o[ND];
+        auto scores = [&](f32x16* s, const unsigned char* k0) {
+#pragma unroll
+            for (int u = 0; u < NT; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int u = 0; u < NT; ++u)
+                    s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(k0 + 32 * u * RB + ak[k]), qf[k], s[u], 0, 0, 0);
+        };
 #pragma unroll
         for (int n = 0; n < ND; ++n)
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
         float m = -INFINITY, l = 0.f;
+        // A trip multiplies this tile's probabilities with its values while the next tile's scores are formed: the matrix cores have those to do
+        // while the vector units do this tile's softmax.  So keys run one tile ahead of values, and both one tile behind their loads.
+        int e1 = 0, e2 = 0;                    // entries of the next tile and the one after
+        unsigned long long ok0 = 0;            // keys of this tile that have a page
         if (span.total > 0) {
-            entries(0);
-            fetch(0);
-            if (span.total > 1) entries(1);
-            stage(0);
-        }
-        __syncthreads();
-        auto tile = [&](int c, auto which) {
-            constexpr int buf = decltype(which)::value;
-            const int kb = span.chunk(c) * KT;
-            const bool more = c + 1 < span.total;
-            if (more) {
-                fetch(c + 1);
-                if (c + 2 < span.total) entries(c + 2);
+            const int e0 = entries(0);
+            if (span.total > 1) e1 = entries(1);
+            if (span.total > 2) e2 = entries(2);
+            ok0 = exists(e0);
+            fetch(0, e0, a.c.k, a.c.ks, sk[0], true, kr);
+            fetch(0, e0, a.c.v, a.c.vs, sv[0], false, vr);
+            stage(sk[0], true, kr);
+            stage(sv[0], false, vr);
+            if (span.total > 1) {
+                fetch(1, e1, a.c.k, a.c.ks, sk[1], true, kr);
+                stage(sk[1], true, kr);
             }
-            __builtin_amdgcn_sched_barrier(0);
-            if (kb <= wmax && (kb + KT - 1 > wmin - W || kb < sinks)) {
-                const unsigned long long okm = __ballot(sok[buf][lane & (KT - 1)]);
-                f32x16 s[NT];
+            landed();
+            meet();
+            scores(s[0], sk[0]);
+            meet();
+        }
+        auto tile = [&](int c, auto which) {
+            constexpr int P = decltype(which)::value;
+            const int kb = span.chunk(c) * KT;
+            const unsigned long long okm = ok0;
+            const int ev = e1, ek = e2;
+            ok0 = exists(e1);
+            e1 = e2;
+            if (c + 3 < span.total) e2 = entries(c + 3);
+            if (c + 2 < span.total) fetch(c + 2, ek, a.c.k, a.c.ks, sk[P], true, kr);
+            if (c + 1 < span.total) fetch(c + 1, ev, a.c.v, a.c.vs, sv[P ^ 1], false, vr);
+            const bool whole = kb + KT - 1 <= wmin && (kb > wmax - W || kb + KT - 1 < sinks) && okm == ~0ull;
+            if (!whole) {                      // key 32 u + 8 (i >> 2) + 4 hh + (i & 3), counted from kb + 32 u + 4 hh
 #pragma unroll
                 for (int u = 0; u < NT; ++u) {
+                    const int from = kb + 32 * u + 4 * hh, hi = mypos - from, lo = mypos - W - from, sink = sinks - from;
+                    const unsigned there = (unsigned)(okm >> (32 * u + 4 * hh));
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
-#pragma unroll
-                    for (int k = 0; k < KS; ++k)
-                        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(sk[buf] + 32 * u * RB + ak[k]), qf[k], s[u], 0, 0, 0);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                const bool whole = kb + KT - 1 <= wmin && (kb > wmax - W || kb + KT - 1 < sinks) && okm == ~0ull;
-                if (!whole) {                  // key 32 u + 8 (i >> 2) + 4 hh + (i & 3), counted from kb + 32 u + 4 hh
-#pragma unroll
-                    for (int u = 0; u < NT; ++u) {
-                        const int from = kb + 32 * u + 4 * hh, hi = mypos - from, lo = mypos - W - from, sink = sinks - from;
-                        const unsigned pages = (unsigned)(okm >> (32 * u + 4 * hh));
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int key = 8 * (i >> 2) + (i & 3);
-                            s[u][i] = (pages & 1u << key) && key <= hi && (key > lo || key < sink) ? s[u][i] : -INFINITY;
-                        }
+                    for (int i = 0; i < 16; ++i) {
+                        const int key = 8 * (i >> 2) + (i & 3);
+                        s[P][u][i] = (there & 1u << key) && key <= hi && (key > lo || key < sink) ? s[P][u][i] : -INFINITY;
                     }
                 }
-                float top = s[0][0];
-#pragma unroll
-                for (int u = 0; u < NT; ++u)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
-                top = fmaxf(top, __shfl_xor(top, 32)) * cs;
-                if (__any(top > m + 8.0f || (m == -INFINITY && top > m))) {
-                    const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
-                    l *= f;
-#pragma unroll
-                    for (int n = 0; n < ND; ++n)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[n][i] *= f;
-                    m = mn;
-                }
-                const float mu = m == -INFINITY ? 0.f : m;
-                u32x4 p[NT][2];
-#pragma unroll
-                for (int u = 0; u < NT; ++u)
-#pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        const float x = __builtin_amdgcn_exp2f(fmaf(s[u][i], cs, -mu)), y = __builtin_amdgcn_exp2f(fmaf(s[u][i + 1], cs, -mu));
-                        l += x + y;
-                        p[u][i >> 3][(i & 7) >> 1] = pack2(x, y);
-                    }
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int u = 0; u < NT; ++u)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                        for (int n = 0; n < ND; ++n) {
-                            bf16x8 x;
-#pragma unroll
-                            for (int jj = 0; jj < 2; ++jj) {
-                                const unsigned char* ad = sv[buf] + (32 * u + 16 * h + 8 * jj) * RB + av[n];
-                                const bf16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)ad);
-#pragma unroll
-                                for (int w = 0; w < 4; ++w) x[4 * jj + w] = v[w];
-                            }
-                            o[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, __builtin_bit_cast(bf16x8, p[u][h]), o[n], 0, 0, 0);
-                        }
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
             }
-            if (more) stage(buf ^ 1);
-            __syncthreads();
+            float top = s[P][0][0];
+#pragma unroll
+            for (int u = 0; u < NT; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[P][u][i]);
+            top = max_halves(top) * cs;
+            if (__any(top > m + 8.0f)) {
+                const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+                l *= f;
+#pragma unroll
+                for (int n = 0; n < ND; ++n)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[n][i] *= f;
+                m = mn;
+            }
+            const float mu = m == -INFINITY ? 0.f : m;
+            scores(s[P ^ 1], sk[P ^ 1]);       // past the last tile: of whatever lies there, and not looked at
+            u32x4 p[NT][2];
+#pragma unroll
+            for (int u = 0; u < NT; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[P][u][i], cs, -mu)), y = __builtin_amdgcn_exp2f(fmaf(s[P][u][i + 1], cs, -mu));
+                    l += x + y;
+                    p[u][i >> 3][(i & 7) >> 1] = pack2(x, y);
+                }
+#pragma unroll
+            for (int u = 0; u < NT; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int n = 0; n < ND; ++n) {
+                        bf16x8 x;
+#pragma unroll
+                        for (int jj = 0; jj < 2; ++jj) {
+                            const unsigned char* ad = sv[P] + (32 * u + 16 * h + 8 * jj) * RB + av[n];
+                            const bf16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)ad);
+#pragma unroll
+                            for (int w = 0; w < 4; ++w) x[4 * jj + w] = v[w];
+                        }
+                        o[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, __builtin_bit_cast(bf16x8, p[u][h]), o[n], 0, 0, 0);
+                    }
+            if (c + 2 < span.total) stage(sk[P], true, kr);
+            if (c + 1 < span.total) stage(sv[P ^ 1], false, vr);
+            landed();
+            meet();
         };
         for (int c = 0; c < span.total; c += 2) {
             tile(c, Const<0>());
@@ -756,7 +805,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
                     bf16x4 x;
 #pragma unroll
                     for (int w = 0; w < 4; ++w) x[w] = (bf16)(none ? 0.f : o[n][4 * g + w] * inv);
-                    if constexpr (__is_same(T, Int4)) {
+                    if constexpr (!DMA) {
 #pragma unroll
                         for (int w = 0; w < 4; ++w) out[R::dim(d + w)] = x[w];
                     } else if (d < D) {
@@ -782,7 +831,7 @@ long long tiles_of(int tokens, int sequences, int group, bool ragged, int cols =
 }
 // Which kernel: 16-column tiles re-read a request's keys for every tile, 128-column ones feed them to four waves through LDS
 bool prompts(const KvView& c, int tokens, int sequences, int q_heads, bool ragged) {
-    return c.dtype != Q3C_KV_F32 && ragged && (long long)tokens * (q_heads / c.heads) >= 64ll * sequences;
+    return c.dtype != Q3C_KV_F32 && !(c.dtype == Q3C_KV_INT4 && c.dim > 128) && ragged && (long long)tokens * (q_heads / c.heads) >= 64ll * sequences;
 }
 
 }  // namespace
@@ -821,8 +870,7 @@ hipError_t q3_launch_kv_attend(const KvAttendArgs& a, hipStream_t s) {
             else kv_prompt_kernel<bf16, 256, 32><<<blocks, 256, 0, s>>>(a, n);
         } else {
             if (dp == 64) kv_prompt_kernel<Int4, 64, 64><<<blocks, 256, 0, s>>>(a, n);
-            else if (dp == 128) kv_prompt_kernel<Int4, 128, 64><<<blocks, 256, 0, s>>>(a, n);
-            else kv_prompt_kernel<Int4, 256, 32><<<blocks, 256, 0, s>>>(a, n);
+            else kv_prompt_kernel<Int4, 128, 32><<<blocks, 256, 0, s>>>(a, n);
         }
         return hipGetLastError();
     }
