@@ -617,6 +617,8 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
             }
         }
     }
+#pragma unroll
+    for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[s]));   // waited for here: a wait in the loop would be for every load in flight
     const Span span = kv_span(a, t, KT);
     const int* table = a.c.table + (long long)max(t.row, 0) * a.c.width;
     const long long page_rows = (long long)a.c.heads << sh, head0 = ((long long)a.layer * a.c.pages * a.c.heads + hk) << sh;
@@ -640,18 +642,28 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
         const bool all = only < t.pmin;
         const int vlo = (all ? t.pmin : only) - W, vhi = all ? t.pmax : only;
         typename R::Raw kr[DMA ? 1 : NR], vr[DMA ? 1 : NR];
-        // the page of each of a tile's keys, one per lane
-        auto entries = [&](int c) { return table[min((span.chunk(c) * KT + (lane & (KT - 1))) >> sh, last_entry)]; };
+        // 64 entries of the table, one per lane, for the keys' fetches and for the values': read again only when a tile leaves them, so that the
+        // wait for them (which is one for every load in flight) comes once in 64 pages
+        int ent[2] = {0, 0}, ent0[2] = {-0x40000000, -0x40000000};
+        unsigned long long good = 0;           // which of the keys' 64 name a page of the pool
         // Rows of one tensor of tile c on their way, to LDS (bf16) or to registers (4 bits: `stage` puts them there).  A row that no column sees is
         // read as zeros: its probabilities are 0, but 0 times an old NaN would still be NaN.
-        auto fetch = [&](int c, int e, const void* tensor, const bf16* steps, unsigned char* lds, bool keys, typename R::Raw* raw) {
-            const int kb = span.chunk(c) * KT;
+        auto fetch = [&](int c, const void* tensor, const bf16* scales, unsigned char* lds, auto which, typename R::Raw* raw) -> unsigned long long {
+            constexpr bool keys = decltype(which)::value;
+            const int kb = span.chunk(c) * KT, e0 = kb >> sh;
+            if (e0 < ent0[keys] || ((kb + KT - 1) >> sh) > ent0[keys] + 63) {
+                ent0[keys] = e0;
+                ent[keys] = table[min(e0 + lane, last_entry)];
+                asm volatile("" : "+v"(ent[keys]));            // waited for here, not at every later use
+                if constexpr (keys) good = __ballot((unsigned)ent[keys] < (unsigned)a.c.pages);
+            }
+            const int e = ent[keys], from = ent0[keys];
             const bool inner = all && kb + KT - 1 <= vhi && (kb > vlo || kb + KT - 1 < sinks);
 #pragma unroll
             for (int i = 0; i < NR; ++i) {
                 const int first = i * RP + wave * RW, tok = kb + first, mine = tok + sub;
                 if constexpr (DMA) {
-                    const int page = __builtin_amdgcn_readlane(e, first);
+                    const int page = __builtin_amdgcn_readlane(e, (tok >> sh) - from);
                     const bool there = (unsigned)page < (unsigned)a.c.pages;
                     const int place = (keys ? lds_k<DP>(row0 + i * RP, slot) : lds_v<DP>(row0 + i * RP, slot)) - RB * (row0 + i * RP);     // the chunk whose place this slot is
                     const unsigned off = (unsigned)(sub * D * 2 + (place < 2 * D ? place : 0));
@@ -660,14 +672,21 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
                     if (there && inner) to_lds(base, off, to);
                     else to_lds(there && mine <= vhi && (mine > vlo || mine < sinks) ? (const void*)(base + off) : (const void*)&kv_zeros, to);
                 } else {
-                    const int page = __shfl(e, row0 + i * RP);
+                    const int page = __shfl(e, ((kb + row0 + i * RP) >> sh) - from);
                     R::zero(raw[i]);
                     if ((unsigned)page < (unsigned)a.c.pages && mine <= vhi && (mine > vlo || mine < sinks)) {
                         const long long at = head0 + (long long)page * page_rows + ((kb + row0 + i * RP) & in_page);
-                        R::load(raw[i], R::base(tensor, at, D), R::steps(steps, at), 0, D, slot);
+                        R::load(raw[i], R::base(tensor, at, D), R::steps(scales, at), 0, D, slot);
                     }
                 }
             }
+            unsigned long long there = ~0ull;  // the tile's keys that have a page
+            if constexpr (keys) {
+                const int first = (kb >> sh) - from, n = ((kb + KT - 1) >> sh) - (kb >> sh) + 1;
+                if ((~good >> first) & ((1ull << n) - 1))
+                    there = __ballot((good >> (((kb + (lane & (KT - 1))) >> sh) - from)) & 1);
+            }
+            return there;
         };
         auto stage = [&](unsigned char* lds, bool keys, const typename R::Raw* raw) {
             if constexpr (!DMA) {
@@ -678,7 +697,6 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
                 }
             }
         };
-        auto exists = [&](int e) { return (unsigned long long)__ballot((unsigned)e < (unsigned)a.c.pages); };
         f32x16 s[2][NT], o[ND];
         auto scores = [&](f32x16* s, const unsigned char* k0) {
 #pragma unroll
@@ -698,19 +716,16 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
         float m = -INFINITY, l = 0.f;
         // A trip multiplies this tile's probabilities with its values while the next tile's scores are formed: the matrix cores have those to do
         // while the vector units do this tile's softmax.  So keys run one tile ahead of values, and both one tile behind their loads.
-        int e1 = 0, e2 = 0;                    // entries of the next tile and the one after
-        unsigned long long ok0 = 0;            // keys of this tile that have a page
+        unsigned long long ok0 = 0, ok1 = 0;   // keys of this tile and the next that have a page
+        const Const<1> keys;
+        const Const<0> values;
         if (span.total > 0) {
-            const int e0 = entries(0);
-            if (span.total > 1) e1 = entries(1);
-            if (span.total > 2) e2 = entries(2);
-            ok0 = exists(e0);
-            fetch(0, e0, a.c.k, a.c.ks, sk[0], true, kr);
-            fetch(0, e0, a.c.v, a.c.vs, sv[0], false, vr);
+            ok0 = fetch(0, a.c.k, a.c.ks, sk[0], keys, kr);
+            fetch(0, a.c.v, a.c.vs, sv[0], values, vr);
             stage(sk[0], true, kr);
             stage(sv[0], false, vr);
             if (span.total > 1) {
-                fetch(1, e1, a.c.k, a.c.ks, sk[1], true, kr);
+                ok1 = fetch(1, a.c.k, a.c.ks, sk[1], keys, kr);
                 stage(sk[1], true, kr);
             }
             landed();
@@ -722,12 +737,9 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
             constexpr int P = decltype(which)::value;
             const int kb = span.chunk(c) * KT;
             const unsigned long long okm = ok0;
-            const int ev = e1, ek = e2;
-            ok0 = exists(e1);
-            e1 = e2;
-            if (c + 3 < span.total) e2 = entries(c + 3);
-            if (c + 2 < span.total) fetch(c + 2, ek, a.c.k, a.c.ks, sk[P], true, kr);
-            if (c + 1 < span.total) fetch(c + 1, ev, a.c.v, a.c.vs, sv[P ^ 1], false, vr);
+            ok0 = ok1;
+            if (c + 2 < span.total) ok1 = fetch(c + 2, a.c.k, a.c.ks, sk[P], keys, kr);
+            if (c + 1 < span.total) fetch(c + 1, a.c.v, a.c.vs, sv[P ^ 1], values, vr);
             const bool whole = kb + KT - 1 <= wmin && (kb > wmax - W || kb + KT - 1 < sinks) && okm == ~0ull;
             if (!whole) {                      // key 32 u + 8 (i >> 2) + 4 hh + (i & 3), counted from kb + 32 u + 4 hh
 #pragma unroll
@@ -757,32 +769,50 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
                 m = mn;
             }
             const float mu = m == -INFINITY ? 0.f : m;
-            scores(s[P ^ 1], sk[P ^ 1]);       // past the last tile: of whatever lies there, and not looked at
+            // The order below is the order of the instructions: each matrix product has its operands' reads of LDS a few products earlier and a share of
+            // the softmax's arithmetic behind it.  (Past the last tile the scores are of whatever lies there, and not looked at.)
+            constexpr int QK = KS * NT, PV = 2 * NT * ND, NE = 16 * NT / 2, AHEAD = 4;      // products, pairs of scores
+            bf16x8 kf[AHEAD], vf[AHEAD];
             u32x4 p[NT][2];
+            auto read_k = [&](int j) { return *(const bf16x8*)(sk[P ^ 1] + 32 * (j % NT) * RB + ak[j / NT]); };
+            auto read_v = [&](int j) {
+                bf16x8 x;
 #pragma unroll
-            for (int u = 0; u < NT; ++u)
+                for (int jj = 0; jj < 2; ++jj) {
+                    const unsigned char* ad = sv[P] + (16 * (j / ND) + 8 * jj) * RB + av[j % ND];
+                    const bf16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)ad);
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const float x = __builtin_amdgcn_exp2f(fmaf(s[P][u][i], cs, -mu)), y = __builtin_amdgcn_exp2f(fmaf(s[P][u][i + 1], cs, -mu));
-                    l += x + y;
-                    p[u][i >> 3][(i & 7) >> 1] = pack2(x, y);
+                    for (int w = 0; w < 4; ++w) x[4 * jj + w] = v[w];
                 }
+                return x;
+            };
+            auto weight = [&](int e) {         // scores 2 e, 2 e + 1 of this tile -> probabilities
+                const int u = e >> 3, i = 2 * (e & 7);
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[P][u][i], cs, -mu)), y = __builtin_amdgcn_exp2f(fmaf(s[P][u][i + 1], cs, -mu));
+                l += x + y;
+                p[u][i >> 3][(i & 7) >> 1] = pack2(x, y);
+            };
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) kf[j] = read_k(j);
 #pragma unroll
             for (int u = 0; u < NT; ++u)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int i = 0; i < 16; ++i) s[P ^ 1][u][i] = 0.f;
 #pragma unroll
-                    for (int n = 0; n < ND; ++n) {
-                        bf16x8 x;
+            for (int j = 0; j < QK; ++j) {
+                s[P ^ 1][j % NT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[j % AHEAD], qf[j / NT], s[P ^ 1][j % NT], 0, 0, 0);
+                if (j + AHEAD < QK) kf[j % AHEAD] = read_k(j + AHEAD);
+                else vf[(j + AHEAD - QK) % AHEAD] = read_v(j + AHEAD - QK);
 #pragma unroll
-                        for (int jj = 0; jj < 2; ++jj) {
-                            const unsigned char* ad = sv[P] + (32 * u + 16 * h + 8 * jj) * RB + av[n];
-                            const bf16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)ad);
+                for (int e = j * NE / QK; e < (j + 1) * NE / QK; ++e) weight(e);
+                __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
-                            for (int w = 0; w < 4; ++w) x[4 * jj + w] = v[w];
-                        }
-                        o[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, __builtin_bit_cast(bf16x8, p[u][h]), o[n], 0, 0, 0);
-                    }
+            for (int j = 0; j < PV; ++j) {
+                o[j % ND] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[j % AHEAD], __builtin_bit_cast(bf16x8, p[j / ND / 2][(j / ND) & 1]), o[j % ND], 0, 0, 0);
+                if (j + AHEAD < PV) vf[j % AHEAD] = read_v(j + AHEAD);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             if (c + 2 < span.total) stage(sk[P], true, kr);
             if (c + 1 < span.total) stage(sv[P ^ 1], false, vr);
             landed();
