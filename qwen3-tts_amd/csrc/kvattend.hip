@@ -622,7 +622,9 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
     const Span span = kv_span(a, t, KT);
     const int* table = a.c.table + (long long)max(t.row, 0) * a.c.width;
     const long long page_rows = (long long)a.c.heads << sh, head0 = ((long long)a.layer * a.c.pages * a.c.heads + hk) << sh;
-    const int in_page = (1 << sh) - 1, last_entry = a.c.width - 1;
+    const int in_page = (1 << sh) - 1, last_entry = a.c.width - 1, row_bytes = 2 * D;
+    const unsigned page_bytes = (unsigned)page_rows * row_bytes;                   // below 2^32: the entry points see to it
+    const char *kbase = (const char*)a.c.k + (DMA ? head0 * row_bytes : 0), *vbase = (const char*)a.c.v + (DMA ? head0 * row_bytes : 0);
     const int W = a.window > 0 ? a.window : 0x7fffffff, sinks = a.window > 0 ? a.sinks : 0;
     // This thread stages 16-byte slot `slot` of rows row0 + i RP; the rows of a wave and i are RW consecutive ones, which lie in one page.
     const int slot = tid & (NCH - 1), row0 = tid / NCH, sub = lane / NCH;
@@ -642,51 +644,67 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
         const bool all = only < t.pmin;
         const int vlo = (all ? t.pmin : only) - W, vhi = all ? t.pmax : only;
         typename R::Raw kr[DMA ? 1 : NR], vr[DMA ? 1 : NR];
-        // 64 entries of the table, one per lane, for the keys' fetches and for the values': read again only when a tile leaves them, so that the
-        // wait for them (which is one for every load in flight) comes once in 64 pages
-        int ent[2] = {0, 0}, ent0[2] = {-0x40000000, -0x40000000};
-        unsigned long long good = 0;           // which of the keys' 64 name a page of the pool
-        // Rows of one tensor of tile c on their way, to LDS (bf16) or to registers (4 bits: `stage` puts them there).  A row that no column sees is
-        // read as zeros: its probabilities are 0, but 0 times an old NaN would still be NaN.
-        auto fetch = [&](int c, const void* tensor, const bf16* scales, unsigned char* lds, auto which, typename R::Raw* raw) -> unsigned long long {
-            constexpr bool keys = decltype(which)::value;
+        // 64 entries of the table, one per lane, read again only when a tile leaves them: the wait for them is one for every load in flight
+        int ent = 0, ent0 = -0x40000000;
+        unsigned long long good = 0;           // which of them name a page of the pool
+        long long place[DMA ? NR : 1];         // where this wave's rows of the tile last asked for begin, in bytes from a tensor's first
+        int page[DMA ? 1 : NR];                // the pages of this thread's
+        // Looks a tile's rows up; returns which of its keys have a page.
+        auto find = [&](int c) -> unsigned long long {
             const int kb = span.chunk(c) * KT, e0 = kb >> sh;
-            if (e0 < ent0[keys] || ((kb + KT - 1) >> sh) > ent0[keys] + 63) {
-                ent0[keys] = e0;
-                ent[keys] = table[min(e0 + lane, last_entry)];
-                asm volatile("" : "+v"(ent[keys]));            // waited for here, not at every later use
-                if constexpr (keys) good = __ballot((unsigned)ent[keys] < (unsigned)a.c.pages);
+            if (e0 < ent0 || ((kb + KT - 1) >> sh) > ent0 + 63) {
+                ent0 = e0;
+                ent = table[min(e0 + lane, last_entry)];
+                asm volatile("" : "+v"(ent));                  // waited for here, not at every later use
+                good = __ballot((unsigned)ent < (unsigned)a.c.pages);
             }
-            const int e = ent[keys], from = ent0[keys];
-            const bool inner = all && kb + KT - 1 <= vhi && (kb > vlo || kb + KT - 1 < sinks);
+            if constexpr (DMA) {
 #pragma unroll
-            for (int i = 0; i < NR; ++i) {
-                const int first = i * RP + wave * RW, tok = kb + first, mine = tok + sub;
-                if constexpr (DMA) {
-                    const int page = __builtin_amdgcn_readlane(e, (tok >> sh) - from);
-                    const bool there = (unsigned)page < (unsigned)a.c.pages;
-                    const int place = (keys ? lds_k<DP>(row0 + i * RP, slot) : lds_v<DP>(row0 + i * RP, slot)) - RB * (row0 + i * RP);     // the chunk whose place this slot is
-                    const unsigned off = (unsigned)(sub * D * 2 + (place < 2 * D ? place : 0));
-                    const char* base = (const char*)tensor + (head0 + (long long)page * page_rows + (tok & in_page)) * D * 2;
-                    const unsigned to = lds_of(lds) + first * RB;
-                    if (there && inner) to_lds(base, off, to);
-                    else to_lds(there && mine <= vhi && (mine > vlo || mine < sinks) ? (const void*)(base + off) : (const void*)&kv_zeros, to);
-                } else {
-                    const int page = __shfl(e, ((kb + row0 + i * RP) >> sh) - from);
+                for (int i = 0; i < NR; ++i) {
+                    const int tok = kb + i * RP + wave * RW;
+                    const unsigned p = (unsigned)__builtin_amdgcn_readlane(ent, (tok >> sh) - ent0);
+                    place[i] = (long long)((unsigned long long)p * page_bytes) + (unsigned)((tok & in_page) * row_bytes);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < NR; ++i) page[i] = __shfl(ent, ((kb + row0 + i * RP) >> sh) - ent0);
+            }
+            const int first = e0 - ent0, n = ((kb + KT - 1) >> sh) - e0 + 1;
+            if ((~good >> first) & ((1ull << n) - 1)) return __ballot((good >> (((kb + (lane & (KT - 1))) >> sh) - ent0)) & 1);
+            return ~0ull;
+        };
+        // Rows of one tensor of that tile on their way, to LDS (bf16) or to registers (4 bits: `stage` puts them there).  A row that no column
+        // sees is read as zeros: its probabilities are 0, but 0 times an old NaN would still be NaN.
+        auto fetch = [&](int c, unsigned long long okm, const char* base, const bf16* scales, unsigned char* lds, auto which, typename R::Raw* raw) {
+            constexpr bool keys = decltype(which)::value;
+            const int kb = span.chunk(c) * KT;
+            if constexpr (DMA) {
+                const bool inner = all && kb + KT - 1 <= vhi && (kb > vlo || kb + KT - 1 < sinks) && okm == ~0ull;
+#pragma unroll
+                for (int i = 0; i < NR; ++i) {
+                    const int first = i * RP + wave * RW;
+                    // the chunk whose place this thread's slot is
+                    const int chunk = (keys ? lds_k<DP>(row0 + i * RP, slot) : lds_v<DP>(row0 + i * RP, slot)) - RB * (row0 + i * RP);
+                    const unsigned off = (unsigned)(sub * row_bytes + (chunk < row_bytes ? chunk : 0)), to = lds_of(lds) + first * RB;
+                    if (inner) {
+                        to_lds(base + place[i], off, to);
+                    } else {
+                        const int mine = kb + first + sub;
+                        const bool ok = (okm >> first & 1) && mine <= vhi && (mine > vlo || mine < sinks);
+                        to_lds(ok ? (const void*)(base + place[i] + off) : (const void*)&kv_zeros, to);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < NR; ++i) {
+                    const int mine = kb + row0 + i * RP;
                     R::zero(raw[i]);
-                    if ((unsigned)page < (unsigned)a.c.pages && mine <= vhi && (mine > vlo || mine < sinks)) {
-                        const long long at = head0 + (long long)page * page_rows + ((kb + row0 + i * RP) & in_page);
-                        R::load(raw[i], R::base(tensor, at, D), R::steps(scales, at), 0, D, slot);
+                    if ((unsigned)page[i] < (unsigned)a.c.pages && mine <= vhi && (mine > vlo || mine < sinks)) {
+                        const long long at = head0 + (long long)page[i] * page_rows + (mine & in_page);
+                        R::load(raw[i], R::base(base, at, D), R::steps(scales, at), 0, D, slot);
                     }
                 }
             }
-            unsigned long long there = ~0ull;  // the tile's keys that have a page
-            if constexpr (keys) {
-                const int first = (kb >> sh) - from, n = ((kb + KT - 1) >> sh) - (kb >> sh) + 1;
-                if ((~good >> first) & ((1ull << n) - 1))
-                    there = __ballot((good >> (((kb + (lane & (KT - 1))) >> sh) - from)) & 1);
-            }
-            return there;
         };
         auto stage = [&](unsigned char* lds, bool keys, const typename R::Raw* raw) {
             if constexpr (!DMA) {
@@ -720,12 +738,14 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
         const Const<1> keys;
         const Const<0> values;
         if (span.total > 0) {
-            ok0 = fetch(0, a.c.k, a.c.ks, sk[0], keys, kr);
-            fetch(0, a.c.v, a.c.vs, sv[0], values, vr);
+            ok0 = find(0);
+            fetch(0, ok0, kbase, a.c.ks, sk[0], keys, kr);
+            fetch(0, ok0, vbase, a.c.vs, sv[0], values, vr);
             stage(sk[0], true, kr);
             stage(sv[0], false, vr);
             if (span.total > 1) {
-                ok1 = fetch(1, a.c.k, a.c.ks, sk[1], keys, kr);
+                ok1 = find(1);
+                fetch(1, ok1, kbase, a.c.ks, sk[1], keys, kr);
                 stage(sk[1], true, kr);
             }
             landed();
@@ -737,9 +757,12 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
             constexpr int P = decltype(which)::value;
             const int kb = span.chunk(c) * KT;
             const unsigned long long okm = ok0;
+            if (c + 1 < span.total) fetch(c + 1, ok1, vbase, a.c.vs, sv[P ^ 1], values, vr);
             ok0 = ok1;
-            if (c + 2 < span.total) ok1 = fetch(c + 2, a.c.k, a.c.ks, sk[P], keys, kr);
-            if (c + 1 < span.total) fetch(c + 1, a.c.v, a.c.vs, sv[P ^ 1], values, vr);
+            if (c + 2 < span.total) {
+                ok1 = find(c + 2);
+                fetch(c + 2, ok1, kbase, a.c.ks, sk[P], keys, kr);
+            }
             const bool whole = kb + KT - 1 <= wmin && (kb > wmax - W || kb + KT - 1 < sinks) && okm == ~0ull;
             if (!whole) {                      // key 32 u + 8 (i >> 2) + 4 hh + (i & 3), counted from kb + 32 u + 4 hh
 #pragma unroll

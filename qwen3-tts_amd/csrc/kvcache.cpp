@@ -20,6 +20,7 @@ int view(const q3c_kv* kv, KvView* c) {
     if (four && kv->head_dim != 64 && kv->head_dim != 128 && kv->head_dim != 256) return Q3C_ERR_UNSUPPORTED;
     if (four && (!kv->k_scale || !kv->v_scale || !aligned(kv->k_scale, 16) || !aligned(kv->v_scale, 16))) return Q3C_ERR_INVALID_ARGUMENT;
     if (kv->kv_heads > 65535 || (long long)kv->pages_per_row * kv->page_size > 0x40000000ll) return Q3C_ERR_UNSUPPORTED;   // grid y; int32 positions
+    if ((long long)kv->kv_heads * kv->page_size * kv->head_dim * 4 >= 0x80000000ll) return Q3C_ERR_UNSUPPORTED;            // a page of one layer
     c->dtype = kv->dtype;
     c->layers = kv->layers; c->pages = kv->pages; c->heads = kv->kv_heads; c->ps_shift = shift; c->dim = kv->head_dim;
     c->rows = kv->rows; c->width = kv->pages_per_row;
