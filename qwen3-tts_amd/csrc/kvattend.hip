@@ -680,18 +680,21 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
             const int kb = span.chunk(c) * KT;
             if constexpr (DMA) {
                 const bool inner = all && kb + KT - 1 <= vhi && (kb > vlo || kb + KT - 1 < sinks) && okm == ~0ull;
-#pragma unroll
-                for (int i = 0; i < NR; ++i) {
-                    const int first = i * RP + wave * RW;
-                    // the chunk whose place this thread's slot is
+                // the chunk whose place this thread's slot is
+                auto source = [&](int i) {
                     const int chunk = (keys ? lds_k<DP>(row0 + i * RP, slot) : lds_v<DP>(row0 + i * RP, slot)) - RB * (row0 + i * RP);
-                    const unsigned off = (unsigned)(sub * row_bytes + (chunk < row_bytes ? chunk : 0)), to = lds_of(lds) + first * RB;
-                    if (inner) {
-                        to_lds(base + place[i], off, to);
-                    } else {
-                        const int mine = kb + first + sub;
+                    return (unsigned)(sub * row_bytes + (chunk < row_bytes ? chunk : 0));
+                };
+                const unsigned to = lds_of(lds) + wave * RW * RB;
+                if (inner) {
+#pragma unroll
+                    for (int i = 0; i < NR; ++i) to_lds(base + place[i], source(i), to + i * RP * RB);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NR; ++i) {
+                        const int first = i * RP + wave * RW, mine = kb + first + sub;
                         const bool ok = (okm >> first & 1) && mine <= vhi && (mine > vlo || mine < sinks);
-                        to_lds(ok ? (const void*)(base + place[i] + off) : (const void*)&kv_zeros, to);
+                        to_lds(ok ? (const void*)(base + place[i] + source(i)) : (const void*)&kv_zeros, to + i * RP * RB);
                     }
                 }
             } else {
@@ -794,8 +797,8 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
             const float mu = m == -INFINITY ? 0.f : m;
             // The order below is the order of the instructions: each matrix product has its operands' reads of LDS a few products earlier and a share of
             // the softmax's arithmetic behind it.  (Past the last tile the scores are of whatever lies there, and not looked at.)
-            constexpr int QK = KS * NT, PV = 2 * NT * ND, NE = 16 * NT / 2, AHEAD = 4;      // products, pairs of scores
-            bf16x8 kf[AHEAD], vf[AHEAD];
+            constexpr int QK = KS * NT, PV = 2 * NT * ND, NE = 16 * NT / 2, AHEAD = DMA ? 5 : 4;      // products, pairs of scores
+            bf16x8 ring[AHEAD];
             u32x4 p[NT][2];
             auto read_k = [&](int j) { return *(const bf16x8*)(sk[P ^ 1] + 32 * (j % NT) * RB + ak[j / NT]); };
             auto read_v = [&](int j) {
@@ -815,25 +818,22 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
                 l += x + y;
                 p[u][i >> 3][(i & 7) >> 1] = pack2(x, y);
             };
+            auto read = [&](int j) { return j < QK ? read_k(j) : read_v(j - QK); };
 #pragma unroll
-            for (int j = 0; j < AHEAD; ++j) kf[j] = read_k(j);
+            for (int j = 0; j < AHEAD; ++j) ring[j] = read(j);
 #pragma unroll
             for (int u = 0; u < NT; ++u)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[P ^ 1][u][i] = 0.f;
 #pragma unroll
-            for (int j = 0; j < QK; ++j) {
-                s[P ^ 1][j % NT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[j % AHEAD], qf[j / NT], s[P ^ 1][j % NT], 0, 0, 0);
-                if (j + AHEAD < QK) kf[j % AHEAD] = read_k(j + AHEAD);
-                else vf[(j + AHEAD - QK) % AHEAD] = read_v(j + AHEAD - QK);
+            for (int j = 0; j < QK + PV; ++j) {
+                const bf16x8 x = ring[j % AHEAD];
+                if (j < QK) s[P ^ 1][j % NT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, qf[j / NT], s[P ^ 1][j % NT], 0, 0, 0);
+                else o[(j - QK) % ND] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, __builtin_bit_cast(bf16x8, p[(j - QK) / ND / 2][((j - QK) / ND) & 1]), o[(j - QK) % ND], 0, 0, 0);
+                if (j + AHEAD < QK + PV) ring[j % AHEAD] = read(j + AHEAD);
+                if (j < QK)
 #pragma unroll
-                for (int e = j * NE / QK; e < (j + 1) * NE / QK; ++e) weight(e);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-#pragma unroll
-            for (int j = 0; j < PV; ++j) {
-                o[j % ND] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[j % AHEAD], __builtin_bit_cast(bf16x8, p[j / ND / 2][(j / ND) & 1]), o[j % ND], 0, 0, 0);
-                if (j + AHEAD < PV) vf[j % AHEAD] = read_v(j + AHEAD);
+                    for (int e = j * NE / QK; e < (j + 1) * NE / QK; ++e) weight(e);
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (c + 2 < span.total) stage(sk[P], true, kr);
