@@ -110,7 +110,7 @@ template <int DP> struct Chunk<bf16, DP> {
         }
     }
     // row: element offset of this lane's key in its page tensor; dimensions past the head's size read its first ones (their q is 0)
-    __device__ __forceinline__ void load_k(int u, const void* base, long long row, int D, int g, const KvView&, long long) {
+    __device__ __forceinline__ void load_k(int u, const void* base, long long row, int D, int g, int, const KvView&, long long) {
         const bf16* p = (const bf16*)base + row * D;
 #pragma unroll
         for (int s = 0; s < NS; ++s) { const int d = 32 * s + 8 * g; k[u][s] = *(const u32x4*)(p + (d < D ? d : 0)); }
@@ -129,17 +129,21 @@ template <int DP> struct Chunk<bf16, DP> {
                 }
         }
     }
-    __device__ __forceinline__ void drop_v(int j) {
+    // keep(u, r): whether key 4 g + r of tile u counts.  An old NaN in a row that does not must not meet its probability 0.
+    template <typename Keep> __device__ __forceinline__ void hide(int, Keep keep) {
 #pragma unroll
-        for (int w = 0; w < VW; ++w) v[j][w] = 0;
+        for (int j = 0; j < 8; ++j)
+            if (!keep(j >> 2, j & 3))
+#pragma unroll
+                for (int w = 0; w < VW; ++w) v[j][w] = 0;
     }
-    __device__ __forceinline__ f32x4 scores(int u, const Q& q) const {
+    __device__ __forceinline__ f32x4 scores(int u, const Q& q, unsigned) const {
         f32x4 s = {0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < NS; ++i) s = mfma_bf16(k[u][i], q.f[i], s);
         return s;
     }
-    __device__ __forceinline__ void weigh(const float* p, f32x4* o) const {
+    __device__ __forceinline__ void weigh(const float* p, f32x4* o, unsigned) const {
         u32x4 b;
 #pragma unroll
         for (int j = 0; j < 4; ++j) b[j] = pack2(p[2 * j], p[2 * j + 1]);
@@ -167,7 +171,7 @@ template <int DP> struct Chunk<float, DP> {
             if (on && 16 * s < D) q.f[s] = *(const f32x4*)(p + 16 * s + 4 * g);
         }
     }
-    __device__ __forceinline__ void load_k(int, const void* base, long long row, int D, int g, const KvView&, long long) {
+    __device__ __forceinline__ void load_k(int, const void* base, long long row, int D, int g, int, const KvView&, long long) {
         const float* p = (const float*)base + row * D + 4 * g;
 #pragma unroll
         for (int s = 0; s < NS; ++s) k[0][s] = *(const f32x4*)(p + (16 * s < D ? 16 * s : 0));
@@ -179,11 +183,14 @@ template <int DP> struct Chunk<float, DP> {
 #pragma unroll
             for (int w = 0; w < DV / 4; ++w) v[r][w] = *(const f32x4*)(p + r * D + 4 * w);
     }
-    __device__ __forceinline__ void drop_v(int j) {
+    template <typename Keep> __device__ __forceinline__ void hide(int, Keep keep) {
 #pragma unroll
-        for (int w = 0; w < DV / 4; ++w) v[j][w] = f32x4{0, 0, 0, 0};
+        for (int j = 0; j < 4; ++j)
+            if (!keep(0, j))
+#pragma unroll
+                for (int w = 0; w < DV / 4; ++w) v[j][w] = f32x4{0, 0, 0, 0};
     }
-    __device__ __forceinline__ f32x4 scores(int, const Q& q) const {
+    __device__ __forceinline__ f32x4 scores(int, const Q& q, unsigned) const {
         f32x4 s = {0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < NS; ++i)
@@ -191,7 +198,7 @@ template <int DP> struct Chunk<float, DP> {
             for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[0][i][e], q.f[i][e], s, 0, 0, 0);
         return s;
     }
-    __device__ __forceinline__ void weigh(const float* p, f32x4* o) const {
+    __device__ __forceinline__ void weigh(const float* p, f32x4* o, unsigned) const {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -205,11 +212,21 @@ template <int DP> struct Chunk<float, DP> {
 // Values: the step goes into the probability, p step in bf16, and a second product with the constant -136 takes the offset out
 // again, chunk by chunk, from the same rounded numbers (one offset for a whole row would cancel against 136 times its sum).
 struct Int4 {};
+// v of lane `from` of this lane's row of 16 (a DPP operand of the instruction that takes it, not one of its own)
+template <int from> __device__ __forceinline__ float row_lane(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + from, 0xf, 0xf, true));
+}
+template <int N> struct Const { static constexpr int value = N; };
+template <int I, int N, typename F> __device__ __forceinline__ void each(F f) {      // f(Const<I>()) .. f(Const<N - 1>())
+    if constexpr (I < N) { f(Const<I>()); each<I + 1, N>(f); }
+}
 template <int D> struct Chunk<Int4, D> {
     static constexpr int TILES = 2, S = D / 32, DV = D / 16;        // S groups; a lane's keys: 4 S bytes, its values: S bytes a key
+    static constexpr int SW = (4 * S + 15) / 16;                    // steps of a lane group's four keys, S each, one per lane of the row
     typedef bf16 act;
     struct Q { u32x4 f[S]; float bias[S]; };
-    unsigned k[2][S], v[8][(S + 3) / 4], ks[2][2 * S], vs[2][2 * S];
+    unsigned k[2][S], v[8][(S + 3) / 4];
+    float ks[2][SW], vs[2][SW];
     static __device__ __forceinline__ void load_q(Q& q, const bf16* p, int, int g, bool on) {
 #pragma unroll
         for (int s = 0; s < S; ++s) {
@@ -235,9 +252,13 @@ template <int D> struct Chunk<Int4, D> {
                 for (int e = 0; e < 4; ++e) d[w + e] = x[e];
             }
     }
-    __device__ __forceinline__ void load_k(int u, const void* base, long long row, int, int g, const KvView& c, long long row4) {
+    static __device__ __forceinline__ void load_steps(float* d, const bf16* p, int cq) {
+#pragma unroll
+        for (int w = 0; w < SW; ++w) d[w] = (float)p[S == 2 ? cq & 7 : 16 * w + cq];
+    }
+    __device__ __forceinline__ void load_k(int u, const void* base, long long row, int, int g, int cq, const KvView& c, long long row4) {
         load_dw<S>(k[u], (const char*)base + row * (D / 2) + g * 4 * S);
-        load_dw<2 * S>(ks[u], c.ks + row4 * S);
+        load_steps(ks[u], c.ks + row4 * S, cq);
     }
     __device__ __forceinline__ void load_v(int u, const void* base, long long row, int, int m, const KvView& c) {
         const char* p = (const char*)base + row * (D / 2) + m * S;
@@ -246,51 +267,52 @@ template <int D> struct Chunk<Int4, D> {
             if constexpr (S == 2) v[4 * u + r][0] = *(const unsigned short*)(p + r * (D / 2));
             else load_dw<S / 4>(v[4 * u + r], p + r * (D / 2));
         }
-        load_dw<2 * S>(vs[u], c.vs + row * S);
+        load_steps(vs[u], c.vs + row * S, m);
     }
-    __device__ __forceinline__ void drop_v(int j) {
+    // keep(u, r): whether key 4 g + r of tile u counts.  Its step is what goes: a NaN there must not meet its probability 0.
+    template <typename Keep> __device__ __forceinline__ void hide(int cq, Keep keep) {
 #pragma unroll
-        for (int s = 0; s < S; ++s) {                               // the step of key j (a NaN there must not meet its probability 0)
-            unsigned& w = vs[j >> 2][((j & 3) * S + s) >> 1];
-            w &= ((j & 3) * S + s) & 1 ? 0x0000ffffu : 0xffff0000u;
-        }
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int w = 0; w < SW; ++w)
+                if (!keep(u, S == 2 ? (cq & 7) >> 1 : (16 * w + cq) / S)) vs[u][w] = 0.f;
     }
-    static __device__ __forceinline__ float step(const unsigned* d, int i) { return i & 1 ? hi_f(d[i >> 1]) : lo_f(d[i >> 1]); }
-    __device__ __forceinline__ f32x4 scores(int u, const Q& q) const {
+    __device__ __forceinline__ f32x4 scores(int u, const Q& q, unsigned magic) const {
         f32x4 t = {0, 0, 0, 0};
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
+        each<0, S>([&](auto si) {
+            constexpr int s = decltype(si)::value;
             u32x4 x;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {                           // bytes s of the lane's m = 4 g + 2 e and + 1
                 unsigned z;
                 if constexpr (S == 2) z = perm(0, k[u][e], 0x0c000c00u | (unsigned)(s + 2) << 16 | (unsigned)s);
                 else z = perm(k[u][(2 * e + 1) * (S / 4) + s / 4], k[u][2 * e * (S / 4) + s / 4], 0x0c000c00u | (unsigned)(s % 4 + 4) << 16 | (unsigned)(s % 4));
-                x[e] = (z & 0x000f000fu) | 0x43004300u;
-                x[e + 2] = ((z >> 4) & 0x000f000fu) | 0x43004300u;
+                x[e] = (z & 0x000f000fu) | magic;
+                x[e + 2] = ((z >> 4) & 0x000f000fu) | magic;
             }
             const f32x4 d = mfma_bf16(x, q.f[s], f32x4{q.bias[s], q.bias[s], q.bias[s], q.bias[s]});
-#pragma unroll
-            for (int r = 0; r < 4; ++r) t[r] = fmaf(step(ks[u], r * S + s), d[r], t[r]);
-        }
+            each<0, 4>([&](auto ri) {
+                constexpr int r = decltype(ri)::value, i = r * S + s;
+                t[r] = fmaf(row_lane<i % 16>(ks[u][i / 16]), d[r], t[r]);
+            });
+        });
         return t;
     }
-    __device__ __forceinline__ void weigh(const float* p, f32x4* o) const {
+    __device__ __forceinline__ void weigh(const float* p, f32x4* o, unsigned magic) const {
         const u32x4 off = {0xc308c308u, 0xc308c308u, 0xc308c308u, 0xc308c308u};       // -136
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
+        each<0, S>([&](auto si) {
+            constexpr int s = decltype(si)::value;
             u32x4 b, lo, hi;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int u = j >> 1, r = 2 * (j & 1);
-                b[j] = pack2(p[2 * j] * step(vs[u], r * S + s), p[2 * j + 1] * step(vs[u], (r + 1) * S + s));
+            each<0, 4>([&](auto ji) {
+                constexpr int j = decltype(ji)::value, u = j >> 1, i = 2 * (j & 1) * S + s, k = i + S;
+                b[j] = pack2(row_lane<i % 16>(vs[u][i / 16]) * p[2 * j], row_lane<k % 16>(vs[u][k / 16]) * p[2 * j + 1]);
                 const unsigned z = perm(v[2 * j + 1][s / 4], v[2 * j][s / 4], 0x0c000c00u | (unsigned)(s % 4 + 4) << 16 | (unsigned)(s % 4));
-                lo[j] = (z & 0x000f000fu) | 0x43004300u;
-                hi[j] = ((z >> 4) & 0x000f000fu) | 0x43004300u;
-            }
+                lo[j] = (z & 0x000f000fu) | magic;
+                hi[j] = ((z >> 4) & 0x000f000fu) | magic;
+            });
             o[2 * s] = mfma_bf16(lo, b, mfma_bf16(off, b, o[2 * s]));
             o[2 * s + 1] = mfma_bf16(hi, b, mfma_bf16(off, b, o[2 * s + 1]));
-        }
+        });
     }
     static __device__ __forceinline__ int dim(int i, int m) { return 16 * i + m; }
 };
@@ -300,7 +322,7 @@ template <int D> struct Chunk<Int4, D> {
 // unnormalised sums go to the workspace and kv_join_kernel joins them.  Bound by memory for single tokens: the next chunk's keys are
 // requested before this one's softmax, its values before this one's scores.
 template <typename T, int DP>
-__global__ void __launch_bounds__(256) kv_attend_kernel(const KvAttendArgs a) {
+__global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_attend_kernel(const KvAttendArgs a) {
     typedef Chunk<T, DP> C;
     typedef typename C::act A;
     constexpr int TB = 16 * C::TILES, NT = DP / 16, LD = DP + 4;
@@ -328,6 +350,8 @@ __global__ void __launch_bounds__(256) kv_attend_kernel(const KvAttendArgs a) {
     const int W = a.window > 0 ? a.window : 0x7fffffff, sinks = a.window > 0 ? a.sinks : 0;
 
     const float cs = a.scale_log2e;
+    unsigned magic = 0x43004300u;              // two bf16 exponents of 128, kept in a register: an and-or takes one constant
+    asm("" : "+v"(magic));
     int only = t.pmin - 1;                     // pmin - 1: all columns at once; else the one position whose columns are wanted (below)
     for (;;) {
         const bool all = only < t.pmin;
@@ -349,7 +373,7 @@ __global__ void __launch_bounds__(256) kv_attend_kernel(const KvAttendArgs a) {
         auto keys = [&](int tb) {
 #pragma unroll
             for (int u = 0; u < C::TILES; ++u)
-                ch.load_k(u, a.c.k, row_of(ek[u], tb + 16 * u + cq), D, g, a.c, row_of(ev[u], tb + 16 * u + 4 * g));
+                ch.load_k(u, a.c.k, row_of(ek[u], tb + 16 * u + cq), D, g, cq, a.c, row_of(ev[u], tb + 16 * u + 4 * g));
         };
         int c = c_begin, tb = 0;
         if (c < c_end) {
@@ -368,18 +392,16 @@ __global__ void __launch_bounds__(256) kv_attend_kernel(const KvAttendArgs a) {
             }
             const int now = tb;
             c += 4;
-            if (c < c_end) {
-                tb = span.chunk(c) * TB;
-                entries(tb);
-            }
+            tb = span.chunk(min(c, c_end - 1)) * TB;       // past the end: the last chunk again, and not looked at
+            entries(tb);
             float x[4 * C::TILES];
 #pragma unroll
             for (int u = 0; u < C::TILES; ++u) {
-                const f32x4 s = ch.scores(u, q);
+                const f32x4 s = ch.scores(u, q, magic);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) x[4 * u + r] = s[r];
             }
-            if (c < c_end) keys(tb);
+            keys(tb);
             const bool whole = now + TB - 1 <= t.pmin && (now > t.pmax - W || now + TB - 1 < sinks) && __all(pages_ok);
             if (!whole) {
 #pragma unroll
@@ -387,8 +409,11 @@ __global__ void __launch_bounds__(256) kv_attend_kernel(const KvAttendArgs a) {
                     const int tok = now + 16 * (j >> 2) + 4 * g + (j & 3);
                     const bool sees = ok[j >> 2] && tok <= mypos && (tok > mypos - W || tok < sinks);
                     x[j] = sees ? x[j] : -INFINITY;
-                    if (!(ok[j >> 2] && tok <= vhi && (tok > vlo || tok < sinks))) ch.drop_v(j);
                 }
+                ch.hide(cq, [&](int u, int r) {
+                    const int tok = now + 16 * u + 4 * g + r;
+                    return ok[u] && tok <= vhi && (tok > vlo || tok < sinks);
+                });
             }
             float top = x[0];
 #pragma unroll
@@ -408,7 +433,7 @@ __global__ void __launch_bounds__(256) kv_attend_kernel(const KvAttendArgs a) {
                 x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], cs, -mu));
                 l += x[j];
             }
-            ch.weigh(x, o);
+            ch.weigh(x, o, magic);
         }
         l += __shfl_xor(l, 16);
         l += __shfl_xor(l, 32);
@@ -560,7 +585,6 @@ __device__ __forceinline__ float max_halves(float x) {           // over lanes l
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-template <int N> struct Const { static constexpr int value = N; };
 
 typedef __attribute__((address_space(3))) void lds_void;
 __device__ const u32x4 kv_zeros = {0, 0, 0, 0};                 // what a row that nobody sees is read from
