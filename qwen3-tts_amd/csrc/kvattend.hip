@@ -317,9 +317,22 @@ template <int D> struct Chunk<Int4, D> {
     static __device__ __forceinline__ int dim(int i, int m) { return 16 * i + m; }
 };
 
-// One workgroup = one tile of columns, one kv head, one of `splits` equal shares of the chunks the tile sees; its four waves take the
-// share's chunks in turn, each with a running maximum and sum of its own, and are joined through LDS at the end.  With splits > 1 the
-// unnormalised sums go to the workspace and kv_join_kernel joins them.  Bound by memory for single tokens: the next chunk's keys are
+// The workspace: for each (tile, kv head) the sums [splits][16][DP], then maxima and weights [splits][16][2], then how many shares it has.
+struct KvShares {
+    float *sums, *ml;
+    int* used;
+    __device__ __forceinline__ KvShares(const KvAttendArgs& a, int tiles, int dp, int tile, int hk) {
+        const long long n = (long long)tiles * a.c.heads, i = (long long)tile * a.c.heads + hk, rows = (long long)a.splits * 16;
+        sums = a.ws + i * rows * dp;
+        ml = a.ws + n * rows * dp + i * rows * 2;
+        used = (int*)(a.ws + n * rows * (dp + 2)) + i;
+    }
+};
+
+// One workgroup = one tile of columns, one kv head, one share (`share` chunks) of those the tile sees: shares of one size, so that long and
+// short rows fill the card alike.  Its four waves take the share's chunks in turn, each with a running maximum and sum of its own, and
+// are joined through LDS at the end.  Where a tile has more than one share the unnormalised sums go to the workspace and
+// kv_join_kernel joins them.  Bound by memory for single tokens: the next chunk's keys are
 // requested before this one's softmax, its values before this one's scores.
 template <typename T, int DP>
 __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_attend_kernel(const KvAttendArgs a) {
@@ -337,12 +350,13 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_attend_kernel(const
     const bool col_on = col < t.ncols;
     int mypos = col_on && t.row >= 0 ? t.first_pos + qtok : -1;
     if (mypos > t.pmax) mypos = -1;
+    const Span span = kv_span(a, t, TB);
+    if (blockIdx.z > 0 && (int)blockIdx.z * a.share >= span.total) return;
+    const bool shared = a.splits > 1 && span.total > a.share;
+    const int c_begin = (int)blockIdx.z * a.share + wave, c_end = shared && (int)blockIdx.z + 1 < a.splits ? min(span.total, ((int)blockIdx.z + 1) * a.share) : span.total;
     typename C::Q q;
     C::load_q(q, (const A*)a.q.p + (long long)(t.tok0 + qtok) * a.q.ts + (long long)(hk * G + col - qtok * G) * a.q.hs, D, g, mypos >= 0);
 
-    const Span span = kv_span(a, t, TB);
-    const int per = (span.total + a.splits - 1) / a.splits;
-    const int c_end = min(span.total, (int)(blockIdx.z + 1) * per), c_begin = (int)blockIdx.z * per + wave;
     const int* table = a.c.table + (long long)max(t.row, 0) * a.c.width;
     const long long page_rows = (long long)a.c.heads << sh;                    // rows of one page, all heads
     const long long head0 = ((long long)a.layer * a.c.pages * a.c.heads + hk) << sh;
@@ -478,13 +492,15 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_attend_kernel(const
         for (int w = 0; w < 4; ++w) r[i] += *(const f32x4*)&so[w][c][d0 + 4 * i] * f[w];
     }
     if (a.splits > 1) {
-        float* ws = a.ws + (((long long)blockIdx.x * gridDim.y + hk) * a.splits + blockIdx.z) * (16 * (DP + 2)) + c * (DP + 2);
+        const KvShares ws(a, gridDim.x, DP, blockIdx.x, hk);
+        if (blockIdx.z == 0 && tid == 0) *ws.used = shared ? min(a.splits, (span.total + a.share - 1) / a.share) : 1;
+        if (shared) {
+            float* o = ws.sums + ((long long)blockIdx.z * 16 + c) * DP + d0;
 #pragma unroll
-        for (int i = 0; i < DP / 64; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) ws[2 + d0 + 4 * i + e] = r[i][e];
-        if (d0 == 0) { ws[0] = mx; ws[1] = l; }
-        return;
+            for (int i = 0; i < DP / 64; ++i) *(f32x4*)(o + 4 * i) = r[i];
+            if (d0 == 0) { ws.ml[2 * (blockIdx.z * 16 + c)] = mx; ws.ml[2 * (blockIdx.z * 16 + c) + 1] = l; }
+            return;
+        }
     }
     const int tk = (t.col0 + c) / G, h = hk * G + t.col0 + c - tk * G;
     const bool none = l == 0.f;
@@ -496,35 +512,44 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_attend_kernel(const
         for (int e = 0; e < 4; ++e) out[4 * i + e] = (A)(none ? 0.f : r[i][e] * inv);
 }
 
-// out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the shares of one tile and head
+// out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the shares s of one tile and head.  Sixteen lanes have a column: each first looks
+// at every sixteenth share's maximum and sum, then sums its dimensions of all.
 template <typename A, int DP>
 __global__ void __launch_bounds__(256) kv_join_kernel(const KvAttendArgs a) {
-    const int tid = threadIdx.x;
+    constexpr int N = DP / 16;
+    const int tid = threadIdx.x, hk = blockIdx.y, G = a.group, D = a.c.dim, c = tid >> 4, j = tid & 15, d0 = j * N;
+    const KvShares ws(a, gridDim.x, DP, blockIdx.x, hk);
     const Tile t = kv_tile(a, blockIdx.x, 16, tid & 63);
     if (!t.on) return;
-    const int hk = blockIdx.y, G = a.group, D = a.c.dim, c = tid >> 4, d0 = (tid & 15) * (DP / 16);
-    if (t.col0 + c >= t.ncols || d0 >= D) return;
-    const float* ws = a.ws + ((long long)blockIdx.x * gridDim.y + hk) * a.splits * (16 * (DP + 2)) + c * (DP + 2);
-    float mx = -INFINITY, l = 0.f;
-    for (int s = 0; s < a.splits; ++s) mx = fmaxf(mx, ws[(long long)s * (16 * (DP + 2))]);
-    const float mu = mx == -INFINITY ? 0.f : mx;
-    float r[DP / 16];
+    const int used = *ws.used;
+    if (used < 2 || t.col0 + (c & ~3) >= t.ncols) return;       // whole waves
+    float m = -INFINITY;
+    for (int s = j; s < used; s += 16) m = fmaxf(m, ws.ml[2 * (s * 16 + c)]);
 #pragma unroll
-    for (int e = 0; e < DP / 16; ++e) r[e] = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-        const float* w = ws + (long long)s * (16 * (DP + 2));
-        const float ls = w[1], f = __builtin_amdgcn_exp2f(w[0] - mu);
-        if (ls == 0.f) continue;
+    for (int k = 1; k < 16; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
+    const float mu = m == -INFINITY ? 0.f : m;
+    float r[N], l = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) r[e] = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < used; ++s) {
+        const float f = __builtin_amdgcn_exp2f(ws.ml[2 * (s * 16 + c)] - mu), ls = ws.ml[2 * (s * 16 + c) + 1];
+        const float* o = ws.sums + ((long long)s * 16 + c) * DP + d0;
         l = fmaf(ls, f, l);
 #pragma unroll
-        for (int e = 0; e < DP / 16; ++e) r[e] = fmaf(w[2 + d0 + e], f, r[e]);
+        for (int e = 0; e < N; e += 4) {
+            const f32x4 x = *(const f32x4*)(o + e);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) r[e + w] = fmaf(x[w], f, r[e + w]);
+        }
     }
+    if (t.col0 + c >= t.ncols || d0 >= D) return;
     const int tk = (t.col0 + c) / G, h = hk * G + t.col0 + c - tk * G;
     const bool none = l == 0.f;
     const float inv = 1.0f / l;
     A* out = (A*)a.out + ((long long)(t.tok0 + tk) * a.q_heads + h) * D + d0;
 #pragma unroll
-    for (int e = 0; e < DP / 16; ++e) out[e] = (A)(none ? 0.f : r[e] * inv);
+    for (int e = 0; e < N; ++e) out[e] = (A)(none ? 0.f : r[e] * inv);
 }
 
 // ---- prompts -----------------------------------------------------------------------------------------------------------------------------
@@ -913,24 +938,29 @@ bool prompts(const KvView& c, int tokens, int sequences, int q_heads, bool ragge
 
 }  // namespace
 
-// How many shares a tile's keys are cut into: as many workgroups as keep 256 compute units busy, each with at least 8 chunks' work
-// (two rounds of its four waves).
-int q3_kv_attend_splits(const KvView& c, int tokens, int sequences, int q_heads, int window, int sinks, int max_len) {
+// How a tile's keys are cut: shares of as many chunks as make about 2048 workgroups of the longest rows there can be (eight per compute
+// unit: short ones then even out what is left), of at least 16 chunks (four rounds of a workgroup's waves), and no more than 256.
+KvSplit q3_kv_attend_split(const KvView& c, int tokens, int sequences, int q_heads, int window, int sinks, int max_len) {
     const int group = q_heads / c.heads, tb = c.dtype == Q3C_KV_F32 ? 16 : 32;
     long long len = (long long)c.width << c.ps_shift;
     if (max_len > 0 && max_len < len) len = max_len;
     if (window > 0 && (long long)window + sinks + tb < len) len = (long long)window + sinks + tb;
     const long long chunks = len / tb + 1, base = (tokens == sequences ? (long long)sequences * ((group + 15) / 16) : (long long)tokens * group / 16 + 1) * c.heads;
-    long long n = (1024 + base - 1) / (base ? base : 1);
-    if (n > (chunks + 7) / 8) n = (chunks + 7) / 8;
-    return (int)(n < 1 ? 1 : n > 128 ? 128 : n);
+    long long share = (chunks * base + 2047) / 2048;
+    if (share < 16) share = 16;
+    if (share < (chunks + 255) / 256) share = (chunks + 255) / 256;
+    share = (share + 3) / 4 * 4;
+    KvSplit s;
+    s.splits = base >= 2048 ? 1 : (int)((chunks + share - 1) / share);
+    s.share = s.splits == 1 ? 0x7fffffff : (int)share;
+    return s;
 }
 size_t q3_kv_attend_ws(const KvView& c, int tokens, int sequences, int q_heads, int splits) {
     if (splits < 2) return 0;
     const int group = q_heads / c.heads;
     const long long tiles = tiles_of(tokens, sequences, group, true);
     const long long flat = tiles_of(tokens, sequences, group, false);
-    return (size_t)((tiles > flat ? tiles : flat) * c.heads * splits) * (16 * (padded_dim(c.dim) + 2)) * sizeof(float);
+    return (size_t)((tiles > flat ? tiles : flat) * c.heads) * ((size_t)splits * 16 * (padded_dim(c.dim) + 2) + 1) * sizeof(float);
 }
 
 hipError_t q3_launch_kv_attend(const KvAttendArgs& a, hipStream_t s) {

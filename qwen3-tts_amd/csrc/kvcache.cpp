@@ -107,7 +107,7 @@ int q3c_kv_attend_workspace_bytes(const q3c_kv* kv, int32_t q_heads, int32_t seq
     if (!bytes) return Q3C_ERR_INVALID_ARGUMENT;
     const int rc = attend_shape(kv, q_heads, sequences, tokens, window, sinks, max_len, &c);
     if (rc) return rc;
-    *bytes = q3_kv_attend_ws(c, tokens, sequences, q_heads, q3_kv_attend_splits(c, tokens, sequences, q_heads, window, sinks, max_len));
+    *bytes = q3_kv_attend_ws(c, tokens, sequences, q_heads, q3_kv_attend_split(c, tokens, sequences, q_heads, window, sinks, max_len).splits);
     return 0;
 }
 
@@ -120,7 +120,9 @@ int q3c_kv_attend(const q3c_kv* kv, int32_t layer, const void* q, int64_t q_ts, 
     if (layer < 0 || layer >= a.c.layers || !(scale > 0.f) || !(scale < 3e38f)) return Q3C_ERR_INVALID_ARGUMENT;
     if (!tokens) return 0;
     if (!strided(q, q_ts, q_hs, act_bytes(a.c)) || !out || !aligned(out, 16)) return Q3C_ERR_INVALID_ARGUMENT;
-    a.splits = q3_kv_attend_splits(a.c, tokens, sequences, q_heads, window, sinks, max_len);
+    const KvSplit cut = q3_kv_attend_split(a.c, tokens, sequences, q_heads, window, sinks, max_len);
+    a.splits = cut.splits;
+    a.share = cut.share;
     const size_t need = q3_kv_attend_ws(a.c, tokens, sequences, q_heads, a.splits);
     if (need && (!workspace || !aligned(workspace, 16))) return Q3C_ERR_INVALID_ARGUMENT;
     if (workspace_bytes < need) return Q3C_ERR_WORKSPACE;

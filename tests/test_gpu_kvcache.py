@@ -89,6 +89,24 @@ def _check_attend(got, want, mag, dot, kv, N, scale, q=None, prompt=False):
     assert bool((off <= bound + 1e-30).all()), f"max excess {float((off - bound).max()):.3e}, max error {float(off.max()):.3e}"
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32", "int4"])
+def test_attend_cuts_rows_of_any_length(dtype):
+    """Long rows are cut into shares that a second kernel joins; how long rows can be is known from the table or said by max_len, which
+    only steers that: a bound that is too low changes nothing.  Rows of one share, of several, and the last one ragged."""
+    g = _gen(23)
+    G, group, D, ps, lens = 1, 2, 64, 32, [40, 5000, 2048, 513, 9001]
+    kv = _cache(dtype, G, D, ps, lens)
+    store = _fill(kv, 0, lens, g)
+    q = _randn(g, 5, G * group, D).mul_(2).to(kv.activations)
+    rows = torch.arange(5, dtype=torch.int32, device=DEV)
+    for window, sinks in ((0, 0), (4000, 40), (10, 3000)):
+        for max_len in (0, 100, 2000, 9001):
+            out = kv.attend(0, q, rows, window=window, sinks=sinks, max_len=max_len)
+            for r, L in enumerate(lens):
+                want, mag, dot = attention(q[r:r + 1], *store[r], [L - 1], window, sinks, D ** -0.5)
+                _check_attend(out[r:r + 1], want, mag, dot, kv, L, D ** -0.5, q[r:r + 1].double())
+
+
 # ---- append ----------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype,D,rot,G,H,ps,norm", [
     ("bf16", 128, 128, 8, 16, 32, True), ("bf16", 128, 64, 2, 14, 8, True), ("bf16", 64, 64, 16, 16, 16, False),
