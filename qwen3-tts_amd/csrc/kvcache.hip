@@ -8,25 +8,11 @@
 
 namespace {
 
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+template <typename T, int N> using Vec = T __attribute__((ext_vector_type(N)));      // N elements as they lie in memory
+template <int N> using Floats = float __attribute__((ext_vector_type(N)));
 
-template <typename T> struct Quad;
-template <> struct Quad<float> { typedef f32x4 type; };
-template <> struct Quad<bf16> { typedef bf16x4 type; };
-
-template <typename T> __device__ __forceinline__ f32x4 kv_load4(const T* p) {
-    const typename Quad<T>::type v = *(const typename Quad<T>::type*)p;
-    f32x4 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = (float)v[i];
-    return r;
-}
-template <typename T> __device__ __forceinline__ void kv_store4(T* p, f32x4 v) {
-    typename Quad<T>::type r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = (T)v[i];
-    *(typename Quad<T>::type*)p = r;
-}
+template <int N, typename T> __device__ __forceinline__ Vec<T, N> kv_load(const T* p) { return *(const Vec<T, N>*)p; }
+template <int N, typename T> __device__ __forceinline__ void kv_store(T* p, Floats<N> v) { *(Vec<T, N>*)p = __builtin_convertvector(v, Vec<T, N>); }
 
 __device__ __forceinline__ void kv_flag(const KvView& c, int bits) { atomicOr(c.status, bits); }
 
@@ -42,53 +28,103 @@ __device__ __forceinline__ int kv_page(const KvView& c, int row, int pos) {
     return (unsigned)p < (unsigned)c.pages ? p : -1;
 }
 
+// Where token `tok` goes: its position and page (-1: none).  false: nothing is to be done for it - it lies behind the last request, or has no
+// valid row or position; then its queries are zeros.
+__device__ __forceinline__ bool kv_place(const KvAppendArgs& a, int tok, bool first, int lane, int& pos, int& page, bool& zero) {
+    int seq, row;
+    zero = false;
+    pos = kv_position(a.c, a.b, tok, lane, seq, row);
+    if (pos < 0) {
+        zero = pos != -1;
+        if (zero && lane == 0 && first) kv_flag(a.c, Q3C_KV_BAD_ROW);
+        return false;
+    }
+    page = kv_page(a.c, row, pos);
+    if (page < 0 && lane == 0 && first) kv_flag(a.c, Q3C_KV_NO_PAGE);
+    if (kv_repeated(a.b.rows, seq, row, lane)) {
+        if (lane == 0 && first) kv_flag(a.c, Q3C_KV_BAD_ROW);
+        page = -1;
+    }
+    return true;
+}
+
 // ---- append -----------------------------------------------------------------------------------------------------------------------
 // y = x * rsqrt(mean(x^2) + eps) * w over a head's dimensions, then its first `rot` dimensions turned by the position's angle:
 // (a, b) = (y_i, y_(i + rot/2)) -> (a cos - b sin, b cos + a sin); sums and products in fp32, one rounding at the store.  The keys
 // and the (unchanged) values go straight to their page.  Bound by memory: 2 reads and writes of each element.
-// One wave = one token and a run of its heads, 8 dimensions per lane as two runs of 4 that are each other's rotation partners, so that
-// the rotation needs no exchange between lanes and the norm one butterfly over the head's lanes.
-template <typename T>
-__device__ __forceinline__ void append_plain(const KvAppendArgs& a, int tok, int unit0, int units, int lane, int lpu_shift, int pos, int row,
-                                             int page, bool store) {
-    const int D = a.c.dim, R = a.rot, lpu = 1 << lpu_shift;
-    const int u = unit0 + (lane >> lpu_shift), ch = lane & (lpu - 1);
-    if (u >= units) return;
-    const int H = a.q_heads, G = a.c.heads;
-    const bool on = 8 * ch < D, turn = 8 * ch < R && u < H + G;
-    const int d0 = turn ? 4 * ch : 8 * ch, d1 = turn ? R / 2 + 4 * ch : 8 * ch + 4;
-    const KvStrided& src = u < H ? a.q : u < H + G ? a.k : a.v;
-    const int h = u < H ? u : u < H + G ? u - H : u - H - G;
-    const T* x = (const T*)src.p + tok * src.ts + h * src.hs;
-    f32x4 lo = {0, 0, 0, 0}, hi = lo;
-    if (on) { lo = kv_load4(x + d0); hi = kv_load4(x + d1); }
-    const float* w = u < H ? a.qw : u < H + G ? a.kw : nullptr;
-    if (u < H + G && (u < H ? a.qw : a.kw)) {
-        float ss = 0.f;
+// A wave has one token and `parts`-th of its heads, VEC pairs per lane as two runs that are each other's rotation partners, so that the
+// rotation needs no exchange between lanes and the norm one butterfly over the head's lanes.  Four runs of heads are requested before
+// the token's place is looked up (offset -> row -> length -> page, four dependent reads): they are what a wave has to wait for once.
+template <typename T, int VEC, bool CACHED>     // CACHED: keys and values go to the pages here too (no 4-bit cache)
+__device__ __forceinline__ void append_plain(const KvAppendArgs& a, int tok, int part, int parts, int lane, int lpu_shift) {
+    constexpr int RUN = 4;
+    const int D = a.c.dim, R = a.rot, H = a.q_heads, G = a.c.heads, units = CACHED ? H + 2 * G : H;
+    const int lpu = 1 << lpu_shift, upw = 64 >> lpu_shift, ch = lane & (lpu - 1);
+    const bool on = 2 * VEC * ch < D, in_turn = 2 * VEC * ch < R;
+    int pos = 0, page = -1;
+    for (int u0 = part * upw + (lane >> lpu_shift); u0 - (lane >> lpu_shift) < units; u0 += RUN * parts * upw) {
+        Vec<T, VEC> x0[RUN], x1[RUN];
+        int d0[RUN], d1[RUN], h[RUN], kind[RUN];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ss = fmaf(lo[i], lo[i], fmaf(hi[i], hi[i], ss));
-        for (int m = 1; m < lpu; m <<= 1) ss += __shfl_xor(ss, m);
-        const float r = 1.0f / sqrtf(ss / (float)D + a.eps);
-        if (on) {
-            lo = lo * r * *(const f32x4*)(w + d0);
-            hi = hi * r * *(const f32x4*)(w + d1);
+        for (int i = 0; i < RUN; ++i) {
+            const int u = u0 + i * parts * upw;
+            kind[i] = u >= units || !on ? 3 : u < H ? 0 : u < H + G ? 1 : 2;
+            h[i] = u - (kind[i] == 0 ? 0 : kind[i] == 1 ? H : H + G);
+            const bool turn = in_turn && kind[i] < 2;
+            d0[i] = turn ? VEC * ch : 2 * VEC * ch;
+            d1[i] = turn ? R / 2 + VEC * ch : 2 * VEC * ch + VEC;
+            if (kind[i] < 3) {
+                const KvStrided& src = kind[i] == 0 ? a.q : kind[i] == 1 ? a.k : a.v;
+                const T* x = (const T*)src.p + tok * src.ts + h[i] * src.hs;
+                x0[i] = kv_load<VEC>(x + d0[i]);
+                x1[i] = kv_load<VEC>(x + d1[i]);
+            } else {
+                x0[i] = x1[i] = (T)0.f;
+            }
+        }
+        if (u0 - (lane >> lpu_shift) == part * upw) {           // the first time round
+            bool zero;
+            if (!kv_place(a, tok, part == 0, lane, pos, page, zero)) {
+                T* q = (T*)a.q_out + (long long)tok * H * D;
+                if (zero)
+                    for (int i = part * 64 + lane; i < H * D; i += parts * 64) q[i] = (T)0.f;
+                return;
+            }
+        }
+        Floats<VEC> co, si;
+        if (in_turn) {
+            co = *(const Floats<VEC>*)(a.cos_t + (long long)pos * (R / 2) + VEC * ch);
+            si = *(const Floats<VEC>*)(a.sin_t + (long long)pos * (R / 2) + VEC * ch);
+        }
+#pragma unroll
+        for (int i = 0; i < RUN; ++i) {
+            if (u0 - (lane >> lpu_shift) + i * parts * upw >= units) break;
+            Floats<VEC> lo = __builtin_convertvector(x0[i], Floats<VEC>), hi = __builtin_convertvector(x1[i], Floats<VEC>);
+            const float* w = kind[i] == 0 ? a.qw : kind[i] == 1 ? a.kw : nullptr;
+            if (a.qw || a.kw) {
+                float ss = 0.f;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) ss = fmaf(lo[e], lo[e], fmaf(hi[e], hi[e], ss));
+                for (int m = 1; m < lpu; m <<= 1) ss += __shfl_xor(ss, m);
+                const float r = 1.0f / sqrtf(ss / (float)D + a.eps);
+                if (w) {
+                    lo = lo * r * *(const Floats<VEC>*)(w + d0[i]);
+                    hi = hi * r * *(const Floats<VEC>*)(w + d1[i]);
+                }
+            }
+            if (in_turn && kind[i] < 2) {
+                const Floats<VEC> y0 = lo, y1 = hi;
+                lo = y0 * co - y1 * si;
+                hi = y1 * co + y0 * si;
+            }
+            T* y = nullptr;
+            if (kind[i] == 0) y = (T*)a.q_out + ((long long)tok * H + h[i]) * D;
+            else if (kind[i] < 3 && page >= 0)
+                y = (T*)(kind[i] == 1 ? a.c.k : a.c.v) +
+                    (((((long long)a.layer * a.c.pages + page) * G + h[i]) << a.c.ps_shift) + (pos & ((1 << a.c.ps_shift) - 1))) * D;
+            if (y) { kv_store<VEC, T>(y + d0[i], lo); kv_store<VEC, T>(y + d1[i], hi); }
         }
     }
-    if (turn) {
-        const f32x4 co = *(const f32x4*)(a.cos_t + (long long)pos * (R / 2) + 4 * ch), si = *(const f32x4*)(a.sin_t + (long long)pos * (R / 2) + 4 * ch);
-        const f32x4 x0 = lo, x1 = hi;
-        lo = x0 * co - x1 * si;
-        hi = x1 * co + x0 * si;
-    }
-    T* y;
-    if (u < H) {
-        y = (T*)a.q_out + ((long long)tok * H + h) * D;
-    } else {
-        if (!store) return;
-        y = (T*)(u < H + G ? a.c.k : a.c.v) +
-            (((((long long)a.layer * a.c.pages + page) * G + h) << a.c.ps_shift) + (pos & ((1 << a.c.ps_shift) - 1))) * D;
-    }
-    if (on) { kv_store4(y + d0, lo); kv_store4(y + d1, hi); }
 }
 
 // A 4-bit row: groups of 32 dimensions share step = bf16(absmax / 7); value n = rint(x / step) in -7 .. 7 is held as n + 8.  Byte
@@ -96,17 +132,22 @@ __device__ __forceinline__ void append_plain(const KvAppendArgs& a, int tok, int
 // owns whole bytes and, dim / 2 being a multiple of 16, both partners of its rotations.  The group maximum is taken on the bits of
 // |x| (integers order like the floats, NaN above infinity), so a group that holds either reads back as NaN throughout.
 template <int D>
-__device__ __forceinline__ void append_int4(const KvAppendArgs& a, int tok, int unit0, int lane, int pos, int page) {
+__device__ __forceinline__ void append_int4(const KvAppendArgs& a, int tok, int unit0, int lane) {
     constexpr int N = D / 16, S = D / 32;
-    const int G = a.c.heads, u = unit0 + (lane >> 4), m = lane & 15;
-    if (u >= 2 * G) return;
-    const bool key = u < G;
+    const int G = a.c.heads, m = lane & 15, u = min(unit0 + (lane >> 4), 2 * G - 1);
+    const bool key = u < G, twin = unit0 + (lane >> 4) != u;         // twin: past the last head, a copy of it that stores nothing
     const int h = key ? u : u - G;
     const KvStrided& src = key ? a.k : a.v;
     const bf16* xp = (const bf16*)src.p + tok * src.ts + h * src.hs + m;
+    bf16 raw[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) raw[i] = xp[16 * i];
+    int pos, page;
+    bool zero;
+    if (!kv_place(a, tok, false, lane, pos, page, zero) || page < 0) return;
     float x[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = (float)xp[16 * i];
+    for (int i = 0; i < N; ++i) x[i] = (float)raw[i];
     if (key && a.kw) {
         float ss = 0.f;
 #pragma unroll
@@ -127,7 +168,6 @@ __device__ __forceinline__ void append_int4(const KvAppendArgs& a, int tok, int 
             x[i + N / 2] = q * c + p * s;
         }
     }
-    if (page < 0) return;
     const long long at = ((((long long)a.layer * a.c.pages + page) * G + h) << a.c.ps_shift) + (pos & ((1 << a.c.ps_shift) - 1));
     unsigned char* out = (unsigned char*)(key ? a.c.k : a.c.v) + at * (D / 2) + m * S;
     unsigned short* steps = (unsigned short*)(key ? a.c.ks : a.c.vs) + at * S;
@@ -145,38 +185,23 @@ __device__ __forceinline__ void append_int4(const KvAppendArgs& a, int tok, int 
             byte = (unsigned)(n0 + 8) | (unsigned)(n1 + 8) << 4;
         }
         bytes |= (unsigned long long)byte << (8 * s);
-        if (m == s) steps[s] = __builtin_bit_cast(unsigned short, st);
+        if (m == s && !twin) steps[s] = __builtin_bit_cast(unsigned short, st);
     }
+    if (twin) return;
     if (S == 2) *(unsigned short*)out = (unsigned short)bytes;
     else if (S == 4) *(unsigned*)out = (unsigned)bytes;
     else *(unsigned long long*)out = bytes;
 }
 
-template <typename T, int D4>      // D4: 0 = cache in T, else head size of a 4-bit cache
-__global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs a, int waves_q, int waves, int lpu_shift) {
+// `parts` waves have a token's heads (D4: its query heads; then one wave for each four of its key and value heads)
+template <typename T, int VEC, int D4>      // D4: 0 = cache in T, else head size of a 4-bit cache
+__global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs a, int parts, int waves, int lpu_shift) {
     const int lane = threadIdx.x & 63;
     const long long w = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tok = (int)(w / waves), part = (int)(w - (long long)tok * waves);
     if (tok >= a.b.tokens) return;
-    int seq, row;
-    const int pos = kv_position(a.c, a.b, tok, lane, seq, row);
-    if (pos == -1) return;                                      // behind the last request
-    const int upw = 64 >> lpu_shift;
-    if (pos < 0) {                                              // nothing to write; the queries read as zeros
-        if (lane == 0 && part == 0) kv_flag(a.c, Q3C_KV_BAD_ROW);
-        T* q = (T*)a.q_out + (long long)tok * a.q_heads * a.c.dim;
-        for (int i = part * 64 + lane; i < a.q_heads * a.c.dim; i += waves * 64) q[i] = (T)0.f;
-        return;
-    }
-    int page = kv_page(a.c, row, pos);
-    if (page < 0 && lane == 0 && part == 0) kv_flag(a.c, Q3C_KV_NO_PAGE);
-    if (kv_repeated(a.b.rows, seq, row, lane)) {
-        if (lane == 0 && part == 0) kv_flag(a.c, Q3C_KV_BAD_ROW);
-        page = -1;
-    }
-    if (D4 == 0) append_plain<T>(a, tok, part * upw, a.q_heads + 2 * a.c.heads, lane, lpu_shift, pos, row, page, page >= 0);
-    else if (part < waves_q) append_plain<T>(a, tok, part * upw, a.q_heads, lane, lpu_shift, pos, row, page, false);
-    else append_int4<D4 ? D4 : 64>(a, tok, (part - waves_q) * 4, lane, pos, page);
+    if (D4 == 0 || part < parts) append_plain<T, VEC, D4 == 0>(a, tok, part, parts, lane, lpu_shift);
+    else append_int4<D4 ? D4 : 64>(a, tok, (part - parts) * 4, lane);
 }
 
 // ---- gather: the stored keys and values of the same tokens, back in one piece (zeros where there is no page) -------------------------
@@ -197,13 +222,13 @@ __global__ void __launch_bounds__(256) kv_gather_kernel(const KvView c, const Kv
     const bool key = u < c.heads;
     const int h = key ? u : u - c.heads;
     O* out = (key ? k_out : v_out) + ((long long)tok * c.heads + h) * c.dim + 8 * ch;
-    f32x4 lo = {0, 0, 0, 0}, hi = lo;
+    Floats<4> lo = {0, 0, 0, 0}, hi = lo;
     if (page >= 0) {
         const long long at = ((((long long)layer * c.pages + page) * c.heads + h) << c.ps_shift) + (pos & ((1 << c.ps_shift) - 1));
         if (D4 == 0) {
             const T* x = (const T*)(key ? c.k : c.v) + at * c.dim + 8 * ch;
-            lo = kv_load4(x);
-            hi = kv_load4(x + 4);
+            lo = __builtin_convertvector(kv_load<4>(x), Floats<4>);
+            hi = __builtin_convertvector(kv_load<4>(x + 4), Floats<4>);
         } else {                                               // dimensions 8 ch .. + 7: one half of eight neighbouring m's bytes
             const int S = c.dim / 32, s = ch >> 2;
             const unsigned char* x = (const unsigned char*)(key ? c.k : c.v) + at * (c.dim / 2) + (ch & 1) * 8 * S + s;
@@ -215,8 +240,8 @@ __global__ void __launch_bounds__(256) kv_gather_kernel(const KvView c, const Kv
             }
         }
     }
-    kv_store4(out, lo);
-    kv_store4(out + 4, hi);
+    kv_store<4, O>(out, lo);
+    kv_store<4, O>(out + 4, hi);
 }
 
 // ---- pages ----------------------------------------------------------------------------------------------------------------------------
@@ -551,25 +576,36 @@ __global__ void __launch_bounds__(256) kv_compact_kernel(const KvView c, const K
     }
 }
 
-int lanes_shift(int dim) {            // lanes of one head, 8 dimensions each, rounded up to a power of two
+int lanes_shift(int dim, int per_lane = 8) {            // lanes of one head, rounded up to a power of two
     int s = 1;
-    while ((8 << s) < dim) ++s;
+    while ((per_lane << s) < dim) ++s;
     return s;
 }
 
 }  // namespace
 
 hipError_t q3_launch_kv_append(const KvAppendArgs& a, hipStream_t s) {
-    const int sh = lanes_shift(a.c.dim), upw = 64 >> sh, d4 = a.c.dtype == Q3C_KV_INT4 ? a.c.dim : 0;
-    const int wq = (a.q_heads + upw - 1) / upw;
-    const int waves = d4 ? wq + (2 * a.c.heads + 3) / 4 : (a.q_heads + 2 * a.c.heads + upw - 1) / upw;
+    const int d4 = a.c.dtype == Q3C_KV_INT4 ? a.c.dim : 0, units = a.q_heads + (d4 ? 0 : 2 * a.c.heads);
+    // bf16: 16-byte accesses (runs of 8) where heads, halves and strides allow it, else 8-byte ones
+    const auto wide = [](const KvStrided& x) { return x.ts % 8 == 0 && x.hs % 8 == 0 && (uintptr_t)x.p % 16 == 0; };
+    const bool v8 = a.c.dtype != Q3C_KV_F32 && a.rot % 16 == 0 && wide(a.q) && (d4 || (wide(a.k) && wide(a.v)));
+    const int sh = lanes_shift(a.c.dim, v8 ? 16 : 8), upw = 64 >> sh, runs = (units + upw - 1) / upw;
+    int parts = runs;                       // waves of a token: few tokens are spread, many keep four runs of heads in flight per wave
+    while (parts > 1 && (long long)a.b.tokens * parts > 4096 && (runs + parts - 1) / parts < 4) parts = (parts + 1) / 2;
+    const int waves = parts + (d4 ? (2 * a.c.heads + 3) / 4 : 0);
     const unsigned blocks = (unsigned)(((long long)a.b.tokens * waves + 3) / 4);
     if (!blocks) return hipSuccess;
-    if (a.c.dtype == Q3C_KV_F32) kv_append_kernel<float, 0><<<blocks, 256, 0, s>>>(a, wq, waves, sh);
-    else if (!d4) kv_append_kernel<bf16, 0><<<blocks, 256, 0, s>>>(a, wq, waves, sh);
-    else if (d4 == 64) kv_append_kernel<bf16, 64><<<blocks, 256, 0, s>>>(a, wq, waves, sh);
-    else if (d4 == 128) kv_append_kernel<bf16, 128><<<blocks, 256, 0, s>>>(a, wq, waves, sh);
-    else kv_append_kernel<bf16, 256><<<blocks, 256, 0, s>>>(a, wq, waves, sh);
+#define Q3_APPEND(T, D4)                                                                    \
+    do {                                                                                    \
+        if (v8) kv_append_kernel<T, 8, D4><<<blocks, 256, 0, s>>>(a, parts, waves, sh);     \
+        else kv_append_kernel<T, 4, D4><<<blocks, 256, 0, s>>>(a, parts, waves, sh);        \
+    } while (0)
+    if (a.c.dtype == Q3C_KV_F32) kv_append_kernel<float, 4, 0><<<blocks, 256, 0, s>>>(a, parts, waves, sh);
+    else if (!d4) Q3_APPEND(bf16, 0);
+    else if (d4 == 64) Q3_APPEND(bf16, 64);
+    else if (d4 == 128) Q3_APPEND(bf16, 128);
+    else Q3_APPEND(bf16, 256);
+#undef Q3_APPEND
     return hipGetLastError();
 }
 
