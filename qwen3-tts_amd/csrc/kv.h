@@ -21,7 +21,7 @@ struct KvAppendArgs {
     int q_heads;
     const float *qw, *kw, *cos_t, *sin_t;                       // norm weights [dim] or null, tables [positions][rot / 2]
     int rot;
-    float eps;
+    float eps, inv_dim;
     void* q_out;                                                // [tokens][q_heads][dim]
 };
 struct KvAttendArgs {
@@ -41,8 +41,8 @@ hipError_t q3_launch_kv_fork(const KvView& c, const int* parents, const int* chi
 hipError_t q3_launch_kv_copy(const KvView& c, const int* src, const int* dst, int count, int* ws, hipStream_t s);
 hipError_t q3_launch_kv_compact(const KvView& c, int* live, int* ws, hipStream_t s);
 struct KvSplit { int splits, share; };
-KvSplit q3_kv_attend_split(const KvView& c, int tokens, int sequences, int q_heads, int window, int sinks, int max_len);
-size_t q3_kv_attend_ws(const KvView& c, int tokens, int sequences, int q_heads, int splits);
+KvSplit q3_kv_attend_split(const KvView& c, int tokens, int sequences, int q_heads, bool ragged, int window, int sinks, int max_len);
+size_t q3_kv_attend_ws(const KvView& c, int tokens, int sequences, int q_heads, bool ragged, int splits);
 hipError_t q3_launch_kv_attend(const KvAttendArgs& a, hipStream_t s);
 
 #ifdef __HIPCC__

@@ -317,43 +317,26 @@ template <int D> struct Chunk<Int4, D> {
     static __device__ __forceinline__ int dim(int i, int m) { return 16 * i + m; }
 };
 
-// The workspace: for each (tile, kv head) the sums [splits][16][DP], then maxima and weights [splits][16][2], then how many shares it has.
-struct KvShares {
-    float *sums, *ml;
-    int* used;
-    __device__ __forceinline__ KvShares(const KvAttendArgs& a, int tiles, int dp, int tile, int hk) {
-        const long long n = (long long)tiles * a.c.heads, i = (long long)tile * a.c.heads + hk, rows = (long long)a.splits * 16;
-        sums = a.ws + i * rows * dp;
-        ml = a.ws + n * rows * dp + i * rows * 2;
-        used = (int*)(a.ws + n * rows * (dp + 2)) + i;
-    }
-};
+// Work on one tile of columns and one kv head: chunks cb .. ce - 1 of those the tile sees, whole (`out`) or as a part of them (unnormalised
+// sums, maxima and weights: `part`).
+struct KvPart { float *sums, *ml; };           // [16][DP], [16][2]
 
-// One workgroup = one tile of columns, one kv head, one share (`share` chunks) of those the tile sees: shares of one size, so that long and
-// short rows fill the card alike.  Its four waves take the share's chunks in turn, each with a running maximum and sum of its own, and
-// are joined through LDS at the end.  Where a tile has more than one share the unnormalised sums go to the workspace and
-// kv_join_kernel joins them.  Bound by memory for single tokens: the next chunk's keys are
-// requested before this one's softmax, its values before this one's scores.
-template <typename T, int DP>
-__global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_attend_kernel(const KvAttendArgs a) {
+// The four waves take the chunks in turn, each with a running maximum and sum of its own, and are joined through LDS at the end.  Bound
+// by memory for single tokens: the next chunk's keys are requested before this one's softmax, its values before this one's scores.
+template <typename T, int DP, typename Part>
+__device__ __forceinline__ void attend_part(const KvAttendArgs& a, const Tile& t, const Span& span, int hk, int cb, int ce, bool whole_row, Part part_of,
+                                            float (*so)[16][DP + 4], float (*sm)[16], float (*sl)[16]) {
     typedef Chunk<T, DP> C;
     typedef typename C::act A;
-    constexpr int TB = 16 * C::TILES, NT = DP / 16, LD = DP + 4;
-    __shared__ __attribute__((aligned(16))) float so[4][16][LD];
-    __shared__ float sm[4][16], sl[4][16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    constexpr int TB = 16 * C::TILES, NT = DP / 16;
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));              // made new for each part: what follows from it is not kept in registers from one to the next
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int cq = lane & 15, g = lane >> 4;
-    const Tile t = kv_tile(a, blockIdx.x, 16, lane);
-    if (!t.on) return;
-    const int hk = blockIdx.y, G = a.group, D = a.c.dim, sh = a.c.ps_shift;
+    const int G = a.group, D = a.c.dim, sh = a.c.ps_shift;
     const int col = t.col0 + cq, qtok = col / G;
-    const bool col_on = col < t.ncols;
-    int mypos = col_on && t.row >= 0 ? t.first_pos + qtok : -1;
+    int mypos = col < t.ncols && t.row >= 0 ? t.first_pos + qtok : -1;
     if (mypos > t.pmax) mypos = -1;
-    const Span span = kv_span(a, t, TB);
-    if (blockIdx.z > 0 && (int)blockIdx.z * a.share >= span.total) return;
-    const bool shared = a.splits > 1 && span.total > a.share;
-    const int c_begin = (int)blockIdx.z * a.share + wave, c_end = shared && (int)blockIdx.z + 1 < a.splits ? min(span.total, ((int)blockIdx.z + 1) * a.share) : span.total;
     typename C::Q q;
     C::load_q(q, (const A*)a.q.p + (long long)(t.tok0 + qtok) * a.q.ts + (long long)(hk * G + col - qtok * G) * a.q.hs, D, g, mypos >= 0);
 
@@ -389,13 +372,13 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_attend_kernel(const
             for (int u = 0; u < C::TILES; ++u)
                 ch.load_k(u, a.c.k, row_of(ek[u], tb + 16 * u + cq), D, g, cq, a.c, row_of(ev[u], tb + 16 * u + 4 * g));
         };
-        int c = c_begin, tb = 0;
-        if (c < c_end) {
+        int c = cb + wave, tb = 0;
+        if (c < ce) {
             tb = span.chunk(c) * TB;
             entries(tb);
             keys(tb);
         }
-        while (c < c_end) {
+        while (c < ce) {
             bool pages_ok = true;
             int ok[C::TILES];
 #pragma unroll
@@ -406,7 +389,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_attend_kernel(const
             }
             const int now = tb;
             c += 4;
-            tb = span.chunk(min(c, c_end - 1)) * TB;       // past the end: the last chunk again, and not looked at
+            tb = span.chunk(min(c, ce - 1)) * TB;          // past the end: the last chunk again, and not looked at
             entries(tb);
             float x[4 * C::TILES];
 #pragma unroll
@@ -491,16 +474,12 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_attend_kernel(const
 #pragma unroll
         for (int w = 0; w < 4; ++w) r[i] += *(const f32x4*)&so[w][c][d0 + 4 * i] * f[w];
     }
-    if (a.splits > 1) {
-        const KvShares ws(a, gridDim.x, DP, blockIdx.x, hk);
-        if (blockIdx.z == 0 && tid == 0) *ws.used = shared ? min(a.splits, (span.total + a.share - 1) / a.share) : 1;
-        if (shared) {
-            float* o = ws.sums + ((long long)blockIdx.z * 16 + c) * DP + d0;
+    if (!whole_row) {
+        const KvPart part = part_of();
 #pragma unroll
-            for (int i = 0; i < DP / 64; ++i) *(f32x4*)(o + 4 * i) = r[i];
-            if (d0 == 0) { ws.ml[2 * (blockIdx.z * 16 + c)] = mx; ws.ml[2 * (blockIdx.z * 16 + c) + 1] = l; }
-            return;
-        }
+        for (int i = 0; i < DP / 64; ++i) *(f32x4*)(part.sums + c * DP + d0 + 4 * i) = r[i];
+        if (d0 == 0) { part.ml[2 * c] = mx; part.ml[2 * c + 1] = l; }
+        return;
     }
     const int tk = (t.col0 + c) / G, h = hk * G + t.col0 + c - tk * G;
     const bool none = l == 0.f;
@@ -512,19 +491,123 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_attend_kernel(const
         for (int e = 0; e < 4; ++e) out[4 * i + e] = (A)(none ? 0.f : r[i][e] * inv);
 }
 
-// out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the shares s of one tile and head.  Sixteen lanes have a column: each first looks
-// at every sixteenth share's maximum and sum, then sums its dimensions of all.
-template <typename A, int DP>
-__global__ void __launch_bounds__(256) kv_join_kernel(const KvAttendArgs a) {
+// ---- single tokens: one new token per row, up to FLAT tiles --------------------------------------------------------------------------
+// A launch of as many workgroups as run at once; all (tile, kv head, chunk) triples in one line, cut into that many equal runs.  So
+// long rows and short ones, few and many, load the card alike, whatever the host does not know about lengths.  A workgroup's run touches
+// whole (tile, head) pairs and at most two in part, its first and its last: two parts per workgroup are all the workspace there is, and
+// kv_flat_join_kernel puts the parts together.  Each workgroup finds the line's layout by itself: the chunk counts of all tiles, summed up.
+constexpr int FLAT = 512;
+constexpr int FLAT_LEAST = 8;                  // chunks of a run: two rounds of its waves
+
+struct KvFlat {                                // the workspace
+    long long* before;                         // [tiles + 1] chunks of the tiles before, for one head
+    float *sums, *ml;                          // parts [2 runs][min(16, group)][DP], [..][2]
+    int cols;
+    __host__ __device__ KvFlat(float* ws, int runs, int dp, int group) {
+        before = (long long*)ws;
+        cols = group < 16 ? group : 16;
+        sums = ws + 2 * (FLAT + 2);
+        ml = sums + 2ll * runs * cols * dp;
+    }
+    __host__ __device__ static size_t bytes(int runs, int dp, int group) {
+        return (2 * (FLAT + 2) + 2ull * runs * (group < 16 ? group : 16) * (dp + 2)) * sizeof(float);
+    }
+};
+__device__ __forceinline__ long long kv_flat_run(long long units, int runs) {
+    const long long n = (units + runs - 1) / runs;
+    return n < FLAT_LEAST ? FLAT_LEAST : n;
+}
+
+// workgroups of a compute unit = waves of a SIMD, by the registers the kernel needs
+__host__ __device__ constexpr int flat_waves(bool four_bits, int dp) { return dp == 256 ? 1 : dp == 64 ? 4 : four_bits ? 3 : 2; }
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(256, flat_waves(__is_same(T, Int4), DP)) kv_flat_kernel(const KvAttendArgs a, int tiles) {
+    typedef Chunk<T, DP> C;
+    typedef typename C::act A;
+    constexpr int TB = 16 * C::TILES;
+    __shared__ __attribute__((aligned(16))) float so[4][16][DP + 4];
+    __shared__ float sm[4][16], sl[4][16];
+    __shared__ long long before[FLAT + 1], wave_sum[4];
+    __shared__ int first_tile;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, runs = gridDim.x, heads = a.c.heads;
+    const KvFlat ws(a.ws, runs, DP, a.group);
+    int n[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {              // thread t counts the chunks of tiles 2 t and 2 t + 1
+        const int x = 2 * tid + k;
+        n[k] = 0;
+        if (x < tiles) n[k] = kv_span(a, kv_tile(a, x, 16, 0), TB).total;
+    }
+    long long sum = (long long)n[0] + n[1];
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+        const long long y = __shfl_up(sum, k);
+        if (lane >= k) sum += y;
+    }
+    if (lane == 63) wave_sum[wave] = sum;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) sum += wave_sum[w];
+    if (2 * tid < tiles) before[2 * tid + 1] = sum - n[1];
+    if (2 * tid + 1 < tiles) before[2 * tid + 2] = sum;
+    if (tid == 0) { before[0] = 0; first_tile = tiles; }
+    __syncthreads();
+    const long long units = before[tiles] * heads, run = kv_flat_run(units, runs);
+    long long u = blockIdx.x * run;
+    const long long end = min(u + run, units);
+    for (int x = tid; x < tiles; x += 256)
+        if (before[x] * heads <= u && u < before[x + 1] * heads) first_tile = x;
+    if (blockIdx.x == 0)
+        for (int x = tid; x <= tiles; x += 256) ws.before[x] = before[x];
+    // tiles that see nothing at all lie nowhere on the line: their outputs are zeros
+    for (int x = blockIdx.x; x < tiles; x += runs)
+        if (before[x] == before[x + 1]) {
+            const Tile t = kv_tile(a, x, 16, 0);
+            if (!t.on) continue;
+            const int cols = min(16, t.ncols - t.col0);
+            for (int i = tid; i < heads * cols * a.c.dim; i += 256) {
+                const int d = i % a.c.dim, c = i / a.c.dim % cols, hk = i / a.c.dim / cols;
+                ((A*)a.out)[((long long)t.tok0 * a.q_heads + hk * a.group + t.col0 + c) * a.c.dim + d] = (A)0.f;
+            }
+        }
+    __syncthreads();
+    if (u >= end) return;
+    int x = __builtin_amdgcn_readfirstlane(first_tile), left = (int)(end - u), slot = 2 * blockIdx.x;
+    int len = __builtin_amdgcn_readfirstlane((int)(before[x + 1] - before[x]));
+    const long long off = u - before[x] * heads;
+    int hk = __builtin_amdgcn_readfirstlane((int)(off / len)), cb = __builtin_amdgcn_readfirstlane((int)(off - (long long)hk * len));
+    for (;;) {
+        const int ce = min(len, cb + left);
+        const Tile t = kv_tile(a, x, 16, lane);
+        attend_part<T, DP>(a, t, kv_span(a, t, TB), hk, cb, ce, cb == 0 && ce == len, [&]() {
+            const KvFlat ws(a.ws, runs, DP, a.group);
+            return KvPart{ws.sums + (long long)slot * ws.cols * DP, ws.ml + (long long)slot * ws.cols * 2};
+        }, so, sm, sl);
+        left -= ce - cb;
+        if (left <= 0) return;
+        __syncthreads();
+        cb = 0;
+        slot |= 1;
+        if (++hk == heads) {
+            hk = 0;
+            do {
+                ++x;
+                len = __builtin_amdgcn_readfirstlane((int)(before[x + 1] - before[x]));
+            } while (len == 0);
+        }
+    }
+}
+
+// out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the n parts of one tile and head, part s at place(s).  Sixteen lanes have a
+// column: each looks at every sixteenth part's maximum, then sums its DP / 16 dimensions of all.
+template <typename A, int DP, typename Place>
+__device__ __forceinline__ void join_parts(const KvAttendArgs& a, const Tile& t, int hk, int n, const float* sums, const float* ml, int cols, Place place) {
     constexpr int N = DP / 16;
-    const int tid = threadIdx.x, hk = blockIdx.y, G = a.group, D = a.c.dim, c = tid >> 4, j = tid & 15, d0 = j * N;
-    const KvShares ws(a, gridDim.x, DP, blockIdx.x, hk);
-    const Tile t = kv_tile(a, blockIdx.x, 16, tid & 63);
-    if (!t.on) return;
-    const int used = *ws.used;
-    if (used < 2 || t.col0 + (c & ~3) >= t.ncols) return;       // whole waves
+    const int tid = threadIdx.x, G = a.group, D = a.c.dim, c = tid >> 4, j = tid & 15, d0 = j * N;
+    if (t.col0 + (c & ~3) >= t.ncols) return;                  // whole waves
+    const int cc = min(c, cols - 1);
     float m = -INFINITY;
-    for (int s = j; s < used; s += 16) m = fmaxf(m, ws.ml[2 * (s * 16 + c)]);
+    for (int s = j; s < n; s += 16) m = fmaxf(m, ml[2 * (place(s) * cols + cc)]);
 #pragma unroll
     for (int k = 1; k < 16; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
     const float mu = m == -INFINITY ? 0.f : m;
@@ -532,13 +615,13 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const KvAttendArgs a) {
 #pragma unroll
     for (int e = 0; e < N; ++e) r[e] = 0.f;
 #pragma unroll 4
-    for (int s = 0; s < used; ++s) {
-        const float f = __builtin_amdgcn_exp2f(ws.ml[2 * (s * 16 + c)] - mu), ls = ws.ml[2 * (s * 16 + c) + 1];
-        const float* o = ws.sums + ((long long)s * 16 + c) * DP + d0;
+    for (int s = 0; s < n; ++s) {
+        const long long row = place(s) * cols + cc;
+        const float f = __builtin_amdgcn_exp2f(ml[2 * row] - mu), ls = ml[2 * row + 1];
         l = fmaf(ls, f, l);
 #pragma unroll
         for (int e = 0; e < N; e += 4) {
-            const f32x4 x = *(const f32x4*)(o + e);
+            const f32x4 x = *(const f32x4*)(sums + row * DP + d0 + e);
 #pragma unroll
             for (int w = 0; w < 4; ++w) r[e + w] = fmaf(x[w], f, r[e + w]);
         }
@@ -550,6 +633,62 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const KvAttendArgs a) {
     A* out = (A*)a.out + ((long long)(t.tok0 + tk) * a.q_heads + h) * D + d0;
 #pragma unroll
     for (int e = 0; e < N; ++e) out[e] = (A)(none ? 0.f : r[e] * inv);
+}
+template <typename A, int DP>
+__global__ void __launch_bounds__(256) kv_flat_join_kernel(const KvAttendArgs a, int tiles, int runs) {
+    const int x = blockIdx.x, hk = blockIdx.y;
+    const KvFlat ws(a.ws, runs, DP, a.group);
+    const long long b0 = ws.before[x], len = ws.before[x + 1] - b0, run = kv_flat_run(ws.before[tiles] * a.c.heads, runs);
+    if (len == 0) return;
+    const long long u = b0 * a.c.heads + hk * len;
+    const int ra = (int)(u / run), rb = (int)((u + len - 1) / run);
+    if (ra == rb) return;
+    const Tile t = kv_tile(a, x, 16, threadIdx.x & 63);
+    if (!t.on) return;
+    // the part of the run in which it begins is that run's first only if it begins with it
+    const long long first = 2ll * ra + (u == ra * run ? 0 : 1);
+    join_parts<A, DP>(a, t, hk, rb - ra + 1, ws.sums, ws.ml, ws.cols, [&](int s) { return s == 0 ? first : 2ll * (ra + s); });
+}
+
+// ---- few columns per request, or many requests --------------------------------------------------------------------------------------
+// One workgroup = one tile of columns, one kv head, one share (`share` chunks) of those the tile sees; where a tile has more than one
+// share kv_join_kernel joins them.  The workspace: for each (tile, kv head) the parts [splits], then how many there are.
+struct KvShares {
+    float *sums, *ml;
+    int* used;
+    __device__ __forceinline__ KvShares(const KvAttendArgs& a, int tiles, int dp, int tile, int hk) {
+        const long long n = (long long)tiles * a.c.heads, i = (long long)tile * a.c.heads + hk, rows = (long long)a.splits * 16;
+        sums = a.ws + i * rows * dp;
+        ml = a.ws + n * rows * dp + i * rows * 2;
+        used = (int*)(a.ws + n * rows * (dp + 2)) + i;
+    }
+};
+template <typename T, int DP>
+__global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_attend_kernel(const KvAttendArgs a) {
+    constexpr int TB = 16 * Chunk<T, DP>::TILES;
+    __shared__ __attribute__((aligned(16))) float so[4][16][DP + 4];
+    __shared__ float sm[4][16], sl[4][16];
+    const Tile t = kv_tile(a, blockIdx.x, 16, threadIdx.x & 63);
+    if (!t.on) return;
+    const int hk = blockIdx.y, z = blockIdx.z;
+    const Span span = kv_span(a, t, TB);
+    if (z > 0 && z * a.share >= span.total) return;
+    const bool shared = a.splits > 1 && span.total > a.share;
+    if (a.splits > 1 && z == 0 && threadIdx.x == 0)
+        *KvShares(a, gridDim.x, DP, blockIdx.x, hk).used = shared ? min(a.splits, (span.total + a.share - 1) / a.share) : 1;
+    const int ce = shared && z + 1 < a.splits ? min(span.total, (z + 1) * a.share) : span.total;       // a bound on lengths that was too low: the last share's
+    attend_part<T, DP>(a, t, span, hk, z * a.share, ce, !shared, [&]() {
+        const KvShares ws(a, gridDim.x, DP, blockIdx.x, hk);
+        return KvPart{ws.sums + z * 16ll * DP, ws.ml + z * 32ll};
+    }, so, sm, sl);
+}
+template <typename A, int DP>
+__global__ void __launch_bounds__(256) kv_join_kernel(const KvAttendArgs a) {
+    const KvShares ws(a, gridDim.x, DP, blockIdx.x, blockIdx.y);
+    const Tile t = kv_tile(a, blockIdx.x, 16, threadIdx.x & 63);
+    if (!t.on) return;
+    const int used = *ws.used;
+    if (used > 1) join_parts<A, DP>(a, t, blockIdx.y, used, ws.sums, ws.ml, 16, [](int s) { return (long long)s; });
 }
 
 // ---- prompts -----------------------------------------------------------------------------------------------------------------------------
@@ -935,39 +1074,56 @@ long long tiles_of(int tokens, int sequences, int group, bool ragged, int cols =
 bool prompts(const KvView& c, int tokens, int sequences, int q_heads, bool ragged) {
     return c.dtype != Q3C_KV_F32 && !(c.dtype == Q3C_KV_INT4 && c.dim > 128) && ragged && (long long)tokens * (q_heads / c.heads) >= 64ll * sequences;
 }
-
-}  // namespace
-
-// How a tile's keys are cut: shares of as many chunks as make about 2048 workgroups of the longest rows there can be (eight per compute
-// unit: short ones then even out what is left), of at least 16 chunks (four rounds of a workgroup's waves), and no more than 256.
-KvSplit q3_kv_attend_split(const KvView& c, int tokens, int sequences, int q_heads, int window, int sinks, int max_len) {
-    const int group = q_heads / c.heads, tb = c.dtype == Q3C_KV_F32 ? 16 : 32;
+// most chunks that one row of the call can see
+long long most_chunks(const KvView& c, int window, int sinks, int max_len) {
+    const int tb = c.dtype == Q3C_KV_F32 ? 16 : 32;
     long long len = (long long)c.width << c.ps_shift;
     if (max_len > 0 && max_len < len) len = max_len;
     if (window > 0 && (long long)window + sinks + tb < len) len = (long long)window + sinks + tb;
-    const long long chunks = len / tb + 1, base = (tokens == sequences ? (long long)sequences * ((group + 15) / 16) : (long long)tokens * group / 16 + 1) * c.heads;
+    return len / tb + 1;
+}
+// Single tokens in a line of runs, unless the whole line is short: then the layout of the line costs more than it evens out (one row under a
+// 4096-token window, 1040 chunks: 20 us against 14; 8 rows of 700 tokens in 4 bits: 17.6 against 11.5; 64 rows of 3200 - 16000: 184 against 218).
+bool flat(const KvView& c, int sequences, int q_heads, bool ragged, int window, int sinks, int max_len) {
+    const long long tiles = (long long)sequences * ((q_heads / c.heads + 15) / 16);
+    return !ragged && tiles <= FLAT && tiles * c.heads * most_chunks(c, window, sinks, max_len) > 8192;
+}
+// workgroups that run at once on 256 compute units
+int flat_runs(const KvView& c) {
+    return 256 * flat_waves(c.dtype == Q3C_KV_INT4, padded_dim(c.dim));
+}
+
+}  // namespace
+
+// How a tile's keys are cut otherwise: shares of as many chunks as make about 2048 workgroups of the longest rows there can be (eight per
+// compute unit: short ones then even out what is left), of at least 8 chunks (two rounds of a workgroup's waves), no more than 256; rows of
+// up to 32 chunks are left whole, since a second launch takes as long as six rounds (700 tokens: 11.5 us whole, 14.2 in shares of 8).
+KvSplit q3_kv_attend_split(const KvView& c, int tokens, int sequences, int q_heads, bool ragged, int window, int sinks, int max_len) {
+    if (flat(c, sequences, q_heads, ragged, window, sinks, max_len)) return KvSplit{0, 0};
+    if (prompts(c, tokens, sequences, q_heads, ragged)) return KvSplit{1, 0x7fffffff};
+    const int group = q_heads / c.heads;
+    const long long chunks = most_chunks(c, window, sinks, max_len), base = tiles_of(tokens, sequences, group, ragged) * c.heads;
     long long share = (chunks * base + 2047) / 2048;
-    if (share < 16) share = 16;
+    if (share < 8) share = 8;
     if (share < (chunks + 255) / 256) share = (chunks + 255) / 256;
     share = (share + 3) / 4 * 4;
     KvSplit s;
-    s.splits = base >= 2048 ? 1 : (int)((chunks + share - 1) / share);
+    s.splits = base >= 2048 || chunks <= 32 ? 1 : (int)((chunks + share - 1) / share);
     s.share = s.splits == 1 ? 0x7fffffff : (int)share;
     return s;
 }
-size_t q3_kv_attend_ws(const KvView& c, int tokens, int sequences, int q_heads, int splits) {
-    if (splits < 2) return 0;
-    const int group = q_heads / c.heads;
-    const long long tiles = tiles_of(tokens, sequences, group, true);
-    const long long flat = tiles_of(tokens, sequences, group, false);
-    return (size_t)((tiles > flat ? tiles : flat) * c.heads) * ((size_t)splits * 16 * (padded_dim(c.dim) + 2) + 1) * sizeof(float);
+size_t q3_kv_attend_ws(const KvView& c, int tokens, int sequences, int q_heads, bool ragged, int splits) {
+    const int group = q_heads / c.heads, dp = padded_dim(c.dim);
+    if (splits == 0) return KvFlat::bytes(flat_runs(c), dp, group);
+    if (splits == 1) return 0;
+    return (size_t)(tiles_of(tokens, sequences, group, ragged) * c.heads) * ((size_t)splits * 16 * (dp + 2) + 1) * sizeof(float);
 }
 
 hipError_t q3_launch_kv_attend(const KvAttendArgs& a, hipStream_t s) {
     const unsigned tiles = (unsigned)tiles_of(a.b.tokens, a.b.sequences, a.group, a.b.offsets != nullptr);
     if (!tiles || !a.b.tokens) return hipSuccess;
-    const dim3 grid(tiles, a.c.heads, a.splits), join(tiles, a.c.heads);
-    const int dp = padded_dim(a.c.dim);
+    const dim3 grid(tiles, a.c.heads, a.splits ? a.splits : 1), join(tiles, a.c.heads);
+    const int dp = padded_dim(a.c.dim), runs = a.splits ? 0 : flat_runs(a.c);
     if (prompts(a.c, a.b.tokens, a.b.sequences, a.q_heads, a.b.offsets != nullptr)) {
         const int n = (int)tiles_of(a.b.tokens, a.b.sequences, a.group, true, 128);
         const unsigned blocks = (unsigned)n * a.c.heads;
@@ -983,8 +1139,13 @@ hipError_t q3_launch_kv_attend(const KvAttendArgs& a, hipStream_t s) {
     }
 #define Q3_ATTEND(T, A, DP)                                                        \
     do {                                                                           \
-        kv_attend_kernel<T, DP><<<grid, 256, 0, s>>>(a);                           \
-        if (a.splits > 1) kv_join_kernel<A, DP><<<join, 256, 0, s>>>(a);           \
+        if (runs) {                                                                \
+            kv_flat_kernel<T, DP><<<runs, 256, 0, s>>>(a, (int)tiles);             \
+            kv_flat_join_kernel<A, DP><<<join, 256, 0, s>>>(a, (int)tiles, runs);  \
+        } else {                                                                   \
+            kv_attend_kernel<T, DP><<<grid, 256, 0, s>>>(a);                       \
+            if (a.splits > 1) kv_join_kernel<A, DP><<<join, 256, 0, s>>>(a);       \
+        }                                                                          \
     } while (0)
 #define Q3_ATTEND_DIM(T, A)                        \
     do {                                           \

@@ -67,6 +67,7 @@ int q3c_kv_append(const q3c_kv* kv, int32_t layer, const void* q, int64_t q_ts, 
     if (!tokens) return 0;
     const size_t e = act_bytes(a.c);
     if (!strided(q, q_ts, q_hs, e) || !strided(k, k_ts, k_hs, e) || !strided(v, v_ts, v_hs, e) || !q_out || !aligned(q_out, 16)) return Q3C_ERR_INVALID_ARGUMENT;
+    if ((q_weight || k_weight) && !(eps > 0.f)) return Q3C_ERR_INVALID_ARGUMENT;
     if (!aligned(q_weight, 16) || !aligned(k_weight, 16)) return Q3C_ERR_INVALID_ARGUMENT;
     if (rot_dim < 0 || rot_dim > a.c.dim || rot_dim % 8) return Q3C_ERR_UNSUPPORTED;
     if (a.c.dtype == Q3C_KV_INT4 && rot_dim && rot_dim != a.c.dim) return Q3C_ERR_UNSUPPORTED;
@@ -77,7 +78,7 @@ int q3c_kv_append(const q3c_kv* kv, int32_t layer, const void* q, int64_t q_ts, 
     a.q = {q, q_ts, q_hs}; a.k = {k, k_ts, k_hs}; a.v = {v, v_ts, v_hs};
     a.q_heads = q_heads;
     a.qw = q_weight; a.kw = k_weight; a.cos_t = cos_table; a.sin_t = sin_table;
-    a.rot = rot_dim; a.eps = eps; a.q_out = q_out;
+    a.rot = rot_dim; a.eps = eps; a.inv_dim = 1.0f / (float)a.c.dim; a.q_out = q_out;
     return done(q3_launch_kv_append(a, (hipStream_t)stream));
 }
 
@@ -107,7 +108,12 @@ int q3c_kv_attend_workspace_bytes(const q3c_kv* kv, int32_t q_heads, int32_t seq
     if (!bytes) return Q3C_ERR_INVALID_ARGUMENT;
     const int rc = attend_shape(kv, q_heads, sequences, tokens, window, sinks, max_len, &c);
     if (rc) return rc;
-    *bytes = q3_kv_attend_ws(c, tokens, sequences, q_heads, q3_kv_attend_split(c, tokens, sequences, q_heads, window, sinks, max_len).splits);
+    size_t most = 0;                       // with offsets and, where there can be none, without
+    for (int ragged = tokens == sequences ? 0 : 1; ragged < 2; ++ragged) {
+        const size_t n = q3_kv_attend_ws(c, tokens, sequences, q_heads, ragged, q3_kv_attend_split(c, tokens, sequences, q_heads, ragged, window, sinks, max_len).splits);
+        if (n > most) most = n;
+    }
+    *bytes = most;
     return 0;
 }
 
@@ -120,10 +126,10 @@ int q3c_kv_attend(const q3c_kv* kv, int32_t layer, const void* q, int64_t q_ts, 
     if (layer < 0 || layer >= a.c.layers || !(scale > 0.f) || !(scale < 3e38f)) return Q3C_ERR_INVALID_ARGUMENT;
     if (!tokens) return 0;
     if (!strided(q, q_ts, q_hs, act_bytes(a.c)) || !out || !aligned(out, 16)) return Q3C_ERR_INVALID_ARGUMENT;
-    const KvSplit cut = q3_kv_attend_split(a.c, tokens, sequences, q_heads, window, sinks, max_len);
+    const KvSplit cut = q3_kv_attend_split(a.c, tokens, sequences, q_heads, offsets != nullptr, window, sinks, max_len);
     a.splits = cut.splits;
     a.share = cut.share;
-    const size_t need = q3_kv_attend_ws(a.c, tokens, sequences, q_heads, a.splits);
+    const size_t need = q3_kv_attend_ws(a.c, tokens, sequences, q_heads, offsets != nullptr, a.splits);
     if (need && (!workspace || !aligned(workspace, 16))) return Q3C_ERR_INVALID_ARGUMENT;
     if (workspace_bytes < need) return Q3C_ERR_WORKSPACE;
     a.layer = layer;

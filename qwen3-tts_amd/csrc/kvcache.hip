@@ -14,6 +14,25 @@ template <int N> using Floats = float __attribute__((ext_vector_type(N)));
 template <int N, typename T> __device__ __forceinline__ Vec<T, N> kv_load(const T* p) { return *(const Vec<T, N>*)p; }
 template <int N, typename T> __device__ __forceinline__ void kv_store(T* p, Floats<N> v) { *(Vec<T, N>*)p = __builtin_convertvector(v, Vec<T, N>); }
 
+// The value of the lane whose number differs in bit k (0 .. 3).  Bits 2 and 3 are taken by mirroring 8 or 16 lanes: right where the lanes
+// that the lower bits tell apart hold one value, as in a butterfly that runs upwards.
+template <typename V> __device__ __forceinline__ V lane_xor(V x, int k) {
+    const int i = __builtin_bit_cast(int, x);
+    return __builtin_bit_cast(V, k == 0   ? __builtin_amdgcn_update_dpp(0, i, 0xb1, 0xf, 0xf, true)
+                                 : k == 1 ? __builtin_amdgcn_update_dpp(0, i, 0x4e, 0xf, 0xf, true)
+                                 : k == 2 ? __builtin_amdgcn_update_dpp(0, i, 0x141, 0xf, 0xf, true)
+                                          : __builtin_amdgcn_update_dpp(0, i, 0x140, 0xf, 0xf, true));
+}
+// the sum over each run of `lanes` (2 .. 32) lanes
+__device__ __forceinline__ float sum_lanes(float x, int lanes) {
+    x += lane_xor(x, 0);
+    if (lanes > 2) x += lane_xor(x, 1);
+    if (lanes > 4) x += lane_xor(x, 2);
+    if (lanes > 8) x += lane_xor(x, 3);
+    if (lanes > 16) x += __shfl_xor(x, 16);
+    return x;
+}
+
 __device__ __forceinline__ void kv_flag(const KvView& c, int bits) { atomicOr(c.status, bits); }
 
 // whether an earlier request of the call names the same table row: its tokens would race for the same places (wave-uniform)
@@ -53,11 +72,11 @@ __device__ __forceinline__ bool kv_place(const KvAppendArgs& a, int tok, bool fi
 // (a, b) = (y_i, y_(i + rot/2)) -> (a cos - b sin, b cos + a sin); sums and products in fp32, one rounding at the store.  The keys
 // and the (unchanged) values go straight to their page.  Bound by memory: 2 reads and writes of each element.
 // A wave has one token and `parts`-th of its heads, VEC pairs per lane as two runs that are each other's rotation partners, so that the
-// rotation needs no exchange between lanes and the norm one butterfly over the head's lanes.  Four runs of heads are requested before
+// rotation needs no exchange between lanes and the norm one butterfly over the head's lanes.  Two runs of heads are requested before
 // the token's place is looked up (offset -> row -> length -> page, four dependent reads): they are what a wave has to wait for once.
 template <typename T, int VEC, bool CACHED>     // CACHED: keys and values go to the pages here too (no 4-bit cache)
 __device__ __forceinline__ void append_plain(const KvAppendArgs& a, int tok, int part, int parts, int lane, int lpu_shift) {
-    constexpr int RUN = 4;
+    constexpr int RUN = 2;
     const int D = a.c.dim, R = a.rot, H = a.q_heads, G = a.c.heads, units = CACHED ? H + 2 * G : H;
     const int lpu = 1 << lpu_shift, upw = 64 >> lpu_shift, ch = lane & (lpu - 1);
     const bool on = 2 * VEC * ch < D, in_turn = 2 * VEC * ch < R;
@@ -105,8 +124,8 @@ __device__ __forceinline__ void append_plain(const KvAppendArgs& a, int tok, int
                 float ss = 0.f;
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) ss = fmaf(lo[e], lo[e], fmaf(hi[e], hi[e], ss));
-                for (int m = 1; m < lpu; m <<= 1) ss += __shfl_xor(ss, m);
-                const float r = 1.0f / sqrtf(ss / (float)D + a.eps);
+                ss = sum_lanes(ss, lpu);
+                const float r = __builtin_amdgcn_rsqf(fmaf(ss, a.inv_dim, a.eps));
                 if (w) {
                     lo = lo * r * *(const Floats<VEC>*)(w + d0[i]);
                     hi = hi * r * *(const Floats<VEC>*)(w + d1[i]);
@@ -152,9 +171,8 @@ __device__ __forceinline__ void append_int4(const KvAppendArgs& a, int tok, int 
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-        for (int k = 1; k < 16; k <<= 1) ss += __shfl_xor(ss, k);
-        const float r = 1.0f / sqrtf(ss / (float)D + a.eps);
+        ss = sum_lanes(ss, 16);
+        const float r = __builtin_amdgcn_rsqf(fmaf(ss, a.inv_dim, a.eps));
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = x[i] * r * a.kw[16 * i + m];
     }
@@ -176,7 +194,7 @@ __device__ __forceinline__ void append_int4(const KvAppendArgs& a, int tok, int 
     for (int s = 0; s < S; ++s) {
         unsigned top = max(__float_as_uint(x[2 * s]) & 0x7fffffffu, __float_as_uint(x[2 * s + 1]) & 0x7fffffffu);
 #pragma unroll
-        for (int k = 1; k < 16; k <<= 1) top = max(top, (unsigned)__shfl_xor((int)top, k));
+        for (int k = 0; k < 4; ++k) top = max(top, lane_xor<unsigned>(top, k));
         const bf16 st = (bf16)(__uint_as_float(top) / 7.0f);
         const float step = (float)st;
         unsigned byte = 0x88;
@@ -229,14 +247,18 @@ __global__ void __launch_bounds__(256) kv_gather_kernel(const KvView c, const Kv
             const T* x = (const T*)(key ? c.k : c.v) + at * c.dim + 8 * ch;
             lo = __builtin_convertvector(kv_load<4>(x), Floats<4>);
             hi = __builtin_convertvector(kv_load<4>(x + 4), Floats<4>);
-        } else {                                               // dimensions 8 ch .. + 7: one half of eight neighbouring m's bytes
-            const int S = c.dim / 32, s = ch >> 2;
-            const unsigned char* x = (const unsigned char*)(key ? c.k : c.v) + at * (c.dim / 2) + (ch & 1) * 8 * S + s;
+        } else {                                               // dimensions 8 ch .. + 7: one half of byte s of eight neighbouring m's S bytes
+            constexpr int S = D4 ? D4 / 32 : 2;
+            const int s = ch >> 2, shift = 8 * (s & 3) + ((ch & 2) ? 4 : 0);
+            const unsigned* x = (const unsigned*)((const unsigned char*)(key ? c.k : c.v) + at * (16 * S) + (ch & 1) * 8 * S);
             const float step = (float)(key ? c.ks : c.vs)[at * S + s];
+            unsigned w[2 * S];
+#pragma unroll
+            for (int i = 0; i < 2 * S; i += 4) *(uint4*)(w + i) = *(const uint4*)(x + i);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int byte = x[i * S], n = (((ch & 2) ? byte >> 4 : byte & 15) - 8);
-                (i < 4 ? lo : hi)[i & 3] = (float)n * step;
+                const unsigned v = S == 2 ? w[i >> 1] >> (16 * (i & 1)) : S == 4 ? w[i] : s < 4 ? w[2 * i & (2 * S - 1)] : w[(2 * i + 1) & (2 * S - 1)];
+                (i < 4 ? lo : hi)[i & 3] = (float)((int)(v >> shift & 15u) - 8) * step;
             }
         }
     }
@@ -590,8 +612,8 @@ hipError_t q3_launch_kv_append(const KvAppendArgs& a, hipStream_t s) {
     const auto wide = [](const KvStrided& x) { return x.ts % 8 == 0 && x.hs % 8 == 0 && (uintptr_t)x.p % 16 == 0; };
     const bool v8 = a.c.dtype != Q3C_KV_F32 && a.rot % 16 == 0 && wide(a.q) && (d4 || (wide(a.k) && wide(a.v)));
     const int sh = lanes_shift(a.c.dim, v8 ? 16 : 8), upw = 64 >> sh, runs = (units + upw - 1) / upw;
-    int parts = runs;                       // waves of a token: few tokens are spread, many keep four runs of heads in flight per wave
-    while (parts > 1 && (long long)a.b.tokens * parts > 4096 && (runs + parts - 1) / parts < 4) parts = (parts + 1) / 2;
+    int parts = runs;                       // waves of a token: few tokens are spread, many keep two runs of heads in flight per wave
+    while (parts > 1 && (long long)a.b.tokens * parts > 4096 && (runs + parts - 1) / parts < 2) parts = (parts + 1) / 2;
     const int waves = parts + (d4 ? (2 * a.c.heads + 3) / 4 : 0);
     const unsigned blocks = (unsigned)(((long long)a.b.tokens * waves + 3) / 4);
     if (!blocks) return hipSuccess;
@@ -618,7 +640,9 @@ hipError_t q3_launch_kv_gather(const KvView& c, const KvBatch& b, int layer, voi
                          : kv_gather_kernel<T, bf16, D4><<<blocks, 256, 0, s>>>(c, b, layer, (bf16*)k_out, (bf16*)v_out, waves, sh))
     if (c.dtype == Q3C_KV_F32) Q3_GATHER(float, 0);
     else if (c.dtype == Q3C_KV_BF16) Q3_GATHER(bf16, 0);
-    else Q3_GATHER(bf16, 1);
+    else if (c.dim == 64) Q3_GATHER(bf16, 64);
+    else if (c.dim == 128) Q3_GATHER(bf16, 128);
+    else Q3_GATHER(bf16, 256);
 #undef Q3_GATHER
     return hipGetLastError();
 }

@@ -33,6 +33,8 @@ Rows = Union[torch.Tensor, Sequence[int]]
 GROUP = 32                                     # dimensions that share a step in a 4-bit cache
 _HELD = {torch.float32: 0, torch.bfloat16: 1, torch.uint8: 2}
 _ACT = (torch.float32, torch.bfloat16, torch.bfloat16)
+# the current device and its stream's handle, without the objects that torch.cuda wraps them in (a call of a generation step is host-bound)
+_device, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 _STATUS = ((1, "a row id outside the table, named twice in a call, or offsets that do not fit a row's length"),
            (2, "no free page was left (or a token was appended that has no page)"),
            (4, "a page id outside the pool, or a copy whose source is another copy's destination"),
@@ -126,6 +128,7 @@ class PagedKV:
         self.rows, self.pages_per_row = int(table.shape[0]), int(table.shape[1])
         self.dtype = ("f32", "bf16", "int4")[code]
         self.activations = _ACT[code]
+        self._act_bytes = 4 if code == 0 else 2
         self.device = k.device
         self._index = k.device.index if k.device.index is not None else torch.cuda.current_device()
         self._lib = _lib.load()
@@ -147,17 +150,18 @@ class PagedKV:
         return self.page_size * self.pages_per_row
 
     def _call(self, fn, *args) -> None:
-        if torch.cuda.current_device() == self._index:
-            rc = fn(self._ref, *args, torch.cuda.current_stream(self._index).cuda_stream)
+        i = self._index
+        if _device() == i:
+            rc = fn(self._ref, *args, _stream(i))
         else:
-            with torch.cuda.device(self._index):
-                rc = fn(self._ref, *args, torch.cuda.current_stream(self._index).cuda_stream)
+            with torch.cuda.device(i):
+                rc = fn(self._ref, *args, _stream(i))
         if rc:
             raise _lib.Q3cError(rc, f"{fn.__name__} failed")
 
     def _ids(self, ids, what: str, most: int, distinct: bool = True) -> torch.Tensor:
         if isinstance(ids, torch.Tensor):
-            if ids.dtype != torch.int32 or ids.dim() != 1 or not ids.is_contiguous() or ids.device != self.device:
+            if ids.dtype != torch.int32 or ids.dim() != 1 or not ids.is_contiguous() or ids.get_device() != self._index:
                 raise ValueError(f"{what} must be a contiguous int32 tensor [n] on {self.device} (or a sequence of ints)")
             return ids
         ids = [int(i) for i in ids]
@@ -175,19 +179,22 @@ class PagedKV:
             if tokens is not None and tokens != n:
                 raise ValueError(f"{tokens} tokens for {n} rows: without offsets every row has one")
             return rows, n, None, n
-        if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.shape[0] != n + 1 or not offsets.is_contiguous() or offsets.device != self.device:
+        if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.shape[0] != n + 1 or not offsets.is_contiguous() or offsets.get_device() != self._index:
             raise ValueError(f"offsets must be a contiguous int32 tensor [{n + 1}] on {self.device}")
         return rows, n, offsets, tokens
 
     def _heads(self, x: torch.Tensor, what: str, heads: Optional[int]) -> torch.Tensor:
         """[tokens, heads, head_dim] in the cache's activation type; copied only where its strides are not what the kernels read."""
-        if x.dim() != 3 or x.shape[2] != self.head_dim or (heads is not None and x.shape[1] != heads) or x.shape[1] < 1:
-            raise ValueError(f"{what} must be [tokens, {'heads' if heads is None else heads}, {self.head_dim}], got {tuple(x.shape)}")
-        if x.dtype != self.activations or x.device != self.device:
+        shape = x.shape
+        if len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads) or shape[1] < 1:
+            raise ValueError(f"{what} must be [tokens, {'heads' if heads is None else heads}, {self.head_dim}], got {tuple(shape)}")
+        if x.dtype != self.activations or x.get_device() != self._index:
             raise ValueError(f"{what} must be {self.activations} on {self.device}, got {x.dtype} on {x.device}")
-        if x.stride(2) != 1 or x.stride(0) % 4 or x.stride(1) % 4 or x.data_ptr() % (4 * x.element_size()):
+        ts, hs, ds = x.stride()
+        quad = 4 * self._act_bytes
+        if ds != 1 or ts % 4 or hs % 4 or x.data_ptr() % quad:
             x = x.contiguous()
-            if x.data_ptr() % (4 * x.element_size()):          # a contiguous view that starts between two quads
+            if x.data_ptr() % quad:                            # a contiguous view that starts between two quads
                 x = x.clone()
         return x
 
@@ -199,7 +206,7 @@ class PagedKV:
     def _out(self, out: Optional[torch.Tensor], shape, dtype, what: str = "out") -> torch.Tensor:
         if out is None:
             return torch.empty(shape, dtype=dtype, device=self.device)
-        if out.dtype != dtype or tuple(out.shape) != tuple(shape) or not out.is_contiguous() or out.device != self.device or out.data_ptr() % 16:
+        if out.dtype != dtype or tuple(out.shape) != tuple(shape) or not out.is_contiguous() or out.get_device() != self._index or out.data_ptr() % 16:
             raise ValueError(f"{what} must be a contiguous, 16-byte aligned {dtype} tensor {tuple(shape)} on {self.device}")
         return out
 
@@ -234,14 +241,16 @@ class PagedKV:
         if not n and T:
             raise ValueError(f"{T} tokens without a row")
         for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-            if w is not None and (w.dtype != torch.float32 or tuple(w.shape) != (self.head_dim,) or not w.is_contiguous() or w.device != self.device or w.data_ptr() % 16):
+            if w is not None and (w.dtype != torch.float32 or w.dim() != 1 or w.shape[0] != self.head_dim or not w.is_contiguous() or w.get_device() != self._index or w.data_ptr() % 16):
                 raise ValueError(f"{name} must be a contiguous, 16-byte aligned float32 tensor [{self.head_dim}] on {self.device}")
+        if (q_weight is not None or k_weight is not None) and not eps > 0:
+            raise ValueError(f"eps must be positive, got {eps}")
         rot = positions = 0
         cos = sin = None
         if rope is not None:
             cos, sin = rope
             for name, t in (("cos", cos), ("sin", sin)):
-                if t.dtype != torch.float32 or t.dim() != 2 or t.shape != cos.shape or not t.is_contiguous() or t.device != self.device or t.data_ptr() % 16:
+                if t.dtype != torch.float32 or t.dim() != 2 or t.shape != cos.shape or not t.is_contiguous() or t.get_device() != self._index or t.data_ptr() % 16:
                     raise ValueError(f"rope's {name} must be a contiguous, 16-byte aligned float32 tensor [positions, rotated / 2] on {self.device}")
             positions, rot = cos.shape[0], 2 * cos.shape[1]
             if rot % 8 or not 0 < rot <= self.head_dim or (self.dtype == "int4" and rot != self.head_dim):
