@@ -109,21 +109,26 @@ template <int DP> struct Chunk<bf16, DP> {
             q.f[s] = u32x4{x[0], x[1], y[0], y[1]};
         }
     }
-    // row: element offset of this lane's key in its page tensor; dimensions past the head's size read its first ones (their q is 0)
-    __device__ __forceinline__ void load_k(int u, const void* base, long long row, int D, int g, int, const KvView&, long long) {
-        const bf16* p = (const bf16*)base + row * D;
+    static __device__ __forceinline__ int row_bytes(int D) { return 2 * D; }
+    static __device__ __forceinline__ int step_bytes() { return 0; }
+    // tile: where row 0 of the 16 rows of tile u lies; dimensions past the head's size read its first ones (their q is 0)
+    __device__ __forceinline__ void load_k(int u, const char* tile, const char*, int D, int g, int cq) {
 #pragma unroll
-        for (int s = 0; s < NS; ++s) { const int d = 32 * s + 8 * g; k[u][s] = *(const u32x4*)(p + (d < D ? d : 0)); }
+        for (int s = 0; s < NS; ++s) {
+            const int d = 32 * s + 8 * g;
+            k[u][s] = *(const u32x4*)(tile + (unsigned)(2 * (cq * D + (d < D ? d : 0))));
+        }
     }
-    __device__ __forceinline__ void load_v(int u, const void* base, long long row, int D, int m, const KvView&) {
-        const bf16* p = (const bf16*)base + row * D + (m * DV < D ? m * DV : 0);
+    __device__ __forceinline__ void load_v(int u, const char* tile, const char*, int D, int g, int m) {
+        const unsigned off = (unsigned)(2 * (4 * g * D + (m * DV < D ? m * DV : 0)));
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            if constexpr (VW == 2) { const u32x2 x = *(const u32x2*)(p + r * D); v[4 * u + r][0] = x[0]; v[4 * u + r][1] = x[1]; }
+            const char* p = tile + 2 * r * D;
+            if constexpr (VW == 2) { const u32x2 x = *(const u32x2*)(p + off); v[4 * u + r][0] = x[0]; v[4 * u + r][1] = x[1]; }
             else
 #pragma unroll
                 for (int w = 0; w < VW; w += 4) {
-                    const u32x4 x = *(const u32x4*)(p + r * D + 2 * w);
+                    const u32x4 x = *(const u32x4*)(p + off + 4 * w);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[4 * u + r][w + e] = x[e];
                 }
@@ -171,17 +176,18 @@ template <int DP> struct Chunk<float, DP> {
             if (on && 16 * s < D) q.f[s] = *(const f32x4*)(p + 16 * s + 4 * g);
         }
     }
-    __device__ __forceinline__ void load_k(int, const void* base, long long row, int D, int g, int, const KvView&, long long) {
-        const float* p = (const float*)base + row * D + 4 * g;
+    static __device__ __forceinline__ int row_bytes(int D) { return 4 * D; }
+    static __device__ __forceinline__ int step_bytes() { return 0; }
+    __device__ __forceinline__ void load_k(int, const char* tile, const char*, int D, int g, int cq) {
 #pragma unroll
-        for (int s = 0; s < NS; ++s) k[0][s] = *(const f32x4*)(p + (16 * s < D ? 16 * s : 0));
+        for (int s = 0; s < NS; ++s) k[0][s] = *(const f32x4*)(tile + (unsigned)(4 * (cq * D + 4 * g + (16 * s < D ? 16 * s : 0))));
     }
-    __device__ __forceinline__ void load_v(int, const void* base, long long row, int D, int m, const KvView&) {
-        const float* p = (const float*)base + row * D + (m * DV < D ? m * DV : 0);
+    __device__ __forceinline__ void load_v(int, const char* tile, const char*, int D, int g, int m) {
+        const unsigned off = (unsigned)(4 * (4 * g * D + (m * DV < D ? m * DV : 0)));
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int w = 0; w < DV / 4; ++w) v[r][w] = *(const f32x4*)(p + r * D + 4 * w);
+            for (int w = 0; w < DV / 4; ++w) v[r][w] = *(const f32x4*)(tile + 4 * r * D + off + 16 * w);
     }
     template <typename Keep> __device__ __forceinline__ void hide(int, Keep keep) {
 #pragma unroll
@@ -252,22 +258,24 @@ template <int D> struct Chunk<Int4, D> {
                 for (int e = 0; e < 4; ++e) d[w + e] = x[e];
             }
     }
-    static __device__ __forceinline__ void load_steps(float* d, const bf16* p, int cq) {
+    static __device__ __forceinline__ int row_bytes(int) { return D / 2; }
+    static __device__ __forceinline__ int step_bytes() { return 2 * S; }
+    static __device__ __forceinline__ void load_steps(float* d, const char* p, int g, int cq) {
 #pragma unroll
-        for (int w = 0; w < SW; ++w) d[w] = (float)p[S == 2 ? cq & 7 : 16 * w + cq];
+        for (int w = 0; w < SW; ++w) d[w] = (float)*(const bf16*)(p + (unsigned)(2 * (4 * g * S + (S == 2 ? cq & 7 : 16 * w + cq))));
     }
-    __device__ __forceinline__ void load_k(int u, const void* base, long long row, int, int g, int cq, const KvView& c, long long row4) {
-        load_dw<S>(k[u], (const char*)base + row * (D / 2) + g * 4 * S);
-        load_steps(ks[u], c.ks + row4 * S, cq);
+    __device__ __forceinline__ void load_k(int u, const char* tile, const char* steps, int, int g, int cq) {
+        load_dw<S>(k[u], tile + (unsigned)(cq * (D / 2) + g * 4 * S));
+        load_steps(ks[u], steps, g, cq);
     }
-    __device__ __forceinline__ void load_v(int u, const void* base, long long row, int, int m, const KvView& c) {
-        const char* p = (const char*)base + row * (D / 2) + m * S;
+    __device__ __forceinline__ void load_v(int u, const char* tile, const char* steps, int, int g, int m) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            if constexpr (S == 2) v[4 * u + r][0] = *(const unsigned short*)(p + r * (D / 2));
-            else load_dw<S / 4>(v[4 * u + r], p + r * (D / 2));
+            const char* p = tile + (unsigned)(4 * g * (D / 2) + m * S) + r * (D / 2);
+            if constexpr (S == 2) v[4 * u + r][0] = *(const unsigned short*)p;
+            else load_dw<S / 4>(v[4 * u + r], p);
         }
-        load_steps(vs[u], c.vs + row * S, m);
+        load_steps(vs[u], steps, g, m);
     }
     // keep(u, r): whether key 4 g + r of tile u counts.  Its step is what goes: a NaN there must not meet its probability 0.
     template <typename Keep> __device__ __forceinline__ void hide(int cq, Keep keep) {
@@ -323,7 +331,7 @@ struct KvPart { float *sums, *ml; };           // [16][DP], [16][2]
 
 // The four waves take the chunks in turn, each with a running maximum and sum of its own, and are joined through LDS at the end.  Bound
 // by memory for single tokens: the next chunk's keys are requested before this one's softmax, its values before this one's scores.
-template <typename T, int DP, typename Part>
+template <typename T, int DP, bool P8, typename Part>
 __device__ __forceinline__ void attend_part(const KvAttendArgs& a, const Tile& t, const Span& span, int hk, int cb, int ce, bool whole_row, Part part_of,
                                             float (*so)[16][DP + 4], float (*sm)[16], float (*sl)[16]) {
     typedef Chunk<T, DP> C;
@@ -340,10 +348,16 @@ __device__ __forceinline__ void attend_part(const KvAttendArgs& a, const Tile& t
     typename C::Q q;
     C::load_q(q, (const A*)a.q.p + (long long)(t.tok0 + qtok) * a.q.ts + (long long)(hk * G + col - qtok * G) * a.q.hs, D, g, mypos >= 0);
 
-    const int* table = a.c.table + (long long)max(t.row, 0) * a.c.width;
-    const long long page_rows = (long long)a.c.heads << sh;                    // rows of one page, all heads
+    // The table is read through the scalar cache (nothing in this launch writes it), apart from the vector loads and their order.  Pages of 16
+    // tokens and more: the 16 rows of a tile lie in one page, so its address is the same for the wave and a lane adds a constant.  (P8: pages
+    // of 8, two to a tile.)
+    typedef const __attribute__((address_space(4))) int* Entries;
+    const Entries table = (Entries)(unsigned long long)(a.c.table + (long long)max(t.row, 0) * a.c.width);
+    const int in_page = (1 << sh) - 1, last_entry = a.c.width - 1, rb = C::row_bytes(D), sb = C::step_bytes();
+    const unsigned page_rows = (unsigned)a.c.heads << sh;                      // rows of one page, all heads
     const long long head0 = ((long long)a.layer * a.c.pages * a.c.heads + hk) << sh;
-    const int in_page = (1 << sh) - 1, last_entry = a.c.width - 1;
+    const char *kb = (const char*)a.c.k + head0 * rb, *vb = (const char*)a.c.v + head0 * rb;
+    const char *ksb = (const char*)a.c.ks + head0 * sb, *vsb = (const char*)a.c.vs + head0 * sb;
     const int W = a.window > 0 ? a.window : 0x7fffffff, sinks = a.window > 0 ? a.sinks : 0;
 
     const float cs = a.scale_log2e;
@@ -357,20 +371,28 @@ __device__ __forceinline__ void attend_part(const KvAttendArgs& a, const Tile& t
 #pragma unroll
         for (int i = 0; i < NT; ++i) o[i] = f32x4{0, 0, 0, 0};
         float m = -INFINITY, l = 0.f;
-        int ek[C::TILES], ev[C::TILES];
+        int e0[C::TILES], e1[C::TILES];        // the pages of a tile's rows 0 .. 7 and 8 .. 15
         C ch;
         auto entries = [&](int tb) {
 #pragma unroll
             for (int u = 0; u < C::TILES; ++u) {
-                ek[u] = table[min((tb + 16 * u + cq) >> sh, last_entry)];
-                ev[u] = table[min((tb + 16 * u + 4 * g) >> sh, last_entry)];
+                e0[u] = table[min((tb + 16 * u) >> sh, last_entry)];
+                e1[u] = P8 ? table[min((tb + 16 * u + 8) >> sh, last_entry)] : e0[u];
             }
         };
-        auto row_of = [&](int e, int tok) { return head0 + (long long)((unsigned)e < (unsigned)a.c.pages ? e : 0) * page_rows + (tok & in_page); };
+        auto good = [&](int e) { return (unsigned)e < (unsigned)a.c.pages; };
+        auto row = [&](const char* base, int e, int first, int bytes) { return base + (unsigned long long)(good(e) ? (unsigned)e : 0u) * (page_rows * (unsigned)bytes) + first * bytes; };
         auto keys = [&](int tb) {
 #pragma unroll
-            for (int u = 0; u < C::TILES; ++u)
-                ch.load_k(u, a.c.k, row_of(ek[u], tb + 16 * u + cq), D, g, cq, a.c, row_of(ev[u], tb + 16 * u + 4 * g));
+            for (int u = 0; u < C::TILES; ++u) {
+                const int first = (tb + 16 * u) & in_page;
+                if constexpr (!P8) {
+                    ch.load_k(u, row(kb, e0[u], first, rb), row(ksb, e0[u], first, sb), D, g, cq);
+                } else {
+                    const int ek = cq & 8 ? e1[u] : e0[u], ev = g & 2 ? e1[u] : e0[u];
+                    ch.load_k(u, row(kb, ek, -(cq & 8), rb), row(ksb, ev, -4 * (g & 2), sb), D, g, cq);
+                }
+            }
         };
         int c = cb + wave, tb = 0;
         if (c < ce) {
@@ -383,9 +405,16 @@ __device__ __forceinline__ void attend_part(const KvAttendArgs& a, const Tile& t
             int ok[C::TILES];
 #pragma unroll
             for (int u = 0; u < C::TILES; ++u) {
-                ch.load_v(u, a.c.v, row_of(ev[u], tb + 16 * u + 4 * g), D, cq, a.c);
-                ok[u] = (unsigned)ev[u] < (unsigned)a.c.pages;
-                pages_ok = pages_ok && ok[u];
+                const int first = (tb + 16 * u) & in_page;
+                if constexpr (!P8) {
+                    ch.load_v(u, row(vb, e0[u], first, rb), row(vsb, e0[u], first, sb), D, g, cq);
+                    ok[u] = good(e0[u]);
+                } else {
+                    const int ev = g & 2 ? e1[u] : e0[u];
+                    ch.load_v(u, row(vb, ev, -4 * (g & 2), rb), row(vsb, ev, -4 * (g & 2), sb), D, g, cq);
+                    ok[u] = good(ev);
+                }
+                pages_ok = pages_ok && good(e0[u]) && good(e1[u]);
             }
             const int now = tb;
             c += 4;
@@ -399,7 +428,7 @@ __device__ __forceinline__ void attend_part(const KvAttendArgs& a, const Tile& t
                 for (int r = 0; r < 4; ++r) x[4 * u + r] = s[r];
             }
             keys(tb);
-            const bool whole = now + TB - 1 <= t.pmin && (now > t.pmax - W || now + TB - 1 < sinks) && __all(pages_ok);
+            const bool whole = now + TB - 1 <= t.pmin && (now > t.pmax - W || now + TB - 1 < sinks) && pages_ok;
             if (!whole) {
 #pragma unroll
                 for (int j = 0; j < 4 * C::TILES; ++j) {
@@ -521,7 +550,7 @@ __device__ __forceinline__ long long kv_flat_run(long long units, int runs) {
 // workgroups of a compute unit = waves of a SIMD, by the registers the kernel needs
 __host__ __device__ constexpr int flat_waves(bool four_bits, int dp) { return dp == 256 ? 1 : dp == 64 ? 4 : four_bits ? 3 : 2; }
 
-template <typename T, int DP>
+template <typename T, int DP, bool P8>
 __global__ void __launch_bounds__(256, flat_waves(__is_same(T, Int4), DP)) kv_flat_kernel(const KvAttendArgs a, int tiles) {
     typedef Chunk<T, DP> C;
     typedef typename C::act A;
@@ -579,7 +608,7 @@ __global__ void __launch_bounds__(256, flat_waves(__is_same(T, Int4), DP)) kv_fl
     for (;;) {
         const int ce = min(len, cb + left);
         const Tile t = kv_tile(a, x, 16, lane);
-        attend_part<T, DP>(a, t, kv_span(a, t, TB), hk, cb, ce, cb == 0 && ce == len, [&]() {
+        attend_part<T, DP, P8>(a, t, kv_span(a, t, TB), hk, cb, ce, cb == 0 && ce == len, [&]() {
             const KvFlat ws(a.ws, runs, DP, a.group);
             return KvPart{ws.sums + (long long)slot * ws.cols * DP, ws.ml + (long long)slot * ws.cols * 2};
         }, so, sm, sl);
@@ -663,7 +692,7 @@ struct KvShares {
         used = (int*)(a.ws + n * rows * (dp + 2)) + i;
     }
 };
-template <typename T, int DP>
+template <typename T, int DP, bool P8>
 __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_attend_kernel(const KvAttendArgs a) {
     constexpr int TB = 16 * Chunk<T, DP>::TILES;
     __shared__ __attribute__((aligned(16))) float so[4][16][DP + 4];
@@ -677,7 +706,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_attend_kernel(const
     if (a.splits > 1 && z == 0 && threadIdx.x == 0)
         *KvShares(a, gridDim.x, DP, blockIdx.x, hk).used = shared ? min(a.splits, (span.total + a.share - 1) / a.share) : 1;
     const int ce = shared && z + 1 < a.splits ? min(span.total, (z + 1) * a.share) : span.total;       // a bound on lengths that was too low: the last share's
-    attend_part<T, DP>(a, t, span, hk, z * a.share, ce, !shared, [&]() {
+    attend_part<T, DP, P8>(a, t, span, hk, z * a.share, ce, !shared, [&]() {
         const KvShares ws(a, gridDim.x, DP, blockIdx.x, hk);
         return KvPart{ws.sums + z * 16ll * DP, ws.ml + z * 32ll};
     }, so, sm, sl);
@@ -1140,10 +1169,12 @@ hipError_t q3_launch_kv_attend(const KvAttendArgs& a, hipStream_t s) {
 #define Q3_ATTEND(T, A, DP)                                                        \
     do {                                                                           \
         if (runs) {                                                                \
-            kv_flat_kernel<T, DP><<<runs, 256, 0, s>>>(a, (int)tiles);             \
+            if (a.c.ps_shift == 3) kv_flat_kernel<T, DP, true><<<runs, 256, 0, s>>>(a, (int)tiles);  \
+            else kv_flat_kernel<T, DP, false><<<runs, 256, 0, s>>>(a, (int)tiles); \
             kv_flat_join_kernel<A, DP><<<join, 256, 0, s>>>(a, (int)tiles, runs);  \
         } else {                                                                   \
-            kv_attend_kernel<T, DP><<<grid, 256, 0, s>>>(a);                       \
+            if (a.c.ps_shift == 3) kv_attend_kernel<T, DP, true><<<grid, 256, 0, s>>>(a);            \
+            else kv_attend_kernel<T, DP, false><<<grid, 256, 0, s>>>(a);           \
             if (a.splits > 1) kv_join_kernel<A, DP><<<join, 256, 0, s>>>(a);       \
         }                                                                          \
     } while (0)
