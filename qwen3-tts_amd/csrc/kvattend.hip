@@ -371,55 +371,44 @@ __device__ __forceinline__ void attend_part(const KvAttendArgs& a, const Tile& t
 #pragma unroll
         for (int i = 0; i < NT; ++i) o[i] = f32x4{0, 0, 0, 0};
         float m = -INFINITY, l = 0.f;
-        int e0[C::TILES], e1[C::TILES];        // the pages of a tile's rows 0 .. 7 and 8 .. 15
-        C ch;
+        struct Pages { int lo[C::TILES], hi[C::TILES]; };                     // of a tile's rows 0 .. 7 and 8 .. 15
         auto entries = [&](int tb) {
+            Pages e;
 #pragma unroll
             for (int u = 0; u < C::TILES; ++u) {
-                e0[u] = table[min((tb + 16 * u) >> sh, last_entry)];
-                e1[u] = P8 ? table[min((tb + 16 * u + 8) >> sh, last_entry)] : e0[u];
+                e.lo[u] = table[min((tb + 16 * u) >> sh, last_entry)];
+                e.hi[u] = P8 ? table[min((tb + 16 * u + 8) >> sh, last_entry)] : e.lo[u];
             }
+            return e;
         };
         auto good = [&](int e) { return (unsigned)e < (unsigned)a.c.pages; };
         auto row = [&](const char* base, int e, int first, int bytes) { return base + (unsigned long long)(good(e) ? (unsigned)e : 0u) * (page_rows * (unsigned)bytes) + first * bytes; };
-        auto keys = [&](int tb) {
+        auto keys = [&](C& ch, const Pages& e, int tb) {
 #pragma unroll
             for (int u = 0; u < C::TILES; ++u) {
                 const int first = (tb + 16 * u) & in_page;
                 if constexpr (!P8) {
-                    ch.load_k(u, row(kb, e0[u], first, rb), row(ksb, e0[u], first, sb), D, g, cq);
+                    ch.load_k(u, row(kb, e.lo[u], first, rb), row(ksb, e.lo[u], first, sb), D, g, cq);
                 } else {
-                    const int ek = cq & 8 ? e1[u] : e0[u], ev = g & 2 ? e1[u] : e0[u];
+                    const int lo = e.lo[u], hi = e.hi[u], ek = cq & 8 ? hi : lo, ev = g & 2 ? hi : lo;
                     ch.load_k(u, row(kb, ek, -(cq & 8), rb), row(ksb, ev, -4 * (g & 2), sb), D, g, cq);
                 }
             }
         };
-        int c = cb + wave, tb = 0;
-        if (c < ce) {
-            tb = span.chunk(c) * TB;
-            entries(tb);
-            keys(tb);
-        }
-        while (c < ce) {
-            bool pages_ok = true;
-            int ok[C::TILES];
+        auto values = [&](C& ch, const Pages& e, int tb) {
 #pragma unroll
             for (int u = 0; u < C::TILES; ++u) {
                 const int first = (tb + 16 * u) & in_page;
                 if constexpr (!P8) {
-                    ch.load_v(u, row(vb, e0[u], first, rb), row(vsb, e0[u], first, sb), D, g, cq);
-                    ok[u] = good(e0[u]);
+                    ch.load_v(u, row(vb, e.lo[u], first, rb), row(vsb, e.lo[u], first, sb), D, g, cq);
                 } else {
-                    const int ev = g & 2 ? e1[u] : e0[u];
+                    const int lo = e.lo[u], hi = e.hi[u], ev = g & 2 ? hi : lo;
                     ch.load_v(u, row(vb, ev, -4 * (g & 2), rb), row(vsb, ev, -4 * (g & 2), sb), D, g, cq);
-                    ok[u] = good(ev);
                 }
-                pages_ok = pages_ok && good(e0[u]) && good(e1[u]);
             }
-            const int now = tb;
-            c += 4;
-            tb = span.chunk(min(c, ce - 1)) * TB;          // past the end: the last chunk again, and not looked at
-            entries(tb);
+        };
+        // one chunk, at token `now` with pages `e`: scores, `between`, softmax, values
+        auto consume = [&](C& ch, const Pages& e, int now, auto between) {
             float x[4 * C::TILES];
 #pragma unroll
             for (int u = 0; u < C::TILES; ++u) {
@@ -427,18 +416,24 @@ __device__ __forceinline__ void attend_part(const KvAttendArgs& a, const Tile& t
 #pragma unroll
                 for (int r = 0; r < 4; ++r) x[4 * u + r] = s[r];
             }
-            keys(tb);
-            const bool whole = now + TB - 1 <= t.pmin && (now > t.pmax - W || now + TB - 1 < sinks) && pages_ok;
+            between();
+            bool whole = now + TB - 1 <= t.pmin && (now > t.pmax - W || now + TB - 1 < sinks);
+#pragma unroll
+            for (int u = 0; u < C::TILES; ++u) whole = whole && good(e.lo[u]) && good(e.hi[u]);
             if (!whole) {
+                auto there = [&](int u) {
+                    const int lo = e.lo[u], hi = e.hi[u];
+                    return good(P8 && (g & 2) ? hi : lo);
+                };
 #pragma unroll
                 for (int j = 0; j < 4 * C::TILES; ++j) {
                     const int tok = now + 16 * (j >> 2) + 4 * g + (j & 3);
-                    const bool sees = ok[j >> 2] && tok <= mypos && (tok > mypos - W || tok < sinks);
+                    const bool sees = there(j >> 2) && tok <= mypos && (tok > mypos - W || tok < sinks);
                     x[j] = sees ? x[j] : -INFINITY;
                 }
                 ch.hide(cq, [&](int u, int r) {
                     const int tok = now + 16 * u + 4 * g + r;
-                    return ok[u] && tok <= vhi && (tok > vlo || tok < sinks);
+                    return there(u) && tok <= vhi && (tok > vlo || tok < sinks);
                 });
             }
             float top = x[0];
@@ -460,6 +455,19 @@ __device__ __forceinline__ void attend_part(const KvAttendArgs& a, const Tile& t
                 l += x[j];
             }
             ch.weigh(x, o, magic);
+        };
+        int c = cb + wave;
+        auto at = [&](int i) { return span.chunk(min(i, ce - 1)) * TB; };      // past the end: the last chunk again, and not looked at
+        if (c < ce) {
+            C ch;
+            Pages p = entries(at(c));
+            keys(ch, p, at(c));
+            do {
+                values(ch, p, at(c));
+                const Pages next = entries(at(c + 4));
+                consume(ch, p, at(c), [&] { keys(ch, next, at(c + 4)); });
+                p = next;
+            } while ((c += 4) < ce);
         }
         l += __shfl_xor(l, 16);
         l += __shfl_xor(l, 32);
