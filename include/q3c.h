@@ -327,7 +327,7 @@ typedef struct q3c_kv {
 } q3c_kv;
 /* Make room for the new tokens: lens[row] grows by each request's count, pages are taken lowest free first, in the order of the call. */
 int q3c_kv_reserve(const q3c_kv* kv, const int32_t* rows, const int32_t* offsets, int32_t sequences, int32_t tokens, void* hip_stream);
-/* Per head of q and k: y = x * rsqrt(mean(x^2) + eps) * weight (NULL weight: no norm), then the first rot_dim dimensions turned by
+/* Per head of q and k: y = x * rsqrt(mean(x^2) + eps) * weight (NULL weight: no norm; eps > 0), then the first rot_dim dimensions turned by
  * the token's position: (a, b) = (y[i], y[i + rot_dim / 2]) -> (a cos - b sin, b cos + a sin), tables [positions][rot_dim / 2] fp32 with
  * positions >= page_size * pages_per_row (rot_dim 0: no rotation; rot_dim a multiple of 8, INT4: 0 or head_dim).  fp32 throughout, rounded once.  k and
  * v go to the pages (INT4: groups of 32 dimensions, step = bf16(max |x| / 7), n = rint(x / step); a group with an infinity or a NaN

@@ -30,6 +30,7 @@ struct KvAttendArgs {
     int q_heads, group, window, sinks;
     float scale_log2e;
     void* out;                                                  // [tokens][q_heads][dim]
+    int most;                                                   // chunks that a row can see
     int splits, share;                                          // shares of a tile's key chunks: most there can be, chunks of one
     float* ws;
 };
@@ -40,7 +41,7 @@ hipError_t q3_launch_kv_release(const KvView& c, const int* rows, int count, int
 hipError_t q3_launch_kv_fork(const KvView& c, const int* parents, const int* children, int count, int* ws, hipStream_t s);
 hipError_t q3_launch_kv_copy(const KvView& c, const int* src, const int* dst, int count, int* ws, hipStream_t s);
 hipError_t q3_launch_kv_compact(const KvView& c, int* live, int* ws, hipStream_t s);
-struct KvSplit { int splits, share; };
+struct KvSplit { int splits, share, most; };
 KvSplit q3_kv_attend_split(const KvView& c, int tokens, int sequences, int q_heads, bool ragged, int window, int sinks, int max_len);
 size_t q3_kv_attend_ws(const KvView& c, int tokens, int sequences, int q_heads, bool ragged, int splits);
 hipError_t q3_launch_kv_attend(const KvAttendArgs& a, hipStream_t s);

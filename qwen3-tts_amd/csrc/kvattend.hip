@@ -83,6 +83,8 @@ __device__ __forceinline__ unsigned pack2(float a, float b) {
     typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{a, b}), bf16x2));
 }
+__device__ __forceinline__ void store4(float* p, f32x4 x) { *(f32x4*)p = x; }
+__device__ __forceinline__ void store4(bf16* p, f32x4 x) { *(u32x2*)p = u32x2{pack2(x[0], x[1]), pack2(x[2], x[3])}; }
 __device__ __forceinline__ float lo_f(unsigned x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float hi_f(unsigned x) { return __uint_as_float(x & 0xffff0000u); }
 
@@ -161,6 +163,14 @@ template <int DP> struct Chunk<bf16, DP> {
         }
     }
     static __device__ __forceinline__ int dim(int i, int m) { return m * DV + i; }      // of row m of output tile i
+    // a lane's values of one column: rows 4 g + r of all tiles
+    template <typename E, typename Get> static __device__ __forceinline__ void store(E* out, int D, int g, Get get) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if ((4 * g + r) * DV < D)
+#pragma unroll
+                for (int i = 0; i < DV; i += 4) store4(out + (4 * g + r) * DV + i, f32x4{get(i, r), get(i + 1, r), get(i + 2, r), get(i + 3, r)});
+    }
 };
 
 template <int DP> struct Chunk<float, DP> {
@@ -211,6 +221,13 @@ template <int DP> struct Chunk<float, DP> {
             for (int i = 0; i < DV; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][i >> 2][i & 3], p[r], o[i], 0, 0, 0);
     }
     static __device__ __forceinline__ int dim(int i, int m) { return m * DV + i; }
+    template <typename E, typename Get> static __device__ __forceinline__ void store(E* out, int D, int g, Get get) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if ((4 * g + r) * DV < D)
+#pragma unroll
+                for (int i = 0; i < DV; i += 4) store4(out + (4 * g + r) * DV + i, f32x4{get(i, r), get(i + 1, r), get(i + 2, r), get(i + 3, r)});
+    }
 };
 
 // 4 bits: a half byte n + 8 under the exponent of 128 IS the bf16 number 128 + (n + 8) (7 fraction bits), one and-or per two values.
@@ -323,15 +340,20 @@ template <int D> struct Chunk<Int4, D> {
         });
     }
     static __device__ __forceinline__ int dim(int i, int m) { return 16 * i + m; }
+    template <typename E, typename Get> static __device__ __forceinline__ void store(E* out, int, int g, Get get) {
+#pragma unroll
+        for (int i = 0; i < DV; ++i) store4(out + 16 * i + 4 * g, f32x4{get(i, 0), get(i, 1), get(i, 2), get(i, 3)});
+    }
 };
 
 // Work on one tile of columns and one kv head: chunks cb .. ce - 1 of those the tile sees, whole (`out`) or as a part of them (unnormalised
 // sums, maxima and weights: `part`).
 struct KvPart { float *sums, *ml; };           // [16][DP], [16][2]
 
-// The four waves take the chunks in turn, each with a running maximum and sum of its own, and are joined through LDS at the end.  Bound
+// The workgroup's waves take the chunks in turn, each with a running maximum and sum of its own, and are joined through LDS at the end
+// (WAVES = 4), or a wave has all of them and writes the result itself (WAVES = 1: no LDS, no barrier, waves on tiles of their own).  Bound
 // by memory for single tokens: the next chunk's keys are requested before this one's softmax, its values before this one's scores.
-template <typename T, int DP, bool P8, typename Part>
+template <typename T, int DP, bool P8, int WAVES, typename Part>
 __device__ __forceinline__ void attend_part(const KvAttendArgs& a, const Tile& t, const Span& span, int hk, int cb, int ce, bool whole_row, Part part_of,
                                             float (*so)[16][DP + 4], float (*sm)[16], float (*sl)[16]) {
     typedef Chunk<T, DP> C;
@@ -339,7 +361,7 @@ __device__ __forceinline__ void attend_part(const KvAttendArgs& a, const Tile& t
     constexpr int TB = 16 * C::TILES, NT = DP / 16;
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));              // made new for each part: what follows from it is not kept in registers from one to the next
-    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = tid & 63, wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
     const int cq = lane & 15, g = lane >> 4;
     const int G = a.group, D = a.c.dim, sh = a.c.ps_shift;
     const int col = t.col0 + cq, qtok = col / G;
@@ -464,14 +486,27 @@ __device__ __forceinline__ void attend_part(const KvAttendArgs& a, const Tile& t
             keys(ch, p, at(c));
             do {
                 values(ch, p, at(c));
-                const Pages next = entries(at(c + 4));
-                consume(ch, p, at(c), [&] { keys(ch, next, at(c + 4)); });
+                const Pages next = entries(at(c + WAVES));
+                consume(ch, p, at(c), [&] { keys(ch, next, at(c + WAVES)); });
                 p = next;
-            } while ((c += 4) < ce);
+            } while ((c += WAVES) < ce);
         }
         l += __shfl_xor(l, 16);
         l += __shfl_xor(l, 32);
-        if (all || mypos == only) {
+        if (WAVES == 1) {
+            if (col < t.ncols && (all || mypos == only)) {
+                if (whole_row) {
+                    const bool none = mypos < 0 || l == 0.f;
+                    const float inv = 1.0f / l;
+                    A* out = (A*)a.out + ((long long)(t.tok0 + qtok) * a.q_heads + hk * G + col - qtok * G) * D;
+                    C::store(out, D, g, [&](int i, int r) { return none ? 0.f : o[i][r] * inv; });
+                } else {
+                    const KvPart part = part_of();
+                    C::store(part.sums + cq * DP, D, g, [&](int i, int r) { return o[i][r]; });
+                    if (g == 0) { part.ml[2 * cq] = mypos < 0 ? -INFINITY : m; part.ml[2 * cq + 1] = mypos < 0 ? 0.f : l; }
+                }
+            }
+        } else if (all || mypos == only) {
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -491,6 +526,7 @@ __device__ __forceinline__ void attend_part(const KvAttendArgs& a, const Tile& t
         }
         if (++only > t.pmax) break;
     }
+    if constexpr (WAVES == 1) return;
     __syncthreads();
     // join the four waves; thread (c, j) takes DP / 16 dimensions of column c
     const int c = tid >> 4, d0 = (tid & 15) * (DP / 16);
@@ -529,33 +565,46 @@ __device__ __forceinline__ void attend_part(const KvAttendArgs& a, const Tile& t
 }
 
 // ---- single tokens: one new token per row, up to FLAT tiles --------------------------------------------------------------------------
-// A launch of as many workgroups as run at once; all (tile, kv head, chunk) triples in one line, cut into that many equal runs.  So
-// long rows and short ones, few and many, load the card alike, whatever the host does not know about lengths.  A workgroup's run touches
-// whole (tile, head) pairs and at most two in part, its first and its last: two parts per workgroup are all the workspace there is, and
+// A launch of as many waves as run at once; all (tile, kv head, chunk) triples in one line, cut into that many equal runs.  So long rows and
+// short ones, few and many, load the card alike, whatever the host does not know about lengths.  A wave's run touches whole (tile,
+// head) pairs and at most two in part, its first and its last: two parts per wave are all the workspace there is, and
 // kv_flat_join_kernel puts the parts together.  Each workgroup finds the line's layout by itself: the chunk counts of all tiles, summed up.
-constexpr int FLAT = 512;
-constexpr int FLAT_LEAST = 8;                  // chunks of a run: two rounds of its waves
+// A run for each wave rather than for each workgroup: no meeting of waves at a pair's end, which short rows have often (64 rows of 512
+// tokens in 4 bits 24 us against 47, in bf16 31 against 44; 32 rows of 16001 in bf16 226 us against 223: 5.5 TB/s).
+constexpr int FLAT = 1024;
+constexpr int FLAT_LEAST = 4;                  // chunks of a run
 
-struct KvFlat {                                // the workspace
-    long long* before;                         // [tiles + 1] chunks of the tiles before, for one head
+struct KvFlat {                                // the workspace (the entry point keeps the line below 2^31 chunks)
+    int* before;                               // [tiles + 1] chunks of the tiles before, for one head
     float *sums, *ml;                          // parts [2 runs][min(16, group)][DP], [..][2]
     int cols;
     __host__ __device__ KvFlat(float* ws, int runs, int dp, int group) {
-        before = (long long*)ws;
+        before = (int*)ws;
         cols = group < 16 ? group : 16;
-        sums = ws + 2 * (FLAT + 2);
+        sums = ws + FLAT + 4;
         ml = sums + 2ll * runs * cols * dp;
     }
     __host__ __device__ static size_t bytes(int runs, int dp, int group) {
-        return (2 * (FLAT + 2) + 2ull * runs * (group < 16 ? group : 16) * (dp + 2)) * sizeof(float);
+        return (FLAT + 4 + 2ull * runs * (group < 16 ? group : 16) * (dp + 2)) * sizeof(float);
     }
 };
-__device__ __forceinline__ long long kv_flat_run(long long units, int runs) {
-    const long long n = (units + runs - 1) / runs;
-    return n < FLAT_LEAST ? FLAT_LEAST : n;
+__device__ __forceinline__ int kv_flat_run(int units, int runs) { return max((units + runs - 1) / runs, FLAT_LEAST); }
+// a tile of single tokens, given its table row and length
+__device__ __forceinline__ Tile kv_flat_tile(const KvAttendArgs& a, int x, int row, int len) {
+    Tile t;
+    const int per = (a.group + 15) / 16;
+    t.on = true;
+    t.seq = t.tok0 = per == 1 ? x : x / per;
+    t.col0 = (x - t.seq * per) * 16;
+    t.ncols = a.group;
+    t.row = row >= 0 && row < a.c.rows ? row : -1;
+    t.first_pos = len - 1;
+    t.pmin = max(t.first_pos, 0);
+    t.pmax = t.row < 0 ? -1 : min(t.first_pos, (a.c.width << a.c.ps_shift) - 1);
+    return t;
 }
 
-// workgroups of a compute unit = waves of a SIMD, by the registers the kernel needs
+// waves of a SIMD, by the registers the kernel needs
 __host__ __device__ constexpr int flat_waves(bool four_bits, int dp) { return dp == 256 ? 1 : dp == 64 ? 4 : four_bits ? 3 : 2; }
 
 template <typename T, int DP, bool P8>
@@ -563,73 +612,85 @@ __global__ void __launch_bounds__(256, flat_waves(__is_same(T, Int4), DP)) kv_fl
     typedef Chunk<T, DP> C;
     typedef typename C::act A;
     constexpr int TB = 16 * C::TILES;
-    __shared__ __attribute__((aligned(16))) float so[4][16][DP + 4];
-    __shared__ float sm[4][16], sl[4][16];
-    __shared__ long long before[FLAT + 1], wave_sum[4];
-    __shared__ int first_tile;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, runs = gridDim.x, heads = a.c.heads;
-    const KvFlat ws(a.ws, runs, DP, a.group);
-    int n[2];
+    constexpr int PER = FLAT / 256;
+    __shared__ int before[FLAT + 1], row_of[FLAT], len_of[FLAT], wave_sum[4], first_tile[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), runs = 4 * gridDim.x, heads = a.c.heads;
+    const int per_token = (a.group + 15) / 16;
+    int n[PER], sum = 0;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {              // thread t counts the chunks of tiles 2 t and 2 t + 1
-        const int x = 2 * tid + k;
+    for (int k = 0; k < PER; ++k) {            // thread t counts the chunks of tiles PER t ..
+        const int x = PER * tid + k;
         n[k] = 0;
-        if (x < tiles) n[k] = kv_span(a, kv_tile(a, x, 16, 0), TB).total;
+        if (x < tiles) {
+            const int row = a.b.rows[per_token == 1 ? x : x / per_token], len = row >= 0 && row < a.c.rows ? a.c.lens[row] : 0;
+            row_of[x] = row;
+            len_of[x] = len;
+            n[k] = kv_span(a, kv_flat_tile(a, x, row, len), TB).total;
+        }
+        sum += n[k];
     }
-    long long sum = (long long)n[0] + n[1];
+    const int mine = sum;
 #pragma unroll
     for (int k = 1; k < 64; k <<= 1) {
-        const long long y = __shfl_up(sum, k);
+        const int y = __shfl_up(sum, k);
         if (lane >= k) sum += y;
     }
     if (lane == 63) wave_sum[wave] = sum;
     __syncthreads();
     for (int w = 0; w < wave; ++w) sum += wave_sum[w];
-    if (2 * tid < tiles) before[2 * tid + 1] = sum - n[1];
-    if (2 * tid + 1 < tiles) before[2 * tid + 2] = sum;
-    if (tid == 0) { before[0] = 0; first_tile = tiles; }
+    const int units = (wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3]) * heads, run = kv_flat_run(units, runs);
+    int b = sum - mine;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int x = PER * tid + k;
+        if (x <= tiles) {
+            before[x] = b;
+            if (blockIdx.x == 0) KvFlat(a.ws, runs, DP, a.group).before[x] = b;
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const int u = (4 * blockIdx.x + w) * run;
+            if (b * heads <= u && u < (b + n[k]) * heads) first_tile[w] = x;
+        }
+        b += n[k];
+    }
+    if (tid == 255 && tiles == FLAT) {
+        before[FLAT] = b;
+        if (blockIdx.x == 0) KvFlat(a.ws, runs, DP, a.group).before[FLAT] = b;
+    }
     __syncthreads();
-    const long long units = before[tiles] * heads, run = kv_flat_run(units, runs);
-    long long u = blockIdx.x * run;
-    const long long end = min(u + run, units);
-    for (int x = tid; x < tiles; x += 256)
-        if (before[x] * heads <= u && u < before[x + 1] * heads) first_tile = x;
-    if (blockIdx.x == 0)
-        for (int x = tid; x <= tiles; x += 256) ws.before[x] = before[x];
     // tiles that see nothing at all lie nowhere on the line: their outputs are zeros
-    for (int x = blockIdx.x; x < tiles; x += runs)
+    for (int x = blockIdx.x; x < tiles; x += gridDim.x)
         if (before[x] == before[x + 1]) {
-            const Tile t = kv_tile(a, x, 16, 0);
-            if (!t.on) continue;
+            const Tile t = kv_flat_tile(a, x, row_of[x], len_of[x]);
             const int cols = min(16, t.ncols - t.col0);
             for (int i = tid; i < heads * cols * a.c.dim; i += 256) {
                 const int d = i % a.c.dim, c = i / a.c.dim % cols, hk = i / a.c.dim / cols;
                 ((A*)a.out)[((long long)t.tok0 * a.q_heads + hk * a.group + t.col0 + c) * a.c.dim + d] = (A)0.f;
             }
         }
-    __syncthreads();
-    if (u >= end) return;
-    int x = __builtin_amdgcn_readfirstlane(first_tile), left = (int)(end - u), slot = 2 * blockIdx.x;
-    int len = __builtin_amdgcn_readfirstlane((int)(before[x + 1] - before[x]));
-    const long long off = u - before[x] * heads;
-    int hk = __builtin_amdgcn_readfirstlane((int)(off / len)), cb = __builtin_amdgcn_readfirstlane((int)(off - (long long)hk * len));
+    const long long u = (long long)(4 * blockIdx.x + wave) * run;
+    if (u >= units) return;
+    int x = __builtin_amdgcn_readfirstlane(first_tile[wave]), left = min(run, units - (int)u), slot = 2 * (4 * blockIdx.x + wave);
+    int len = __builtin_amdgcn_readfirstlane(before[x + 1] - before[x]);
+    const int off = (int)u - __builtin_amdgcn_readfirstlane(before[x]) * heads;
+    int hk = off / len, cb = off - hk * len;
     for (;;) {
         const int ce = min(len, cb + left);
-        const Tile t = kv_tile(a, x, 16, lane);
-        attend_part<T, DP, P8>(a, t, kv_span(a, t, TB), hk, cb, ce, cb == 0 && ce == len, [&]() {
+        const Tile t = kv_flat_tile(a, x, __builtin_amdgcn_readfirstlane(row_of[x]), __builtin_amdgcn_readfirstlane(len_of[x]));
+        attend_part<T, DP, P8, 1>(a, t, kv_span(a, t, TB), hk, cb, ce, cb == 0 && ce == len, [&]() {
             const KvFlat ws(a.ws, runs, DP, a.group);
             return KvPart{ws.sums + (long long)slot * ws.cols * DP, ws.ml + (long long)slot * ws.cols * 2};
-        }, so, sm, sl);
+        }, nullptr, nullptr, nullptr);
         left -= ce - cb;
         if (left <= 0) return;
-        __syncthreads();
         cb = 0;
         slot |= 1;
         if (++hk == heads) {
             hk = 0;
             do {
                 ++x;
-                len = __builtin_amdgcn_readfirstlane((int)(before[x + 1] - before[x]));
+                len = __builtin_amdgcn_readfirstlane(before[x + 1] - before[x]);
             } while (len == 0);
         }
     }
@@ -675,13 +736,11 @@ template <typename A, int DP>
 __global__ void __launch_bounds__(256) kv_flat_join_kernel(const KvAttendArgs a, int tiles, int runs) {
     const int x = blockIdx.x, hk = blockIdx.y;
     const KvFlat ws(a.ws, runs, DP, a.group);
-    const long long b0 = ws.before[x], len = ws.before[x + 1] - b0, run = kv_flat_run(ws.before[tiles] * a.c.heads, runs);
+    const int b0 = ws.before[x], len = ws.before[x + 1] - b0, run = kv_flat_run(ws.before[tiles] * a.c.heads, runs);
     if (len == 0) return;
-    const long long u = b0 * a.c.heads + hk * len;
-    const int ra = (int)(u / run), rb = (int)((u + len - 1) / run);
+    const int u = b0 * a.c.heads + hk * len, ra = u / run, rb = (u + len - 1) / run;
     if (ra == rb) return;
-    const Tile t = kv_tile(a, x, 16, threadIdx.x & 63);
-    if (!t.on) return;
+    const Tile t = kv_flat_tile(a, x, 0, 1);                    // columns only
     // the part of the run in which it begins is that run's first only if it begins with it
     const long long first = 2ll * ra + (u == ra * run ? 0 : 1);
     join_parts<A, DP>(a, t, hk, rb - ra + 1, ws.sums, ws.ml, ws.cols, [&](int s) { return s == 0 ? first : 2ll * (ra + s); });
@@ -714,10 +773,21 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_attend_kernel(const
     if (a.splits > 1 && z == 0 && threadIdx.x == 0)
         *KvShares(a, gridDim.x, DP, blockIdx.x, hk).used = shared ? min(a.splits, (span.total + a.share - 1) / a.share) : 1;
     const int ce = shared && z + 1 < a.splits ? min(span.total, (z + 1) * a.share) : span.total;       // a bound on lengths that was too low: the last share's
-    attend_part<T, DP, P8>(a, t, span, hk, z * a.share, ce, !shared, [&]() {
+    attend_part<T, DP, P8, 4>(a, t, span, hk, z * a.share, ce, !shared, [&]() {
         const KvShares ws(a, gridDim.x, DP, blockIdx.x, hk);
         return KvPart{ws.sums + z * 16ll * DP, ws.ml + z * 32ll};
     }, so, sm, sl);
+}
+
+// many pairs: a wave for each (tile, kv head), when `alone` below holds
+template <typename T, int DP, bool P8>
+__global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_short_kernel(const KvAttendArgs a) {
+    const long long w = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int x = (int)(w / a.c.heads), hk = (int)(w - (long long)x * a.c.heads);
+    const Tile t = kv_tile(a, x, 16, threadIdx.x & 63);
+    if (!t.on) return;
+    const Span span = kv_span(a, t, 16 * Chunk<T, DP>::TILES);
+    attend_part<T, DP, P8, 1>(a, t, span, hk, 0, span.total, true, [] { return KvPart{nullptr, nullptr}; }, nullptr, nullptr, nullptr);
 }
 template <typename A, int DP>
 __global__ void __launch_bounds__(256) kv_join_kernel(const KvAttendArgs a) {
@@ -1122,12 +1192,12 @@ long long most_chunks(const KvView& c, int window, int sinks, int max_len) {
 // Single tokens in a line of runs, unless the whole line is short: then the layout of the line costs more than it evens out (one row under a
 // 4096-token window, 1040 chunks: 20 us against 14; 8 rows of 700 tokens in 4 bits: 17.6 against 11.5; 64 rows of 3200 - 16000: 184 against 218).
 bool flat(const KvView& c, int sequences, int q_heads, bool ragged, int window, int sinks, int max_len) {
-    const long long tiles = (long long)sequences * ((q_heads / c.heads + 15) / 16);
-    return !ragged && tiles <= FLAT && tiles * c.heads * most_chunks(c, window, sinks, max_len) > 8192;
+    const long long tiles = (long long)sequences * ((q_heads / c.heads + 15) / 16), line = tiles * c.heads * most_chunks(c, window, sinks, 0);
+    return !ragged && tiles <= FLAT && line < 0x70000000ll && tiles * c.heads * most_chunks(c, window, sinks, max_len) > 8192;
 }
-// workgroups that run at once on 256 compute units
+// waves that run at once on 256 compute units
 int flat_runs(const KvView& c) {
-    return 256 * flat_waves(c.dtype == Q3C_KV_INT4, padded_dim(c.dim));
+    return 1024 * flat_waves(c.dtype == Q3C_KV_INT4, padded_dim(c.dim));
 }
 
 }  // namespace
@@ -1136,8 +1206,8 @@ int flat_runs(const KvView& c) {
 // compute unit: short ones then even out what is left), of at least 8 chunks (two rounds of a workgroup's waves), no more than 256; rows of
 // up to 32 chunks are left whole, since a second launch takes as long as six rounds (700 tokens: 11.5 us whole, 14.2 in shares of 8).
 KvSplit q3_kv_attend_split(const KvView& c, int tokens, int sequences, int q_heads, bool ragged, int window, int sinks, int max_len) {
-    if (flat(c, sequences, q_heads, ragged, window, sinks, max_len)) return KvSplit{0, 0};
-    if (prompts(c, tokens, sequences, q_heads, ragged)) return KvSplit{1, 0x7fffffff};
+    if (flat(c, sequences, q_heads, ragged, window, sinks, max_len)) return KvSplit{0, 0, 0};
+    if (prompts(c, tokens, sequences, q_heads, ragged)) return KvSplit{1, 0x7fffffff, 0};
     const int group = q_heads / c.heads;
     const long long chunks = most_chunks(c, window, sinks, max_len), base = tiles_of(tokens, sequences, group, ragged) * c.heads;
     long long share = (chunks * base + 2047) / 2048;
@@ -1147,6 +1217,7 @@ KvSplit q3_kv_attend_split(const KvView& c, int tokens, int sequences, int q_hea
     KvSplit s;
     s.splits = base >= 2048 || chunks <= 32 ? 1 : (int)((chunks + share - 1) / share);
     s.share = s.splits == 1 ? 0x7fffffff : (int)share;
+    s.most = (int)(chunks < 0x7fffffff ? chunks : 0x7fffffff);
     return s;
 }
 size_t q3_kv_attend_ws(const KvView& c, int tokens, int sequences, int q_heads, bool ragged, int splits) {
@@ -1174,12 +1245,23 @@ hipError_t q3_launch_kv_attend(const KvAttendArgs& a, hipStream_t s) {
         }
         return hipGetLastError();
     }
+    const long long pairs = (long long)tiles * a.c.heads;
+    // A wave for each pair, with no meeting of waves, once there are pairs enough: for short rows (at most 16 chunks: four waves would have
+    // four rounds) from one wave per SIMD on (1024 pairs: 128 tokens in bf16 7.5 us against 10.3 with four waves for each, 330 new tokens x 5
+    // under a window of 72 in f32 15.7 against 21.6; 512 pairs of 64 tokens 6.5 against 6.0), for longer single tokens from eight (1100 rows
+    // of 500 tokens in 4 bits 138 us against 175, bf16 410 against 409).  Not for longer pieces, whose tiles are as unlike as their
+    // positions (4 x 2048 new tokens in f32: 433 us against 366).
+    const bool alone = a.splits == 1 && ((a.most <= 16 && pairs >= 1024) || (!a.b.offsets && pairs >= 8192));
+    const unsigned solo = alone ? (unsigned)((pairs + 3) / 4) : 0;
 #define Q3_ATTEND(T, A, DP)                                                        \
     do {                                                                           \
         if (runs) {                                                                \
-            if (a.c.ps_shift == 3) kv_flat_kernel<T, DP, true><<<runs, 256, 0, s>>>(a, (int)tiles);  \
-            else kv_flat_kernel<T, DP, false><<<runs, 256, 0, s>>>(a, (int)tiles); \
+            if (a.c.ps_shift == 3) kv_flat_kernel<T, DP, true><<<runs / 4, 256, 0, s>>>(a, (int)tiles);  \
+            else kv_flat_kernel<T, DP, false><<<runs / 4, 256, 0, s>>>(a, (int)tiles); \
             kv_flat_join_kernel<A, DP><<<join, 256, 0, s>>>(a, (int)tiles, runs);  \
+        } else if (solo) {                                                         \
+            if (a.c.ps_shift == 3) kv_short_kernel<T, DP, true><<<solo, 256, 0, s>>>(a);             \
+            else kv_short_kernel<T, DP, false><<<solo, 256, 0, s>>>(a);            \
         } else {                                                                   \
             if (a.c.ps_shift == 3) kv_attend_kernel<T, DP, true><<<grid, 256, 0, s>>>(a);            \
             else kv_attend_kernel<T, DP, false><<<grid, 256, 0, s>>>(a);           \

@@ -129,6 +129,7 @@ int q3c_kv_attend(const q3c_kv* kv, int32_t layer, const void* q, int64_t q_ts, 
     const KvSplit cut = q3_kv_attend_split(a.c, tokens, sequences, q_heads, offsets != nullptr, window, sinks, max_len);
     a.splits = cut.splits;
     a.share = cut.share;
+    a.most = cut.most;
     const size_t need = q3_kv_attend_ws(a.c, tokens, sequences, q_heads, offsets != nullptr, a.splits);
     if (need && (!workspace || !aligned(workspace, 16))) return Q3C_ERR_INVALID_ARGUMENT;
     if (workspace_bytes < need) return Q3C_ERR_WORKSPACE;
