@@ -74,6 +74,7 @@ __device__ __forceinline__ bool kv_place(const KvAppendArgs& a, int tok, bool fi
 // A wave has one token and `parts`-th of its heads, VEC pairs per lane as two runs that are each other's rotation partners, so that the
 // rotation needs no exchange between lanes and the norm one butterfly over the head's lanes.  Two runs of heads are requested before
 // the token's place is looked up (offset -> row -> length -> page, four dependent reads): they are what a wave has to wait for once.
+// 28143 tokens of 16 + 8 + 8 heads of 128 in bf16: 113 us, 4.1 TB/s; 64 single tokens 4.8 us.
 template <typename T, int VEC, bool CACHED>     // CACHED: keys and values go to the pages here too (no 4-bit cache)
 __device__ __forceinline__ void append_plain(const KvAppendArgs& a, int tok, int part, int parts, int lane, int lpu_shift) {
     constexpr int RUN = 2;
@@ -146,72 +147,97 @@ __device__ __forceinline__ void append_plain(const KvAppendArgs& a, int tok, int
     }
 }
 
+// x / d, rounded to nearest as the division is, with y = 1 / d rounded to nearest: the remainder of the first guess is exact in an fma, which
+// makes the second one right (Markstein); d at least 2^-100 and the quotients below 2^20, so that nothing over- or underflows on the way.
+__device__ __forceinline__ float divide(float x, float d, float y) {
+    const float q = x * y;
+    return fmaf(fmaf(-d, q, x), y, q);
+}
+
 // A 4-bit row: groups of 32 dimensions share step = bf16(absmax / 7); value n = rint(x / step) in -7 .. 7 is held as n + 8.  Byte
-// [m][s] of the row (m < 16, s < dim / 32) packs dimensions 32 s + m (low half) and 32 s + 16 + m: lane m of a head's 16 lanes then
-// owns whole bytes and, dim / 2 being a multiple of 16, both partners of its rotations.  The group maximum is taken on the bits of
+// [m][s] of the row (m < 16, s < dim / 32) packs dimensions 32 s + m (low half) and 32 s + 16 + m.  A lane has M neighbouring m of a
+// head: whole bytes and, dim / 2 being a multiple of 16, both partners of its rotations.  The group maximum is taken on the bits of
 // |x| (integers order like the floats, NaN above infinity), so a group that holds either reads back as NaN throughout.
+// M = 4: 8-byte loads, two steps of each butterfly, 36.7 us for 10756 tokens of 16 + 8 + 8 heads of 128 (3.9 TB/s; 2: 39, 1: 45 us, where
+// most of the time went to instructions).  A wave for a token's queries and one for its keys and values: both in one took 39 us.
+constexpr int M4 = 4;                         // bytes of each group that a lane has: a head takes 16 / M4 lanes
 template <int D>
 __device__ __forceinline__ void append_int4(const KvAppendArgs& a, int tok, int unit0, int lane) {
-    constexpr int N = D / 16, S = D / 32;
-    const int G = a.c.heads, m = lane & 15, u = min(unit0 + (lane >> 4), 2 * G - 1);
-    const bool key = u < G, twin = unit0 + (lane >> 4) != u;         // twin: past the last head, a copy of it that stores nothing
+    constexpr int N = D / 16, S = D / 32, M = M4, LPU = 16 / M;
+    typedef Floats<M> F;
+    const int G = a.c.heads, m = M * (lane % LPU), u = min(unit0 + lane / LPU, 2 * G - 1);
+    const bool key = u < G, twin = unit0 + lane / LPU != u;          // twin: past the last head, a copy of it that stores nothing
     const int h = key ? u : u - G;
     const KvStrided& src = key ? a.k : a.v;
     const bf16* xp = (const bf16*)src.p + tok * src.ts + h * src.hs + m;
-    bf16 raw[N];
+    Vec<bf16, M> raw[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) raw[i] = xp[16 * i];
+    for (int i = 0; i < N; ++i) raw[i] = kv_load<M>(xp + 16 * i);
     int pos, page;
     bool zero;
     if (!kv_place(a, tok, false, lane, pos, page, zero) || page < 0) return;
-    float x[N];
+    F x[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = (float)raw[i];
+    for (int i = 0; i < N; ++i) x[i] = __builtin_convertvector(raw[i], F);
     if (key && a.kw) {
         float ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) ss = fmaf(x[i], x[i], ss);
-        ss = sum_lanes(ss, 16);
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < M; ++j) ss = fmaf(x[i][j], x[i][j], ss);
+        ss = sum_lanes(ss, LPU);
         const float r = __builtin_amdgcn_rsqf(fmaf(ss, a.inv_dim, a.eps));
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = x[i] * r * a.kw[16 * i + m];
+        for (int i = 0; i < N; ++i) x[i] = x[i] * r * *(const F*)(a.kw + 16 * i + m);
     }
     if (key && a.rot) {
         const float* co = a.cos_t + (long long)pos * (D / 2) + m;
         const float* si = a.sin_t + (long long)pos * (D / 2) + m;
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) {
-            const float c = co[16 * i], s = si[16 * i], p = x[i], q = x[i + N / 2];
+            const F c = *(const F*)(co + 16 * i), s = *(const F*)(si + 16 * i), p = x[i], q = x[i + N / 2];
             x[i] = p * c - q * s;
             x[i + N / 2] = q * c + p * s;
         }
     }
     const long long at = ((((long long)a.layer * a.c.pages + page) * G + h) << a.c.ps_shift) + (pos & ((1 << a.c.ps_shift) - 1));
-    unsigned char* out = (unsigned char*)(key ? a.c.k : a.c.v) + at * (D / 2) + m * S;
-    unsigned short* steps = (unsigned short*)(key ? a.c.ks : a.c.vs) + at * S;
-    unsigned long long bytes = 0;
+    Vec<unsigned, M * S / 4> bytes = 0;
+    Vec<unsigned short, S> steps;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-        unsigned top = max(__float_as_uint(x[2 * s]) & 0x7fffffffu, __float_as_uint(x[2 * s + 1]) & 0x7fffffffu);
+        unsigned top = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) top = max(top, lane_xor<unsigned>(top, k));
-        const bf16 st = (bf16)(__uint_as_float(top) / 7.0f);
-        const float step = (float)st;
-        unsigned byte = 0x88;
-        if (step > 0.f && step < INFINITY) {
-            const int n0 = (int)fminf(fmaxf(rintf(x[2 * s] / step), -7.f), 7.f), n1 = (int)fminf(fmaxf(rintf(x[2 * s + 1] / step), -7.f), 7.f);
-            byte = (unsigned)(n0 + 8) | (unsigned)(n1 + 8) << 4;
+        for (int j = 0; j < M; ++j) top = max(top, max(__float_as_uint(x[2 * s][j]) & 0x7fffffffu, __float_as_uint(x[2 * s + 1][j]) & 0x7fffffffu));
+#pragma unroll
+        for (int k = 0; 1 << k < LPU; ++k) top = max(top, lane_xor<unsigned>(top, k));
+        const bool plain = top - 0x0e000000u < 0x7f800000u - 0x0e000000u;      // 2^-99 .. finite
+        const bf16 st = (bf16)(plain ? divide(__uint_as_float(top), 7.0f, 1.0f / 7.0f) : __uint_as_float(top) / 7.0f);
+        const float step = (float)st, inv = 1.0f / step;
+        steps[s] = __builtin_bit_cast(unsigned short, st);
+        const bool some = step > 0.f && step < INFINITY;
+#pragma unroll
+        for (int j = 0; j < M; ++j) {
+            const float x0 = x[2 * s][j], x1 = x[2 * s + 1][j];
+            float n0, n1;
+            if (step >= 0x1p-100f) {
+                n0 = divide(x0, step, inv);
+                n1 = divide(x1, step, inv);
+            } else {
+                n0 = x0 / step;
+                n1 = x1 / step;
+            }
+            n0 = fminf(fmaxf(rintf(n0), -7.f), 7.f);
+            n1 = fminf(fmaxf(rintf(n1), -7.f), 7.f);
+            const unsigned byte = some ? (unsigned)((int)n0 + 8) | (unsigned)((int)n1 + 8) << 4 : 0x88u;
+            bytes[(j * S + s) / 4] |= byte << (8 * ((j * S + s) & 3));
         }
-        bytes |= (unsigned long long)byte << (8 * s);
-        if (m == s && !twin) steps[s] = __builtin_bit_cast(unsigned short, st);
     }
     if (twin) return;
-    if (S == 2) *(unsigned short*)out = (unsigned short)bytes;
-    else if (S == 4) *(unsigned*)out = (unsigned)bytes;
-    else *(unsigned long long*)out = bytes;
+    *(Vec<unsigned, M * S / 4>*)((unsigned char*)(key ? a.c.k : a.c.v) + at * (D / 2) + m * S) = bytes;
+    if (m == 0) *(Vec<unsigned short, S>*)((unsigned short*)(key ? a.c.ks : a.c.vs) + at * S) = steps;
 }
 
-// `parts` waves have a token's heads (D4: its query heads; then one wave for each four of its key and value heads)
+// `parts` waves have a token's heads (D4: its query heads; then one wave for each 4 * M4 of its key and value heads)
 template <typename T, int VEC, int D4>      // D4: 0 = cache in T, else head size of a 4-bit cache
 __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs a, int parts, int waves, int lpu_shift) {
     const int lane = threadIdx.x & 63;
@@ -219,10 +245,12 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs a, in
     const int tok = (int)(w / waves), part = (int)(w - (long long)tok * waves);
     if (tok >= a.b.tokens) return;
     if (D4 == 0 || part < parts) append_plain<T, VEC, D4 == 0>(a, tok, part, parts, lane, lpu_shift);
-    else append_int4<D4 ? D4 : 64>(a, tok, (part - parts) * 4, lane);
+    else append_int4<D4 ? D4 : 64>(a, tok, (part - parts) * (4 * M4), lane);
 }
 
 // ---- gather: the stored keys and values of the same tokens, back in one piece (zeros where there is no page) -------------------------
+// Bound by the wait for a token's place (four dependent reads) and by memory: a wave has up to RUN runs of a token's heads in flight (4 bits,
+// 10756 tokens of 8 + 8 heads of 128 as bf16: 13.6 us against 16.3 with one run per wave; 4.1 TB/s).
 template <typename T, typename O, int D4>
 __global__ void __launch_bounds__(256) kv_gather_kernel(const KvView c, const KvBatch b, int layer, O* __restrict__ k_out, O* __restrict__ v_out,
                                                         int waves, int lpu_shift) {
@@ -235,35 +263,50 @@ __global__ void __launch_bounds__(256) kv_gather_kernel(const KvView c, const Kv
     if (pos == -1) return;
     const int page = pos < 0 ? -1 : kv_page(c, row, pos);
     if (pos < 0 && lane == 0 && part == 0) kv_flag(c, Q3C_KV_BAD_ROW);
-    const int lpu = 1 << lpu_shift, u = part * (64 >> lpu_shift) + (lane >> lpu_shift), ch = lane & (lpu - 1);
-    if (u >= 2 * c.heads || 8 * ch >= c.dim) return;
-    const bool key = u < c.heads;
-    const int h = key ? u : u - c.heads;
-    O* out = (key ? k_out : v_out) + ((long long)tok * c.heads + h) * c.dim + 8 * ch;
-    Floats<4> lo = {0, 0, 0, 0}, hi = lo;
-    if (page >= 0) {
-        const long long at = ((((long long)layer * c.pages + page) * c.heads + h) << c.ps_shift) + (pos & ((1 << c.ps_shift) - 1));
-        if (D4 == 0) {
-            const T* x = (const T*)(key ? c.k : c.v) + at * c.dim + 8 * ch;
-            lo = __builtin_convertvector(kv_load<4>(x), Floats<4>);
-            hi = __builtin_convertvector(kv_load<4>(x + 4), Floats<4>);
-        } else {                                               // dimensions 8 ch .. + 7: one half of byte s of eight neighbouring m's S bytes
-            constexpr int S = D4 ? D4 / 32 : 2;
-            const int s = ch >> 2, shift = 8 * (s & 3) + ((ch & 2) ? 4 : 0);
-            const unsigned* x = (const unsigned*)((const unsigned char*)(key ? c.k : c.v) + at * (16 * S) + (ch & 1) * 8 * S);
-            const float step = (float)(key ? c.ks : c.vs)[at * S + s];
-            unsigned w[2 * S];
+    constexpr int S = D4 ? D4 / 32 : 2, RUN = D4 == 256 ? 2 : 4;
+    const int lpu = 1 << lpu_shift, upw = 64 >> lpu_shift, ch = lane & (lpu - 1), s = ch >> 2, units = 2 * c.heads;
+    const int in_page = pos & ((1 << c.ps_shift) - 1);
+    for (int u0 = part * upw; u0 < units; u0 += RUN * waves * upw) {
+        Vec<T, 8> x[RUN];
+        Vec<unsigned, 4> w[RUN][S / 2];
+        bf16 step[RUN];
 #pragma unroll
-            for (int i = 0; i < 2 * S; i += 4) *(uint4*)(w + i) = *(const uint4*)(x + i);
+        for (int r = 0; r < RUN; ++r) {
+            const int u = u0 + r * waves * upw + (lane >> lpu_shift), h = u < c.heads ? u : u - c.heads;
+            x[r] = (T)0.f;
+            step[r] = (bf16)0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const unsigned v = S == 2 ? w[i >> 1] >> (16 * (i & 1)) : S == 4 ? w[i] : s < 4 ? w[2 * i & (2 * S - 1)] : w[(2 * i + 1) & (2 * S - 1)];
-                (i < 4 ? lo : hi)[i & 3] = (float)((int)(v >> shift & 15u) - 8) * step;
+            for (int i = 0; i < S / 2; ++i) w[r][i] = 0;
+            if (u >= units || 8 * ch >= c.dim || page < 0) continue;
+            const void* p = u < c.heads ? c.k : c.v;
+            const long long at = ((((long long)layer * c.pages + page) * c.heads + h) << c.ps_shift) + in_page;
+            if (D4 == 0) {
+                x[r] = kv_load<8>((const T*)p + at * c.dim + 8 * ch);
+            } else {                                           // dimensions 8 ch .. + 7: one half of byte s of eight neighbouring m's S bytes
+#pragma unroll
+                for (int i = 0; i < S / 2; ++i) w[r][i] = *(const Vec<unsigned, 4>*)((const unsigned char*)p + at * (16 * S) + (ch & 1) * 8 * S + 16 * i);
+                step[r] = (u < c.heads ? c.ks : c.vs)[at * S + s];
             }
         }
+#pragma unroll
+        for (int r = 0; r < RUN; ++r) {
+            const int u = u0 + r * waves * upw + (lane >> lpu_shift), h = u < c.heads ? u : u - c.heads;
+            if (u >= units || 8 * ch >= c.dim) continue;
+            Floats<8> y = __builtin_convertvector(x[r], Floats<8>);
+            if (D4) {
+                const int shift = 8 * (s & 3) + ((ch & 2) ? 4 : 0);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const unsigned v = S == 2   ? w[r][0][i >> 1] >> (16 * (i & 1))
+                                       : S == 4 ? w[r][i >> 2 & (S / 2 - 1)][i & 3]
+                                       : s < 4  ? w[r][i >> 1 & (S / 2 - 1)][2 * i & 3]
+                                                : w[r][i >> 1 & (S / 2 - 1)][(2 * i + 1) & 3];
+                    y[i] = page < 0 ? 0.f : (float)((int)(v >> shift & 15u) - 8) * (float)step[r];
+                }
+            }
+            kv_store<8, O>((u < c.heads ? k_out : v_out) + ((long long)tok * c.heads + h) * c.dim + 8 * ch, y);
+        }
     }
-    kv_store<4, O>(out, lo);
-    kv_store<4, O>(out + 4, hi);
 }
 
 // ---- pages ----------------------------------------------------------------------------------------------------------------------------
@@ -614,7 +657,7 @@ hipError_t q3_launch_kv_append(const KvAppendArgs& a, hipStream_t s) {
     const int sh = lanes_shift(a.c.dim, v8 ? 16 : 8), upw = 64 >> sh, runs = (units + upw - 1) / upw;
     int parts = runs;                       // waves of a token: few tokens are spread, many keep two runs of heads in flight per wave
     while (parts > 1 && (long long)a.b.tokens * parts > 4096 && (runs + parts - 1) / parts < 2) parts = (parts + 1) / 2;
-    const int waves = parts + (d4 ? (2 * a.c.heads + 3) / 4 : 0);
+    const int waves = parts + (d4 ? (2 * a.c.heads + 4 * M4 - 1) / (4 * M4) : 0);
     const unsigned blocks = (unsigned)(((long long)a.b.tokens * waves + 3) / 4);
     if (!blocks) return hipSuccess;
 #define Q3_APPEND(T, D4)                                                                    \
@@ -632,7 +675,9 @@ hipError_t q3_launch_kv_append(const KvAppendArgs& a, hipStream_t s) {
 }
 
 hipError_t q3_launch_kv_gather(const KvView& c, const KvBatch& b, int layer, void* k_out, void* v_out, int out_dtype, hipStream_t s) {
-    const int sh = lanes_shift(c.dim), upw = 64 >> sh, waves = (2 * c.heads + upw - 1) / upw;
+    const int sh = lanes_shift(c.dim), upw = 64 >> sh, runs = (2 * c.heads + upw - 1) / upw;
+    int waves = runs;                       // of a token: few tokens are spread, many keep several heads in flight per wave
+    while (waves > 1 && (long long)b.tokens * waves > 4096 && (runs + waves - 1) / waves < 4) waves = (waves + 1) / 2;
     const unsigned blocks = (unsigned)(((long long)b.tokens * waves + 3) / 4);
     if (!blocks) return hipSuccess;
 #define Q3_GATHER(T, D4)                                                                                                       \
