@@ -308,7 +308,7 @@ int q3c_wav_to_pcm16(const float* wav_dev, int64_t samples, int16_t* pcm_dev, vo
  * A call names its requests by `rows` [sequences] (table rows, distinct) and their new tokens by `offsets` [sequences + 1]: request
  * i's are tokens offsets[i] .. offsets[i + 1] - 1 of the call's `tokens`; NULL: one each (tokens == sequences).  The last new token of
  * a request stands at position lens[row] - 1: q3c_kv_reserve first makes room (lens grows), then every layer appends and attends.
- * Tokens from offsets[sequences] on are neither read nor written.  What a list, an offset or a table entry says is checked on the
+ * Tokens before offsets[0] and from offsets[sequences] on are neither read nor written.  What a list, an offset or a table entry says is checked on the
  * device: a token whose row is bad or named before in the call, or that has no page, is not stored (its query is zeros if its row or
  * position is bad), keys without a page are seen by nobody, and the bit in `status` says so. */
 typedef enum q3c_kv_dtype { Q3C_KV_F32 = 0, Q3C_KV_BF16 = 1, Q3C_KV_INT4 = 2 } q3c_kv_dtype;

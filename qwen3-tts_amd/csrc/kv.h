@@ -54,14 +54,14 @@ __device__ __forceinline__ int kv_find(const int* __restrict__ offsets, int n, i
     for (int i = 0; i < n; i += 64) b += __popcll(__ballot(i + lane < n && offsets[min(i + lane, n - 1) + 1] <= t));
     return b;
 }
-// The cache position of new token t (wave-uniform); -1: it lies behind the last request, -2: bad row, or a position outside the row's
+// The cache position of new token t (wave-uniform); -1: it lies before the first request or behind the last, -2: bad row, or a position outside the row's
 // table.  `seq`, `row`: its request and table row.
 __device__ __forceinline__ int kv_position(const KvView& c, const KvBatch& b, int t, int lane, int& seq, int& row) {
     int back = 1;
     seq = t;
     if (b.offsets) {
         seq = kv_find(b.offsets, b.sequences, t, lane);
-        if (seq >= b.sequences) return -1;
+        if (seq >= b.sequences || (seq == 0 && t < b.offsets[0])) return -1;
         back = b.offsets[seq + 1] - t;
         if (back < 1) return -2;                                // offsets that do not ascend
     }

@@ -380,7 +380,7 @@ __device__ __forceinline__ void attend_part(const KvAttendArgs& a, const Tile& t
     const long long head0 = ((long long)a.layer * a.c.pages * a.c.heads + hk) << sh;
     const char *kb = (const char*)a.c.k + head0 * rb, *vb = (const char*)a.c.v + head0 * rb;
     const char *ksb = (const char*)a.c.ks + head0 * sb, *vsb = (const char*)a.c.vs + head0 * sb;
-    const int W = a.window > 0 ? a.window : 0x7fffffff, sinks = a.window > 0 ? a.sinks : 0;
+    const int W = a.window > 0 ? min(a.window, 1 << 30) : 1 << 30, sinks = a.window > 0 ? a.sinks : 0;
 
     const float cs = a.scale_log2e;
     unsigned magic = 0x43004300u;              // two bf16 exponents of 128, kept in a register: an and-or takes one constant
@@ -920,7 +920,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
     const int in_page = (1 << sh) - 1, last_entry = a.c.width - 1, row_bytes = 2 * D;
     const unsigned page_bytes = (unsigned)page_rows * row_bytes;                   // below 2^32: the entry points see to it
     const char *kbase = (const char*)a.c.k + (DMA ? head0 * row_bytes : 0), *vbase = (const char*)a.c.v + (DMA ? head0 * row_bytes : 0);
-    const int W = a.window > 0 ? a.window : 0x7fffffff, sinks = a.window > 0 ? a.sinks : 0;
+    const int W = a.window > 0 ? min(a.window, 1 << 30) : 1 << 30, sinks = a.window > 0 ? a.sinks : 0;
     // This thread stages 16-byte slot `slot` of rows row0 + i RP; the rows of a wave and i are RW consecutive ones, which lie in one page.
     const int slot = tid & (NCH - 1), row0 = tid / NCH, sub = lane / NCH;
     const float cs = a.scale_log2e;

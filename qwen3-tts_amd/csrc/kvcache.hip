@@ -458,19 +458,20 @@ __global__ void __launch_bounds__(256) kv_release_kernel(const KvView c, const i
         if (threadIdx.x == 0 && blockIdx.y == 0) kv_flag(c, Q3C_KV_BAD_ROW);
         return;
     }
-    const int j = blockIdx.y * 256 + threadIdx.x;
-    if (!trim && j == 0) c.lens[row] = 0;
-    if (j >= c.width) return;
-    if (trim) {
-        const long long begin = (long long)j << c.ps_shift, end = begin + (1 << c.ps_shift);
-        if (begin < sinks || end > (long long)c.lens[row] - window) return;
+    if (!trim && blockIdx.y == 0 && threadIdx.x == 0) c.lens[row] = 0;
+    const long long left = trim ? (long long)c.lens[row] - window : 0;      // trim: pages end by here
+    for (int j = blockIdx.y * 256 + threadIdx.x; j < c.width; j += gridDim.y * 256) {
+        if (trim) {
+            const long long begin = (long long)j << c.ps_shift, end = begin + (1 << c.ps_shift);
+            if (begin < sinks || end > left) continue;
+        }
+        int* e = c.table + (long long)row * c.width + j;
+        if (*e < 0) continue;
+        const int p = atomicExch(e, -1);
+        if (p < 0) continue;
+        if (p >= c.pages) kv_flag(c, Q3C_KV_BAD_PAGE);
+        else if (atomicSub(c.refs + p, 1) <= 0) { atomicAdd(c.refs + p, 1); kv_flag(c, Q3C_KV_BAD_PAGE); }
     }
-    int* e = c.table + (long long)row * c.width + j;
-    if (*e < 0) return;
-    const int p = atomicExch(e, -1);
-    if (p < 0) return;
-    if (p >= c.pages) { kv_flag(c, Q3C_KV_BAD_PAGE); return; }
-    if (atomicSub(c.refs + p, 1) <= 0) { atomicAdd(c.refs + p, 1); kv_flag(c, Q3C_KV_BAD_PAGE); }
 }
 
 // fork, first launch: which pairs are good, and a free page for each partly filled last one.  ws: [count] source page or -1, [count]
@@ -698,7 +699,8 @@ hipError_t q3_launch_kv_reserve(const KvView& c, const KvBatch& b, hipStream_t s
 }
 
 hipError_t q3_launch_kv_release(const KvView& c, const int* rows, int count, int trim, int window, int sinks, hipStream_t s) {
-    if (count > 0) kv_release_kernel<<<dim3(count, (c.width + 255) / 256), 256, 0, s>>>(c, rows, trim, window, sinks);
+    const int blocks = (c.width + 255) / 256;
+    if (count > 0) kv_release_kernel<<<dim3(count, blocks < 4096 ? blocks : 4096), 256, 0, s>>>(c, rows, trim, window, sinks);
     return hipGetLastError();
 }
 

@@ -15,9 +15,14 @@ generation, and nothing in them reads device values on the host: a whole step ca
     kv.release(ended_rows)
 
 `rows` are table rows, one per request: an int32 tensor on the device (distinct; checked there) or a sequence of ints (checked here).
-`offsets` (int32 [len(rows) + 1] on the device) gives each row's new tokens in a ragged call; without it every row has one.  `dtype`
-"f32" and "bf16" hold what the activations are; "int4" holds bf16 activations in 4 bits with a step per 32 dimensions.  There is no
-backward pass: a cache is state, and this package trains nothing.
+`offsets` (int32 [len(rows) + 1] on the device) gives each row's new tokens in a ragged call; without it every row has one; tokens
+before offsets[0] and from offsets[-1] on belong to no row and are left alone.  `dtype` "f32" and "bf16" hold what the activations are;
+"int4" holds bf16 activations in 4 bits with a step per 32 dimensions.  There is no backward pass: a cache is state, this package trains
+nothing, and tensors that ask for gradients are refused where autograd is on.
+
+Every call runs on the current stream of the cache's device.  attend and gather calls may run beside each other on any streams; a call
+that changes the cache (the others) must be ordered with those around it, as writes to a tensor are.  Calls that are captured into a
+graph take `rows` as a tensor: a sequence is copied to the device by the call.
 """
 from __future__ import annotations
 
@@ -190,6 +195,8 @@ class PagedKV:
             raise ValueError(f"{what} must be [tokens, {'heads' if heads is None else heads}, {self.head_dim}], got {tuple(shape)}")
         if x.dtype != self.activations or x.get_device() != self._index:
             raise ValueError(f"{what} must be {self.activations} on {self.device}, got {x.dtype} on {x.device}")
+        if x.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{what} requires a gradient, and the cache's operators have none: call them under torch.no_grad()")
         ts, hs, ds = x.stride()
         quad = 4 * self._act_bytes
         if ds != 1 or ts % 4 or hs % 4 or x.data_ptr() % quad:

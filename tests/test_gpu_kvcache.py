@@ -693,3 +693,226 @@ def test_attend_prompts_of_many_tiles(dtype, D, G, group, ps, window, sinks):
         pos = [lens[r] - new[r] + p for p in some]
         want, mag, dot = attention(q[start + i], *store[r], pos, window, sinks, scale)
         _check_attend(out[start + i], want, mag, dot, kv, lens[r], scale, q[start + i].double(), prompt=True)
+
+
+# ---- calls of unusual shape ----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["bf16", "f32", "int4"])
+def test_tokens_before_the_first_request_are_left_alone(dtype):
+    """A batch padded in front: offsets that begin at 3.  Nothing of the padding reaches the cache, nothing is written to its outputs."""
+    g = _gen(31)
+    G, group, D, ps, lens, new = 2, 2, 64, 8, [30, 21], [4, 9]
+    kv = _cache(dtype, G, D, ps, lens)
+    _fill(kv, 0, lens, g)
+    rows = torch.tensor([1, 0], dtype=torch.int32, device=DEV)
+    q, k, v = (_randn(g, 16 + 2, n, D, dtype=kv.activations) for n in (G * group, G, G))
+    off = _offsets(new)
+    held = [t.clone() for t in (kv.k, kv.v)]
+    want = kv.append(0, q[3:16], k[3:16], v[3:16], rows, off)
+    seen = kv.attend(0, q[3:16], rows, off, window=10, sinks=2)
+    after = [t.clone() for t in (kv.k, kv.v)]
+    kk, vv = kv.gather(0, rows, off, tokens=13)
+    for t, h in zip((kv.k, kv.v), held):
+        t.copy_(h)
+    out = torch.full_like(q, 5.0)
+    kv.append(0, q, k, v, rows, off + 3, out=out)
+    assert torch.equal(out[3:16], want) and bool((out[:3] == 5.0).all()) and bool((out[16:] == 5.0).all())
+    for t, a in zip((kv.k, kv.v), after):
+        assert torch.equal(t.view(torch.uint8), a.view(torch.uint8))
+    out.fill_(5.0)
+    kv.attend(0, q, rows, off + 3, window=10, sinks=2, out=out)
+    assert torch.equal(out[3:16], seen) and bool((out[:3] == 5.0).all()) and bool((out[16:] == 5.0).all())
+    k3, v3 = kv.gather(0, rows, off + 3, tokens=18)
+    assert torch.equal(k3[3:16], kk) and torch.equal(v3[3:16], vv)
+    lens0 = kv.lens.tolist()
+    kv.reserve(rows, off + 3, tokens=18)
+    assert kv.lens.tolist() == [lens0[0] + 9, lens0[1] + 4]
+    kv.check()
+
+
+@pytest.mark.parametrize("dtype,D,G,H", [("bf16", 80, 3, 5 * 3), ("bf16", 128, 8, 16), ("f32", 48, 5, 5), ("int4", 64, 9, 9), ("int4", 128, 3, 21), ("int4", 256, 10, 10)])
+def test_many_tokens_at_once_are_the_same_as_a_few(dtype, D, G, H):
+    """append and gather give a wave more of a token's heads when tokens are many: the same values, bit for bit, as in small calls."""
+    g = _gen(D + G)
+    lens, ps = [2500, 901], 16
+    kv = _cache(dtype, G, D, ps, lens)
+    T = sum(lens)
+    x = _randn(g, T, H + 2 * G, D).mul_(3).to(kv.activations)
+    q, k, v = x.split([H, G, G], 1)
+    wq, wk = (torch.rand(D, generator=g, device=DEV) + 0.5 for _ in range(2))
+    from qwen3_tts_amd.kvcache import rope_tables
+    rope = rope_tables(kv.max_tokens, D, device=DEV)
+    rows = torch.arange(2, dtype=torch.int32, device=DEV)
+    out = kv.append(0, q, k, v, rows, _offsets(lens), q_weight=wq, k_weight=wk, rope=rope)
+    got = {t: kv.gather(0, rows, _offsets(lens), tokens=T, dtype=t) for t in ("f32", "bf16")}
+    whole = [t.clone() for t in (kv.k, kv.v)]
+    some, at = torch.empty_like(out), 0
+    for r, L in enumerate(lens):
+        for i in range(0, L, 100):
+            n = min(100, L - i)
+            kv.lens[r] = i + n
+            s = slice(at + i, at + i + n)
+            one = rows[r:r + 1]
+            some[s] = kv.append(0, q[s], k[s], v[s], one, _offsets([n]), q_weight=wq, k_weight=wk, rope=rope)
+            for t in ("f32", "bf16"):
+                kk, vv = kv.gather(0, one, _offsets([n]), tokens=n, dtype=t)
+                assert torch.equal(kk, got[t][0][s]) and torch.equal(vv, got[t][1][s])
+        at += L
+    assert torch.equal(some, out)
+    for t, w in zip((kv.k, kv.v), whole):
+        assert torch.equal(t.view(torch.uint8), w.view(torch.uint8))
+    if dtype != "int4":
+        assert torch.equal(got["f32"][1], v.float()) and torch.equal(got["bf16"][1], v.to(torch.bfloat16))
+    kv.check()
+
+
+def _some_rows(kv, out, q, store, lens, rows, some, window, sinks, scale):
+    for i in some:
+        r = rows[i]
+        if 0 <= r < kv.rows and lens[r]:
+            want, mag, dot = attention(q[i:i + 1], *store[r], [lens[r] - 1], window, sinks, scale)
+            _check_attend(out[i:i + 1], want, mag, dot, kv, lens[r], scale, q[i:i + 1].double())
+        else:
+            assert bool((out[i] == 0).all()), i
+
+
+@pytest.mark.parametrize("dtype,D,G,group,ps,S", [("bf16", 128, 8, 2, 32, 300), ("bf16", 64, 1, 20, 8, 400), ("f32", 64, 4, 1, 16, 1024), ("int4", 128, 8, 2, 32, 200),
+                                                  ("int4", 64, 2, 3, 8, 1000), ("bf16", 256, 2, 1, 64, 700), ("int4", 256, 1, 4, 128, 1024), ("f32", 256, 1, 1, 256, 1023),
+                                                  ("bf16", 128, 8, 2, 32, 1030), ("f32", 48, 8, 2, 16, 1100), ("int4", 64, 8, 1, 8, 1025)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 5)])
+def test_attend_single_tokens_of_many_rows(dtype, D, G, group, ps, S, window, sinks):
+    """Hundreds of rows of all lengths, empty ones and bad ids among them: one line of runs up to a thousand rows, a wave for each beyond."""
+    g = _gen(S + D)
+    r = torch.Generator().manual_seed(S)
+    lens = torch.randint(1, 60, (S,), generator=r).tolist()
+    lens[0], lens[1], lens[2], lens[S // 2], lens[-1] = 1, 0, 1900, 700, 0
+    for i in range(3, S, 17):
+        lens[i] = 0
+    kv = _cache(dtype, G, D, ps, lens, width=-(-6000 // ps))
+    store = _fill(kv, 0, lens, g)
+    rows = torch.randperm(S, generator=r).tolist()
+    rows[5], rows[6] = -1, S + 4
+    q = _randn(g, S, G * group, D).mul_(2).to(kv.activations)
+    out = torch.full_like(q, 7.0)
+    kv.attend(0, q, torch.tensor(rows, dtype=torch.int32, device=DEV), window=window, sinks=sinks, out=out)
+    where = {x: i for i, x in enumerate(rows)}
+    some = [where[x] for x in (0, 1, 2, 3, S // 2, S - 1, S - 2, S - 3) if x in where] + [0, 5, 6, S - 1, S // 3]
+    _some_rows(kv, out, q, store, lens, rows, some, window, sinks, D ** -0.5)
+    nothing = torch.tensor([i for i, x in enumerate(rows) if not 0 <= x < S or not lens[x]], device=DEV)
+    assert bool((out[nothing] == 0).all()) and bool(torch.isfinite(out).all())
+    kv.lens.zero_()                                                # and rows that see nothing, all of them
+    assert bool((kv.attend(0, q, torch.tensor(rows, dtype=torch.int32, device=DEV), window=window, sinks=sinks) == 0).all())
+
+
+@pytest.mark.parametrize("dtype,D,G,group,ps", [("bf16", 128, 8, 2, 32), ("f32", 64, 8, 1, 16), ("int4", 128, 8, 2, 8), ("f32", 256, 16, 1, 32), ("bf16", 48, 16, 3, 16)])
+def test_attend_many_short_pieces(dtype, D, G, group, ps):
+    """Many short rows with a few new tokens each: a wave for each tile.  Rows that no token of a tile but its neighbours sees hold NaN."""
+    g = _gen(D + G + 1)
+    S = 140
+    r = torch.Generator().manual_seed(3)
+    new = torch.randint(0, 8, (S,), generator=r).tolist()
+    lens = [n + p for n, p in zip(new, torch.randint(0, 90, (S,), generator=r).tolist())]
+    kv = _cache(dtype, G, D, ps, lens, width=-(-200 // ps))
+    store = _fill(kv, 0, lens, g)
+    T = sum(new)
+    q = _randn(g, T + 3, G * group, D).mul_(2).to(kv.activations)
+    rows = torch.arange(S, dtype=torch.int32, device=DEV)
+    out = torch.full_like(q, 7.0)
+    kv.attend(0, q, rows, _offsets(new), window=30, sinks=3, out=out)
+    assert bool((out[T:] == 7.0).all())
+    start = [sum(new[:i]) for i in range(S)]
+    for i in (0, 1, 2, 50, 77, 138, 139):
+        if new[i]:
+            s = slice(start[i], start[i] + new[i])
+            want, mag, dot = attention(q[s], *store[i], list(range(lens[i] - new[i], lens[i])), 30, 3, D ** -0.5)
+            _check_attend(out[s], want, mag, dot, kv, lens[i], D ** -0.5, q[s].double(), prompt=True)
+    i = next(i for i in range(S) if new[i] >= 5 and lens[i] - new[i] > 40)
+    bad = lens[i] - 2                                               # seen by the last two of the row's tokens
+    page, slot = int(kv.table[i, bad // ps]), bad % ps
+    if dtype == "int4":
+        kv.v_scale[0, page, 0, slot, 0] = float("nan")
+    else:
+        kv.v[0, page, 0, slot, 3] = float("nan")
+    again = kv.attend(0, q, rows, _offsets(new), window=30, sinks=3)
+    end = start[i] + new[i]
+    assert not bool(torch.isfinite(again[end - 2:end]).all(-1).all(-1).any())
+    assert torch.equal(again[:end - 2], out[:end - 2]) and torch.equal(again[end:T], out[end:T])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "int4"])
+def test_captured_calls_of_long_rows_follow_their_lengths(dtype):
+    """A call in one line of runs and a whole prompt, captured; lengths, tables and queries change between replays, with eager work of the
+    same cache between them.  Every replay equals the eager call."""
+    g = _gen(41)
+    G, H, D, ps, S = 8, 16, 128, 32, 40
+    lens = [1000 - 20 * i for i in range(S)]
+    kv = _cache(dtype, G, D, ps, lens, width=60)
+    _fill(kv, 0, lens, g)
+    rows = torch.arange(S, dtype=torch.int32, device=DEV)
+    q = _randn(g, S, H, D, dtype=torch.bfloat16)
+    qp = _randn(g, 300, H, D, dtype=torch.bfloat16)
+    off = _offsets([200, 100])
+    s = torch.cuda.Stream()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=s):
+            graphs.append((graph, kv.attend(0, q, rows, window=1000, sinks=4), kv.attend(0, qp, rows[:2], off)))
+    for i in range(4):
+        q.copy_(_randn(g, S, H, D))
+        qp.copy_(_randn(g, 300, H, D))
+        kv.lens.copy_(torch.tensor([max(0, n - 231 * i * (j % 3)) for j, n in enumerate(lens)], dtype=torch.int32))
+        kv.table[2:4] = kv.table[2:4].flip(0).clone()
+        a, b = kv.attend(0, q, rows, window=1000, sinks=4), kv.attend(0, qp, rows[:2], off)
+        torch.cuda.synchronize()
+        streams = (torch.cuda.current_stream(), s)
+        for st, (graph, _, _) in zip(streams, graphs):              # both at once
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, c, d in graphs:
+            # bits: a row that took over a table whose last places nobody wrote sees their NaN
+            assert torch.equal(a.view(torch.int16), c.view(torch.int16)) and torch.equal(b.view(torch.int16), d.view(torch.int16)), i
+
+
+def test_rows_of_a_very_wide_table():
+    """A table of 2^25 entries a row: release, trim, reserve, fork and attend reach the last of them."""
+    from qwen3_tts_amd.kvcache import PagedKV
+    g = _gen(51)
+    W, ps, D = 1 << 25, 8, 64
+    kv = PagedKV(1, 1, D, 12, ps, rows=2, pages_per_row=W, dtype="f32", device=DEV)
+    kv.lens[0] = W * ps - 9                                          # as after a long stream whose pages were trimmed
+    kv.table[0, 0], kv.table[0, W - 2] = 0, 1
+    kv.refs[:2] = 1
+    kv.reserve([0], _offsets([8]), tokens=8)
+    assert int(kv.table[0, W - 1]) == 2 and int(kv.lens[0]) == W * ps - 1
+    x = _randn(g, 8, 1, D)
+    rows = torch.zeros(1, dtype=torch.int32, device=DEV)
+    kv.append(0, x, x, x, rows, _offsets([8]))
+    out = kv.attend(0, x[-1:], rows, window=2 ** 31 - 1, sinks=2 ** 31 - 1)
+    near = kv.attend(0, x[-1:], rows, window=8)
+    want, mag, dot = attention(x[-1:], x, x, [7], 0, 0, D ** -0.5)
+    _check_attend(near, want, mag, dot, kv, 8, D ** -0.5)
+    kk = torch.cat([x.new_zeros(8 + 7, 1, D), x])                    # the first page, what the last but one held before
+    want, mag, dot = attention(x[-1:], kk, kk, [22], 0, 0, D ** -0.5)
+    _check_attend(out, want, mag, dot, kv, 23, D ** -0.5)
+    kv.fork([0], [1])
+    assert int(kv.table[1, W - 2]) == 1 and int(kv.table[1, W - 1]) == 3
+    kv.trim([1], window=7, sinks=0)
+    assert kv.table[1, :1].tolist() == [-1] and int(kv.table[1, W - 2]) == -1 and int(kv.table[1, W - 1]) == 3
+    kv.check()
+    kv.release([0, 1])
+    assert kv.free_pages() == 12 and bool((kv.table == -1).all())
+    kv.check()
+
+
+def test_tensors_that_ask_for_gradients_are_refused():
+    kv = _cache("f32", 1, 64, 16, [20])
+    rows = torch.zeros(1, dtype=torch.int32, device=DEV)
+    q, k = (torch.zeros(1, 1, 64, device=DEV, requires_grad=r) for r in (True, False))
+    for call in (lambda: kv.attend(0, q, rows), lambda: kv.append(0, q, k, k, rows), lambda: kv.append(0, k, k, q, rows)):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+    with torch.no_grad():
+        kv.append(0, q, q, q, rows)
+    kv.check()
