@@ -763,8 +763,8 @@ convgemm_kernel(const ConvGemmArgs p) {
     const int half = lane >> 5, l31 = lane & 31;
     mark(2);
     // lean-register shapes: the epilogue's per-lane row offsets must not be computed before the main loop and carried through
-    // it (they are loop-invariant, so the compiler would): an opaque zero defined HERE goes into every one of them
-    if constexpr (LEAN_REGS) asm volatile("" : "+v"(late0));
+    // it (they are loop-invariant, so the compiler would): an opaque zero defined HERE goes into every one of them (a scalar: a vector register for it is one too many)
+    if constexpr (LEAN_REGS) asm volatile("" : "+s"(late0));
     if constexpr (FUSE2 && !INNER_LDS) {      // the compiler's wait for the parameters lands here, where the DMA queue is empty
 #pragma unroll
         for (int j = 0; j < WN; ++j) asm volatile("" : "+v"(ia[j]), "+v"(iib[j]), "+v"(ibias[j]));
