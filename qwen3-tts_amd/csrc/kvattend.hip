@@ -925,14 +925,18 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
     const int slot = tid & (NCH - 1), row0 = tid / NCH, sub = lane / NCH;
     const float cs = a.scale_log2e;
     // LDS places of this lane's operands; tiles, halves and buffers are constants added to them
-    int ak[KS], av[ND];
+    constexpr bool FEW = DP == 256;            // registers are short: places from the first one by exclusive or, where they are used
+    int ak[FEW ? 1 : KS], av[FEW ? 1 : ND];
     {
         const int q4 = (lane >> 2) & 3, p4 = lane & 3, c16 = (lane >> 4) & 1;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) ak[k] = lds_k<DP>(r, 2 * k + hh);
+        for (int k = 0; k < (FEW ? 1 : KS); ++k) ak[k] = lds_k<DP>(r, 2 * k + hh);
 #pragma unroll
-        for (int n = 0; n < ND; ++n) av[n] = lds_v<DP>(4 * hh + q4, 4 * n + 2 * c16 + (p4 >> 1)) + 8 * (p4 & 1);
+        for (int n = 0; n < (FEW ? 1 : ND); ++n) av[n] = lds_v<DP>(4 * hh + q4, 4 * n + 2 * c16 + (p4 >> 1)) + 8 * (p4 & 1);
     }
+
+    auto key_at = [&](int k) { return FEW ? ak[0] ^ (32 * k) : ak[FEW ? 0 : k]; };
+    auto value_at = [&](int n) { return FEW ? av[0] ^ (64 * n) : av[FEW ? 0 : n]; };
 
     int only = t.pmin - 1;                     // as in kv_attend_kernel: a second look, position by position, where a result is not finite
     for (;;) {
@@ -1023,7 +1027,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
             for (int k = 0; k < KS; ++k)
 #pragma unroll
                 for (int u = 0; u < NT; ++u)
-                    s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(k0 + 32 * u * RB + ak[k]), qf[k], s[u], 0, 0, 0);
+                    s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(k0 + 32 * u * RB + key_at(k)), qf[k], s[u], 0, 0, 0);
         };
 #pragma unroll
         for (int n = 0; n < ND; ++n)
@@ -1054,6 +1058,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
         auto tile = [&](int c, auto which) {
             constexpr int P = decltype(which)::value;
             const int kb = span.chunk(c) * KT;
+            if constexpr (FEW) asm volatile("" : "+v"(ak[0]), "+v"(av[0]));
             const unsigned long long okm = ok0;
             if (c + 1 < span.total) fetch(c + 1, ok1, vbase, a.c.vs, sv[P ^ 1], values, vr);
             ok0 = ok1;
@@ -1095,12 +1100,12 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
             constexpr int QK = KS * NT, PV = 2 * NT * ND, NE = 16 * NT / 2, AHEAD = DMA ? 5 : 4;      // products, pairs of scores
             bf16x8 ring[AHEAD];
             u32x4 p[NT][2];
-            auto read_k = [&](int j) { return *(const bf16x8*)(sk[P ^ 1] + 32 * (j % NT) * RB + ak[j / NT]); };
+            auto read_k = [&](int j) { return *(const bf16x8*)(sk[P ^ 1] + 32 * (j % NT) * RB + key_at(j / NT)); };
             auto read_v = [&](int j) {
                 bf16x8 x;
 #pragma unroll
                 for (int jj = 0; jj < 2; ++jj) {
-                    const unsigned char* ad = sv[P] + (16 * (j / ND) + 8 * jj) * RB + av[j % ND];
+                    const unsigned char* ad = sv[P] + (16 * (j / ND) + 8 * jj) * RB + value_at(j % ND);
                     const bf16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)ad);
 #pragma unroll
                     for (int w = 0; w < 4; ++w) x[4 * jj + w] = v[w];
@@ -1177,9 +1182,19 @@ int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 long long tiles_of(int tokens, int sequences, int group, bool ragged, int cols = 16) {
     return ragged ? (long long)tokens * group / cols + sequences : (long long)sequences * ((group + cols - 1) / cols);
 }
-// Which kernel: 16-column tiles re-read a request's keys for every tile, 128-column ones feed them to four waves through LDS
+// Which kernel: 16-column tiles re-read a request's keys for every tile, but cut them over workgroups; 128-column ones feed them to four
+// waves through LDS, and a row's keys stay with one workgroup.  The second kind needs enough columns per request to fill its tiles and
+// enough (16-column tile, kv head) pairs that whole rows keep the card busy.  Measured, 128 columns against 16 (us; 16 heads on 8):
+//   bf16, D = 128: 64 x 16 new tokens behind 984 (1024 pairs) 49 / 89, 2 x 1000 under a window of 500 (2000) 26 / 53, 6 x 64 behind 3936 (384)
+//     90 / 121, 1 x 400 (400) 16 / 14, 1 x 100 (100) 10 / 6; of 16 columns: 300 x 8 behind 292 102 / 99, 700 x 8 behind 52 115 / 64
+//   4 bits, where each workgroup has its own keys to unpack, D = 128: 24 x 500 (12000) 120 / 149, 64 x 128 behind 872 (8192) 191 / 210, 64 x 64
+//     (4096) 157 / 116, 2 x 1000 under a window of 500 (2000) 43 / 40, 6 x 128 behind 3872 (768) 189 / 89, 1 x 400 (400) 29 / 12
+//   4 bits, D = 256: 8 x 200 behind 3800 (1600) 378 / 513, 24 x 500 325 / 575, 64 x 64 (4096) 464 / 386, 3 x 235 (705) 40 / 31
 bool prompts(const KvView& c, int tokens, int sequences, int q_heads, bool ragged) {
-    return c.dtype != Q3C_KV_F32 && !(c.dtype == Q3C_KV_INT4 && c.dim > 128) && ragged && (long long)tokens * (q_heads / c.heads) >= 64ll * sequences;
+    if (c.dtype == Q3C_KV_F32 || !ragged) return false;
+    const bool four = c.dtype == Q3C_KV_INT4;
+    const long long columns = (long long)tokens * (q_heads / c.heads), least = !four ? 512 : c.dim == 256 ? 1536 : 6144;
+    return columns >= (four ? 256ll : 32ll) * sequences && columns / 16 * c.heads >= least;
 }
 // most chunks that one row of the call can see
 long long most_chunks(const KvView& c, int window, int sinks, int max_len) {
@@ -1241,7 +1256,8 @@ hipError_t q3_launch_kv_attend(const KvAttendArgs& a, hipStream_t s) {
             else kv_prompt_kernel<bf16, 256, 32><<<blocks, 256, 0, s>>>(a, n);
         } else {
             if (dp == 64) kv_prompt_kernel<Int4, 64, 64><<<blocks, 256, 0, s>>>(a, n);
-            else kv_prompt_kernel<Int4, 128, 32><<<blocks, 256, 0, s>>>(a, n);
+            else if (dp == 128) kv_prompt_kernel<Int4, 128, 32><<<blocks, 256, 0, s>>>(a, n);
+            else kv_prompt_kernel<Int4, 256, 32><<<blocks, 256, 0, s>>>(a, n);
         }
         return hipGetLastError();
     }

@@ -385,14 +385,16 @@ __device__ __forceinline__ int plan_owner(const int* base, int n, int rank) {
     return lo;
 }
 
-// Block-uniform walk over a list in LDS tiles: each(j, list[j]) for all j < count, by every thread.
+// Walk of threads 0 .. live - 1 over a list in LDS tiles (the whole workgroup calls it): each(j, list[j]) for all j < count.  Waves that have
+// none of those threads only help to load: the comparisons of all sixteen would take most of a plan's time (120 pairs: 15 us against 13).
 template <typename Each>
-__device__ __forceinline__ void plan_walk(const int* __restrict__ list, int count, int* tile /* PLAN_T, 16-byte aligned */, Each each) {
+__device__ __forceinline__ void plan_walk(const int* __restrict__ list, int count, int live, int* tile /* PLAN_T, 16-byte aligned */, Each each) {
     for (int j0 = 0; j0 < count; j0 += PLAN_T) {
         const int n = min(PLAN_T, count - j0);
         __syncthreads();
         if ((int)threadIdx.x < n) tile[threadIdx.x] = list[j0 + threadIdx.x];
         __syncthreads();
+        if ((int)(threadIdx.x & ~63u) >= live) continue;
         for (int j = 0; j < n; j += 4) {
             const int4 v = *(const int4*)(tile + j);
             each(j0 + j, v.x);
@@ -414,7 +416,7 @@ __global__ void __launch_bounds__(PLAN_T) kv_reserve_kernel(const KvView c, cons
         bool ok = row >= 0 && row < c.rows;
         if (ok) old = max(c.lens[row], 0);
         if (tid < n && b.offsets) add = min(max(b.offsets[i + 1], 0), b.tokens) - min(max(b.offsets[i], 0), b.tokens);
-        plan_walk(b.rows, s0 + n, tile, [&](int j, int r) { ok = ok && (j >= i || r != row); });   // named twice: the first counts
+        plan_walk(b.rows, s0 + n, n, tile, [&](int j, int r) { ok = ok && (j >= i || r != row); });   // named twice: the first counts
         if (tid < n) {
             ok = ok && add >= 0;
             if (ok) {
@@ -478,7 +480,7 @@ __global__ void __launch_bounds__(256) kv_release_kernel(const KvView c, const i
 // destination page, [count] 1 = good pair.
 __global__ void __launch_bounds__(PLAN_T) kv_fork_plan_kernel(const KvView c, const int* __restrict__ parents, const int* __restrict__ children,
                                                               int count, int* __restrict__ ws) {
-    __shared__ int lds[17 + PLAN_K * 16], base[PLAN_T];
+    __shared__ int lds[17 + PLAN_K * 16], taker[PLAN_T];             // taker: of the page of each rank
     __shared__ __attribute__((aligned(16))) int tile[PLAN_T];
     const int tid = threadIdx.x;
     for (int s0 = 0; s0 < count; s0 += PLAN_T) {
@@ -488,7 +490,7 @@ __global__ void __launch_bounds__(PLAN_T) kv_fork_plan_kernel(const KvView c, co
         bool ok = up >= 0 && up < c.rows && ch >= 0 && ch < c.rows;
         if (ok) ok = c.lens[ch] == 0;
         // a child must be empty and named once (the first counts), and no row of the call both parent and child
-        plan_walk(children, count, tile, [&](int j, int r) { ok = ok && (j >= i || r != ch) && r != up; });
+        plan_walk(children, count, n, tile, [&](int j, int r) { ok = ok && (j >= i || r != ch) && r != up; });
         if (tid < n) {
             int src = -1;
             if (ok) {
@@ -504,12 +506,11 @@ __global__ void __launch_bounds__(PLAN_T) kv_fork_plan_kernel(const KvView c, co
         }
         int total;
         const int ex = plan_scan(need, lds, total);
-        if (tid < n) base[tid] = ex;
+        if (need) taker[ex] = tid;
         __syncthreads();
         const int got = plan_pages(c, 0, c.pages, total, lds, [](int r) { return r == 0; }, [&](int rank, int p) {
             c.refs[p] = 1;
-            // of equal bases the last is the one that needs a page (those before it need none)
-            ws[count + s0 + plan_owner(base, n, rank)] = p;
+            ws[count + s0 + taker[rank]] = p;
         });
         if (tid < n && need && ex >= got) ws[i] = -1;
         if (got < total && tid == 0) kv_flag(c, Q3C_KV_NO_PAGE);

@@ -916,3 +916,64 @@ def test_tensors_that_ask_for_gradients_are_refused():
     with torch.no_grad():
         kv.append(0, q, q, q, rows)
     kv.check()
+
+
+@pytest.mark.parametrize("dtype,D,G,group,ps", [("bf16", 128, 2, 8, 32), ("bf16", 64, 1, 20, 8), ("bf16", 256, 4, 3, 64), ("bf16", 80, 3, 5, 16), ("bf16", 16, 12, 1, 256),
+                                                ("int4", 64, 8, 17, 16), ("int4", 128, 17, 8, 8), ("int4", 128, 8, 17, 32), ("int4", 256, 4, 9, 128), ("int4", 256, 12, 3, 8)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (72, 0), (90, 10)])
+def test_attend_prompts_with_many_heads(dtype, D, G, group, ps, window, sinks):
+    """Enough columns for the kernel that shares key tiles between waves, in each type and head size: a whole prompt, a piece behind a past,
+    a row of one token, an empty one; a missing page and one outside the pool; NaN where no query of a token looks; captured."""
+    g = _gen(D * 7 + group + window)
+    lens, new = [400, 333, 1, 0, 170], [400, 200, 1, 0, 160]
+    kv = _cache(dtype, G, D, ps, lens)
+    store = _fill(kv, 0, lens, g)
+    T = sum(new)
+    q = _randn(g, T + 2, G * group, D).mul_(2).to(kv.activations)
+    out = torch.full_like(q, 5.0)
+    rows = torch.arange(5, dtype=torch.int32, device=DEV)
+    kv.attend(0, q, rows, _offsets(new), window=window, sinks=sinks, out=out)
+    kv.check()
+    assert bool((out[T:] == 5.0).all())
+    scale = D ** -0.5
+    for r, start, some in ((0, 0, [0, 31, 64, 127, 257, 399]), (1, 400, [0, 63, 199]), (2, 600, [0]), (4, 601, [0, 159])):
+        i = torch.tensor(some, device=DEV)
+        pos = [lens[r] - new[r] + p for p in some]
+        want, mag, dot = attention(q[start + i], *store[r], pos, window, sinks, scale)
+        _check_attend(out[start + i], want, mag, dot, kv, lens[r], scale, q[start + i].double(), prompt=True)
+    graph, off = torch.cuda.CUDAGraph(), _offsets(new)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        again = kv.attend(0, q, rows, off, window=window, sinks=sinks)
+    for _ in range(3):
+        again.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(again[:T], out[:T])
+
+    page, slot = int(kv.table[1, 250 // ps]), 250 % ps              # position 250 of the second row: token 117 of its piece
+    where = kv.v_scale[0, page, G - 1, slot, 1:2] if dtype == "int4" else kv.v[0, page, G - 1, slot, 3:4]
+    was = where.clone()
+    where.fill_(float("inf") if dtype == "int4" else float("nan"))
+    got = kv.attend(0, q, rows, _offsets(new), window=window, sinks=sinks)
+    where.copy_(was)
+    sees = torch.zeros(T, dtype=torch.bool, device=DEV)
+    sees[400 + 117:600 if not window else min(600, 400 + 117 + window)] = True
+    # Not bit for bit what it was: such a tile is computed again position by position, and the maximum that its probabilities are rounded against
+    # moves for a whole wave at a time.  Each result by itself is within the bound of the formula, in which the bad row has no part.
+    assert bool(torch.isfinite(got[:T][~sees]).all())
+    for tok in (0, 63, 110, 116, 189, 199):
+        if not bool(sees[400 + tok]):
+            want, mag, dot = attention(q[400 + tok:401 + tok], *store[1], [133 + tok], window, sinks, scale)
+            _check_attend(got[400 + tok:401 + tok], want, mag, dot, kv, 333, scale, q[400 + tok:401 + tok].double(), prompt=True)
+    assert not bool(torch.isfinite(got[:T][sees][:, (G - 1) * group:]).all(-1).any())
+
+    kv.table[0, 32 // ps] = -1
+    kv.table[0, 300 // ps] = kv.pages + 1
+    there = torch.ones(400, dtype=torch.bool, device=DEV)
+    for p in (32, 300):
+        there[p // ps * ps:p // ps * ps + ps] = False
+    got = kv.attend(0, q, rows, _offsets(new), window=window, sinks=sinks)
+    i = torch.tensor([0, 31, 64, 127, 257, 330, 399], device=DEV)
+    want, mag, dot = attention(q[i], *store[0], i.tolist(), window, sinks, scale, there)
+    _check_attend(got[i], want, mag, dot, kv, 400, scale, q[i].double(), prompt=True)
