@@ -74,7 +74,7 @@ __device__ __forceinline__ bool kv_place(const KvAppendArgs& a, int tok, bool fi
 // A wave has one token and `parts`-th of its heads, VEC pairs per lane as two runs that are each other's rotation partners, so that the
 // rotation needs no exchange between lanes and the norm one butterfly over the head's lanes.  Two runs of heads are requested before
 // the token's place is looked up (offset -> row -> length -> page, four dependent reads): they are what a wave has to wait for once.
-// 28143 tokens of 16 + 8 + 8 heads of 128 in bf16: 113 us, 4.1 TB/s; 64 single tokens 4.8 us.
+// 28144 tokens of 16 + 8 + 8 heads of 128 in bf16: 113 us, 4.1 TB/s; 64 single tokens 4.8 us.
 template <typename T, int VEC, bool CACHED>     // CACHED: keys and values go to the pages here too (no 4-bit cache)
 __device__ __forceinline__ void append_plain(const KvAppendArgs& a, int tok, int part, int parts, int lane, int lpu_shift) {
     constexpr int RUN = 2;
