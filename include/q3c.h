@@ -310,7 +310,8 @@ int q3c_wav_to_pcm16(const float* wav_dev, int64_t samples, int16_t* pcm_dev, vo
  * a request stands at position lens[row] - 1: q3c_kv_reserve first makes room (lens grows), then every layer appends and attends.
  * Tokens before offsets[0] and from offsets[sequences] on are neither read nor written.  What a list, an offset or a table entry says is checked on the
  * device: a token whose row is bad or named before in the call, or that has no page, is not stored (its query is zeros if its row or
- * position is bad), keys without a page are seen by nobody, and the bit in `status` says so. */
+ * position is bad), keys without a page are seen by nobody, and the bit in `status` says so.  Calls whose launch would pass 2^32 threads
+ * along one axis (tokens * heads from 2^27 on, copies of some ten thousand pages of many layers) are Q3C_ERR_UNSUPPORTED. */
 typedef enum q3c_kv_dtype { Q3C_KV_F32 = 0, Q3C_KV_BF16 = 1, Q3C_KV_INT4 = 2 } q3c_kv_dtype;
 typedef enum q3c_kv_status {
     Q3C_KV_BAD_ROW = 1,      /* a row id outside the table, named twice, or offsets that do not fit the row's length */

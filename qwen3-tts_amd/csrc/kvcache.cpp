@@ -40,9 +40,14 @@ int batch(const int32_t* rows, const int32_t* offsets, int32_t sequences, int32_
 bool strided(const void* p, int64_t ts, int64_t hs, size_t elem) { return p && aligned(p, 4 * elem) && ts % 4 == 0 && hs % 4 == 0 && ts >= 0 && hs >= 0; }
 int done(hipError_t e) { return e == hipSuccess ? 0 : Q3C_ERR_HIP; }
 size_t act_bytes(const KvView& c) { return c.dtype == Q3C_KV_F32 ? 4 : 2; }
-bool pieces_fit(const KvView& c, int count) {      // one workgroup per 16 KB of a pair: the grid has to stay below 2^31
-    const long long page = ((long long)c.heads << c.ps_shift) * c.dim * 4;
-    return ((page + 16383) / 16384 * 4 * c.layers + 1) * count < 0x7fffffffll;
+// A launch has fewer than 2^32 threads along x: below 2^24 workgroups of 256.
+constexpr long long MOST_BLOCKS = 1 << 24;
+bool pieces_fit(const KvView& c, int count) {      // one workgroup per 16 KB of a pair
+    const long long page = ((long long)c.heads << c.ps_shift) * c.dim * (c.dtype == Q3C_KV_F32 ? 4 : 2);
+    return ((page + 16383) / 16384 * 4 * c.layers + 1) * count < MOST_BLOCKS;
+}
+bool heads_fit(int tokens, long long heads) {      // append, gather: at most a wave per head while tokens are few, per four of them beyond
+    return tokens * heads < 8 * MOST_BLOCKS;
 }
 
 }  // namespace
@@ -73,7 +78,7 @@ int q3c_kv_append(const q3c_kv* kv, int32_t layer, const void* q, int64_t q_ts, 
     if (a.c.dtype == Q3C_KV_INT4 && rot_dim && rot_dim != a.c.dim) return Q3C_ERR_UNSUPPORTED;
     if (rot_dim && (!cos_table || !sin_table || !aligned(cos_table, 16) || !aligned(sin_table, 16))) return Q3C_ERR_INVALID_ARGUMENT;
     if (rot_dim && positions < ((int64_t)a.c.width << a.c.ps_shift)) return Q3C_ERR_INVALID_ARGUMENT;
-    if ((long long)tokens * (q_heads + 2ll * a.c.heads) >= 0x40000000ll) return Q3C_ERR_UNSUPPORTED;
+    if (!heads_fit(tokens, q_heads + 2ll * a.c.heads)) return Q3C_ERR_UNSUPPORTED;
     a.layer = layer;
     a.q = {q, q_ts, q_hs}; a.k = {k, k_ts, k_hs}; a.v = {v, v_ts, v_hs};
     a.q_heads = q_heads;
@@ -90,7 +95,7 @@ int q3c_kv_gather(const q3c_kv* kv, int32_t layer, const int32_t* rows, const in
     if (layer < 0 || layer >= c.layers || (out_precision != Q3C_PRECISION_F32 && out_precision != Q3C_PRECISION_BF16)) return Q3C_ERR_INVALID_ARGUMENT;
     if (!tokens) return 0;
     if (!k_out || !v_out || !aligned(k_out, 16) || !aligned(v_out, 16)) return Q3C_ERR_INVALID_ARGUMENT;
-    if ((long long)tokens * 2 * c.heads >= 0x40000000ll) return Q3C_ERR_UNSUPPORTED;
+    if (!heads_fit(tokens, 2ll * c.heads)) return Q3C_ERR_UNSUPPORTED;
     return done(q3_launch_kv_gather(c, b, layer, k_out, v_out, out_precision == Q3C_PRECISION_F32 ? Q3_F32 : Q3_BF16, (hipStream_t)stream));
 }
 
@@ -98,7 +103,9 @@ static int attend_shape(const q3c_kv* kv, int32_t q_heads, int32_t sequences, in
     const int rc = view(kv, c);
     if (rc) return rc;
     if (q_heads < 1 || q_heads % c->heads || sequences < 0 || tokens < 0 || window < 0 || sinks < 0 || max_len < 0) return Q3C_ERR_INVALID_ARGUMENT;
-    if (tokens > (1 << 24) || sequences > (1 << 24) || (long long)tokens * q_heads >= 0x40000000ll) return Q3C_ERR_UNSUPPORTED;
+    // a workgroup per 16 columns along x, per 128 columns and kv head, or a wave per 16 columns and kv head
+    const long long columns = (long long)tokens * (q_heads / c->heads), tiles = columns / 16 + sequences;
+    if (tiles >= MOST_BLOCKS || (columns / 128 + sequences) * c->heads >= MOST_BLOCKS || tiles * c->heads >= 4 * MOST_BLOCKS) return Q3C_ERR_UNSUPPORTED;
     return 0;
 }
 
@@ -156,6 +163,7 @@ int q3c_kv_release(const q3c_kv* kv, const int32_t* rows, int32_t count, void* s
     const int rc = view(kv, &c);
     if (rc) return rc;
     if (count < 0 || (count && !rows)) return Q3C_ERR_INVALID_ARGUMENT;
+    if (count >= MOST_BLOCKS) return Q3C_ERR_UNSUPPORTED;
     return done(q3_launch_kv_release(c, rows, count, 0, 0, 0, (hipStream_t)stream));
 }
 int q3c_kv_trim(const q3c_kv* kv, const int32_t* rows, int32_t count, int32_t window, int32_t sinks, void* stream) {
@@ -163,6 +171,7 @@ int q3c_kv_trim(const q3c_kv* kv, const int32_t* rows, int32_t count, int32_t wi
     const int rc = view(kv, &c);
     if (rc) return rc;
     if (count < 0 || (count && !rows) || window < 1 || sinks < 0) return Q3C_ERR_INVALID_ARGUMENT;
+    if (count >= MOST_BLOCKS) return Q3C_ERR_UNSUPPORTED;
     return done(q3_launch_kv_release(c, rows, count, 1, window, sinks, (hipStream_t)stream));
 }
 int q3c_kv_copy_pages(const q3c_kv* kv, const int32_t* src, const int32_t* dst, int32_t count, void* workspace, size_t workspace_bytes, void* stream) {

@@ -106,6 +106,20 @@ def test_c_entry_points_refuse_bad_calls():
     assert lib.q3c_kv_gather(kv, 0, PTR, None, 1, 1, PTR, PTR, 2, None) == INVALID and lib.q3c_kv_gather(kv, 0, PTR, None, 1, 1, None, PTR, 1, None) == INVALID
 
 
+def test_calls_larger_than_a_launch_are_refused():
+    """A launch has fewer than 2^32 threads along its first axis: calls whose grid would pass that are refused before anything runs."""
+    lib, kv, n = _lib.load(), _kv(), C.c_size_t()
+    for heads, seqs, tokens, rc in ((2, 1, 1 << 20, OK), (256, 1, 1 << 21, UNSUPPORTED), (2, 1 << 23, 1 << 23, UNSUPPORTED), (2, 1 << 22, 1 << 22, OK)):
+        assert lib.q3c_kv_attend_workspace_bytes(kv, heads, seqs, tokens, 0, 0, 0, C.byref(n)) == rc, (heads, seqs, tokens)
+        if rc:
+            assert lib.q3c_kv_attend(kv, 0, PTR, 256, 64, heads, PTR, PTR, seqs, tokens, 0, 0, 1.0, 0, PTR, PTR, 1 << 40, None) == rc
+    assert lib.q3c_kv_append(kv, 0, PTR, 256, 64, PTR, 128, 64, PTR, 128, 64, 60, PTR, PTR, 1, 1 << 21, None, None, None, None, 0, 0, 1e-6, PTR, None) == UNSUPPORTED
+    assert lib.q3c_kv_gather(_kv(kv_heads=64), 0, PTR, PTR, 1, 1 << 20, PTR, PTR, 1, None) == UNSUPPORTED
+    assert lib.q3c_kv_release(kv, PTR, 1 << 24, None) == UNSUPPORTED and lib.q3c_kv_trim(kv, PTR, 1 << 24, 4, 0, None) == UNSUPPORTED
+    assert lib.q3c_kv_copy_pages(_kv(layers=64), PTR, PTR, 1 << 17, PTR, 1 << 40, None) == UNSUPPORTED
+    assert lib.q3c_kv_fork(_kv(layers=64), PTR, PTR, 1 << 17, PTR, 1 << 40, None) == UNSUPPORTED
+
+
 def test_rope_tables_of_far_positions():
     cos, sin = rope_tables(200001, 8, theta=1e6, device="cpu")
     import math
