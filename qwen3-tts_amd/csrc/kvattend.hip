@@ -570,7 +570,8 @@ __device__ __forceinline__ void attend_part(const KvAttendArgs& a, const Tile& t
 // head) pairs and at most two in part, its first and its last: two parts per wave are all the workspace there is, and
 // kv_flat_join_kernel puts the parts together.  Each workgroup finds the line's layout by itself: the chunk counts of all tiles, summed up.
 // A run for each wave rather than for each workgroup: no meeting of waves at a pair's end, which short rows have often (64 rows of 512
-// tokens in 4 bits 24 us against 47, in bf16 31 against 44; 32 rows of 16001 in bf16 226 us against 223: 5.5 TB/s).
+// tokens in 4 bits 24 us against 47, in bf16 31 against 44; 32 rows of 3200 - 16001 in bf16 226 us against 223: 5.5 TB/s; 64 such rows in 4 bits 164 us, 4.8 TB/s, where
+// unpacking on the vector units is what is left).
 constexpr int FLAT = 1024;
 constexpr int FLAT_LEAST = 4;                  // chunks of a run
 
@@ -747,7 +748,8 @@ __global__ void __launch_bounds__(256) kv_flat_join_kernel(const KvAttendArgs a,
 }
 
 // ---- few columns per request, or many requests --------------------------------------------------------------------------------------
-// One workgroup = one tile of columns, one kv head, one share (`share` chunks) of those the tile sees; where a tile has more than one
+// Bound by latency where it is called: 8 rows of 700 tokens in 4 bits 10.7 us (six rounds of four waves), one row under a window of 4096 7.9
+// and 3.9 to join.  One workgroup = one tile of columns, one kv head, one share (`share` chunks) of those the tile sees; where a tile has more than one
 // share kv_join_kernel joins them.  The workspace: for each (tile, kv head) the parts [splits], then how many there are.
 struct KvShares {
     float *sums, *ml;
@@ -807,7 +809,8 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const KvAttendArgs a) {
 // is allowed to lag: the sums are rescaled only when a column's maximum has grown by more than 2^8 (fp32 sums and bf16 probabilities have
 // the range), which a causal row does a few times in all.
 // Workgroups of one (request, kv head) sit eight apart in launch order, heads fastest: on the eight XCDs, whose workgroups are dealt
-// round robin, a head's keys stay in one L2.  Long columns start first.
+// round robin, a head's keys stay in one L2.  Long columns start first.  16503 new tokens in 6 requests under a window of 2048 (bf16, 16 heads
+// on 8 of 128): 250 us, 820 TFLOP/s of what is visible; the same on 16-column tiles 978.
 // 4 bits: values n * step are rounded to bf16 on their way into LDS (operands of the matrix cores), four bytes of the row = one 16-byte
 // chunk; the order of dimensions in a row is then the packed one, which Q's load and the output's store follow.
 template <typename T, int DP> struct Row;                       // chunk ch of a row: 8 values as 16 bytes

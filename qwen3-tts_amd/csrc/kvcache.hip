@@ -74,7 +74,7 @@ __device__ __forceinline__ bool kv_place(const KvAppendArgs& a, int tok, bool fi
 // A wave has one token and `parts`-th of its heads, VEC pairs per lane as two runs that are each other's rotation partners, so that the
 // rotation needs no exchange between lanes and the norm one butterfly over the head's lanes.  Two runs of heads are requested before
 // the token's place is looked up (offset -> row -> length -> page, four dependent reads): they are what a wave has to wait for once.
-// 28144 tokens of 16 + 8 + 8 heads of 128 in bf16: 113 us, 4.1 TB/s; 64 single tokens 4.8 us.
+// 28144 tokens of 16 + 8 + 8 heads of 128 in bf16: 113 us, 4.2 TB/s; 64 single tokens 4.8 us.
 template <typename T, int VEC, bool CACHED>     // CACHED: keys and values go to the pages here too (no 4-bit cache)
 __device__ __forceinline__ void append_plain(const KvAppendArgs& a, int tok, int part, int parts, int lane, int lpu_shift) {
     constexpr int RUN = 2;
@@ -311,7 +311,8 @@ __global__ void __launch_bounds__(256) kv_gather_kernel(const KvView c, const Kv
 
 // ---- pages ----------------------------------------------------------------------------------------------------------------------------
 // One workgroup plans each operation, so that page numbers come out the same whatever runs beside it: free pages are handed out
-// lowest first, to requests in the order of the call.  That bounds its time by a few dependent reads of memory, not by bandwidth.
+// lowest first, to requests in the order of the call.  That bounds its time by a few dependent reads of memory, not by bandwidth:
+// 6.3 us for a token of each of 64 rows, 12.5 for 120 forks, 8.2 for a compaction of 1 900 pages.
 constexpr int PLAN_T = 1024, PLAN_K = 8;      // a scan step looks at PLAN_T * PLAN_K pages
 
 // Exclusive prefix sums of one value per thread over the workgroup, and its total.  `sums`: 17 ints of LDS.
@@ -519,7 +520,8 @@ __global__ void __launch_bounds__(PLAN_T) kv_fork_plan_kernel(const KvView c, co
 }
 
 // ---- moving pages -----------------------------------------------------------------------------------------------------------------------
-// A pair's work is cut into pieces of at most 16 KB of one (layer, tensor): 256 lanes x 16 bytes x 4 in flight.
+// A pair's work is cut into pieces of at most 16 KB of one (layer, tensor): 256 lanes x 16 bytes x 4 in flight.  685 MB of moved pages: 285 us,
+// 4.8 TB/s read and written, what a large copy reaches.
 struct KvPieces { int per_page[4]; long long bytes[4]; char* base[4]; int per_layer, layers, pages; };
 
 __host__ __device__ __forceinline__ KvPieces kv_pieces(const KvView& c) {
