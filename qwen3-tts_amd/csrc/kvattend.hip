@@ -803,7 +803,7 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const KvAttendArgs a) {
 // ---- prompts -----------------------------------------------------------------------------------------------------------------------------
 // Many columns per request (prompts, long pieces; bf16 and 4 bits): bound by the matrix cores and the LDS that feeds them.  One
 // workgroup = 128 columns of one request and kv head, 32 per wave; keys and values go through LDS in tiles of KT, two buffers
-// deep: while a tile is multiplied the next one's rows are on their way to registers, and one barrier per tile hands them over.
+// deep: while a tile is multiplied the next one's rows are on their way (bf16: to LDS; 4 bits: to registers), and one barrier per tile hands them over.
 // A wave computes S^T = K Q^T on 32 x 32 x 16 products, so that a lane holds scores of one column and its probabilities are, register
 // for register, the B operand of O^T = V^T P^T; V^T comes from the row-major image by transposed LDS reads.  The probabilities' maximum
 // is allowed to lag: the sums are rescaled only when a column's maximum has grown by more than 2^8 (fp32 sums and bf16 probabilities have

@@ -38,6 +38,7 @@ Rows = Union[torch.Tensor, Sequence[int]]
 GROUP = 32                                     # dimensions that share a step in a 4-bit cache
 _HELD = {torch.float32: 0, torch.bfloat16: 1, torch.uint8: 2}
 _ACT = (torch.float32, torch.bfloat16, torch.bfloat16)
+_MOST = 2 ** 31 - 1
 # the current device and its stream's handle, without the objects that torch.cuda wraps them in (a call of a generation step is host-bound)
 _device, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 _STATUS = ((1, "a row id outside the table, named twice in a call, or offsets that do not fit a row's length"),
@@ -186,10 +187,13 @@ class PagedKV:
             return rows, n, None, n
         if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.shape[0] != n + 1 or not offsets.is_contiguous() or offsets.get_device() != self._index:
             raise ValueError(f"offsets must be a contiguous int32 tensor [{n + 1}] on {self.device}")
+        if tokens is not None and not 0 <= tokens <= 1 << 24:
+            raise ValueError(f"a call takes at most 2^24 tokens, got {tokens}")
         return rows, n, offsets, tokens
 
     def _heads(self, x: torch.Tensor, what: str, heads: Optional[int]) -> torch.Tensor:
-        """[tokens, heads, head_dim] in the cache's activation type; copied only where its strides are not what the kernels read."""
+        """[tokens, heads, head_dim] in the cache's activation type; copied only where its strides are not what the kernels read: multiples of
+        four (the stride of a dimension of one element may be anything, and is passed on rounded down)."""
         shape = x.shape
         if len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads) or shape[1] < 1:
             raise ValueError(f"{what} must be [tokens, {'heads' if heads is None else heads}, {self.head_dim}], got {tuple(shape)}")
@@ -199,7 +203,7 @@ class PagedKV:
             raise ValueError(f"{what} requires a gradient, and the cache's operators have none: call them under torch.no_grad()")
         ts, hs, ds = x.stride()
         quad = 4 * self._act_bytes
-        if ds != 1 or ts % 4 or hs % 4 or x.data_ptr() % quad:
+        if ds != 1 or (ts % 4 and shape[0] != 1) or (hs % 4 and shape[1] != 1) or x.data_ptr() % quad:
             x = x.contiguous()
             if x.data_ptr() % quad:                            # a contiguous view that starts between two quads
                 x = x.clone()
@@ -265,8 +269,8 @@ class PagedKV:
             if positions < self.max_tokens:
                 raise ValueError(f"rope covers {positions} positions, a row can hold {self.max_tokens}")
         out = self._out(out, (T, H, self.head_dim), self.activations)
-        self._call(self._lib.q3c_kv_append, self._layer(layer), q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-                   v.data_ptr(), v.stride(0), v.stride(1), H, rows.data_ptr(), None if offsets is None else offsets.data_ptr(), n, T,
+        self._call(self._lib.q3c_kv_append, self._layer(layer), q.data_ptr(), q.stride(0) & -4, q.stride(1) & -4, k.data_ptr(), k.stride(0) & -4, k.stride(1) & -4,
+                   v.data_ptr(), v.stride(0) & -4, v.stride(1) & -4, H, rows.data_ptr(), None if offsets is None else offsets.data_ptr(), n, T,
                    None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
                    None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(), positions, rot, eps, out.data_ptr())
         return out
@@ -300,8 +304,8 @@ class PagedKV:
         T, H = q.shape[0], q.shape[1]
         if H % self.kv_heads:
             raise ValueError(f"{H} query heads do not share {self.kv_heads} kv heads evenly")
-        if window < 0 or sinks < 0 or max_len < 0:
-            raise ValueError("window, sinks and max_len must not be negative")
+        if window < 0 or sinks < 0 or max_len < 0 or window > _MOST or sinks > _MOST or max_len > _MOST:
+            raise ValueError("window, sinks and max_len must be from 0 to 2^31 - 1")
         scale = self.head_dim ** -0.5 if scale is None else float(scale)
         if not 0.0 < scale < 3e38:
             raise ValueError(f"scale must be positive and finite, got {scale}")
@@ -321,7 +325,7 @@ class PagedKV:
             need = self._need[key] = int(size.value)
         # a workspace of its own for each call: calls on two streams, or two captured graphs, share none
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        self._call(self._lib.q3c_kv_attend, self._layer(layer), q.data_ptr(), q.stride(0), q.stride(1), H, rows.data_ptr(),
+        self._call(self._lib.q3c_kv_attend, self._layer(layer), q.data_ptr(), q.stride(0) & -4, q.stride(1) & -4, H, rows.data_ptr(),
                    None if offsets is None else offsets.data_ptr(), n, T, window, sinks, scale, max_len, out.data_ptr(),
                    None if ws is None else ws.data_ptr(), need)
         return out
@@ -344,8 +348,8 @@ class PagedKV:
 
     def trim(self, rows: Rows, window: int, sinks: int = 0) -> None:
         """Pages that no later `attend` with this window and these sinks sees go back to the pool."""
-        if window < 1 or sinks < 0:
-            raise ValueError("trim needs window >= 1 and sinks >= 0")
+        if not 1 <= window <= _MOST or not 0 <= sinks <= _MOST:
+            raise ValueError("trim needs window >= 1 and sinks >= 0 (below 2^31)")
         rows = self._ids(rows, "rows", self.rows)
         self._call(self._lib.q3c_kv_trim, rows.data_ptr(), rows.shape[0], window, sinks)
 

@@ -977,3 +977,44 @@ def test_attend_prompts_with_many_heads(dtype, D, G, group, ps, window, sinks):
     i = torch.tensor([0, 31, 64, 127, 257, 330, 399], device=DEV)
     want, mag, dot = attention(q[i], *store[0], i.tolist(), window, sinks, scale, there)
     _check_attend(got[i], want, mag, dot, kv, 400, scale, q[i].double(), prompt=True)
+
+
+def test_numbers_that_32_bits_do_not_hold_are_refused():
+    kv = _cache("bf16", 1, 64, 16, [20])
+    rows = torch.zeros(1, dtype=torch.int32, device=DEV)
+    q = torch.zeros(1, 1, 64, dtype=torch.bfloat16, device=DEV)
+    for kw in (dict(window=2 ** 32 + 5), dict(window=4, sinks=2 ** 31), dict(max_len=2 ** 33 + 1)):
+        with pytest.raises(ValueError):
+            kv.attend(0, q, rows, **kw)
+    for window, sinks in ((2 ** 32 + 1, 0), (1, 2 ** 32)):
+        with pytest.raises(ValueError):
+            kv.trim(rows, window, sinks)
+    for call in (lambda: kv.reserve(rows, _offsets([1]), tokens=2 ** 32), lambda: kv.gather(0, rows, _offsets([1]), tokens=2 ** 32 + 1),
+                 lambda: kv.reserve(rows, _offsets([1]), tokens=-1)):
+        with pytest.raises(ValueError):
+            call()
+    assert int(kv.lens[0]) == 20 and kv.table[0, :2].tolist().count(-1) == 0
+    kv.check()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32", "int4"])
+def test_one_token_of_a_projection_of_odd_width(dtype):
+    """q, k and v as views of one row of a wider matrix: its row stride, 3 past a multiple of four, belongs to a dimension of one element."""
+    g = _gen(61)
+    G, H, D = 1, 2, 64
+    kv = _cache(dtype, G, D, 16, [20, 7])
+    _fill(kv, 0, [20, 7], g)
+    for T in (1, 2):
+        x = _randn(g, 3, (H + 2 * G) * D + 3, dtype=kv.activations)
+        q, k, v = (t.unflatten(1, (-1, D))[:T] for t in x[:, :(H + 2 * G) * D].split([H * D, G * D, G * D], 1))
+        rows = torch.arange(T, dtype=torch.int32, device=DEV)
+        assert q.stride(0) % 4
+        a = kv.append(0, q, k, v, rows)
+        assert torch.equal(a, q)
+        kk, vv = kv.gather(0, rows)
+        out = kv.attend(0, q, rows)
+        copies = [t.clone(memory_format=torch.contiguous_format) for t in (q, k, v)]
+        kv.append(0, *copies, rows)
+        k2, v2 = kv.gather(0, rows)
+        assert torch.equal(kk, k2) and torch.equal(vv, v2) and torch.equal(kv.attend(0, copies[0], rows), out)
+    kv.check()
