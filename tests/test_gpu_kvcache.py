@@ -1018,3 +1018,54 @@ def test_one_token_of_a_projection_of_odd_width(dtype):
         k2, v2 = kv.gather(0, rows)
         assert torch.equal(kk, k2) and torch.equal(vv, v2) and torch.equal(kv.attend(0, copies[0], rows), out)
     kv.check()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "int4"])
+def test_captured_page_operations_replay(dtype):
+    """fork, append, gather, copy, trim, release and compact captured in one graph and replayed four times, each time equal to the same calls
+    run eagerly on a twin, with eager work of both between."""
+    from qwen3_tts_amd.kvcache import PagedKV
+    G, D, ps = 2, 64, 8
+    pair = [PagedKV(2, G, D, 90, ps, rows=6, pages_per_row=20, dtype=dtype, device=DEV) for _ in range(2)]
+    rows = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    children = torch.tensor([3, 2, 5], dtype=torch.int32, device=DEV)
+    parents = torch.tensor([0, 1, 0], dtype=torch.int32, device=DEV)
+    src, dst = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([1, 3, 3], [80, 81, 80]))
+    x = torch.zeros(3, G, D, dtype=torch.bfloat16, device=DEV)
+    g = _gen(71)
+    for kv in pair:
+        kv.reserve(rows, _offsets([45, 70]), tokens=115)
+        y = _randn(_gen(72), 115, G, D, dtype=torch.bfloat16)
+        for layer in (0, 1):
+            kv.append(layer, y, y, -y, rows, _offsets([45, 70]))
+
+    def calls(kv):
+        kv.fork(parents, children)
+        kv.reserve(children)
+        kv.append(1, x, x, x, children)
+        kv.copy_pages(src, dst)
+        kv.trim(children, 20, 3)
+        live = kv.compact()
+        k, v = kv.gather(1, children)
+        out = kv.attend(1, x, children, window=20, sinks=3)
+        kv.release(children)
+        return live, k, v, out
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = calls(pair[0])
+    for i in range(4):
+        x.copy_(_randn(g, 3, G, D))
+        graph.replay()
+        want = calls(pair[1])
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), i
+        for n in ("table", "lens", "refs"):
+            assert torch.equal(getattr(pair[0], n), getattr(pair[1], n)), (i, n)
+        assert torch.equal(pair[0].k, pair[1].k) and torch.equal(pair[0].v, pair[1].v)
+        for kv in pair:                                            # the parents grow between
+            kv.check()
+            kv.reserve(rows)
+            for layer in (0, 1):
+                kv.append(layer, x[:2], x[:2], x[1:], rows)
