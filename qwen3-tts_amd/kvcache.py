@@ -135,6 +135,7 @@ class PagedKV:
         self.dtype = ("f32", "bf16", "int4")[code]
         self.activations = _ACT[code]
         self._act_bytes = 4 if code == 0 else 2
+        self._max_tokens = ps * self.pages_per_row
         self.device = k.device
         self._index = k.device.index if k.device.index is not None else torch.cuda.current_device()
         self._lib = _lib.load()
@@ -153,7 +154,7 @@ class PagedKV:
     @property
     def max_tokens(self) -> int:
         """Tokens that one row can hold."""
-        return self.page_size * self.pages_per_row
+        return self._max_tokens
 
     def _call(self, fn, *args) -> None:
         i = self._index
@@ -191,9 +192,10 @@ class PagedKV:
             raise ValueError(f"a call takes at most 2^24 tokens, got {tokens}")
         return rows, n, offsets, tokens
 
-    def _heads(self, x: torch.Tensor, what: str, heads: Optional[int]) -> torch.Tensor:
-        """[tokens, heads, head_dim] in the cache's activation type; copied only where its strides are not what the kernels read: multiples of
-        four (the stride of a dimension of one element may be anything, and is passed on rounded down)."""
+    def _heads(self, x: torch.Tensor, what: str, heads: Optional[int]):
+        """[tokens, heads, head_dim] in the cache's activation type -> (tensor, shape, pointer, token stride, head stride); copied only
+        where its strides are not what the kernels read: multiples of four (the stride of a dimension of one element may be anything, and is
+        passed on rounded down)."""
         shape = x.shape
         if len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads) or shape[1] < 1:
             raise ValueError(f"{what} must be [tokens, {'heads' if heads is None else heads}, {self.head_dim}], got {tuple(shape)}")
@@ -202,12 +204,20 @@ class PagedKV:
         if x.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{what} requires a gradient, and the cache's operators have none: call them under torch.no_grad()")
         ts, hs, ds = x.stride()
-        quad = 4 * self._act_bytes
-        if ds != 1 or (ts % 4 and shape[0] != 1) or (hs % 4 and shape[1] != 1) or x.data_ptr() % quad:
+        p, quad = x.data_ptr(), 4 * self._act_bytes
+        if ds != 1 or (ts % 4 and shape[0] != 1) or (hs % 4 and shape[1] != 1) or p % quad:
             x = x.contiguous()
             if x.data_ptr() % quad:                            # a contiguous view that starts between two quads
                 x = x.clone()
-        return x
+            ts, hs, ds = x.stride()
+            p = x.data_ptr()
+        return x, shape, p, ts & -4, hs & -4
+
+    def _table(self, t: torch.Tensor, dims: int, what: str, shape: str) -> int:
+        p = t.data_ptr()
+        if t.dtype != torch.float32 or t.dim() != dims or not t.is_contiguous() or t.get_device() != self._index or p % 16:
+            raise ValueError(f"{what} must be a contiguous, 16-byte aligned float32 tensor {shape} on {self.device}")
+        return p
 
     def _layer(self, layer: int) -> int:
         if not 0 <= layer < self.layers:
@@ -243,36 +253,38 @@ class PagedKV:
         dimensions wide; None: none), k and v stored, q returned (`out`, or a new tensor) [tokens, heads, head_dim].  q, k, v: [tokens,
         heads, head_dim], any strides - views of one projection's output are read in place.  q tokens behind offsets[-1] are left as
         they are in `out` (undefined in a new tensor)."""
-        q = self._heads(q, "q", None)
-        k, v = self._heads(k, "k", self.kv_heads), self._heads(v, "v", self.kv_heads)
-        T, H = q.shape[0], q.shape[1]
-        if k.shape[0] != T or v.shape[0] != T:
-            raise ValueError(f"q, k and v hold {T}, {k.shape[0]} and {v.shape[0]} tokens")
+        q, (T, H, D), qp, qt, qh = self._heads(q, "q", None)
+        k, ks, kp, kt, kh = self._heads(k, "k", self.kv_heads)
+        v, vs, vp, vt, vh = self._heads(v, "v", self.kv_heads)
+        if ks[0] != T or vs[0] != T:
+            raise ValueError(f"q, k and v hold {T}, {ks[0]} and {vs[0]} tokens")
         rows, n, offsets, _ = self._batch(rows, offsets, T)
         if not n and T:
             raise ValueError(f"{T} tokens without a row")
-        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-            if w is not None and (w.dtype != torch.float32 or w.dim() != 1 or w.shape[0] != self.head_dim or not w.is_contiguous() or w.get_device() != self._index or w.data_ptr() % 16):
-                raise ValueError(f"{name} must be a contiguous, 16-byte aligned float32 tensor [{self.head_dim}] on {self.device}")
-        if (q_weight is not None or k_weight is not None) and not eps > 0:
-            raise ValueError(f"eps must be positive, got {eps}")
+        wq = None if q_weight is None else self._table(q_weight, 1, "q_weight", f"[{D}]")
+        wk = None if k_weight is None else self._table(k_weight, 1, "k_weight", f"[{D}]")
+        if wq is not None or wk is not None:
+            for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+                if w is not None and w.shape[0] != D:
+                    raise ValueError(f"{name} must be a contiguous, 16-byte aligned float32 tensor [{D}] on {self.device}")
+            if not eps > 0:
+                raise ValueError(f"eps must be positive, got {eps}")
         rot = positions = 0
-        cos = sin = None
+        cp = sp = None
         if rope is not None:
             cos, sin = rope
-            for name, t in (("cos", cos), ("sin", sin)):
-                if t.dtype != torch.float32 or t.dim() != 2 or t.shape != cos.shape or not t.is_contiguous() or t.get_device() != self._index or t.data_ptr() % 16:
-                    raise ValueError(f"rope's {name} must be a contiguous, 16-byte aligned float32 tensor [positions, rotated / 2] on {self.device}")
-            positions, rot = cos.shape[0], 2 * cos.shape[1]
-            if rot % 8 or not 0 < rot <= self.head_dim or (self.dtype == "int4" and rot != self.head_dim):
-                raise ValueError(f"rope rotates {rot} of {self.head_dim} dimensions: a multiple of 8 is wanted (all of them in a 4-bit cache)")
+            cp, sp = self._table(cos, 2, "rope's cos", "[positions, rotated / 2]"), self._table(sin, 2, "rope's sin", "[positions, rotated / 2]")
+            positions, half = cos.shape
+            if sin.shape != cos.shape:
+                raise ValueError(f"rope's cos and sin must have one shape, got {tuple(cos.shape)} and {tuple(sin.shape)}")
+            rot = 2 * half
+            if rot % 8 or not 0 < rot <= D or (self.dtype == "int4" and rot != D):
+                raise ValueError(f"rope rotates {rot} of {D} dimensions: a multiple of 8 is wanted (all of them in a 4-bit cache)")
             if positions < self.max_tokens:
                 raise ValueError(f"rope covers {positions} positions, a row can hold {self.max_tokens}")
-        out = self._out(out, (T, H, self.head_dim), self.activations)
-        self._call(self._lib.q3c_kv_append, self._layer(layer), q.data_ptr(), q.stride(0) & -4, q.stride(1) & -4, k.data_ptr(), k.stride(0) & -4, k.stride(1) & -4,
-                   v.data_ptr(), v.stride(0) & -4, v.stride(1) & -4, H, rows.data_ptr(), None if offsets is None else offsets.data_ptr(), n, T,
-                   None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
-                   None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(), positions, rot, eps, out.data_ptr())
+        out = self._out(out, (T, H, D), self.activations)
+        self._call(self._lib.q3c_kv_append, self._layer(layer), qp, qt, qh, kp, kt, kh, vp, vt, vh, H, rows.data_ptr(),
+                   None if offsets is None else offsets.data_ptr(), n, T, wq, wk, cp, sp, positions, rot, eps, out.data_ptr())
         return out
 
     def gather(self, layer: int, rows: Rows, offsets: Optional[torch.Tensor] = None, tokens: Optional[int] = None,
@@ -300,19 +312,18 @@ class PagedKV:
         h // (heads / kv_heads)) -> the same shape; a token that sees nothing gives zeros; tokens behind offsets[-1] are left as they are
         in `out` (undefined in a new tensor).  `scale`: head_dim ** -0.5 unless given.  `max_len`: no row is longer than this (0: not
         known); a good bound helps to cut the work of long rows."""
-        q = self._heads(q, "q", None)
-        T, H = q.shape[0], q.shape[1]
+        q, (T, H, D), qp, qt, qh = self._heads(q, "q", None)
         if H % self.kv_heads:
             raise ValueError(f"{H} query heads do not share {self.kv_heads} kv heads evenly")
         if window < 0 or sinks < 0 or max_len < 0 or window > _MOST or sinks > _MOST or max_len > _MOST:
             raise ValueError("window, sinks and max_len must be from 0 to 2^31 - 1")
-        scale = self.head_dim ** -0.5 if scale is None else float(scale)
+        scale = D ** -0.5 if scale is None else float(scale)
         if not 0.0 < scale < 3e38:
             raise ValueError(f"scale must be positive and finite, got {scale}")
         rows, n, offsets, _ = self._batch(rows, offsets, T)
         if not n and T:
             raise ValueError(f"{T} tokens without a row")
-        out = self._out(out, (T, H, self.head_dim), self.activations)
+        out = self._out(out, (T, H, D), self.activations)
         key = (H, n, T, window, sinks, max_len)
         need = self._need.get(key)
         if need is None:
@@ -325,7 +336,7 @@ class PagedKV:
             need = self._need[key] = int(size.value)
         # a workspace of its own for each call: calls on two streams, or two captured graphs, share none
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        self._call(self._lib.q3c_kv_attend, self._layer(layer), q.data_ptr(), q.stride(0) & -4, q.stride(1) & -4, H, rows.data_ptr(),
+        self._call(self._lib.q3c_kv_attend, self._layer(layer), qp, qt, qh, H, rows.data_ptr(),
                    None if offsets is None else offsets.data_ptr(), n, T, window, sinks, scale, max_len, out.data_ptr(),
                    None if ws is None else ws.data_ptr(), need)
         return out
