@@ -813,36 +813,38 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const KvAttendArgs a) {
 // on 8 of 128): 250 us, 820 TFLOP/s of what is visible; the same on 16-column tiles 978.
 // 4 bits: values n * step are rounded to bf16 on their way into LDS (operands of the matrix cores), four bytes of the row = one 16-byte
 // chunk; the order of dimensions in a row is then the packed one, which Q's load and the output's store follow.
+// global, not flat: a flat load would be waited for with every use of LDS
+typedef const __attribute__((address_space(1))) unsigned mem_u32;
+typedef const __attribute__((address_space(1))) u32x2 mem_u32x2;
+__device__ const u32x4 kv_zeros = {0, 0, 0, 0}, kv_eights = {0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u};      // what a row that nobody sees is read from
 template <typename T, int DP> struct Row;                       // chunk ch of a row: 8 values as 16 bytes
-template <int DP> struct Row<bf16, DP> {
-    static constexpr int WORDS = 4;
-    struct Raw { u32x4 x; };
-    static __device__ __forceinline__ const char* base(const void* p, long long row, int D) { return (const char*)p + row * D * 2; }
-    static __device__ __forceinline__ const bf16* steps(const bf16* p, long long) { return p; }
-    static __device__ __forceinline__ void load(Raw& r, const char* base, const bf16*, int row, int D, int ch) {
-        r.x = *(const u32x4*)(base + (unsigned)(row * D * 2 + 16 * ch));
-    }
-    static __device__ __forceinline__ void zero(Raw& r) { r.x = u32x4{0, 0, 0, 0}; }
-    static __device__ __forceinline__ u32x4 value(const Raw& r) { return r.x; }
+template <int DP> struct Row<bf16, DP> {                       // goes to LDS as it is
+    static constexpr float UP = 1.0f;
+    struct Raw {};
     static __device__ __forceinline__ int dim(int d) { return d; }      // of place d of a row
 };
 template <int D> struct Row<Int4, D> {
     static constexpr int S = D / 32;
+    static constexpr float UP = 16.0f;         // what keys and values are divided by in LDS: a power of two
     struct Raw { unsigned x; u32x2 st; };
     static __device__ __forceinline__ const char* base(const void* p, long long row, int) { return (const char*)p + row * (D / 2); }
     static __device__ __forceinline__ const bf16* steps(const bf16* p, long long row) { return p + row * S; }
-    static __device__ __forceinline__ void load(Raw& r, const char* base, const bf16* steps, int row, int, int ch) {
-        r.x = *(const unsigned*)(base + (unsigned)(row * (D / 2) + 4 * ch));
-        if constexpr (S == 2) { r.st[0] = *(const unsigned*)(steps + row * S); r.st[1] = r.st[0]; }
-        else r.st = *(const u32x2*)(steps + row * S + (S == 8 ? 4 * (ch & 1) : 0));
+    // (`ch`'s steps of a row begin at 4 (ch & 1) where there are eight.)  No branch: a row that is not `ok` is read from constants that make zeros.
+    static __device__ __forceinline__ void load(Raw& r, bool ok, const char* row, const bf16* steps, int ch) {
+        const void *x = ok ? (const void*)(row + 4 * ch) : (const void*)&kv_eights, *st = ok ? (const void*)(steps + (S == 8 ? 4 * (ch & 1) : 0)) : (const void*)&kv_zeros;
+        r.x = *(mem_u32*)x;
+        if constexpr (S == 2) r.st[0] = *(mem_u32*)st;
+        else r.st = *(mem_u32x2*)st;
     }
-    static __device__ __forceinline__ void zero(Raw& r) { r.x = 0x88888888u; r.st = u32x2{0, 0}; }
+    // n * step / UP as u * (step / UP) - 8 (step / UP) with u = n + 8, exact in one fma of a converted byte; UP keeps 8 steps from overflowing
     static __device__ __forceinline__ u32x4 value(const Raw& r) {
+        const unsigned lo = r.x & 0x0f0f0f0fu, hi = (r.x >> 4) & 0x0f0f0f0fu;
         u32x4 v;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-            const float st = b & 1 ? hi_f(r.st[b >> 1]) : lo_f(r.st[b >> 1]);
-            v[b] = pack2((float)((int)(r.x >> (8 * b) & 15u) - 8) * st, (float)((int)(r.x >> (8 * b + 4) & 15u) - 8) * st);
+            const unsigned w = r.st[S == 2 ? 0 : b >> 1];
+            const float st = (b & 1 ? hi_f(w) : lo_f(w)) * (1.0f / UP), z = -8.0f * st;
+            v[b] = pack2(fmaf((float)(lo >> (8 * b) & 255u), st, z), fmaf((float)(hi >> (8 * b) & 255u), st, z));
         }
         return v;
     }
@@ -861,7 +863,6 @@ __device__ __forceinline__ float max_halves(float x) {           // over lanes l
 }
 
 typedef __attribute__((address_space(3))) void lds_void;
-__device__ const u32x4 kv_zeros = {0, 0, 0, 0};                 // what a row that nobody sees is read from
 
 // 16 bytes per lane from memory to LDS at `lds` (uniform) + 16 lane, outside the compiler's count of loads: `landed` waits for them.
 // (M0 belongs to no value of the compiler's; its own uses write it right before.)
@@ -926,7 +927,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
     const int W = a.window > 0 ? min(a.window, 1 << 30) : 1 << 30, sinks = a.window > 0 ? a.sinks : 0;
     // This thread stages 16-byte slot `slot` of rows row0 + i RP; the rows of a wave and i are RW consecutive ones, which lie in one page.
     const int slot = tid & (NCH - 1), row0 = tid / NCH, sub = lane / NCH;
-    const float cs = a.scale_log2e;
+    const float cs = a.scale_log2e * R::UP;
     // LDS places of this lane's operands; tiles, halves and buffers are constants added to them
     constexpr bool FEW = DP == 256;            // registers are short: places from the first one by exclusive or, where they are used
     int ak[FEW ? 1 : KS], av[FEW ? 1 : ND];
@@ -1003,11 +1004,9 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
 #pragma unroll
                 for (int i = 0; i < NR; ++i) {
                     const int mine = kb + row0 + i * RP;
-                    R::zero(raw[i]);
-                    if ((unsigned)page[i] < (unsigned)a.c.pages && mine <= vhi && (mine > vlo || mine < sinks)) {
-                        const long long at = head0 + (long long)page[i] * page_rows + (mine & in_page);
-                        R::load(raw[i], R::base(base, at, D), R::steps(scales, at), 0, D, slot);
-                    }
+                    const bool ok = (unsigned)page[i] < (unsigned)a.c.pages && mine <= vhi && (mine > vlo || mine < sinks);
+                    const long long at = head0 + (long long)page[i] * page_rows + (mine & in_page);
+                    R::load(raw[i], ok, R::base(base, at, D), R::steps(scales, at), slot);
                 }
             }
         };
@@ -1150,7 +1149,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
         }
         l += __shfl_xor(l, 32);
         if (col < t.ncols && (all || mypos == only)) {
-            const float inv = 1.0f / l;
+            const float inv = R::UP / l;
             const bool none = mypos < 0 || l == 0.f;
             bf16* out = (bf16*)a.out + ((long long)(t.tok0 + qtok) * a.q_heads + hk * G + col - qtok * G) * D;
 #pragma unroll
