@@ -130,7 +130,7 @@ int q3c_kv_attend(const q3c_kv* kv, int32_t layer, const void* q, int64_t q_ts, 
     KvAttendArgs a = {};
     int rc = attend_shape(kv, q_heads, sequences, tokens, window, sinks, max_len, &a.c);
     if (rc || (rc = batch(rows, offsets, sequences, tokens, &a.b))) return rc;
-    if (layer < 0 || layer >= a.c.layers || !(scale > 0.f) || !(scale < 3e38f)) return Q3C_ERR_INVALID_ARGUMENT;
+    if (layer < 0 || layer >= a.c.layers || !(scale > 0.f) || !(scale < 1e37f)) return Q3C_ERR_INVALID_ARGUMENT;
     if (!tokens) return 0;
     if (!strided(q, q_ts, q_hs, act_bytes(a.c)) || !out || !aligned(out, 16)) return Q3C_ERR_INVALID_ARGUMENT;
     const KvSplit cut = q3_kv_attend_split(a.c, tokens, sequences, q_heads, offsets != nullptr, window, sinks, max_len);

@@ -318,8 +318,8 @@ class PagedKV:
         if window < 0 or sinks < 0 or max_len < 0 or window > _MOST or sinks > _MOST or max_len > _MOST:
             raise ValueError("window, sinks and max_len must be from 0 to 2^31 - 1")
         scale = D ** -0.5 if scale is None else float(scale)
-        if not 0.0 < scale < 3e38:
-            raise ValueError(f"scale must be positive and finite, got {scale}")
+        if not 0.0 < scale < 1e37:
+            raise ValueError(f"scale must be positive and below 1e37, got {scale}")
         rows, n, offsets, _ = self._batch(rows, offsets, T)
         if not n and T:
             raise ValueError(f"{T} tokens without a row")

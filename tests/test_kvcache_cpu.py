@@ -120,6 +120,13 @@ def test_calls_larger_than_a_launch_are_refused():
     assert lib.q3c_kv_fork(_kv(layers=64), PTR, PTR, 1 << 17, PTR, 1 << 40, None) == UNSUPPORTED
 
 
+def test_a_scale_that_overflows_is_refused():
+    """The scale is held times log2(e), and times 16 where keys are: 1e37 is the last decade whose products fp32 holds."""
+    lib, kv = _lib.load(), _kv()
+    for scale in (1e37, 3e38, 0.0, -1.0):
+        assert lib.q3c_kv_attend(kv, 0, PTR, 256, 64, 4, PTR, None, 1, 1, 0, 0, scale, 0, PTR, PTR, 1 << 30, None) == INVALID, scale
+
+
 def test_rope_tables_of_far_positions():
     cos, sin = rope_tables(200001, 8, theta=1e6, device="cpu")
     import math
