@@ -150,6 +150,19 @@ class PagedKV:
         self._ref = C.byref(c)
         self._need = {}                        # attend: workspace bytes by the sizes of the call
 
+    @property
+    def state(self) -> Tuple[Optional[torch.Tensor], ...]:
+        """k, v, k_scale, v_scale, table, lens, status: what `torch.ops.q3tts.kv_append` and `kv_attend` take last, so that a traced program
+        knows what they write and read."""
+        return self.k, self.v, self.k_scale, self.v_scale, self.table, self.lens, self.status
+
+    def over(self, state: Sequence[Optional[torch.Tensor]]) -> "PagedKV":
+        """This cache, or one over `state` (tensors like self.state) where those are others than its own."""
+        if all(a is b or (a is not None and b is not None and a.data_ptr() == b.data_ptr()) for a, b in zip(state, self.state)):
+            return self
+        k, v, k_scale, v_scale, table, lens, status = state
+        return PagedKV.from_tensors(k, v, table, lens, self.refs, k_scale, v_scale, status)
+
     # ---- what every call does ------------------------------------------------------------------------------------------------
     @property
     def max_tokens(self) -> int:

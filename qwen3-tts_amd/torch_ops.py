@@ -12,6 +12,7 @@ tensors raises NotImplementedError from the dispatcher.
 """
 from __future__ import annotations
 
+import re
 from typing import Dict, Optional
 
 import torch
@@ -111,8 +112,11 @@ def _(x, alpha, beta, eps):
 
 # ---- paged key/value cache (kvcache.PagedKV, registered under a handle like a decoder) ---------------------------------------------
 #     h = torch_ops.register_kv(kv)
-#     q = torch.ops.q3tts.kv_append(q, k, v, rows, None, wq, wk, cos, sin, 1e-6, h, layer)      # writes the cache behind the handle
-#     o = torch.ops.q3tts.kv_attend(q, rows, None, 4096, 4, h, layer)
+#     q = torch.ops.q3tts.kv_append(q, k, v, rows, None, wq, wk, cos, sin, 1e-6, h, layer, *kv.state)
+#     o = torch.ops.q3tts.kv_attend(q, rows, None, 4096, 4, h, layer, *kv.state)
+# The cache's tensors are arguments, and the schema names those that kv_append writes: a traced program then keeps an append whose queries
+# nobody takes, and its order against the attends around it.  Eager calls may leave them out (the handle's own are meant); a program that is
+# traced without them is refused, since nothing in it would say that one call writes what the next one reads.
 _caches: Dict[int, object] = {}
 
 
@@ -134,24 +138,48 @@ def _kv(handle: int):
         raise KeyError(f"no cache registered under handle {handle}") from None
 
 
-@torch.library.custom_op("q3tts::kv_append", mutates_args=(), device_types="cuda")
-def kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rows: torch.Tensor, offsets: Optional[torch.Tensor],
-              q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
-              eps: float, handle: int, layer: int) -> torch.Tensor:
-    return _kv(handle).append(layer, q, k, v, rows, offsets, q_weight=q_weight, k_weight=k_weight,
-                              rope=None if cos is None else (cos, sin), eps=eps)
+def _kv_over(handle: int, state):
+    """The handle's cache; over other tensors where a compiler has put copies in the place of its own."""
+    kv = _kv(handle)
+    return kv if all(t is None for t in state) else kv.over(state)
 
 
-@kv_append.register_fake
-def _(q, k, v, rows, offsets, q_weight, k_weight, cos, sin, eps, handle, layer):
+def _traced(state) -> None:
+    if state[0] is None:
+        raise RuntimeError("a traced program has to pass the cache's tensors to kv_append and kv_attend (*kv.state, the last arguments)")
+
+
+def _kv_append(q, k, v, rows, offsets, q_weight, k_weight, cos, sin, eps, handle, layer, *state):
+    return _kv_over(handle, state).append(layer, q, k, v, rows, offsets, q_weight=q_weight, k_weight=k_weight,
+                                          rope=None if cos is None else (cos, sin), eps=eps)
+
+
+def _kv_append_fake(q, k, v, rows, offsets, q_weight, k_weight, cos, sin, eps, handle, layer, *state):
+    _traced(state)
     return q.new_empty(q.shape)
 
 
-@torch.library.custom_op("q3tts::kv_attend", mutates_args=(), device_types="cuda")
-def kv_attend(q: torch.Tensor, rows: torch.Tensor, offsets: Optional[torch.Tensor], window: int, sinks: int, handle: int, layer: int) -> torch.Tensor:
-    return _kv(handle).attend(layer, q, rows, offsets, window=window, sinks=sinks)
+def _kv_attend(q, rows, offsets, window, sinks, handle, layer, *state):
+    return _kv_over(handle, state).attend(layer, q, rows, offsets, window=window, sinks=sinks)
 
 
-@kv_attend.register_fake
-def _(q, rows, offsets, window, sinks, handle, layer):
+def _kv_attend_fake(q, rows, offsets, window, sinks, handle, layer, *state):
+    _traced(state)
     return q.new_empty(q.shape)
+
+
+def _plain(fn):
+    """The kernel with all arguments by position, left out ones as None (the dispatcher drops trailing defaults)."""
+    return lambda *a: fn(*(a + (None,) * (fn.__code__.co_argcount + 7 - len(a))))
+
+
+_KV_STATE = ("Tensor(a!)? k_pages=None, Tensor(b!)? v_pages=None, Tensor(c!)? k_steps=None, Tensor(d!)? v_steps=None, "
+             "Tensor? table=None, Tensor? lens=None, Tensor(e!)? status=None")
+torch.library.define("q3tts::kv_append", "(Tensor q, Tensor k, Tensor v, Tensor rows, Tensor? offsets, Tensor? q_weight, Tensor? k_weight, "
+                     "Tensor? cos, Tensor? sin, float eps, int handle, int layer, " + _KV_STATE + ") -> Tensor")
+torch.library.define("q3tts::kv_attend", "(Tensor q, Tensor rows, Tensor? offsets, int window, int sinks, int handle, int layer, "
+                     + re.sub(r"\(.!\)", "", _KV_STATE) + ") -> Tensor")
+for _name, _fn, _fake in (("kv_append", _kv_append, _kv_append_fake), ("kv_attend", _kv_attend, _kv_attend_fake)):
+    torch.library.impl("q3tts::" + _name, "cuda")(_plain(_fn))
+    torch.library.register_fake("q3tts::" + _name)(_plain(_fake))
+kv_append, kv_attend = torch.ops.q3tts.kv_append, torch.ops.q3tts.kv_attend

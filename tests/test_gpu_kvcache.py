@@ -1069,3 +1069,41 @@ def test_captured_page_operations_replay(dtype):
             kv.reserve(rows)
             for layer in (0, 1):
                 kv.append(layer, x[:2], x[:2], x[1:], rows)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "int4"])
+def test_a_traced_step_is_the_eager_one(dtype):
+    """Two layers whose first append's queries nobody takes, and attends before and behind an append: compiled, where functionalization gives
+    the ops copies of the cache, the outputs and the cache are bit for bit those of the calls made eagerly on a twin."""
+    from qwen3_tts_amd import torch_ops
+    from qwen3_tts_amd.kvcache import PagedKV
+    g = _gen(81)
+    G, H, D = 2, 4, 64
+    pair = [PagedKV(2, G, D, 30, 16, rows=3, pages_per_row=8, dtype=dtype, device=DEV) for _ in range(2)]
+    rows, off = torch.tensor([2, 0], dtype=torch.int32, device=DEV), _offsets([40, 33])
+    x = [_randn(g, 73, n, D, dtype=torch.bfloat16) for n in (H, G, G)]
+    y = [_randn(g, 2, n, D, dtype=torch.bfloat16) for n in (H, G, G)]
+    handles = [torch_ops.register_kv(kv) for kv in pair]
+
+    def prefill(kv, h, q, k, v):
+        for layer in (0, 1):
+            torch.ops.q3tts.kv_append(q, k, v, rows, off, None, None, None, None, 1e-6, h, layer, *kv.state)
+
+    def step(kv, h, q, k, v):
+        a = torch.ops.q3tts.kv_attend(q, rows, None, 20, 2, h, 1, *kv.state)
+        torch.ops.q3tts.kv_append(q, k, v, rows, None, None, None, None, None, 1e-6, h, 1, *kv.state)
+        return a, torch.ops.q3tts.kv_attend(q, rows, None, 20, 2, h, 1, *kv.state)
+    results = []
+    for kv, h, wrap in zip(pair, handles, (lambda f: f, lambda f: torch.compile(f, backend="aot_eager", fullgraph=True))):
+        kv.reserve(rows, off, tokens=73)
+        wrap(lambda *a, kv=kv, h=h: prefill(kv, h, *a))(*x)
+        kv.reserve(rows)
+        results.append(wrap(lambda *a, kv=kv, h=h: step(kv, h, *a))(*y))
+        kv.check()
+    (a0, b0), (a1, b1) = results
+    assert torch.equal(a0, a1) and torch.equal(b0, b1) and not torch.equal(a0, b0)
+    for s, t in zip(pair[0].state, pair[1].state):
+        assert s is None and t is None or torch.equal(s, t)
+    for h in handles:
+        torch_ops.unregister_kv(h)
+    torch._dynamo.reset()

@@ -153,3 +153,106 @@ def test_the_plain_restatement_itself():
     assert p.fork([0], [1]) == [(2, 3)] and p.refs == [2, 2, 1, 1, 0, 0]
     p.release([0])
     assert p.refs == [1, 1, 0, 1, 0, 0] and p.compact() == ([(3, 2)], 3) and p.table[1] == [0, 1, 2, -1]
+
+
+class _Stub:
+    """Stands for a cache where only the order of calls and what they write counts: append adds to the tensors that it is given."""
+
+    def __init__(self, state, calls):
+        self.state, self.calls = state, calls
+
+    def over(self, state):
+        return _Stub(state, self.calls)
+
+    def append(self, layer, q, k, v, rows, offsets, **kw):
+        self.calls.append(("append", layer))
+        self.state[0][layer] += k.sum()
+        self.state[1][layer] += 1
+        return q * 2
+
+    def attend(self, layer, q, rows, offsets, **kw):
+        self.calls.append(("attend", layer))
+        return q + self.state[0][layer] + self.state[5][0]
+
+
+@pytest.fixture
+def traced_ops():
+    """The two ops with CPU kernels, over a stub of a cache -> (handle, stub, its state)."""
+    from qwen3_tts_amd import torch_ops
+    state = [torch.zeros(3), torch.zeros(3), None, None, torch.zeros(2, 2, dtype=torch.int32), torch.full((2,), 7, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)]
+    lib = torch.library.Library("q3tts", "FRAGMENT")
+    lib.impl("kv_append", torch_ops._plain(torch_ops._kv_append), "CPU")
+    lib.impl("kv_attend", torch_ops._plain(torch_ops._kv_attend), "CPU")
+    stub = _Stub(state, [])
+    h = torch_ops.register_kv(stub)
+    yield h, stub, state
+    torch_ops.unregister_kv(h)
+    lib._destroy()
+    torch._dynamo.reset()
+
+
+def _programs(h, state):
+    ops = torch.ops.q3tts
+
+    def append(q, rows, layer):
+        return ops.kv_append(q, q, q, rows, None, None, None, None, None, 1e-6, h, layer, *state)
+
+    def attend(q, rows, layer):
+        return ops.kv_attend(q, rows, None, 0, 0, h, layer, *state)
+
+    def prefill(q, rows):                      # a cached prompt: nobody takes the hidden states
+        for layer in range(3):
+            append(q, rows, layer)
+        return q + 1
+
+    def between(q, rows):
+        a = attend(q, rows, 1)
+        append(q, rows, 1)
+        return a, attend(q, rows, 1)
+
+    def step(q, rows):
+        for layer in range(3):
+            q = attend(append(q, rows, layer), rows, layer)
+        return q
+    return {"prefill": (prefill, ["append"] * 3), "between": (between, ["attend", "append", "attend"]), "step": (step, ["append", "attend"] * 3)}
+
+
+@pytest.mark.parametrize("name", ["prefill", "between", "step"])
+@pytest.mark.parametrize("backend", ["aot_eager", "inductor"])
+def test_a_traced_program_keeps_its_cache_calls(traced_ops, name, backend):
+    """An append whose queries are not wanted is no dead code, and attends on either side of one are not one call: compiled programs make
+    the calls that eager ones make, in their order, with the same results and the same cache."""
+    h, stub, state = traced_ops
+    fn, calls = _programs(h, state)[name]
+    q, rows = torch.tensor([1.0, 2.0]), torch.zeros(1, dtype=torch.int32)
+    want, k, v = fn(q, rows), state[0].clone(), state[1].clone()
+    assert [c for c, _ in stub.calls] == calls
+    for t in state[:2]:
+        t.zero_()
+    stub.calls.clear()
+    got = torch.compile(fn, backend=backend, fullgraph=True)(q, rows)
+    assert [c for c, _ in stub.calls] == calls
+    for a, b in zip(*((x if isinstance(x, tuple) else (x,)) for x in (got, want))):
+        assert torch.equal(a, b)
+    assert torch.equal(state[0], k) and torch.equal(state[1], v)
+
+
+def test_dead_code_elimination_leaves_appends(traced_ops):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    h, stub, state = traced_ops
+    prefill, _ = _programs(h, state)["prefill"]
+    graph = make_fx(prefill)(torch.ones(2), torch.zeros(1, dtype=torch.int32))
+    graph.graph.eliminate_dead_code()
+    assert sum(n.target is torch.ops.q3tts.kv_append.default for n in graph.graph.nodes) == 3
+    schema = torch.ops.q3tts.kv_append.default._schema
+    assert [a.name for a in schema.arguments if a.alias_info is not None and a.alias_info.is_write] == ["k_pages", "v_pages", "k_steps", "v_steps", "status"]
+
+
+def test_a_program_traced_without_the_caches_tensors_is_refused(traced_ops):
+    h, stub, state = traced_ops
+    q, rows = torch.ones(2), torch.zeros(1, dtype=torch.int32)
+    for fn in (lambda q, r: torch.ops.q3tts.kv_append(q, q, q, r, None, None, None, None, None, 1e-6, h, 0),
+               lambda q, r: torch.ops.q3tts.kv_attend(q, r, None, 0, 0, h, 0)):
+        assert fn(q, rows).shape == q.shape                         # eagerly the handle's own tensors are meant
+        with pytest.raises(Exception, match="has to pass the cache's tensors"):
+            torch.compile(fn, backend="aot_eager", fullgraph=True)(q, rows)
