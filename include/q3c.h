@@ -308,13 +308,15 @@ int q3c_wav_to_pcm16(const float* wav_dev, int64_t samples, int16_t* pcm_dev, vo
  * A call names its requests by `rows` [sequences] (table rows, distinct) and their new tokens by `offsets` [sequences + 1]: request
  * i's are tokens offsets[i] .. offsets[i + 1] - 1 of the call's `tokens`; NULL: one each (tokens == sequences).  The last new token of
  * a request stands at position lens[row] - 1: q3c_kv_reserve first makes room (lens grows), then every layer appends and attends.
- * Tokens before offsets[0] and from offsets[sequences] on are neither read nor written.  What a list, an offset or a table entry says is checked on the
- * device: a token whose row is bad or named before in the call, or that has no page, is not stored (its query is zeros if its row or
- * position is bad), keys without a page are seen by nobody, and the bit in `status` says so.  Calls whose launch would pass 2^32 threads
+ * Tokens before offsets[0] and from offsets[sequences] on are neither read nor written; an offset outside 0 .. tokens counts as the nearer end.
+ * What a list, an offset or a table entry says is checked on the device: a token whose row is bad or named before in the call, or that has
+ * no page, is not stored (its query is zeros if its row or position is bad), keys without a page are seen by nobody.  A bit in `status` says
+ * so, set by every call but q3c_kv_attend: that one reports nothing (a bad row's outputs are zeros), since the append before it with
+ * the same rows and offsets has.  Calls whose launch would pass 2^32 threads
  * along one axis (tokens * heads from 2^27 on, copies of some ten thousand pages of many layers) are Q3C_ERR_UNSUPPORTED. */
 typedef enum q3c_kv_dtype { Q3C_KV_F32 = 0, Q3C_KV_BF16 = 1, Q3C_KV_INT4 = 2 } q3c_kv_dtype;
 typedef enum q3c_kv_status {
-    Q3C_KV_BAD_ROW = 1,      /* a row id outside the table, named twice, or offsets that do not fit the row's length */
+    Q3C_KV_BAD_ROW = 1,      /* a row id outside the table, named twice, or offsets that do not fit the row's length or the call's tokens */
     Q3C_KV_NO_PAGE = 2,      /* no free page was left, or a token was appended that has no page */
     Q3C_KV_BAD_PAGE = 4,     /* a page id outside the pool, a count below zero, or a copy pair that was refused */
     Q3C_KV_FULL_ROW = 8      /* a row's length passed page_size * pages_per_row */

@@ -11,7 +11,8 @@ struct KvView {
     bf16 *ks, *vs;                      // 4 bits: steps [layers][pages][heads][page][dim / 32]
     int *table, *lens, *refs, *status;
 };
-// new tokens of a call: request i's are offsets[i] .. offsets[i+1] - 1 (null: token i alone), its last one at position lens[row] - 1
+// new tokens of a call: request i's are offsets[i] .. offsets[i+1] - 1 (null: token i alone), its last one at position lens[row] - 1.  An offset
+// outside 0 .. tokens counts as the nearer end, in every kernel: reserve, append, gather and attend place a token alike.
 struct KvBatch { const int* rows; const int* offsets; int sequences, tokens; };
 struct KvStrided { const void* p; long long ts, hs; };          // [token][head][dim], strides in elements, dim contiguous
 
@@ -62,7 +63,7 @@ __device__ __forceinline__ int kv_position(const KvView& c, const KvBatch& b, in
     if (b.offsets) {
         seq = kv_find(b.offsets, b.sequences, t, lane);
         if (seq >= b.sequences || (seq == 0 && t < b.offsets[0])) return -1;
-        back = b.offsets[seq + 1] - t;
+        back = min(b.offsets[seq + 1], b.tokens) - t;
         if (back < 1) return -2;                                // offsets that do not ascend
     }
     row = b.rows[seq];
@@ -70,4 +71,6 @@ __device__ __forceinline__ int kv_position(const KvView& c, const KvBatch& b, in
     const long long pos = (long long)c.lens[row] - back;
     return pos < 0 || pos >= ((long long)c.width << c.ps_shift) ? -2 : (int)pos;
 }
+// Whether the call's offsets end behind its tokens; true for its last token alone, whose wave reports it.
+__device__ __forceinline__ bool kv_ends_behind(const KvBatch& b, int t) { return b.offsets && t == b.tokens - 1 && b.offsets[b.sequences] > b.tokens; }
 #endif

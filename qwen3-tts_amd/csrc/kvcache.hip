@@ -53,6 +53,7 @@ __device__ __forceinline__ bool kv_place(const KvAppendArgs& a, int tok, bool fi
     int seq, row;
     zero = false;
     pos = kv_position(a.c, a.b, tok, lane, seq, row);
+    if (first && lane == 0 && kv_ends_behind(a.b, tok)) kv_flag(a.c, Q3C_KV_BAD_ROW);
     if (pos < 0) {
         zero = pos != -1;
         if (zero && lane == 0 && first) kv_flag(a.c, Q3C_KV_BAD_ROW);
@@ -260,6 +261,7 @@ __global__ void __launch_bounds__(256) kv_gather_kernel(const KvView c, const Kv
     if (tok >= b.tokens) return;
     int seq, row;
     const int pos = kv_position(c, b, tok, lane, seq, row);
+    if (part == 0 && lane == 0 && kv_ends_behind(b, tok)) kv_flag(c, Q3C_KV_BAD_ROW);
     if (pos == -1) return;
     const int page = pos < 0 ? -1 : kv_page(c, row, pos);
     if (pos < 0 && lane == 0 && part == 0) kv_flag(c, Q3C_KV_BAD_ROW);
@@ -416,7 +418,11 @@ __global__ void __launch_bounds__(PLAN_T) kv_reserve_kernel(const KvView c, cons
         int need = 0, row = tid < n ? b.rows[i] : -1, old = 0, add = 1;
         bool ok = row >= 0 && row < c.rows;
         if (ok) old = max(c.lens[row], 0);
-        if (tid < n && b.offsets) add = min(max(b.offsets[i + 1], 0), b.tokens) - min(max(b.offsets[i], 0), b.tokens);
+        if (tid < n && b.offsets) {
+            const int end = b.offsets[i + 1];
+            add = min(max(end, 0), b.tokens) - min(max(b.offsets[i], 0), b.tokens);
+            if (end > b.tokens) kv_flag(c, Q3C_KV_BAD_ROW);
+        }
         plan_walk(b.rows, s0 + n, n, tile, [&](int j, int r) { ok = ok && (j >= i || r != row); });   // named twice: the first counts
         if (tid < n) {
             ok = ok && add >= 0;

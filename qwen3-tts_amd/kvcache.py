@@ -16,7 +16,8 @@ generation, and nothing in them reads device values on the host: a whole step ca
 
 `rows` are table rows, one per request: an int32 tensor on the device (distinct; checked there) or a sequence of ints (checked here).
 `offsets` (int32 [len(rows) + 1] on the device) gives each row's new tokens in a ragged call; without it every row has one; tokens
-before offsets[0] and from offsets[-1] on belong to no row and are left alone.  `dtype` "f32" and "bf16" hold what the activations are;
+before offsets[0] and from offsets[-1] on belong to no row and are left alone.  Offsets that end behind the call's tokens count as ending there
+(`check` says so).  `dtype` "f32" and "bf16" hold what the activations are;
 "int4" holds bf16 activations in 4 bits with a step per 32 dimensions.  There is no backward pass: a cache is state, this package trains
 nothing, and tensors that ask for gradients are refused where autograd is on.
 
@@ -41,7 +42,7 @@ _ACT = (torch.float32, torch.bfloat16, torch.bfloat16)
 _MOST = 2 ** 31 - 1
 # the current device and its stream's handle, without the objects that torch.cuda wraps them in (a call of a generation step is host-bound)
 _device, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
-_STATUS = ((1, "a row id outside the table, named twice in a call, or offsets that do not fit a row's length"),
+_STATUS = ((1, "a row id outside the table, named twice in a call, or offsets that do not fit a row's length or the call's tokens"),
            (2, "no free page was left (or a token was appended that has no page)"),
            (4, "a page id outside the pool, or a copy whose source is another copy's destination"),
            (8, "a row grew past page_size * pages_per_row tokens"))
@@ -324,7 +325,8 @@ class PagedKV:
         those with j > p - window or j < `sinks`.  q [tokens, heads, head_dim] (heads a multiple of kv_heads; head h reads kv head
         h // (heads / kv_heads)) -> the same shape; a token that sees nothing gives zeros; tokens behind offsets[-1] are left as they are
         in `out` (undefined in a new tensor).  `scale`: head_dim ** -0.5 unless given.  `max_len`: no row is longer than this (0: not
-        known); a good bound helps to cut the work of long rows."""
+        known); a good bound helps to cut the work of long rows.  What is wrong with rows, offsets or pages is not reported here but by
+        the append before it: attend leaves `status` alone."""
         q, (T, H, D), qp, qt, qh = self._heads(q, "q", None)
         if H % self.kv_heads:
             raise ValueError(f"{H} query heads do not share {self.kv_heads} kv heads evenly")

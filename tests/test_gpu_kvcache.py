@@ -1107,3 +1107,56 @@ def test_a_traced_step_is_the_eager_one(dtype):
     for h in handles:
         torch_ops.unregister_kv(h)
     torch._dynamo.reset()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32", "int4"])
+def test_offsets_that_end_behind_the_tokens_mean_one_thing(dtype):
+    """Offsets [0, 3, 9] in a call of 5 tokens: every call takes the second row's tokens to be the two that are there, and reports it."""
+    from qwen3_tts_amd import _lib
+    g = _gen(91)
+    G, H, D = 2, 4, 64
+    kv = _cache(dtype, G, D, 16, [20, 30])
+    store = _fill(kv, 0, [20, 30], g)
+    kv.check()
+    rows, off, fits = torch.tensor([0, 1], dtype=torch.int32, device=DEV), _offsets([3, 6]), _offsets([3, 2])
+    x = [_randn(g, 5, n, D, dtype=kv.activations) for n in (H, G, G)]
+    kv.reserve(rows, off, tokens=5)
+    assert kv.lens.tolist() == [23, 32]
+    with pytest.raises(_lib.Q3cError, match="the call's tokens"):
+        kv.check()
+    q = kv.append(0, *x, rows, off)
+    with pytest.raises(_lib.Q3cError, match="the call's tokens"):
+        kv.check()
+    assert torch.equal(q, x[0])
+    back = kv.gather(0, rows, off, tokens=5, dtype="f32")
+    with pytest.raises(_lib.Q3cError, match="the call's tokens"):
+        kv.check()
+    kk, vv = kv.gather(0, rows, fits, tokens=5, dtype="f32")
+    assert torch.equal(back[0], kk) and torch.equal(back[1], vv)
+    if dtype != "int4":
+        assert torch.equal(kk, x[1].float()) and torch.equal(vv, x[2].float())
+    out = kv.attend(0, q, rows, off)
+    kv.check()
+    for r, s, L in ((0, slice(0, 3), 23), (1, slice(3, 5), 32)):
+        k, v = (torch.cat([a, b[s].double()]) for a, b in zip(store[r], (kk, vv)))
+        n = s.stop - s.start
+        want, mag, dot = attention(q[s], k, v, list(range(L - n, L)), 0, 0, D ** -0.5)
+        _check_attend(out[s], want, mag, dot, kv, L, D ** -0.5, q[s].double())
+
+
+def test_attend_leaves_the_status_alone():
+    """Bad rows, missing pages and pages outside the pool give zeros and unseen keys; what says so is the append before."""
+    from qwen3_tts_amd import _lib
+    g = _gen(92)
+    kv = _cache("bf16", 1, 64, 16, [40, 20])
+    _fill(kv, 0, [40, 20], g)
+    kv.check()
+    kv.table[0, 0], kv.table[1, 1] = kv.pages + 3, -1
+    rows = torch.tensor([0, 1, 7], dtype=torch.int32, device=DEV)
+    q, k = _randn(g, 3, 2, 64, dtype=torch.bfloat16), _randn(g, 3, 1, 64, dtype=torch.bfloat16)
+    out = kv.attend(0, q, rows)
+    kv.check()
+    assert bool((out[2] == 0).all()) and bool(torch.isfinite(out).all())
+    kv.append(0, q, k, k, rows)
+    with pytest.raises(_lib.Q3cError, match="row id.*has no page"):
+        kv.check()
