@@ -88,6 +88,12 @@ __device__ __forceinline__ void store4(bf16* p, f32x4 x) { *(u32x2*)p = u32x2{pa
 __device__ __forceinline__ float lo_f(unsigned x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float hi_f(unsigned x) { return __uint_as_float(x & 0xffff0000u); }
 
+// global, not flat: a flat load would be waited for with every use of LDS
+typedef const __attribute__((address_space(1))) unsigned mem_u32;
+typedef const __attribute__((address_space(1))) u32x2 mem_u32x2;
+typedef const __attribute__((address_space(1))) f32x4 mem_f32x4;
+__device__ const u32x4 kv_zeros = {0, 0, 0, 0};                 // what dimensions past the head's size are read from, and rows that nobody sees
+
 // ---- the cache types: how a wave holds one chunk of keys and values, and multiplies with it --------------------------------------------
 // Scores are computed transposed, S^T = K Q^T with 16 keys x 16 columns per tile: lane (c, g) = (lane & 15, lane >> 4) reads key
 // row c as the A operand, and gets in return the scores of column c with keys 4 g .. 4 g + 3.  Those are, register for register, the
@@ -113,7 +119,7 @@ template <int DP> struct Chunk<bf16, DP> {
     }
     static __device__ __forceinline__ int row_bytes(int D) { return 2 * D; }
     static __device__ __forceinline__ int step_bytes() { return 0; }
-    // tile: where row 0 of the 16 rows of tile u lies; dimensions past the head's size read its first ones (their q is 0)
+    // tile: where row 0 of the 16 rows of tile u lies; dimensions past the head's size read its first ones (`scores` takes zeros for them)
     __device__ __forceinline__ void load_k(int u, const char* tile, const char*, int D, int g, int cq) {
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
@@ -144,10 +150,16 @@ template <int DP> struct Chunk<bf16, DP> {
 #pragma unroll
                 for (int w = 0; w < VW; ++w) v[j][w] = 0;
     }
-    __device__ __forceinline__ f32x4 scores(int u, const Q& q, unsigned) const {
+    // Past the head's size q is 0, but 0 times what a key has in another dimension is NaN where that is infinite.
+    __device__ __forceinline__ f32x4 scores(int u, const Q& q, unsigned, int D, int g) const {
         f32x4 s = {0, 0, 0, 0};
+        if (D == DP) {
 #pragma unroll
-        for (int i = 0; i < NS; ++i) s = mfma_bf16(k[u][i], q.f[i], s);
+            for (int i = 0; i < NS; ++i) s = mfma_bf16(k[u][i], q.f[i], s);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NS; ++i) s = mfma_bf16(32 * i + 8 * g < D ? k[u][i] : u32x4{0, 0, 0, 0}, q.f[i], s);
+        }
         return s;
     }
     __device__ __forceinline__ void weigh(const float* p, f32x4* o, unsigned) const {
@@ -189,8 +201,10 @@ template <int DP> struct Chunk<float, DP> {
     static __device__ __forceinline__ int row_bytes(int D) { return 4 * D; }
     static __device__ __forceinline__ int step_bytes() { return 0; }
     __device__ __forceinline__ void load_k(int, const char* tile, const char*, int D, int g, int cq) {
+        // past the head's size (D is a multiple of 16): zeros, as in bf16's scores, but from memory - a branch around the products there costs
+        // the loads that run beside them (4 prompts of 2 048 tokens, 16 heads of 64: 425 us against 375)
 #pragma unroll
-        for (int s = 0; s < NS; ++s) k[0][s] = *(const f32x4*)(tile + (unsigned)(4 * (cq * D + 4 * g + (16 * s < D ? 16 * s : 0))));
+        for (int s = 0; s < NS; ++s) k[0][s] = *(mem_f32x4*)((16 * s < D ? tile : (const char*)&kv_zeros) + (16 * s < D ? (unsigned)(4 * (cq * D + 4 * g + 16 * s)) : 0u));
     }
     __device__ __forceinline__ void load_v(int, const char* tile, const char*, int D, int g, int m) {
         const unsigned off = (unsigned)(4 * (4 * g * D + (m * DV < D ? m * DV : 0)));
@@ -206,7 +220,7 @@ template <int DP> struct Chunk<float, DP> {
 #pragma unroll
                 for (int w = 0; w < DV / 4; ++w) v[j][w] = f32x4{0, 0, 0, 0};
     }
-    __device__ __forceinline__ f32x4 scores(int, const Q& q, unsigned) const {
+    __device__ __forceinline__ f32x4 scores(int, const Q& q, unsigned, int, int) const {
         f32x4 s = {0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < NS; ++i)
@@ -302,7 +316,7 @@ template <int D> struct Chunk<Int4, D> {
             for (int w = 0; w < SW; ++w)
                 if (!keep(u, S == 2 ? (cq & 7) >> 1 : (16 * w + cq) / S)) vs[u][w] = 0.f;
     }
-    __device__ __forceinline__ f32x4 scores(int u, const Q& q, unsigned magic) const {
+    __device__ __forceinline__ f32x4 scores(int u, const Q& q, unsigned magic, int, int) const {
         f32x4 t = {0, 0, 0, 0};
         each<0, S>([&](auto si) {
             constexpr int s = decltype(si)::value;
@@ -434,7 +448,7 @@ __device__ __forceinline__ void attend_part(const KvAttendArgs& a, const Tile& t
             float x[4 * C::TILES];
 #pragma unroll
             for (int u = 0; u < C::TILES; ++u) {
-                const f32x4 s = ch.scores(u, q, magic);
+                const f32x4 s = ch.scores(u, q, magic, D, g);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) x[4 * u + r] = s[r];
             }
@@ -813,10 +827,7 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const KvAttendArgs a) {
 // on 8 of 128): 250 us, 820 TFLOP/s of what is visible; the same on 16-column tiles 978.
 // 4 bits: values n * step are rounded to bf16 on their way into LDS (operands of the matrix cores), four bytes of the row = one 16-byte
 // chunk; the order of dimensions in a row is then the packed one, which Q's load and the output's store follow.
-// global, not flat: a flat load would be waited for with every use of LDS
-typedef const __attribute__((address_space(1))) unsigned mem_u32;
-typedef const __attribute__((address_space(1))) u32x2 mem_u32x2;
-__device__ const u32x4 kv_zeros = {0, 0, 0, 0}, kv_eights = {0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u};      // what a row that nobody sees is read from
+__device__ const u32x4 kv_eights = {0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u};      // 4 bits: n = 0
 template <typename T, int DP> struct Row;                       // chunk ch of a row: 8 values as 16 bytes
 template <int DP> struct Row<bf16, DP> {                       // goes to LDS as it is
     static constexpr float UP = 1.0f;
@@ -982,12 +993,11 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
             constexpr bool keys = decltype(which)::value;
             const int kb = span.chunk(c) * KT;
             if constexpr (DMA) {
-                const bool inner = all && kb + KT - 1 <= vhi && (kb > vlo || kb + KT - 1 < sinks) && okm == ~0ull;
+                // Past the head's size keys are zeros: q is 0 there, but 0 times an infinity would be NaN.  (Values: rows of the product that nobody stores.)
+                const bool inner = all && kb + KT - 1 <= vhi && (kb > vlo || kb + KT - 1 < sinks) && okm == ~0ull && (!keys || row_bytes == RB);
                 // the chunk whose place this thread's slot is
-                auto source = [&](int i) {
-                    const int chunk = (keys ? lds_k<DP>(row0 + i * RP, slot) : lds_v<DP>(row0 + i * RP, slot)) - RB * (row0 + i * RP);
-                    return (unsigned)(sub * row_bytes + (chunk < row_bytes ? chunk : 0));
-                };
+                auto chunk = [&](int i) { return (keys ? lds_k<DP>(row0 + i * RP, slot) : lds_v<DP>(row0 + i * RP, slot)) - RB * (row0 + i * RP); };
+                auto source = [&](int i) { return (unsigned)(sub * row_bytes + (chunk(i) < row_bytes ? chunk(i) : 0)); };
                 const unsigned to = lds_of(lds) + wave * RW * RB;
                 if (inner) {
 #pragma unroll
@@ -996,7 +1006,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
 #pragma unroll
                     for (int i = 0; i < NR; ++i) {
                         const int first = i * RP + wave * RW, mine = kb + first + sub;
-                        const bool ok = (okm >> first & 1) && mine <= vhi && (mine > vlo || mine < sinks);
+                        const bool ok = (okm >> first & 1) && mine <= vhi && (mine > vlo || mine < sinks) && (!keys || chunk(i) < row_bytes);
                         to_lds(ok ? (const void*)(base + place[i] + source(i)) : (const void*)&kv_zeros, to + i * RP * RB);
                     }
                 }

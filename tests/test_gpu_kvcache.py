@@ -1160,3 +1160,51 @@ def test_attend_leaves_the_status_alone():
     kv.append(0, q, k, k, rows)
     with pytest.raises(_lib.Q3cError, match="row id.*has no page"):
         kv.check()
+
+
+@pytest.mark.parametrize("dtype,D,G,group,ps", [("bf16", 80, 4, 8, 16), ("bf16", 16, 8, 4, 8), ("bf16", 208, 4, 8, 32), ("f32", 80, 2, 2, 16), ("f32", 48, 2, 2, 8),
+                                                ("f32", 208, 1, 2, 32), ("bf16", 128, 4, 8, 16), ("f32", 64, 2, 2, 16)])
+def test_a_key_of_minus_infinity_has_no_weight_in_any_head_size(dtype, D, G, group, ps):
+    """A key whose product with every query is -inf counts as little as one that is not there, also where the head is padded to the matrix
+    instructions' size: through single tokens (short, long and many rows), pieces and prompts."""
+    g = _gen(D + G)
+    lens = [260, 410, 33]
+    kv = _cache(dtype, G, D, ps, lens, width=1024)
+    store = _fill(kv, 0, lens, g)
+    there = [torch.ones(L, dtype=torch.bool, device=DEV) for L in lens]
+    for r, pos, dim in ((0, 7, 3), (0, 100, 0), (1, 200, 1), (1, 31, 7), (2, 9, D - 1)):
+        kv.k[0, int(kv.table[r, pos // ps]), :, pos % ps, dim] = -float("inf")
+        there[r][pos] = False
+
+    def queries(n):
+        q = _randn(g, n, G * group, D).to(kv.activations)
+        for d in (0, 1, 3, 7, D - 1):
+            q[..., d] = q[..., d].abs() + 0.5
+        return q
+
+    def look(out, q, rows, pos):
+        assert bool(torch.isfinite(out).all())
+        for i, (r, p) in enumerate(zip(rows, pos)):
+            want, mag, dot = attention(q[i:i + 1], *store[r], [p], 0, 0, D ** -0.5, there[r])
+            _check_attend(out[i:i + 1], want, mag, dot, kv, lens[r], D ** -0.5, q[i:i + 1].double())
+    rows = torch.arange(3, dtype=torch.int32, device=DEV)
+    q = queries(3)
+    for max_len in (410, 0):                                        # whole rows, and (a table of 1 024 pages) rows that are cut
+        look(kv.attend(0, q, rows, max_len=max_len), q, range(3), [L - 1 for L in lens])
+    many = torch.arange(600, dtype=torch.int32, device=DEV) % 3
+    q = queries(600)
+    for max_len in (410, 0):
+        out = kv.attend(0, q, many, max_len=max_len)
+        look(out[:3], q[:3], range(3), [L - 1 for L in lens])
+        look(out[-3:], q[-3:], range(3), [L - 1 for L in lens])
+    for new in ([5, 3, 2], lens):
+        q = queries(sum(new))
+        out = kv.attend(0, q, rows, _offsets(new))
+        at = 0
+        for r, (L, n) in enumerate(zip(lens, new)):
+            some = sorted({0, n // 2, n - 1})
+            i = torch.tensor([at + x for x in some], device=DEV)
+            look(out[i], q[i], [r] * len(some), [L - n + x for x in some])
+            at += n
+    out = kv.attend(0, q, rows, _offsets(lens), window=50, sinks=10)
+    assert bool(torch.isfinite(out).all())
