@@ -345,7 +345,9 @@ int q3c_kv_gather(const q3c_kv* kv, int32_t layer, const int32_t* rows, const in
                   void* v_out, int32_t out_precision, void* hip_stream);
 /* out[t][h] = sum_j softmax_j(scale * q[t][h] . k_j) v_j over the keys j that token t at position p sees: j <= p, and with window > 0
  * also j > p - window or j < sinks.  Head h reads kv head h / (q_heads / kv_heads).  A token that sees nothing gives zeros (0 < scale < 1e37).  A
- * key or value that a token does not see has no part in its output, whatever it holds (how probabilities are rounded may differ).  max_len: no row's length is above it (0:
+ * key or value that a token does not see has no part in its output, whatever it holds (how probabilities are rounded may differ).  fp32 throughout,
+ * but for operands of the matrix cores: with bf16 activations probabilities are rounded to bf16 (INT4: times the value's step), and calls
+ * of many columns over INT4 round values to bf16 as well; keys never are.  max_len: no row's length is above it (0:
  * not known); it only steers how the work is split.  Workspace: q3c_kv_attend_workspace_bytes of the same arguments, 16-byte aligned. */
 int q3c_kv_attend_workspace_bytes(const q3c_kv* kv, int32_t q_heads, int32_t sequences, int32_t tokens, int32_t window, int32_t sinks,
                                   int32_t max_len, size_t* bytes);

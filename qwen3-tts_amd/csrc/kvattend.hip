@@ -5,6 +5,7 @@
 namespace {
 
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
@@ -825,8 +826,11 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const KvAttendArgs a) {
 // Workgroups of one (request, kv head) sit eight apart in launch order, heads fastest: on the eight XCDs, whose workgroups are dealt
 // round robin, a head's keys stay in one L2.  Long columns start first.  16503 new tokens in 6 requests under a window of 2048 (bf16, 16 heads
 // on 8 of 128): 250 us, 820 TFLOP/s of what is visible; the same on 16-column tiles 978.
-// 4 bits: values n * step are rounded to bf16 on their way into LDS (operands of the matrix cores), four bytes of the row = one 16-byte
-// chunk; the order of dimensions in a row is then the packed one, which Q's load and the output's store follow.
+// 4 bits: four bytes of the row = one 16-byte chunk; the order of dimensions in a row is then the packed one, which Q's load and the output's
+// store follow.  Scores are sums of many terms, whose roundings would move a probability by several bf16 steps: keys n * step are
+// fp16 operands, whose 11 bits hold the product of 3 and 8 bits exactly, each key divided by a power of two of its largest step that a
+// score gets back in fp32, and each query by one of its own (errors below 2^-24 of the largest step and |q|: less than single tokens take
+// with their -136).  Values are rounded to bf16: one more rounding of what a weighted mean averages, like that of its weights.
 __device__ const u32x4 kv_eights = {0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u};      // 4 bits: n = 0
 template <typename T, int DP> struct Row;                       // chunk ch of a row: 8 values as 16 bytes
 template <int DP> struct Row<bf16, DP> {                       // goes to LDS as it is
@@ -836,7 +840,7 @@ template <int DP> struct Row<bf16, DP> {                       // goes to LDS as
 };
 template <int D> struct Row<Int4, D> {
     static constexpr int S = D / 32;
-    static constexpr float UP = 16.0f;         // what keys and values are divided by in LDS: a power of two
+    static constexpr float UP = 16.0f;         // what values are divided by in LDS: a power of two
     struct Raw { unsigned x; u32x2 st; };
     static __device__ __forceinline__ const char* base(const void* p, long long row, int) { return (const char*)p + row * (D / 2); }
     static __device__ __forceinline__ const bf16* steps(const bf16* p, long long row) { return p + row * S; }
@@ -846,6 +850,29 @@ template <int D> struct Row<Int4, D> {
         r.x = *(mem_u32*)x;
         if constexpr (S == 2) r.st[0] = *(mem_u32*)st;
         else r.st = *(mem_u32x2*)st;
+    }
+    // A key's power of two: 2^10 steps of the largest one's exponent (`biased`, 12 .. 253, so that it and its reciprocal are normal numbers)
+    static __device__ __forceinline__ unsigned exponent(const Raw& r) {
+        typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+        u16x2 top = __builtin_bit_cast(u16x2, r.st[0] & 0x7fff7fffu);
+        if constexpr (S > 2) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, r.st[1] & 0x7fff7fffu));
+        unsigned most = max((unsigned)top[0], (unsigned)top[1]);
+        if constexpr (S == 8) most = max(most, (unsigned)__builtin_amdgcn_update_dpp(0, (int)most, 0xb1, 0xf, 0xf, true));    // the row's other steps
+        return min(max(most >> 7, 12u), 253u);
+    }
+    static __device__ __forceinline__ float grown(unsigned biased) { return __uint_as_float((biased - 10) << 23); }      // what its scores are multiplied by
+    // n * step / grown as fp16, exact (a step far below the largest one: to 2^-24)
+    static __device__ __forceinline__ u32x4 key(const Raw& r, unsigned biased) {
+        const unsigned lo = r.x & 0x0f0f0f0fu, hi = (r.x >> 4) & 0x0f0f0f0fu;
+        const float f = __uint_as_float((264 - biased) << 23);
+        u32x4 v;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const unsigned w = r.st[S == 2 ? 0 : b >> 1];
+            const float st = (b & 1 ? hi_f(w) : lo_f(w)) * f, z = -8.0f * st;
+            v[b] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(fmaf((float)(lo >> (8 * b) & 255u), st, z), fmaf((float)(hi >> (8 * b) & 255u), st, z)));
+        }
+        return v;
     }
     // n * step / UP as u * (step / UP) - 8 (step / UP) with u = n + 8, exact in one fma of a converted byte; UP keeps 8 steps from overflowing
     static __device__ __forceinline__ u32x4 value(const Raw& r) {
@@ -897,6 +924,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
     constexpr bool DMA = !__is_same(T, Int4);
     constexpr int RB = 2 * DP, NCH = DP / 8, KS = DP / 16, ND = DP / 32, NT = KT / 32, RP = 256 / NCH, NR = KT / RP, RW = RP / 4;
     __shared__ __attribute__((aligned(16))) unsigned char sk[2][KT * RB], sv[2][KT * RB];
+    __shared__ __attribute__((aligned(16))) float grown[2][DMA ? 4 : KT];      // 4 bits: of each key of a tile
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hk = blockIdx.x % a.c.heads, G = a.group, D = a.c.dim, sh = a.c.ps_shift;
     const Tile t = kv_tile(a, tiles - 1 - (int)(blockIdx.x / a.c.heads), 128, lane);
@@ -927,6 +955,30 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
             }
         }
     }
+    float cs = a.scale_log2e;
+    if constexpr (!DMA) {                      // this column's query as fp16, its largest dimension in 2^14 .. 2^15
+        unsigned top = 0;
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const unsigned w = __builtin_bit_cast(u32x4, qf[s])[e];
+                top = max(top, max(w & 0x7fff0000u, w << 16 & 0x7fff0000u));
+            }
+        top = __float_as_uint(max_halves(__uint_as_float(top >> 1))) << 1;        // (shifted: no NaN among what a maximum of floats is taken of)
+        const unsigned biased = max(top >> 23, 15u);
+        const float f = __uint_as_float((268 - biased) << 23);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const u32x4 w = __builtin_bit_cast(u32x4, qf[s]);
+            u32x4 h;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[e] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(lo_f(w[e]) * f, hi_f(w[e]) * f));
+            qf[s] = __builtin_bit_cast(bf16x8, h);
+        }
+        // kept off 0 and infinity, which times a masked score or a score of 0 would be NaN
+        cs = fminf(fmaxf(cs * __uint_as_float((biased - 14) << 23), 0x1p-126f), 0x1.fffffep127f);
+    }
 #pragma unroll
     for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[s]));   // waited for here: a wait in the loop would be for every load in flight
     const Span span = kv_span(a, t, KT);
@@ -938,7 +990,6 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
     const int W = a.window > 0 ? min(a.window, 1 << 30) : 1 << 30, sinks = a.window > 0 ? a.sinks : 0;
     // This thread stages 16-byte slot `slot` of rows row0 + i RP; the rows of a wave and i are RW consecutive ones, which lie in one page.
     const int slot = tid & (NCH - 1), row0 = tid / NCH, sub = lane / NCH;
-    const float cs = a.scale_log2e * R::UP;
     // LDS places of this lane's operands; tiles, halves and buffers are constants added to them
     constexpr bool FEW = DP == 256;            // registers are short: places from the first one by exclusive or, where they are used
     int ak[FEW ? 1 : KS], av[FEW ? 1 : ND];
@@ -1020,12 +1071,33 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
                 }
             }
         };
-        auto stage = [&](unsigned char* lds, bool keys, const typename R::Raw* raw) {
+        auto stage = [&](int buffer, bool keys, const typename R::Raw* raw) {
             if constexpr (!DMA) {
 #pragma unroll
                 for (int i = 0; i < NR; ++i) {
                     const int row = row0 + i * RP;
-                    *(u32x4*)(lds + (keys ? lds_k<DP>(row, slot) : lds_v<DP>(row, slot))) = R::value(raw[i]);
+                    if (keys) {
+                        const unsigned biased = R::exponent(raw[i]);
+                        *(u32x4*)(sk[buffer] + lds_k<DP>(row, slot)) = R::key(raw[i], biased);
+                        if (slot == 0) grown[buffer][row] = R::grown(biased);
+                    } else {
+                        *(u32x4*)(sv[buffer] + lds_v<DP>(row, slot)) = R::value(raw[i]);
+                    }
+                }
+            }
+        };
+        auto product = [&](bf16x8 x, bf16x8 q, f32x16 c) {
+            if constexpr (DMA) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, q, c, 0, 0, 0);
+            else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, q), c, 0, 0, 0);
+        };
+        // 4 bits: a tile's scores, multiplied by what its keys were divided by
+        auto grow = [&](f32x16* s, const float* by) {
+            if constexpr (!DMA) {
+#pragma unroll
+                for (int j = 0; j < 4 * NT; ++j) {
+                    const f32x4 x = *(const f32x4*)(by + 8 * j + 4 * hh);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[j / 4][4 * (j % 4) + e] *= x[e];
                 }
             }
         };
@@ -1039,7 +1111,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
             for (int k = 0; k < KS; ++k)
 #pragma unroll
                 for (int u = 0; u < NT; ++u)
-                    s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(k0 + 32 * u * RB + key_at(k)), qf[k], s[u], 0, 0, 0);
+                    s[u] = product(*(const bf16x8*)(k0 + 32 * u * RB + key_at(k)), qf[k], s[u]);
         };
 #pragma unroll
         for (int n = 0; n < ND; ++n)
@@ -1055,16 +1127,17 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
             ok0 = find(0);
             fetch(0, ok0, kbase, a.c.ks, sk[0], keys, kr);
             fetch(0, ok0, vbase, a.c.vs, sv[0], values, vr);
-            stage(sk[0], true, kr);
-            stage(sv[0], false, vr);
+            stage(0, true, kr);
+            stage(0, false, vr);
             if (span.total > 1) {
                 ok1 = find(1);
                 fetch(1, ok1, kbase, a.c.ks, sk[1], keys, kr);
-                stage(sk[1], true, kr);
+                stage(1, true, kr);
             }
             landed();
             meet();
             scores(s[0], sk[0]);
+            grow(s[0], grown[0]);
             meet();
         }
         auto tile = [&](int c, auto which) {
@@ -1140,7 +1213,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
 #pragma unroll
             for (int j = 0; j < QK + PV; ++j) {
                 const bf16x8 x = ring[j % AHEAD];
-                if (j < QK) s[P ^ 1][j % NT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, qf[j / NT], s[P ^ 1][j % NT], 0, 0, 0);
+                if (j < QK) s[P ^ 1][j % NT] = product(x, qf[j / NT], s[P ^ 1][j % NT]);
                 else o[(j - QK) % ND] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, __builtin_bit_cast(bf16x8, p[(j - QK) / ND / 2][((j - QK) / ND) & 1]), o[(j - QK) % ND], 0, 0, 0);
                 if (j + AHEAD < QK + PV) ring[j % AHEAD] = read(j + AHEAD);
                 if (j < QK)
@@ -1148,8 +1221,9 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
                     for (int e = j * NE / QK; e < (j + 1) * NE / QK; ++e) weight(e);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (c + 2 < span.total) stage(sk[P], true, kr);
-            if (c + 1 < span.total) stage(sv[P ^ 1], false, vr);
+            grow(s[P ^ 1], grown[P ^ 1]);
+            if (c + 2 < span.total) stage(P, true, kr);
+            if (c + 1 < span.total) stage(P ^ 1, false, vr);
             landed();
             meet();
         };
@@ -1199,9 +1273,11 @@ long long tiles_of(int tokens, int sequences, int group, bool ragged, int cols =
 // enough (16-column tile, kv head) pairs that whole rows keep the card busy.  Measured, 128 columns against 16 (us; 16 heads on 8):
 //   bf16, D = 128: 64 x 16 new tokens behind 984 (1024 pairs) 49 / 89, 2 x 1000 under a window of 500 (2000) 26 / 53, 6 x 64 behind 3936 (384)
 //     90 / 121, 1 x 400 (400) 16 / 14, 1 x 100 (100) 10 / 6; of 16 columns: 300 x 8 behind 292 102 / 99, 700 x 8 behind 52 115 / 64
-//   4 bits, where each workgroup has its own keys to unpack, D = 128: 24 x 500 (12000) 120 / 149, 64 x 128 behind 872 (8192) 191 / 210, 64 x 64
-//     (4096) 157 / 116, 2 x 1000 under a window of 500 (2000) 43 / 40, 6 x 128 behind 3872 (768) 189 / 89, 1 x 400 (400) 29 / 12
-//   4 bits, D = 256: 8 x 200 behind 3800 (1600) 378 / 513, 24 x 500 325 / 575, 64 x 64 (4096) 464 / 386, 3 x 235 (705) 40 / 31
+//   4 bits, where each workgroup has its own keys to unpack, D = 128: 24 x 500 (12000) 132 / 160, 64 x 128 behind 872 (8192) 215 / 233,
+//     2 x 1000 under a window of 500 (2000) 43 / 38, 6 x 128 behind 3872 (768) 205 / 89, 1 x 400 (400) 31 / 12; of 128 columns a request:
+//     64 x 64 (4096) 157 / 116
+//   4 bits, D = 64: 24 x 500 (12000) 84 / 100; D = 256: 8 x 200 behind 3800 (1600) 389 / 514, 24 x 500 340 / 576, 3 x 235 (705) 42 / 30;
+//     of 128 columns a request: 64 x 64 (4096) 464 / 386
 bool prompts(const KvView& c, int tokens, int sequences, int q_heads, bool ragged) {
     if (c.dtype == Q3C_KV_F32 || !ragged) return false;
     const bool four = c.dtype == Q3C_KV_INT4;

@@ -324,7 +324,8 @@ class PagedKV:
         """Attention of the rows' newest tokens over the cache: the token at position p sees the keys j <= p, with `window` > 0 only
         those with j > p - window or j < `sinks`.  q [tokens, heads, head_dim] (heads a multiple of kv_heads; head h reads kv head
         h // (heads / kv_heads)) -> the same shape; a token that sees nothing gives zeros; tokens behind offsets[-1] are left as they are
-        in `out` (undefined in a new tensor).  `scale`: head_dim ** -0.5 unless given.  `max_len`: no row is longer than this (0: not
+        in `out` (undefined in a new tensor).  fp32 inside, but that probabilities (and over a 4-bit cache, in calls of many tokens, values)
+        are rounded to bf16 where they are operands of bf16 products.  `scale`: head_dim ** -0.5 unless given.  `max_len`: no row is longer than this (0: not
         known); a good bound helps to cut the work of long rows.  What is wrong with rows, offsets or pages is not reported here but by
         the append before it: attend leaves `status` alone."""
         q, (T, H, D), qp, qt, qh = self._heads(q, "q", None)

@@ -1208,3 +1208,41 @@ def test_a_key_of_minus_infinity_has_no_weight_in_any_head_size(dtype, D, G, gro
             at += n
     out = kv.attend(0, q, rows, _offsets(lens), window=50, sinks=10)
     assert bool(torch.isfinite(out).all())
+
+
+@pytest.mark.parametrize("D,G,group,ps", [(64, 8, 8, 8), (64, 16, 4, 32), (128, 8, 8, 16), (128, 16, 4, 32), (256, 8, 2, 64), (256, 4, 8, 8)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (500, 7)])
+def test_prompts_over_four_bits_take_keys_as_they_are(D, G, group, ps, window, sinks):
+    """A prompt on the kernel of 128 columns is held to the bound of single tokens, and one rounding of the values to bf16 (u of the mean of |v|):
+    nothing is rounded in front of the scores.  Steps and queries of very unlike sizes among it, and a key whose step is NaN."""
+    g = _gen(D + G + window)
+    lens, new = [900, 777], [850, 777]
+    kv = _cache("int4", G, D, ps, lens)
+    off = _offsets(lens)
+    k, v = (_randn(g, sum(lens), G, D).mul_(2) for _ in range(2))
+    k[::7] *= 2.0 ** -30                                            # whole keys
+    k[:, :, :32] *= 2.0 ** -12                                      # a group of every key
+    k[3::11] *= 2.0 ** 5
+    rows = torch.arange(2, dtype=torch.int32, device=DEV)
+    kv.append(0, k.bfloat16(), k.bfloat16(), v.bfloat16(), rows, off)
+    kk, vv = kv.gather(0, rows, off, tokens=sum(lens), dtype="f32")
+    store = list(zip(kk.double().split(lens), vv.double().split(lens)))
+    kv.k_scale[0, int(kv.table[1, 600 // ps]), 0, 600 % ps, 1] = float("nan")
+    q = _randn(g, sum(new), G * group, D).mul_(2)
+    q[::3] *= 2.0 ** -40
+    q[1::5, :, : D // 2] *= 2.0 ** -9
+    q = q.bfloat16()
+    out = kv.attend(0, q, rows, _offsets(new), window=window, sinks=sinks)
+    scale = D ** -0.5
+    for r, start, some in ((0, 0, [0, 127, 128, 400, 849]), (1, 850, [0, 31, 64, 300, 599])):
+        i = torch.tensor([start + x for x in some], device=DEV)
+        pos = [lens[r] - new[r] + x for x in some]
+        want, mag, dot = attention(q[i], *store[r], pos, window, sinks, scale)
+        score = (D + 4) * 2.0 ** -24 * dot * scale + 8 * 144 * 2.0 ** -24 * float(q[i].double().abs().sum(-1).max()) * float(kv.k_scale.float().nan_to_num(0.0).max()) * scale
+        u = 2.0 ** -8
+        bound = (2 * u * 1.05 + 2 * score + 2.0 ** -20 + lens[r] * 2.0 ** -24) * mag + u * want.abs() * 1.01
+        off_by = (out[i].double() - want).abs()
+        assert bool((off_by <= bound + 1e-30).all()), (r, float((off_by - bound).max()))
+    after = [850 + x for x in (600, 601, 776)]
+    assert not bool(torch.isfinite(out[after][:, :group]).any()) if not window else not bool(torch.isfinite(out[after[:2]][:, :group]).any())
+    assert bool(torch.isfinite(out[after][:, group:]).all())
