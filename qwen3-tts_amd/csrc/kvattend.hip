@@ -361,6 +361,35 @@ template <int D> struct Chunk<Int4, D> {
     }
 };
 
+// A matrix product spreads an infinite or NaN value row to columns that do not see it (0 times it is NaN).  So where a result is not finite and the
+// tile's columns differ in what they see, a position's columns are computed again with the rows that it does not see taken out.  Finite data
+// never comes there, and a second look is taken only where it can change something: for columns whose weights are finite (if they are
+// not, a score of the column's own is not, and every look gives NaN), and if one of the rows that only some columns see - from the
+// first position to the last, and as many at the window's far end - is not finite.  This looks
+// for such a row, each thread at every n-th from i0 on.
+template <typename T> __device__ __forceinline__ bool partly_seen_bad(const KvAttendArgs& a, const Tile& t, int hk, int W, int sinks, int i0, int n) {
+    const int differ = t.pmax - t.pmin, D = a.c.dim;
+    bool bad = false;
+    for (int i = i0; i < 2 * differ; i += n) {
+        const int tok = i < differ ? t.pmin + 1 + i : t.pmin - W + 1 + i - differ;
+        if (tok < 0 || (i >= differ && tok < sinks)) continue;
+        const int page = a.c.table[(long long)t.row * a.c.width + (tok >> a.c.ps_shift)];
+        if ((unsigned)page >= (unsigned)a.c.pages) continue;
+        const long long row = ((((long long)a.layer * a.c.pages + page) * a.c.heads + hk) << a.c.ps_shift) + (tok & ((1 << a.c.ps_shift) - 1));
+        if constexpr (__is_same(T, float)) {
+            const u32x4* v = (const u32x4*)((const float*)a.c.v + row * D);
+            for (int d = 0; d < D / 4; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bad |= (v[d][e] & 0x7f800000u) == 0x7f800000u;
+        } else {                               // 4 bits: the steps
+            const int words = __is_same(T, bf16) ? D / 2 : D / 64;
+            const unsigned* v = __is_same(T, bf16) ? (const unsigned*)a.c.v + row * words : (const unsigned*)a.c.vs + row * words;
+            for (int d = 0; d < words; ++d) bad |= (v[d] & 0x7f80u) == 0x7f80u || (v[d] & 0x7f800000u) == 0x7f800000u;
+        }
+    }
+    return bad;
+}
+
 // Work on one tile of columns and one kv head: chunks cb .. ce - 1 of those the tile sees, whole (`out`) or as a part of them (unnormalised
 // sums, maxima and weights: `part`).
 struct KvPart { float *sums, *ml; };           // [16][DP], [16][2]
@@ -400,7 +429,8 @@ __device__ __forceinline__ void attend_part(const KvAttendArgs& a, const Tile& t
     const float cs = a.scale_log2e;
     unsigned magic = 0x43004300u;              // two bf16 exponents of 128, kept in a register: an and-or takes one constant
     asm("" : "+v"(magic));
-    int only = t.pmin - 1;                     // pmin - 1: all columns at once; else the one position whose columns are wanted (below)
+    int only = t.pmin - 1;                     // pmin - 1: all columns at once; else the one position whose columns are wanted (a second look)
+    unsigned long long again = 0;              // lanes whose columns want one
     for (;;) {
         const bool all = only < t.pmin;
         const int vlo = (all ? t.pmin : only) - W, vhi = all ? t.pmax : only;       // a value row counts if vlo < its position <= vhi
@@ -528,18 +558,19 @@ __device__ __forceinline__ void attend_part(const KvAttendArgs& a, const Tile& t
                 for (int r = 0; r < 4; ++r) so[wave][cq][C::dim(i, 4 * g + r)] = o[i][r];
             if (g == 0) { sm[wave][cq] = mypos < 0 ? -INFINITY : m; sl[wave][cq] = mypos < 0 ? 0.f : l; }
         }
-        // A matrix product spreads an infinite or NaN value row to columns that do not see it (0 times it is NaN).  So when a result is
-        // not finite and the tile's columns differ in what they see, each position is computed again with the rows it does not see
-        // taken out, and only its own columns kept.  Finite data never comes here.
         if (all) {
             float bad = 0.f;
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) bad += o[i][r] * 0.f;
-            if (t.pmax <= t.pmin || !__any(mypos >= 0 && bad != 0.f)) break;
+            if (t.pmax <= t.pmin) break;
+            again = __ballot(mypos >= 0 && bad != 0.f && l * 0.f == 0.f);
+            if (!again || !__any(partly_seen_bad<T>(a, t, hk, W, sinks, lane, 64))) break;
         }
-        if (++only > t.pmax) break;
+        do ++only;
+        while (only <= t.pmax && !(again & __ballot(mypos == only)));
+        if (only > t.pmax) break;
     }
     if constexpr (WAVES == 1) return;
     __syncthreads();
@@ -924,6 +955,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
     constexpr bool DMA = !__is_same(T, Int4);
     constexpr int RB = 2 * DP, NCH = DP / 8, KS = DP / 16, ND = DP / 32, NT = KT / 32, RP = 256 / NCH, NR = KT / RP, RW = RP / 4;
     __shared__ __attribute__((aligned(16))) unsigned char sk[2][KT * RB], sv[2][KT * RB];
+    __shared__ unsigned long long again[4];    // lanes whose columns want a second look (in LDS: no register is left to carry it)
     __shared__ __attribute__((aligned(16))) float grown[2][DMA ? 4 : KT];      // 4 bits: of each key of a tile
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hk = blockIdx.x % a.c.heads, G = a.group, D = a.c.dim, sh = a.c.ps_shift;
@@ -1004,7 +1036,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
     auto key_at = [&](int k) { return FEW ? ak[0] ^ (32 * k) : ak[FEW ? 0 : k]; };
     auto value_at = [&](int n) { return FEW ? av[0] ^ (64 * n) : av[FEW ? 0 : n]; };
 
-    int only = t.pmin - 1;                     // as in kv_attend_kernel: a second look, position by position, where a result is not finite
+    int only = t.pmin - 1;                     // as in attend_part: a second look where partly_seen_bad says
     for (;;) {
         const bool all = only < t.pmin;
         const int vlo = (all ? t.pmin : only) - W, vhi = all ? t.pmax : only;
@@ -1182,7 +1214,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
             const float mu = m == -INFINITY ? 0.f : m;
             // The order below is the order of the instructions: each matrix product has its operands' reads of LDS a few products earlier and a share of
             // the softmax's arithmetic behind it.  (Past the last tile the scores are of whatever lies there, and not looked at.)
-            constexpr int QK = KS * NT, PV = 2 * NT * ND, NE = 16 * NT / 2, AHEAD = DMA ? 5 : 4;      // products, pairs of scores
+            constexpr int QK = KS * NT, PV = 2 * NT * ND, NE = 16 * NT / 2, AHEAD = DMA ? 5 : 3;      // products, pairs of scores
             bf16x8 ring[AHEAD];
             u32x4 p[NT][2];
             auto read_k = [&](int j) { return *(const bf16x8*)(sk[P ^ 1] + 32 * (j % NT) * RB + key_at(j / NT)); };
@@ -1258,9 +1290,14 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
             for (int n = 0; n < ND; ++n)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) bad += o[n][i] * 0.f;
-            if (!__syncthreads_or(t.pmax > t.pmin && mypos >= 0 && bad != 0.f)) return;
+            if (t.pmax <= t.pmin) return;
+            const unsigned long long bits = __ballot(mypos >= 0 && bad != 0.f && l * 0.f == 0.f);
+            if (lane == 0) again[wave] = bits;
+            if (!__syncthreads_or(bits != 0) || !__syncthreads_or(partly_seen_bad<T>(a, t, hk, W, sinks, tid, 256))) return;
         }
-        if (++only > t.pmax) return;
+        do ++only;
+        while (only <= t.pmax && !__syncthreads_or((again[wave] & __ballot(mypos == only)) != 0));
+        if (only > t.pmax) return;
     }
 }
 

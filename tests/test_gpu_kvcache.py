@@ -1246,3 +1246,83 @@ def test_prompts_over_four_bits_take_keys_as_they_are(D, G, group, ps, window, s
     after = [850 + x for x in (600, 601, 776)]
     assert not bool(torch.isfinite(out[after][:, :group]).any()) if not window else not bool(torch.isfinite(out[after[:2]][:, :group]).any())
     assert bool(torch.isfinite(out[after][:, group:]).all())
+
+
+def _time(call):
+    """The least of some runs, in ms."""
+    for _ in range(3):
+        call()
+    best = math.inf
+    for _ in range(7):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        for _ in range(3):
+            call()
+        b.record()
+        b.synchronize()
+        best = min(best, a.elapsed_time(b) / 3)
+    return best
+
+
+SECOND = [("bf16", 128, 4, 4, 16), ("bf16", 64, 1, 2, 32), ("bf16", 80, 4, 8, 16), ("int4", 128, 8, 8, 32), ("int4", 64, 1, 3, 8), ("int4", 256, 4, 4, 16), ("f32", 64, 2, 2, 16)]
+
+
+@pytest.mark.parametrize("dtype,D,G,group,ps", SECOND)
+def test_one_bad_row_or_token_does_not_multiply_the_time(dtype, D, G, group, ps):
+    """A value that is not finite, seen by every later token (the first position, a sink), and a query that is not: neither is worth a second
+    look at every tile, one for each of its positions.  Four times are left for the tile that holds the row."""
+    g = _gen(D + G + 5)
+    lens = [1700]
+    kv = _cache(dtype, G, D, ps, lens)
+    _fill(kv, 0, lens, g)
+    rows, off = torch.zeros(1, dtype=torch.int32, device=DEV), _offsets([1500])
+    q = _randn(g, 1500, G * group, D).to(kv.activations)
+    out = torch.empty_like(q)
+
+    def run():
+        return kv.attend(0, q, rows, off, window=0, out=out)
+    clean = _time(run)
+    keep = out.clone()
+    q[777] = float("nan")
+    query = _time(run)
+    assert bool(torch.isnan(out[777]).all()) and bool(torch.isfinite(out[:777]).all()) and bool(torch.isfinite(out[778:]).all())
+    q[777] = 0.0
+    page = int(kv.table[0, 0])
+    (kv.v_scale if dtype == "int4" else kv.v)[0, page, G - 1, 2, 1] = float("inf")
+    value = _time(run)
+    assert torch.equal(out[:777, :(G - 1) * group], keep[:777, :(G - 1) * group]) and not bool(torch.isfinite(out[:, (G - 1) * group:]).all(-1).any())
+    assert query < 4 * clean and value < 4 * clean, (clean, query, value)
+
+
+@pytest.mark.parametrize("dtype,D,G,group,ps", SECOND)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (300, 3)])
+def test_bad_values_stay_with_the_tokens_that_see_them(dtype, D, G, group, ps, window, sinks):
+    """Infinities and NaN in values of other dimensions: one at the first position (a sink of all), one between, one that enters and leaves the
+    window inside tiles.  Every output element is finite or not as the rows that its token sees say, and the finite ones are right."""
+    g = _gen(D + G + 6)
+    lens, new = [1000, 60], [900, 60]
+    kv = _cache(dtype, G, D, ps, lens)
+    store = [[k.clone(), v.clone()] for k, v in _fill(kv, 0, lens, g)]
+    bad = {0: (1, float("inf")), 333: (40, float("nan")), 650: (D - 1, -float("inf")), 651: (D - 1, float("inf"))}
+    for pos, (dim, x) in bad.items():
+        page, slot = int(kv.table[0, pos // ps]), pos % ps
+        if dtype == "int4":
+            kv.v_scale[0, page, :, slot, dim // 32] = x
+            store[0][1][pos, :, dim // 32 * 32:dim // 32 * 32 + 32] = float("nan")      # n times an infinite step: of either sign, or NaN
+        else:
+            kv.v[0, page, :, slot, dim] = x
+            store[0][1][pos, :, dim] = x
+    q = _randn(g, sum(new), G * group, D).to(kv.activations)
+    rows = torch.arange(2, dtype=torch.int32, device=DEV)
+    out = kv.attend(0, q, rows, _offsets(new), window=window, sinks=sinks)
+    some = [0, 1, 127, 128, 230, 232, 233, 240, 255, 256, 400, 530, 532, 533, 534, 548, 549, 550, 551, 560, 700, 830, 845, 849, 850, 851, 852, 899]
+    for i in some:
+        p = 100 + i
+        see = [x for x in range(p + 1) if not window or x > p - window or x < sinks]
+        v, finite = store[0][1][see], torch.isfinite(store[0][1][see]).all(0)                        # [G, D]
+        finite = finite.repeat_interleave(group, 0)
+        assert torch.equal(torch.isfinite(out[i]), finite), i
+        want, mag, dot = attention(q[i:i + 1], store[0][0], store[0][1].nan_to_num(0.0, 0.0, 0.0), [p], window, sinks, D ** -0.5)
+        got = torch.where(finite, out[i], want[0].to(out.dtype))
+        _check_attend(got[None], want, mag, dot, kv, p + 1, D ** -0.5, q[i:i + 1].double(), prompt=True)
+    assert bool(torch.isfinite(out[900:]).all())
