@@ -1321,19 +1321,24 @@ bool prompts(const KvView& c, int tokens, int sequences, int q_heads, bool ragge
     const long long columns = (long long)tokens * (q_heads / c.heads), least = !four ? 512 : c.dim == 256 ? 1536 : 6144;
     return columns >= (four ? 256ll : 32ll) * sequences && columns / 16 * c.heads >= least;
 }
-// most chunks that one row of the call can see
-long long most_chunks(const KvView& c, int window, int sinks, int max_len) {
+// The most chunks that a tile of `positions` neighbouring ones can see (of a row no longer than max_len, if that is given): its sinks', and those
+// that window + positions - 1 tokens touch, which begin anywhere in a chunk.
+long long most_chunks(const KvView& c, int window, int sinks, int max_len, int positions) {
     const int tb = c.dtype == Q3C_KV_F32 ? 16 : 32;
     long long len = (long long)c.width << c.ps_shift;
     if (max_len > 0 && max_len < len) len = max_len;
-    if (window > 0 && (long long)window + sinks + tb < len) len = (long long)window + sinks + tb;
-    return len / tb + 1;
+    long long n = len / tb + 1;
+    if (window > 0) {
+        const long long seen = ((long long)sinks + tb - 1) / tb + ((long long)window + positions - 1 + tb - 2) / tb + 1;
+        if (seen < n) n = seen;
+    }
+    return n;
 }
 // Single tokens in a line of runs, unless the whole line is short: then the layout of the line costs more than it evens out (one row under a
 // 4096-token window, 1040 chunks: 20 us against 14; 8 rows of 700 tokens in 4 bits: 17.6 against 11.5; 64 rows of 3200 - 16000: 184 against 218).
 bool flat(const KvView& c, int sequences, int q_heads, bool ragged, int window, int sinks, int max_len) {
-    const long long tiles = (long long)sequences * ((q_heads / c.heads + 15) / 16), line = tiles * c.heads * most_chunks(c, window, sinks, 0);
-    return !ragged && tiles <= FLAT && line < 0x70000000ll && tiles * c.heads * most_chunks(c, window, sinks, max_len) > 8192;
+    const long long tiles = (long long)sequences * ((q_heads / c.heads + 15) / 16), line = tiles * c.heads * most_chunks(c, window, sinks, 0, 1);
+    return !ragged && tiles <= FLAT && line < 0x70000000ll && tiles * c.heads * most_chunks(c, window, sinks, max_len, 1) > 8192;
 }
 // waves that run at once on 256 compute units
 int flat_runs(const KvView& c) {
@@ -1349,7 +1354,7 @@ KvSplit q3_kv_attend_split(const KvView& c, int tokens, int sequences, int q_hea
     if (flat(c, sequences, q_heads, ragged, window, sinks, max_len)) return KvSplit{0, 0, 0};
     if (prompts(c, tokens, sequences, q_heads, ragged)) return KvSplit{1, 0x7fffffff, 0};
     const int group = q_heads / c.heads;
-    const long long chunks = most_chunks(c, window, sinks, max_len), base = tiles_of(tokens, sequences, group, ragged) * c.heads;
+    const long long chunks = most_chunks(c, window, sinks, max_len, ragged ? 16 : 1), base = tiles_of(tokens, sequences, group, ragged) * c.heads;
     long long share = (chunks * base + 2047) / 2048;
     if (share < 8) share = 8;
     if (share < (chunks + 255) / 256) share = (chunks + 255) / 256;

@@ -120,6 +120,21 @@ def test_calls_larger_than_a_launch_are_refused():
     assert lib.q3c_kv_fork(_kv(layers=64), PTR, PTR, 1 << 17, PTR, 1 << 40, None) == UNSUPPORTED
 
 
+@pytest.mark.parametrize("dtype,tb", [(0, 16), (1, 32)])
+def test_shares_cover_the_chunks_that_a_window_can_touch(dtype, tb):
+    """How a long row is cut follows from the most chunks of 16 or 32 tokens that a tile can see under the window: a bound, held here against all
+    places of a window of one position and of 16 (the workspace says how many shares of 8 chunks there are; none: at most 32 chunks, uncut)."""
+    lib, kv, n = _lib.load(), _kv(dtype=dtype, pages=4096, pages_per_row=4096), C.c_size_t()
+    for window in list(range(1, 5)) + list(range(tb * 31 - 20, tb * 33 + 20, 3)) + list(range(1200, 1300, 5)) + list(range(1210, 1222)):
+        for sinks in (0, 1, 5, tb, tb + 1):
+            assert lib.q3c_kv_attend_workspace_bytes(kv, 2, 1, 1, window, sinks, 0, C.byref(n)) == OK
+            shares = (n.value // (4 * 2) - 1) // (16 * 66)            # of each of the two heads: shares of [16][64 + 2], one count
+            for positions in (1, 16):
+                first = 10 * tb + sinks + window                       # far behind the sinks: the most there is
+                most = max(-(-sinks // tb) + (p + positions - 1) // tb - (p - window + 1) // tb + 1 for p in range(first, first + tb))
+                assert most <= (8 * shares if n.value else 32), (window, sinks, positions)
+
+
 def test_a_scale_that_overflows_is_refused():
     """The scale is held times log2(e), and times 16 where keys are: 1e37 is the last decade whose products fp32 holds."""
     lib, kv = _lib.load(), _kv()
