@@ -48,6 +48,11 @@ _STATUS = ((1, "a row id outside the table, named twice in a call, or offsets th
            (8, "a row grew past page_size * pages_per_row tokens"))
 
 
+def _no_gradient(t: torch.Tensor, what: str) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} requires a gradient, and the cache's operators have none: call them under torch.no_grad()")
+
+
 def rope_tables(positions: int, rot_dim: int, theta: float = 10000.0, device: Union[str, torch.device] = "cuda:0") -> Tuple[torch.Tensor, torch.Tensor]:
     """(cos, sin), float32 [positions, rot_dim / 2] each, of position * theta^(-2 i / rot_dim): angles in float64, so that far positions
     are as exact as near ones."""
@@ -127,6 +132,7 @@ class PagedKV:
                 raise ValueError(f"{n} must be contiguous and on {k.device}")
             if n in ("k", "v", "k_scale", "v_scale") and t.data_ptr() % 16:
                 raise ValueError(f"{n} must be 16-byte aligned")
+            _no_gradient(t, n)
         if k.device.type != "cuda":
             raise RuntimeError("qwen3_tts_amd.kvcache needs a ROCm GPU (MI355X); there is no CPU fallback")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
@@ -215,8 +221,8 @@ class PagedKV:
             raise ValueError(f"{what} must be [tokens, {'heads' if heads is None else heads}, {self.head_dim}], got {tuple(shape)}")
         if x.dtype != self.activations or x.get_device() != self._index:
             raise ValueError(f"{what} must be {self.activations} on {self.device}, got {x.dtype} on {x.device}")
-        if x.requires_grad and torch.is_grad_enabled():
-            raise ValueError(f"{what} requires a gradient, and the cache's operators have none: call them under torch.no_grad()")
+        if x.requires_grad:
+            _no_gradient(x, what)
         ts, hs, ds = x.stride()
         p, quad = x.data_ptr(), 4 * self._act_bytes
         if ds != 1 or (ts % 4 and shape[0] != 1) or (hs % 4 and shape[1] != 1) or p % quad:
@@ -231,6 +237,8 @@ class PagedKV:
         p = t.data_ptr()
         if t.dtype != torch.float32 or t.dim() != dims or not t.is_contiguous() or t.get_device() != self._index or p % 16:
             raise ValueError(f"{what} must be a contiguous, 16-byte aligned float32 tensor {shape} on {self.device}")
+        if t.requires_grad:
+            _no_gradient(t, what)
         return p
 
     def _layer(self, layer: int) -> int:
@@ -243,6 +251,7 @@ class PagedKV:
             return torch.empty(shape, dtype=dtype, device=self.device)
         if out.dtype != dtype or tuple(out.shape) != tuple(shape) or not out.is_contiguous() or out.get_device() != self._index or out.data_ptr() % 16:
             raise ValueError(f"{what} must be a contiguous, 16-byte aligned {dtype} tensor {tuple(shape)} on {self.device}")
+        _no_gradient(out, what)
         return out
 
     def check(self) -> None:

@@ -1326,3 +1326,23 @@ def test_bad_values_stay_with_the_tokens_that_see_them(dtype, D, G, group, ps, w
         got = torch.where(finite, out[i], want[0].to(out.dtype))
         _check_attend(got[None], want, mag, dot, kv, p + 1, D ** -0.5, q[i:i + 1].double(), prompt=True)
     assert bool(torch.isfinite(out[900:]).all())
+
+
+def test_weights_tables_and_outputs_that_ask_for_gradients_are_refused():
+    """A module's parameters, as they are, outside torch.no_grad(): their gradients would be cut off without a word."""
+    kv = _cache("bf16", 1, 64, 16, [20])
+    rows = torch.zeros(1, dtype=torch.int32, device=DEV)
+    q = torch.ones(1, 1, 64, dtype=torch.bfloat16, device=DEV)
+    w = torch.nn.Parameter(torch.ones(64, device=DEV))
+    cos, sin = (torch.ones(kv.max_tokens, 32, device=DEV, requires_grad=r) for r in (True, False))
+    out = torch.zeros(1, 1, 64, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    calls = [lambda: kv.append(0, q, q, q, rows, q_weight=w), lambda: kv.append(0, q, q, q, rows, k_weight=w), lambda: kv.append(0, q, q, q, rows, rope=(cos, sin)),
+             lambda: kv.append(0, q, q, q, rows, rope=(sin, cos)), lambda: kv.append(0, q, q, q, rows, out=out), lambda: kv.attend(0, q, rows, out=out)]
+    for call in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+    assert bool(torch.isnan(kv.k[0, int(kv.table[0, 1]), 0, 3]).all())      # nothing was written
+    with torch.no_grad():
+        for call in calls:
+            call()
+    kv.check()

@@ -42,6 +42,15 @@ def test_tensors_that_are_refused():
             PagedKV(**{**dict(layers=1, kv_heads=1, head_dim=64, pages=2, device="cpu"), **kw})
 
 
+def test_cache_tensors_that_ask_for_gradients_are_refused():
+    good = _tensors()
+    for n in ("k", "v"):
+        with pytest.raises(ValueError, match=f"{n} requires a gradient"):
+            PagedKV.from_tensors(**{**good, n: good[n].clone().requires_grad_()})
+        with pytest.raises(RuntimeError, match="no CPU fallback"), torch.no_grad():
+            PagedKV.from_tensors(**{**good, n: good[n].clone().requires_grad_()})
+
+
 def _kv(**change):
     c = _lib.Q3cKv()
     c.struct_size = C.sizeof(_lib.Q3cKv)
