@@ -28,6 +28,7 @@ graph take `rows` as a tensor: a sequence is copied to the device by the call.
 from __future__ import annotations
 
 import ctypes as C
+import operator
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
@@ -191,7 +192,7 @@ class PagedKV:
             if ids.dtype != torch.int32 or ids.dim() != 1 or not ids.is_contiguous() or ids.get_device() != self._index:
                 raise ValueError(f"{what} must be a contiguous int32 tensor [n] on {self.device} (or a sequence of ints)")
             return ids
-        ids = [int(i) for i in ids]
+        ids = [operator.index(i) for i in ids]                  # whole numbers only: 1.9 is no row
         for i in ids:
             if not 0 <= i < most:
                 raise IndexError(f"{what}: {i} is not in [0, {most})")

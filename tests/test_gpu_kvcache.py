@@ -1346,3 +1346,15 @@ def test_weights_tables_and_outputs_that_ask_for_gradients_are_refused():
         for call in calls:
             call()
     kv.check()
+
+
+def test_ids_that_are_no_whole_numbers_are_refused():
+    import numpy as np
+    kv = _cache("bf16", 1, 64, 16, [20, 7])
+    for call in (lambda: kv.release([0.9]), lambda: kv.trim([1.0], 4), lambda: kv.copy_pages([0.5], [1]), lambda: kv.fork([0], ["1"]), lambda: kv.reserve([None])):
+        with pytest.raises(TypeError):
+            call()
+    assert kv.lens.tolist() == [20, 7]
+    kv.reserve(np.array([1, 0]))
+    assert kv.lens.tolist() == [21, 8]
+    kv.check()
