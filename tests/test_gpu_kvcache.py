@@ -1358,3 +1358,95 @@ def test_ids_that_are_no_whole_numbers_are_refused():
     kv.reserve(np.array([1, 0]))
     assert kv.lens.tolist() == [21, 8]
     kv.check()
+
+
+# ---- which kernel a call takes, and what only long rows reach ------------------------------------------------------------------------
+def _kernels(call):
+    """Names of the cache's kernels that a call launches."""
+    import re
+    from torch.profiler import ProfilerActivity, profile
+    call()
+    torch.cuda.synchronize()
+    with profile(activities=[ProfilerActivity.CUDA]) as p:
+        call()
+        torch.cuda.synchronize()
+    return {m.group(1) for e in p.key_averages() for m in [re.search(r"(kv_[a-z_]+?_kernel)", e.key)] if m}
+
+
+def _check_tight(got, q, k, v, pos, window, sinks, kv, N, there=None, prompt=False):
+    """As _check_attend, but keys count as unrounded everywhere; `prompt`: values over 4 bits are rounded to bf16 once (u of the mean of |v|)."""
+    scale = kv.head_dim ** -0.5
+    want, mag, dot = attention(q, k, v, pos, window, sinks, scale, there)
+    if not (prompt and kv.dtype == "int4"):
+        return _check_attend(got, want, mag, dot, kv, N, scale, q.double())
+    u = 2.0 ** -8
+    top = float(kv.k_scale.float().nan_to_num(0.0).max())
+    score = (kv.head_dim + 4) * 2.0 ** -24 * dot * scale + 8 * 144 * 2.0 ** -24 * float(q.double().abs().sum(-1).max()) * top * scale
+    bound = (2 * u * 1.05 + 2 * score + 2.0 ** -20 + N * 2.0 ** -24) * mag + u * want.abs() * 1.01
+    off_by = (got.double() - want).abs()
+    assert bool((off_by <= bound + 1e-30).all()), f"max excess {float((off_by - bound).max()):.3e}"
+
+
+@pytest.mark.parametrize("dtype,D,G,group,ps,L", [("bf16", 128, 2, 8, 8, 1600), ("bf16", 64, 4, 4, 32, 3100), ("bf16", 256, 2, 8, 16, 1300), ("bf16", 80, 4, 4, 8, 1500),
+                                                  ("int4", 64, 8, 8, 8, 1600), ("int4", 128, 8, 8, 32, 3100), ("int4", 256, 4, 8, 8, 1500)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (700, 5), (130, 1000)])
+def test_prompts_over_more_pages_than_a_wave_has_lanes(dtype, D, G, group, ps, L, window, sinks):
+    """The prompt kernel holds 64 entries of the table at a time: rows of 81 to 200 pages, read from front to back, and from the sinks to the window's
+    start; whole prompts and a piece behind a past; a missing page and one outside the pool among the later ones."""
+    g = _gen(D + L + window)
+    lens, new = [L, L - 77], [L, 500]
+    kv = _cache(dtype, G, D, ps, lens)
+    store = _fill(kv, 0, lens, g)
+    there = [torch.ones(n, dtype=torch.bool, device=DEV) for n in lens]
+    for r, pos, value in ((0, L - 300, -1), (1, L - 400, kv.pages + 5), (1, 65 * ps, -1)):
+        j = pos // ps
+        kv.table[r, j] = value
+        there[r][j * ps:(j + 1) * ps] = False
+    q = _randn(g, sum(new), G * group, D).mul_(2).to(kv.activations)
+    rows = torch.arange(2, dtype=torch.int32, device=DEV)
+    out = torch.empty_like(q)
+    assert _kernels(lambda: kv.attend(0, q, rows, _offsets(new), window=window, sinks=sinks, out=out)) == {"kv_prompt_kernel"}
+    for r, start, some in ((0, 0, [0, 63, 64 * ps - 1, 64 * ps, 65 * ps + 3, L - 301, L - 150, L - 1]), (1, L, [0, 5, 130, 499])):
+        i = torch.tensor([start + x for x in some], device=DEV)
+        _check_tight(out[i], q[i], *store[r], [lens[r] - new[r] + x for x in some], window, sinks, kv, L, there[r], prompt=True)
+
+
+@pytest.mark.parametrize("dtype,D,G,group,ps", [("bf16", 128, 2, 2, 16), ("bf16", 64, 1, 5, 8), ("bf16", 256, 1, 4, 32), ("bf16", 80, 2, 3, 8), ("int4", 128, 2, 2, 16), ("int4", 64, 1, 7, 8),
+                                                ("int4", 256, 2, 1, 64), ("f32", 64, 2, 2, 16), ("f32", 128, 1, 3, 8)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (3000, 40)])
+def test_pieces_behind_a_long_past_are_cut_and_joined(dtype, D, G, group, ps, window, sinks):
+    """A few tokens of each request behind thousands: tiles of several positions whose keys are cut into shares."""
+    g = _gen(D + G + window)
+    lens, new = [6001, 4096, 70, 5333], [5, 19, 2, 40]
+    kv = _cache(dtype, G, D, ps, lens)
+    store = _fill(kv, 0, lens, g)
+    q = _randn(g, sum(new), G * group, D).mul_(2).to(kv.activations)
+    rows = torch.arange(4, dtype=torch.int32, device=DEV)
+    out = torch.empty_like(q)
+    assert _kernels(lambda: kv.attend(0, q, rows, _offsets(new), window=window, sinks=sinks, out=out)) == {"kv_attend_kernel", "kv_join_kernel"}
+    at = 0
+    for r, n in enumerate(new):
+        some = sorted({0, n // 2, n - 1})
+        i = torch.tensor([at + x for x in some], device=DEV)
+        _check_tight(out[i], q[i], *store[r], [lens[r] - n + x for x in some], window, sinks, kv, lens[r])
+        at += n
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32", "int4"])
+def test_which_kernel_a_call_takes(dtype):
+    """The rule for each kernel, by a call on either side of it: many columns a request, one token of long rows, short rows, and the rest."""
+    G, group, D, ps = 8, 4, 128, 32
+    kv = _cache(dtype, G, D, ps, [1] * 600, width=300)
+    rows = torch.arange(600, dtype=torch.int32, device=DEV)
+
+    def names(new, n, **kw):
+        q = torch.zeros(new * n, G * group, D, dtype=kv.activations, device=DEV)
+        off = None if new == 1 else torch.arange(0, new * n + 1, new, dtype=torch.int32, device=DEV)
+        return _kernels(lambda: kv.attend(0, q, rows[:n], off, **kw))
+    flat, cut, whole, short, prompt = {"kv_flat_kernel", "kv_flat_join_kernel"}, {"kv_attend_kernel", "kv_join_kernel"}, {"kv_attend_kernel"}, {"kv_short_kernel"}, {"kv_prompt_kernel"}
+    assert names(1, 64) == flat and names(1, 64, max_len=200) == whole
+    assert names(1, 2) == (flat if dtype == "f32" else cut) and names(1, 2, max_len=500) == whole       # (fp32 chunks are half as long)
+    assert names(1, 600, max_len=200) == flat and names(1, 600, max_len=15) == short
+    assert names(4, 300, window=60) == short and names(4, 20, window=60) == whole
+    assert names(800, 4) == (whole if dtype == "f32" else prompt)
+    assert names(10, 4) == cut
