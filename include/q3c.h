@@ -344,11 +344,12 @@ int q3c_kv_append(const q3c_kv* kv, int32_t layer, const void* q, int64_t q_toke
 int q3c_kv_gather(const q3c_kv* kv, int32_t layer, const int32_t* rows, const int32_t* offsets, int32_t sequences, int32_t tokens, void* k_out,
                   void* v_out, int32_t out_precision, void* hip_stream);
 /* out[t][h] = sum_j softmax_j(scale * q[t][h] . k_j) v_j over the keys j that token t at position p sees: j <= p, and with window > 0
- * also j > p - window or j < sinks.  Head h reads kv head h / (q_heads / kv_heads).  A token that sees nothing gives zeros (0 < scale < 1e37).  A
- * key or value that a token does not see has no part in its output, whatever it holds (how probabilities are rounded may differ).  fp32 throughout,
- * but for operands of the matrix cores: with bf16 activations probabilities are rounded to bf16 (INT4: times the value's step), and calls
- * of many columns over INT4 round values to bf16 as well; keys never are.  max_len: no row's length is above it (0:
- * not known); it only steers how the work is split.  Workspace: q3c_kv_attend_workspace_bytes of the same arguments, 16-byte aligned. */
+ * also j > p - window or j < sinks; 0 < scale < 1e37.  Head h reads kv head h / (q_heads / kv_heads).  A token that sees nothing, or whose
+ * scores are all -inf, gives zeros.  A key or value that a token does not see has no part in its output, whatever it holds (how
+ * probabilities are rounded may differ).  fp32 throughout, but for operands of the matrix cores: with bf16 activations probabilities are
+ * rounded to bf16 (INT4: times the value's step), and calls of many columns over INT4 round values to bf16 as well; keys never are.
+ * max_len: no row's length is above it (0: not known); it only steers how the work is split.  Workspace: q3c_kv_attend_workspace_bytes of
+ * the same arguments, 16-byte aligned. */
 int q3c_kv_attend_workspace_bytes(const q3c_kv* kv, int32_t q_heads, int32_t sequences, int32_t tokens, int32_t window, int32_t sinks,
                                   int32_t max_len, size_t* bytes);
 int q3c_kv_attend(const q3c_kv* kv, int32_t layer, const void* q, int64_t q_token_stride, int64_t q_head_stride, int32_t q_heads,
@@ -359,7 +360,8 @@ int q3c_kv_attend(const q3c_kv* kv, int32_t layer, const void* q, int64_t q_toke
  * later query of a sliding window sees go back (all their tokens >= sinks and at least `window` before the row's end).  copy: page
  * dst[i] = page src[i] in every layer; of pairs with one destination the last counts, a pair whose source is another's destination
  * is refused.  compact: the live pages move to the front of the pool (live pages behind the first *live_dev ones, ascending, to the
- * free ones before, ascending); table and counts follow, *live_dev = their number.  Workspaces in device memory, 4-byte aligned:
+ * free ones before, ascending); table and counts follow, *live_dev = their number; nothing says where a page went, so a page that is held by its
+ * count alone, without a table entry, cannot be followed: hold pages by a row of the table.  Workspaces in device memory, 4-byte aligned:
  * fork 12 * count bytes, copy 4 * count, compact 8 * pages + 16. */
 int q3c_kv_fork(const q3c_kv* kv, const int32_t* parents, const int32_t* children, int32_t count, void* workspace, size_t workspace_bytes, void* hip_stream);
 int q3c_kv_release(const q3c_kv* kv, const int32_t* rows, int32_t count, void* hip_stream);

@@ -365,8 +365,8 @@ template <int D> struct Chunk<Int4, D> {
 // tile's columns differ in what they see, a position's columns are computed again with the rows that it does not see taken out.  Finite data
 // never comes there, and a second look is taken only where it can change something: for columns whose weights are finite (if they are
 // not, a score of the column's own is not, and every look gives NaN), and if one of the rows that only some columns see - from the
-// first position to the last, and as many at the window's far end - is not finite.  This looks
-// for such a row, each thread at every n-th from i0 on.
+// first position to the last, and as many at the window's far end - is not finite.  This looks for such a row, each thread at every n-th
+// of them from i0 on.
 template <typename T> __device__ __forceinline__ bool partly_seen_bad(const KvAttendArgs& a, const Tile& t, int hk, int W, int sinks, int i0, int n) {
     const int differ = t.pmax - t.pmin, D = a.c.dim;
     bool bad = false;
@@ -856,7 +856,7 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const KvAttendArgs a) {
 // the range), which a causal row does a few times in all.
 // Workgroups of one (request, kv head) sit eight apart in launch order, heads fastest: on the eight XCDs, whose workgroups are dealt
 // round robin, a head's keys stay in one L2.  Long columns start first.  16503 new tokens in 6 requests under a window of 2048 (bf16, 16 heads
-// on 8 of 128): 250 us, 820 TFLOP/s of what is visible; the same on 16-column tiles 978.
+// on 8 of 128): 253 us, 810 TFLOP/s of what is visible; the same on 16-column tiles 978.
 // 4 bits: four bytes of the row = one 16-byte chunk; the order of dimensions in a row is then the packed one, which Q's load and the output's
 // store follow.  Scores are sums of many terms, whose roundings would move a probability by several bf16 steps: keys n * step are
 // fp16 operands, whose 11 bits hold the product of 3 and 8 bits exactly, each key divided by a power of two of its largest step that a
@@ -934,6 +934,7 @@ __device__ __forceinline__ float max_halves(float x) {           // over lanes l
 typedef __attribute__((address_space(3))) void lds_void;
 
 // 16 bytes per lane from memory to LDS at `lds` (uniform) + 16 lane, outside the compiler's count of loads: `landed` waits for them.
+// (M0 is a reserved register: the compiler gives it to no value, and takes it in no list of what an asm block changes.)
 // (M0 belongs to no value of the compiler's; its own uses write it right before.)
 __device__ __forceinline__ void to_lds(const char* base, unsigned off, unsigned lds) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory");

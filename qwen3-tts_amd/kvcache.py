@@ -333,11 +333,13 @@ class PagedKV:
                scale: Optional[float] = None, max_len: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Attention of the rows' newest tokens over the cache: the token at position p sees the keys j <= p, with `window` > 0 only
         those with j > p - window or j < `sinks`.  q [tokens, heads, head_dim] (heads a multiple of kv_heads; head h reads kv head
-        h // (heads / kv_heads)) -> the same shape; a token that sees nothing gives zeros; tokens behind offsets[-1] are left as they are
-        in `out` (undefined in a new tensor).  fp32 inside, but that probabilities (and over a 4-bit cache, in calls of many tokens, values)
-        are rounded to bf16 where they are operands of bf16 products.  `scale`: head_dim ** -0.5 unless given.  `max_len`: no row is longer than this (0: not
-        known); a good bound helps to cut the work of long rows.  What is wrong with rows, offsets or pages is not reported here but by
-        the append before it: attend leaves `status` alone."""
+        h // (heads / kv_heads)) -> the same shape; a token that sees nothing, or whose scores are all -inf, gives zeros; tokens behind
+        offsets[-1] are left as they are in `out` (undefined in a new tensor).  fp32 inside, but that probabilities (and over a 4-bit cache, in
+        calls of many tokens, values) are rounded to bf16 where they are operands of bf16 products.  `scale`: head_dim ** -0.5 unless given.
+        `max_len`: no row is longer than this (0: not known); a good bound helps to cut the work of long rows.  What is wrong with rows, offsets
+        or pages is not reported here but by the append before it: attend leaves `status` alone.
+        The rows of a call are treated alike: one token behind a very long past, in a call with prompts, is not spread over the card as in a call
+        of its own (100 000 tokens beside a prompt of 2 000: 2.0 ms against 54 + 123 us apart).  Make two calls of such a batch."""
         q, (T, H, D), qp, qt, qh = self._heads(q, "q", None)
         if H % self.kv_heads:
             raise ValueError(f"{H} query heads do not share {self.kv_heads} kv heads evenly")

@@ -1450,3 +1450,21 @@ def test_which_kernel_a_call_takes(dtype):
     assert names(4, 300, window=60) == short and names(4, 20, window=60) == whole
     assert names(800, 4) == (whole if dtype == "f32" else prompt)
     assert names(10, 4) == cut
+
+
+@pytest.mark.parametrize("dtype,D", [("bf16", 64), ("bf16", 80), ("f32", 64), ("f32", 256)])
+def test_scores_that_are_all_minus_infinity_give_zeros(dtype, D):
+    """Rows whose every visible key is -inf against the query: as if nothing were seen, in single tokens, cut rows, pieces and prompts."""
+    g = _gen(D)
+    G, group, lens = 4, 8, [3000, 500]
+    kv = _cache(dtype, G, D, 16, lens, width=1024)
+    _fill(kv, 0, lens, g)
+    kv.k[0, :, :, :, 5] = -float("inf")
+    rows = torch.arange(2, dtype=torch.int32, device=DEV)
+    for new in (None, [3, 2], [700, 500]):
+        T = 2 if new is None else sum(new)
+        q = _randn(g, T, G * group, D).to(kv.activations)
+        q[..., 5] = q[..., 5].abs() + 0.5
+        for max_len in (0, 500):
+            out = kv.attend(0, q, rows, None if new is None else _offsets(new), max_len=max_len)
+            assert bool((out == 0).all()), (new, max_len)
