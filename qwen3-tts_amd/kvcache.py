@@ -168,6 +168,8 @@ class PagedKV:
         """This cache, or one over `state` (tensors like self.state) where those are others than its own."""
         if all(a is b or (a is not None and b is not None and a.data_ptr() == b.data_ptr()) for a, b in zip(state, self.state)):
             return self
+        if any((a is None) != (b is None) for a, b in zip(state, self.state)):
+            raise ValueError("all of the cache's tensors are wanted, in the order of `state`")
         k, v, k_scale, v_scale, table, lens, status = state
         return PagedKV.from_tensors(k, v, table, lens, self.refs, k_scale, v_scale, status)
 

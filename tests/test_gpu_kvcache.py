@@ -1468,3 +1468,22 @@ def test_scores_that_are_all_minus_infinity_give_zeros(dtype, D):
         for max_len in (0, 500):
             out = kv.attend(0, q, rows, None if new is None else _offsets(new), max_len=max_len)
             assert bool((out == 0).all()), (new, max_len)
+
+
+def test_part_of_the_state_is_refused():
+    from qwen3_tts_amd import torch_ops
+    kv = _cache("bf16", 1, 64, 16, [20])
+    _fill(kv, 0, [20], _gen(1))
+    rows, q = torch.zeros(1, dtype=torch.int32, device=DEV), torch.ones(1, 2, 64, dtype=torch.bfloat16, device=DEV)
+    h = torch_ops.register_kv(kv)
+    want = kv.attend(0, q, rows)
+    assert torch.equal(torch.ops.q3tts.kv_attend(q, rows, None, 0, 0, h, 0, *kv.state), want)
+    for some in (kv.state[:2], (None,) + kv.state[1:]):
+        with pytest.raises(ValueError, match="all of the cache's tensors"):
+            torch.ops.q3tts.kv_attend(q, rows, None, 0, 0, h, 0, *some)
+    other = tuple(None if t is None else t.clone() for t in kv.state)
+    other[0].zero_()                                                # uniform weights: the mean of the values
+    out = torch.ops.q3tts.kv_attend(q, rows, None, 0, 0, h, 0, *other)
+    mean = kv.gather(0, rows, _offsets([20]), tokens=20, dtype="f32")[1].double().mean(0)
+    assert float((out[0].double() - mean).abs().max()) <= 2.0 ** -8 * 2 * float(kv.v.float().nan_to_num(0.0).abs().max())
+    torch_ops.unregister_kv(h)
