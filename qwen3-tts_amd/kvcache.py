@@ -57,6 +57,8 @@ def _no_gradient(t: torch.Tensor, what: str) -> None:
 def rope_tables(positions: int, rot_dim: int, theta: float = 10000.0, device: Union[str, torch.device] = "cuda:0") -> Tuple[torch.Tensor, torch.Tensor]:
     """(cos, sin), float32 [positions, rot_dim / 2] each, of position * theta^(-2 i / rot_dim): angles in float64, so that far positions
     are as exact as near ones."""
+    if positions < 1 or rot_dim < 2 or rot_dim % 2:
+        raise ValueError(f"rope tables need a position and an even number of rotated dimensions, got {positions} and {rot_dim}")
     inv = theta ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
     ang = torch.arange(positions, dtype=torch.float64)[:, None] * inv
     return ang.cos().float().to(device), ang.sin().float().to(device)

@@ -160,6 +160,13 @@ def test_rope_tables_of_far_positions():
             assert abs(float(cos[p, i]) - math.cos(a)) < 1e-7 and abs(float(sin[p, i]) - math.sin(a)) < 1e-7
 
 
+def test_rope_tables_of_odd_sizes_are_refused():
+    """15 dimensions would make 8 angles of theta^(-2 i / 15), which append takes for 16 dimensions'."""
+    for positions, rot in ((10, 15), (10, 0), (10, -2), (0, 16)):
+        with pytest.raises(ValueError):
+            rope_tables(positions, rot, device="cpu")
+
+
 def test_the_plain_restatement_itself():
     """Fixed points that need no second implementation: uniform weights, a window of one token, rotation keeps lengths."""
     g = torch.Generator().manual_seed(0)
