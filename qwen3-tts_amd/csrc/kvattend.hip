@@ -101,7 +101,9 @@ __device__ const u32x4 kv_zeros = {0, 0, 0, 0};                 // what dimensio
 // B operand of O^T = V^T P^T when the contraction takes the keys in that order, so probabilities never leave the lane; and because
 // the order of the output rows is free too, lane (m, g) loads for the A operand the DV = DP / 16 consecutive dimensions m DV .. of its
 // keys - whole rows, straight from memory - and transposes that small block in registers (one v_perm per two values).  Nothing
-// passes through LDS.  A chunk is two tiles (32 keys) for bf16 and 4 bits, one (16 keys) for f32.
+// passes through LDS.  A chunk is two tiles (32 keys) for bf16 and 4 bits, one (16 keys) for f32.  Where values are bf16 the products take
+// probabilities in bf16 too, rounded once (their sum is of the unrounded ones): the rounding of each weight is averaged over the keys,
+// the output's own is not (32 rows to 16 001 tokens: 1.8e-3 of the output against 1.7e-3 with fp32 weights).
 template <typename T, int DP> struct Chunk;
 
 template <int DP> struct Chunk<bf16, DP> {
