@@ -952,16 +952,19 @@ __device__ __forceinline__ void meet() {                        // a barrier tha
 }
 __device__ __forceinline__ unsigned lds_of(const void* p) { return (unsigned)(unsigned long long)(lds_void*)p; }
 
-template <typename T, int DP, int KT>
+// PAD: the head is smaller than DP.  Kernels of their own, so that the others have neither its branches nor its registers (one kernel for both: D = 80
+// 118 us and D = 256 261 for 4 x 2 000 tokens, against 104 and 257).
+template <typename T, int DP, int KT, bool PAD>
 __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const KvAttendArgs a, int tiles) {
     typedef Row<T, DP> R;
     constexpr bool DMA = !__is_same(T, Int4);
+    static_assert(DMA || !PAD, "4-bit heads have the sizes of the tiles");
     constexpr int RB = 2 * DP, NCH = DP / 8, KS = DP / 16, ND = DP / 32, NT = KT / 32, RP = 256 / NCH, NR = KT / RP, RW = RP / 4;
     __shared__ __attribute__((aligned(16))) unsigned char sk[2][KT * RB], sv[2][KT * RB];
     __shared__ unsigned long long again[4];    // lanes whose columns want a second look (in LDS: no register is left to carry it)
     __shared__ __attribute__((aligned(16))) float grown[2][DMA ? 4 : KT];      // 4 bits: of each key of a tile
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int hk = blockIdx.x % a.c.heads, G = a.group, D = a.c.dim, sh = a.c.ps_shift;
+    const int hk = blockIdx.x % a.c.heads, G = a.group, D = PAD ? a.c.dim : DP, sh = a.c.ps_shift;
     const Tile t = kv_tile(a, tiles - 1 - (int)(blockIdx.x / a.c.heads), 128, lane);
     if (!t.on) return;
     const int r = lane & 31, hh = lane >> 5;
@@ -1039,6 +1042,14 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
     auto key_at = [&](int k) { return FEW ? ak[0] ^ (32 * k) : ak[FEW ? 0 : k]; };
     auto value_at = [&](int n) { return FEW ? av[0] ^ (64 * n) : av[FEW ? 0 : n]; };
 
+    // Past the head's size keys are zeros: q is 0 there, but 0 times an infinity would be NaN.  (Values: rows of the product that nobody stores.)
+    if constexpr (PAD) {
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+            if (lds_k<DP>(row0 + i * RP, slot) - RB * (row0 + i * RP) >= row_bytes)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) *(u32x4*)(sk[b] + RB * (row0 + i * RP) + 16 * slot) = u32x4{0, 0, 0, 0};
+    }
     int only = t.pmin - 1;                     // as in attend_part: a second look where partly_seen_bad says
     for (;;) {
         const bool all = only < t.pmin;
@@ -1079,20 +1090,23 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
             constexpr bool keys = decltype(which)::value;
             const int kb = span.chunk(c) * KT;
             if constexpr (DMA) {
-                // Past the head's size keys are zeros: q is 0 there, but 0 times an infinity would be NaN.  (Values: rows of the product that nobody stores.)
-                const bool inner = all && kb + KT - 1 <= vhi && (kb > vlo || kb + KT - 1 < sinks) && okm == ~0ull && (!keys || row_bytes == RB);
+                const bool inner = all && kb + KT - 1 <= vhi && (kb > vlo || kb + KT - 1 < sinks) && okm == ~0ull;
                 // the chunk whose place this thread's slot is
                 auto chunk = [&](int i) { return (keys ? lds_k<DP>(row0 + i * RP, slot) : lds_v<DP>(row0 + i * RP, slot)) - RB * (row0 + i * RP); };
-                auto source = [&](int i) { return (unsigned)(sub * row_bytes + (chunk(i) < row_bytes ? chunk(i) : 0)); };
+                auto source = [&](int i) { return (unsigned)(sub * row_bytes + (!PAD || chunk(i) < row_bytes ? chunk(i) : 0)); };
                 const unsigned to = lds_of(lds) + wave * RW * RB;
-                if (inner) {
+                if (inner && (!keys || !PAD)) {
 #pragma unroll
                     for (int i = 0; i < NR; ++i) to_lds(base + place[i], source(i), to + i * RP * RB);
+                } else if (PAD && inner) {     // lanes past the head's size leave the zeros that lie there
+#pragma unroll
+                    for (int i = 0; i < NR; ++i)
+                        if (chunk(i) < row_bytes) to_lds(base + place[i], source(i), to + i * RP * RB);
                 } else {
 #pragma unroll
                     for (int i = 0; i < NR; ++i) {
                         const int first = i * RP + wave * RW, mine = kb + first + sub;
-                        const bool ok = (okm >> first & 1) && mine <= vhi && (mine > vlo || mine < sinks) && (!keys || chunk(i) < row_bytes);
+                        const bool ok = (okm >> first & 1) && mine <= vhi && (mine > vlo || mine < sinks) && (!keys || !PAD || chunk(i) < row_bytes);
                         to_lds(ok ? (const void*)(base + place[i] + source(i)) : (const void*)&kv_zeros, to + i * RP * RB);
                     }
                 }
@@ -1383,14 +1397,18 @@ hipError_t q3_launch_kv_attend(const KvAttendArgs& a, hipStream_t s) {
     if (prompts(a.c, a.b.tokens, a.b.sequences, a.q_heads, a.b.offsets != nullptr)) {
         const int n = (int)tiles_of(a.b.tokens, a.b.sequences, a.group, true, 128);
         const unsigned blocks = (unsigned)n * a.c.heads;
-        if (a.c.dtype == Q3C_KV_BF16) {
-            if (dp == 64) kv_prompt_kernel<bf16, 64, 64><<<blocks, 256, 0, s>>>(a, n);
-            else if (dp == 128) kv_prompt_kernel<bf16, 128, 64><<<blocks, 256, 0, s>>>(a, n);
-            else kv_prompt_kernel<bf16, 256, 32><<<blocks, 256, 0, s>>>(a, n);
+        if (a.c.dtype == Q3C_KV_BF16 && a.c.dim != dp) {
+            if (dp == 64) kv_prompt_kernel<bf16, 64, 64, true><<<blocks, 256, 0, s>>>(a, n);
+            else if (dp == 128) kv_prompt_kernel<bf16, 128, 64, true><<<blocks, 256, 0, s>>>(a, n);
+            else kv_prompt_kernel<bf16, 256, 32, true><<<blocks, 256, 0, s>>>(a, n);
+        } else if (a.c.dtype == Q3C_KV_BF16) {
+            if (dp == 64) kv_prompt_kernel<bf16, 64, 64, false><<<blocks, 256, 0, s>>>(a, n);
+            else if (dp == 128) kv_prompt_kernel<bf16, 128, 64, false><<<blocks, 256, 0, s>>>(a, n);
+            else kv_prompt_kernel<bf16, 256, 32, false><<<blocks, 256, 0, s>>>(a, n);
         } else {
-            if (dp == 64) kv_prompt_kernel<Int4, 64, 64><<<blocks, 256, 0, s>>>(a, n);
-            else if (dp == 128) kv_prompt_kernel<Int4, 128, 32><<<blocks, 256, 0, s>>>(a, n);
-            else kv_prompt_kernel<Int4, 256, 32><<<blocks, 256, 0, s>>>(a, n);
+            if (dp == 64) kv_prompt_kernel<Int4, 64, 64, false><<<blocks, 256, 0, s>>>(a, n);
+            else if (dp == 128) kv_prompt_kernel<Int4, 128, 32, false><<<blocks, 256, 0, s>>>(a, n);
+            else kv_prompt_kernel<Int4, 256, 32, false><<<blocks, 256, 0, s>>>(a, n);
         }
         return hipGetLastError();
     }
