@@ -364,30 +364,29 @@ template <int D> struct Chunk<Int4, D> {
 };
 
 // A matrix product spreads an infinite or NaN value row to columns that do not see it (0 times it is NaN).  So where a result is not finite and the
-// tile's columns differ in what they see, a position's columns are computed again with the rows that it does not see taken out.  Finite data
-// never comes there, and a second look is taken only where it can change something: for columns whose weights are finite (if they are
-// not, a score of the column's own is not, and every look gives NaN), and if one of the rows that only some columns see - from the
-// first position to the last, and as many at the window's far end - is not finite.  This looks for such a row, each thread at every n-th
-// of them from i0 on.
-template <typename T> __device__ __forceinline__ bool partly_seen_bad(const KvAttendArgs& a, const Tile& t, int hk, int W, int sinks, int i0, int n) {
-    const int differ = t.pmax - t.pmin, D = a.c.dim;
+// tile's columns differ in what they see, columns are computed again with the rows that they do not see taken out: positions from .. to at a
+// time, between which no such row enters or leaves.  Finite data never comes there, and a second look is taken only where it can change
+// something: for columns whose weights are finite (if they are not, a score of the column's own is not, and every look gives NaN), and if
+// one of the rows that only some columns see - from the second position to the last, and as many at the window's far end - is not finite.
+// Whether the tile's position pmin + 1 + i sees the row that it is the first to see (i < pmax - pmin), or not the one that the position before
+// is the last to see (i further on by that), and that row is not finite: where a run of positions ends.
+template <typename T> __device__ __forceinline__ bool ends_run(const KvAttendArgs& a, const Tile& t, int hk, int W, int sinks, int i) {
+    asm volatile("" : "+v"(i));                // what follows from it is made here, not carried through the kernel in registers
+    const int differ = t.pmax - t.pmin, D = a.c.dim, tok = i < differ ? t.pmin + 1 + i : t.pmin - W + 1 + i - differ;
+    if (i >= 2 * differ || tok < 0 || (i >= differ && tok < sinks)) return false;
+    const int page = a.c.table[(long long)t.row * a.c.width + (tok >> a.c.ps_shift)];
+    if ((unsigned)page >= (unsigned)a.c.pages) return false;
+    const long long row = ((((long long)a.layer * a.c.pages + page) * a.c.heads + hk) << a.c.ps_shift) + (tok & ((1 << a.c.ps_shift) - 1));
     bool bad = false;
-    for (int i = i0; i < 2 * differ; i += n) {
-        const int tok = i < differ ? t.pmin + 1 + i : t.pmin - W + 1 + i - differ;
-        if (tok < 0 || (i >= differ && tok < sinks)) continue;
-        const int page = a.c.table[(long long)t.row * a.c.width + (tok >> a.c.ps_shift)];
-        if ((unsigned)page >= (unsigned)a.c.pages) continue;
-        const long long row = ((((long long)a.layer * a.c.pages + page) * a.c.heads + hk) << a.c.ps_shift) + (tok & ((1 << a.c.ps_shift) - 1));
-        if constexpr (__is_same(T, float)) {
-            const u32x4* v = (const u32x4*)((const float*)a.c.v + row * D);
-            for (int d = 0; d < D / 4; ++d)
+    if constexpr (__is_same(T, float)) {
+        const u32x4* v = (const u32x4*)((const float*)a.c.v + row * D);
+        for (int d = 0; d < D / 4; ++d)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) bad |= (v[d][e] & 0x7f800000u) == 0x7f800000u;
-        } else {                               // 4 bits: the steps
-            const int words = __is_same(T, bf16) ? D / 2 : D / 64;
-            const unsigned* v = __is_same(T, bf16) ? (const unsigned*)a.c.v + row * words : (const unsigned*)a.c.vs + row * words;
-            for (int d = 0; d < words; ++d) bad |= (v[d] & 0x7f80u) == 0x7f80u || (v[d] & 0x7f800000u) == 0x7f800000u;
-        }
+            for (int e = 0; e < 4; ++e) bad |= (v[d][e] & 0x7f800000u) == 0x7f800000u;
+    } else {                                   // 4 bits: the steps
+        const int words = __is_same(T, bf16) ? D / 2 : D / 64;
+        const unsigned* v = __is_same(T, bf16) ? (const unsigned*)a.c.v + row * words : (const unsigned*)a.c.vs + row * words;
+        for (int d = 0; d < words; ++d) bad |= (v[d] & 0x7f80u) == 0x7f80u || (v[d] & 0x7f800000u) == 0x7f800000u;
     }
     return bad;
 }
@@ -431,11 +430,11 @@ __device__ __forceinline__ void attend_part(const KvAttendArgs& a, const Tile& t
     const float cs = a.scale_log2e;
     unsigned magic = 0x43004300u;              // two bf16 exponents of 128, kept in a register: an and-or takes one constant
     asm("" : "+v"(magic));
-    int only = t.pmin - 1;                     // pmin - 1: all columns at once; else the one position whose columns are wanted (a second look)
-    unsigned long long again = 0;              // lanes whose columns want one
+    int from = t.pmin, to = t.pmax;            // positions that are looked at: all, then runs of them for the columns of lanes `again`
+    unsigned long long again = ~0ull;
+    unsigned ends = 0;                         // bit i: a run ends behind position pmin + i
     for (;;) {
-        const bool all = only < t.pmin;
-        const int vlo = (all ? t.pmin : only) - W, vhi = all ? t.pmax : only;       // a value row counts if vlo < its position <= vhi
+        const int vlo = from - W, vhi = to;    // a value row counts if vlo < its position <= vhi
         f32x4 o[NT];
 #pragma unroll
         for (int i = 0; i < NT; ++i) o[i] = f32x4{0, 0, 0, 0};
@@ -541,7 +540,7 @@ __device__ __forceinline__ void attend_part(const KvAttendArgs& a, const Tile& t
         l += __shfl_xor(l, 16);
         l += __shfl_xor(l, 32);
         if (WAVES == 1) {
-            if (col < t.ncols && (all || mypos == only)) {
+            if (col < t.ncols && (ends == 0 || (mypos >= from && mypos <= to))) {
                 if (whole_row) {
                     const bool none = mypos < 0 || l == 0.f;
                     const float inv = 1.0f / l;
@@ -553,26 +552,34 @@ __device__ __forceinline__ void attend_part(const KvAttendArgs& a, const Tile& t
                     if (g == 0) { part.ml[2 * cq] = mypos < 0 ? -INFINITY : m; part.ml[2 * cq + 1] = mypos < 0 ? 0.f : l; }
                 }
             }
-        } else if (all || mypos == only) {
+        } else if (ends == 0 || (mypos >= from && mypos <= to)) {
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) so[wave][cq][C::dim(i, 4 * g + r)] = o[i][r];
             if (g == 0) { sm[wave][cq] = mypos < 0 ? -INFINITY : m; sl[wave][cq] = mypos < 0 ? 0.f : l; }
         }
-        if (all) {
+        if (ends == 0) {
             float bad = 0.f;
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) bad += o[i][r] * 0.f;
-            if (t.pmax <= t.pmin) break;
+            const int differ = t.pmax - t.pmin;                                     // below 16
+            if (differ <= 0) break;
             again = __ballot(mypos >= 0 && bad != 0.f && l * 0.f == 0.f);
-            if (!again || !__any(partly_seen_bad<T>(a, t, hk, W, sinks, lane, 64))) break;
+            if (!again) break;
+            const unsigned long long rows = __ballot(ends_run<T>(a, t, hk, W, sinks, lane));
+            ends = (unsigned)(rows | rows >> differ) & ((1u << differ) - 1);
+            if (!ends) break;
+            to = t.pmin - 1;
         }
-        do ++only;
-        while (only <= t.pmax && !(again & __ballot(mypos == only)));
-        if (only > t.pmax) break;
+        do {
+            from = to + 1;
+            const unsigned rest = from > t.pmax ? 0 : ends >> (from - t.pmin);
+            to = rest ? from + __builtin_ctz(rest) : t.pmax;
+        } while (from <= t.pmax && !(again & __ballot(mypos >= from && mypos <= to)));
+        if (from > t.pmax) break;
     }
     if constexpr (WAVES == 1) return;
     __syncthreads();
@@ -961,7 +968,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
     static_assert(DMA || !PAD, "4-bit heads have the sizes of the tiles");
     constexpr int RB = 2 * DP, NCH = DP / 8, KS = DP / 16, ND = DP / 32, NT = KT / 32, RP = 256 / NCH, NR = KT / RP, RW = RP / 4;
     __shared__ __attribute__((aligned(16))) unsigned char sk[2][KT * RB], sv[2][KT * RB];
-    __shared__ unsigned long long again[4];    // lanes whose columns want a second look (in LDS: no register is left to carry it)
+    __shared__ unsigned long long again[4], ends[4];           // as in attend_part, in LDS: no register is left to carry them
     __shared__ __attribute__((aligned(16))) float grown[2][DMA ? 4 : KT];      // 4 bits: of each key of a tile
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hk = blockIdx.x % a.c.heads, G = a.group, D = PAD ? a.c.dim : DP, sh = a.c.ps_shift;
@@ -1050,10 +1057,10 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
 #pragma unroll
                 for (int b = 0; b < 2; ++b) *(u32x4*)(sk[b] + RB * (row0 + i * RP) + 16 * slot) = u32x4{0, 0, 0, 0};
     }
-    int only = t.pmin - 1;                     // as in attend_part: a second look where partly_seen_bad says
+    int from = t.pmin, to = t.pmax;            // as in attend_part
+    bool all = true;
     for (;;) {
-        const bool all = only < t.pmin;
-        const int vlo = (all ? t.pmin : only) - W, vhi = all ? t.pmax : only;
+        const int vlo = from - W, vhi = to;
         typename R::Raw kr[DMA ? 1 : NR], vr[DMA ? 1 : NR];
         // 64 entries of the table, one per lane, read again only when a tile leaves them: the wait for them is one for every load in flight
         int ent = 0, ent0 = -0x40000000;
@@ -1090,7 +1097,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
             constexpr bool keys = decltype(which)::value;
             const int kb = span.chunk(c) * KT;
             if constexpr (DMA) {
-                const bool inner = all && kb + KT - 1 <= vhi && (kb > vlo || kb + KT - 1 < sinks) && okm == ~0ull;
+                const bool inner = kb + KT - 1 <= vhi && (kb > vlo || kb + KT - 1 < sinks) && okm == ~0ull;
                 // the chunk whose place this thread's slot is
                 auto chunk = [&](int i) { return (keys ? lds_k<DP>(row0 + i * RP, slot) : lds_v<DP>(row0 + i * RP, slot)) - RB * (row0 + i * RP); };
                 auto source = [&](int i) { return (unsigned)(sub * row_bytes + (!PAD || chunk(i) < row_bytes ? chunk(i) : 0)); };
@@ -1281,7 +1288,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
             if (c + 1 < span.total) tile(c + 1, Const<1>());
         }
         l += __shfl_xor(l, 32);
-        if (col < t.ncols && (all || mypos == only)) {
+        if (col < t.ncols && (all || (mypos >= from && mypos <= to))) {
             const float inv = R::UP / l;
             const bool none = mypos < 0 || l == 0.f;
             bf16* out = (bf16*)a.out + ((long long)(t.tok0 + qtok) * a.q_heads + hk * G + col - qtok * G) * D;
@@ -1307,14 +1314,24 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) kv_prompt_kernel(const
             for (int n = 0; n < ND; ++n)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) bad += o[n][i] * 0.f;
-            if (t.pmax <= t.pmin) return;
+            const int differ = t.pmax - t.pmin;                                     // below 128
+            if (differ <= 0) return;
             const unsigned long long bits = __ballot(mypos >= 0 && bad != 0.f && l * 0.f == 0.f);
             if (lane == 0) again[wave] = bits;
-            if (!__syncthreads_or(bits != 0) || !__syncthreads_or(partly_seen_bad<T>(a, t, hk, W, sinks, tid, 256))) return;
+            if (!__syncthreads_or(bits != 0)) return;
+            const unsigned long long rows = __ballot(ends_run<T>(a, t, hk, W, sinks, tid));
+            if (lane == 0) ends[wave] = rows;
+            if (!__syncthreads_or(rows != 0)) return;
+            all = false;
+            to = t.pmin - 1;
         }
-        do ++only;
-        while (only <= t.pmax && !__syncthreads_or((again[wave] & __ballot(mypos == only)) != 0));
-        if (only > t.pmax) return;
+        do {
+            from = to + 1;
+            auto end = [&](int i) { return ends[i >> 6] >> (i & 63) & 1; };
+            for (to = min(from, t.pmax); to < t.pmax && !end(to - t.pmin) && !end(to - t.pmin + t.pmax - t.pmin);) ++to;
+            to = __builtin_amdgcn_readfirstlane(to);
+        } while (from <= t.pmax && !__syncthreads_or((again[wave] & __ballot(mypos >= from && mypos <= to)) != 0));
+        if (from > t.pmax) return;
     }
 }
 

@@ -1487,3 +1487,30 @@ def test_part_of_the_state_is_refused():
     mean = kv.gather(0, rows, _offsets([20]), tokens=20, dtype="f32")[1].double().mean(0)
     assert float((out[0].double() - mean).abs().max()) <= 2.0 ** -8 * 2 * float(kv.v.float().nan_to_num(0.0).abs().max())
     torch_ops.unregister_kv(h)
+
+
+@pytest.mark.parametrize("dtype,D,G,group,ps", SECOND)
+@pytest.mark.parametrize("window", [0, 700])
+def test_a_bad_token_amid_a_prompt_costs_its_tile_a_look_or_two(dtype, D, G, group, ps, window):
+    """A token whose key and value are NaN, as a bad hidden state makes them, in the middle of a prompt: the positions of its tile before and
+    behind it are looked at as two runs, not one by one (which took up to 33 looks), and so where it leaves the window."""
+    g = _gen(D + G + 8)
+    lens, pos = [1700], 200 + 901
+    kv = _cache(dtype, G, D, ps, lens)
+    _fill(kv, 0, lens, g)
+    rows, off = torch.zeros(1, dtype=torch.int32, device=DEV), _offsets([1500])
+    q = _randn(g, 1500, G * group, D).to(kv.activations)
+    out = torch.empty_like(q)
+
+    def run():
+        return kv.attend(0, q, rows, off, window=window, out=out)
+    clean = _time(run)
+    keep = out.clone()
+    for t in (kv.k_scale, kv.v_scale) if dtype == "int4" else (kv.k, kv.v):
+        t[0, int(kv.table[0, pos // ps]), :, pos % ps] = float("nan")
+    bad = _time(run)
+    sees = torch.zeros(1500, dtype=torch.bool, device=DEV)
+    sees[901:min(1500, 901 + window) if window else 1500] = True
+    assert bool(torch.isnan(out[sees]).all()) and bool(torch.isfinite(out[~sees]).all())
+    assert torch.equal(out[:700], keep[:700])                       # (tiles that the token is in may round their probabilities otherwise)
+    assert bad < 4 * clean, (clean, bad)
