@@ -865,7 +865,7 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const KvAttendArgs a) {
 // the range), which a causal row does a few times in all.
 // Workgroups of one (request, kv head) sit eight apart in launch order, heads fastest: on the eight XCDs, whose workgroups are dealt
 // round robin, a head's keys stay in one L2.  Long columns start first.  16503 new tokens in 6 requests under a window of 2048 (bf16, 16 heads
-// on 8 of 128): 253 us, 810 TFLOP/s of what is visible; the same on 16-column tiles 978.
+// on 8 of 128): 250 us, 820 TFLOP/s of what is visible; the same on 16-column tiles 978.
 // 4 bits: four bytes of the row = one 16-byte chunk; the order of dimensions in a row is then the packed one, which Q's load and the output's
 // store follow.  Scores are sums of many terms, whose roundings would move a probability by several bf16 steps: keys n * step are
 // fp16 operands, whose 11 bits hold the product of 3 and 8 bits exactly, each key divided by a power of two of its largest step that a

@@ -75,7 +75,7 @@ __device__ __forceinline__ bool kv_place(const KvAppendArgs& a, int tok, bool fi
 // A wave has one token and `parts`-th of its heads, VEC pairs per lane as two runs that are each other's rotation partners, so that the
 // rotation needs no exchange between lanes and the norm one butterfly over the head's lanes.  Two runs of heads are requested before
 // the token's place is looked up (offset -> row -> length -> page, four dependent reads): they are what a wave has to wait for once.
-// 28144 tokens of 16 + 8 + 8 heads of 128 in bf16: 113 us, 4.2 TB/s; 64 single tokens 4.8 us.
+// 28144 tokens of 16 + 8 + 8 heads of 128 in bf16: 114 us, 4.2 TB/s; 64 single tokens 4.8 us.
 template <typename T, int VEC, bool CACHED>     // CACHED: keys and values go to the pages here too (no 4-bit cache)
 __device__ __forceinline__ void append_plain(const KvAppendArgs& a, int tok, int part, int parts, int lane, int lpu_shift) {
     constexpr int RUN = 2;
@@ -159,7 +159,7 @@ __device__ __forceinline__ float divide(float x, float d, float y) {
 // [m][s] of the row (m < 16, s < dim / 32) packs dimensions 32 s + m (low half) and 32 s + 16 + m.  A lane has M neighbouring m of a
 // head: whole bytes and, dim / 2 being a multiple of 16, both partners of its rotations.  The group maximum is taken on the bits of
 // |x| (integers order like the floats, NaN above infinity), so a group that holds either reads back as NaN throughout.
-// M = 4: 8-byte loads, two steps of each butterfly, 36.7 us for 10756 tokens of 16 + 8 + 8 heads of 128 (3.9 TB/s; 2: 39, 1: 45 us, where
+// M = 4: 8-byte loads, two steps of each butterfly, 37 us for 10756 tokens of 16 + 8 + 8 heads of 128 (3.9 TB/s; 2: 39, 1: 45 us, where
 // most of the time went to instructions).  A wave for a token's queries and one for its keys and values: both in one took 39 us.
 constexpr int M4 = 4;                         // bytes of each group that a lane has: a head takes 16 / M4 lanes
 template <int D>
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs a, in
 
 // ---- gather: the stored keys and values of the same tokens, back in one piece (zeros where there is no page) -------------------------
 // Bound by the wait for a token's place (four dependent reads) and by memory: a wave has up to RUN runs of a token's heads in flight (4 bits,
-// 10756 tokens of 8 + 8 heads of 128 as bf16: 13.6 us against 16.3 with one run per wave; 4.1 TB/s).
+// 10756 tokens of 8 + 8 heads of 128 as bf16: 13.9 us against 16.3 with one run per wave; 4.1 TB/s).
 template <typename T, typename O, int D4>
 __global__ void __launch_bounds__(256) kv_gather_kernel(const KvView c, const KvBatch b, int layer, O* __restrict__ k_out, O* __restrict__ v_out,
                                                         int waves, int lpu_shift) {
